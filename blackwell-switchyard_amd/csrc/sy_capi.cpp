@@ -1076,6 +1076,105 @@ int64_t sy_probe_grid(int64_t bytes) {
   return g < 1 ? 1 : (g > 32768 ? 32768 : g);
 }
 
+// The cache's sizes and strides, into *out; nothing here reads device memory.
+static int cache_args(const sy_paged* c, CacheArgs* out) {
+  if (!c) return SY_ERR_NULL;
+  if (!valid_dtype(c->dtype)) return SY_ERR_DTYPE;
+  const int64_t big = 0x7fffffff;
+  if (c->n_seq < 0 || c->n_tok < 0 || c->n_seq > big / 2 || c->n_tok > big / 2 || c->n_pages < 1 ||
+      c->n_pages > big || c->table_cols < 0 || c->page < 1 || (c->page & (c->page - 1)) != 0 ||
+      c->page > (1 << 20) || c->table_cols > big / c->page || c->kv_heads < 1 || c->heads < c->kv_heads ||
+      c->heads % c->kv_heads != 0 || c->heads > 0xffff || c->hd < 8 || c->hd > 256 || c->hd % 8 != 0)
+    return SY_ERR_SHAPE;
+  if (c->n_tok != 0 && (c->n_seq == 0 || (!c->starts && c->n_tok % c->n_seq != 0))) return SY_ERR_SHAPE;
+  const int64_t chunk = 16 / esize(c->dtype);
+  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->table_stride < 0) return SY_ERR_STRIDE;
+  if (c->page_stride % chunk != 0 || c->head_stride % chunk != 0 || c->row_stride % chunk != 0)
+    return SY_ERR_STRIDE;
+  if (c->n_tok == 0) return SY_OK;
+  if (!c->k || !c->v || !c->lengths || (c->table_cols != 0 && !c->table)) return SY_ERR_NULL;
+  if (!al16(c->k) || !al16(c->v)) return SY_ERR_SHAPE;
+  int shift = 0;
+  while ((1 << shift) < c->page) ++shift;
+  *out = CacheArgs{c->k, c->v, c->table, c->lengths, c->starts, c->page_stride, c->head_stride, c->row_stride,
+                   c->table_stride, (int)c->n_seq, (int)c->n_tok, (int)(c->n_tok / c->n_seq), (int)c->n_pages,
+                   shift, c->heads, c->kv_heads, c->heads / c->kv_heads, c->hd, c->table_cols << shift};
+  return SY_OK;
+}
+
+int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride,
+                    const float* cosv, const float* sinv, int64_t n_pos, int64_t prefix_len, void* q,
+                    int fill, void* stream) {
+  AppendArgs a{};
+  const int rc = cache_args(c, &a.c);
+  if (rc != SY_OK) return rc;
+  if (n_pos < 0 || prefix_len < 0 || prefix_len > 0x7fffffff || (fill != 0 && fill != 1)) return SY_ERR_SHAPE;
+  if (tok_stride < 0 || head_stride < 0) return SY_ERR_STRIDE;
+  if (c->n_tok == 0) return SY_OK;
+  if (!qkv || !q || (n_pos != 0 && (!cosv || !sinv))) return SY_ERR_NULL;
+  if (!al16(q)) return SY_ERR_SHAPE;
+  a.qkv = qkv;
+  a.tok_stride = tok_stride;
+  a.head_stride = head_stride;
+  a.cosv = cosv;
+  a.sinv = sinv;
+  a.n_pos = n_pos;
+  a.offset = prefix_len;
+  a.q = q;
+  a.fill = fill;
+  return status(launch_append(a, c->dtype, (hipStream_t)stream));
+}
+
+int64_t sy_paged_attention_workspace_bytes(const sy_paged* c, int64_t prefix_len) {
+  CacheArgs a{};
+  const int rc = cache_args(c, &a);
+  if (rc != SY_OK) return rc;
+  if (prefix_len < 0 || prefix_len > 0x7fffffff) return SY_ERR_SHAPE;
+  if (c->n_tok == 0) return 0;
+  const int64_t bytes = attend_workspace(a, prefix_len, c->dtype);
+  return bytes < 0 ? SY_ERR_SHAPE : bytes;
+}
+
+int sy_paged_attention(const sy_paged* c, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                       void* out, const int32_t* prefix_pages, int64_t prefix_len, float scale, int fill,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
+  AttendArgs a{};
+  const int rc = cache_args(c, &a.c);
+  if (rc != SY_OK) return rc;
+  if (prefix_len < 0 || prefix_len > 0x7fffffff || (fill != 0 && fill != 1)) return SY_ERR_SHAPE;
+  const int64_t chunk = 16 / esize(c->dtype);
+  if (q_tok_stride < 0 || q_head_stride < 0 || q_tok_stride % chunk != 0 || q_head_stride % chunk != 0)
+    return SY_ERR_STRIDE;
+  if (c->n_tok == 0) return SY_OK;
+  if (!q || !out || (prefix_len != 0 && !prefix_pages)) return SY_ERR_NULL;
+  if (!al16(q) || !al16(out)) return SY_ERR_SHAPE;
+  const int64_t need = attend_workspace(a.c, prefix_len, c->dtype);
+  if (need < 0) return SY_ERR_SHAPE;
+  if (need > 0 && (!workspace || workspace_bytes < need || !al16(workspace))) return SY_ERR_WORKSPACE;
+  a.q = q;
+  a.q_tok_stride = q_tok_stride;
+  a.q_head_stride = q_head_stride;
+  a.out = out;
+  a.prefix_pages = prefix_pages;
+  a.prefix_len = prefix_len;
+  a.scale = scale;
+  a.fill = fill;
+  a.workspace = workspace;
+  return status(launch_attend(a, c->dtype, (hipStream_t)stream));
+}
+
+int sy_sample(const void* logits, const float* u, int64_t* tokens, const sy_sampling* how, int64_t n_rows,
+              int64_t vocab, int64_t row_stride, int dtype, void* stream) {
+  if (!how) return SY_ERR_NULL;
+  if (!valid_dtype(dtype)) return SY_ERR_DTYPE;
+  if (n_rows < 0 || n_rows > 0x7fffffff || vocab < 1 || vocab > (1 << 18)) return SY_ERR_SHAPE;
+  if (row_stride < 0) return SY_ERR_STRIDE;
+  if (n_rows == 0) return SY_OK;
+  if (!logits || !u || !tokens) return SY_ERR_NULL;
+  const SampleArgs a{logits, u, tokens, *how, n_rows, row_stride, (int)vocab};
+  return status(launch_sample(a, dtype, (hipStream_t)stream));
+}
+
 int sy_bw_probe(int kind, const void* src, void* dst, int64_t bytes, void* stream) {
   if (kind < 0 || kind > 3) return SY_ERR_OP;
   if (bytes <= 0 || bytes % 16 != 0 || (kind == 3 && bytes % 144 != 0)) return SY_ERR_SHAPE;

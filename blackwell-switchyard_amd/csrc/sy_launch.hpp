@@ -426,6 +426,54 @@ hipError_t launch_rope_qkv(const RopeArgs& a, int dtype, hipStream_t s);
 hipError_t launch_swiglu(const void* gu, const void* go, void* out, int64_t n_tok, int f, int dtype,
                          hipStream_t s);
 
+// A paged cache and the operators over it (sy_cache.hip). All sizes checked on the host.
+struct CacheArgs {
+  void* k;
+  void* v;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* starts;  // nullptr: `each` rows a sequence
+  int64_t page_stride, head_stride, row_stride, table_stride;  // elements
+  int n_seq, n_tok, each, n_pages, page_shift, heads, kv_heads, group, hd;
+  int64_t cap;  // tokens a row of the table can hold
+};
+struct AppendArgs {
+  CacheArgs c;
+  const void* qkv;
+  int64_t tok_stride, head_stride;
+  const float* cosv;
+  const float* sinv;
+  int64_t n_pos, offset;
+  void* q;
+  int fill;
+};
+struct AttendArgs {
+  CacheArgs c;
+  const void* q;
+  int64_t q_tok_stride, q_head_stride;
+  void* out;
+  const int32_t* prefix_pages;
+  int64_t prefix_len;
+  float scale;
+  int fill;
+  void* workspace;
+};
+hipError_t launch_append(const AppendArgs& a, int dtype, hipStream_t s);
+// Bytes of workspace of an attention call, or -1 where its tiles pass 32 bits.
+int64_t attend_workspace(const CacheArgs& c, int64_t prefix_len, int dtype);
+hipError_t launch_attend(const AttendArgs& a, int dtype, hipStream_t s);
+
+// Sampling (sy_sample.hip).
+struct SampleArgs {
+  const void* logits;
+  const float* u;
+  int64_t* tokens;
+  sy_sampling how;
+  int64_t n_rows, row_stride;
+  int vocab;
+};
+hipError_t launch_sample(const SampleArgs& a, int dtype, hipStream_t s);
+
 // Generic kernels, the dw reduction and the probes (sy_generic.hip).
 hipError_t launch_fwd_generic(const FwdArgs& a, hipStream_t s);
 hipError_t launch_sol_generic(const FwdArgs& a, hipStream_t s);

@@ -20,6 +20,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "../../include/switchyard.h"
@@ -571,6 +572,160 @@ std::optional<Tensor> swiglu(const Tensor& gu) {
   return SwiGlu::run(gu);
 }
 
+// -------------------------------------------------------------------- serving
+
+bool whole(const Tensor& t) {  // a dense int32 GPU tensor that nothing intercepts
+  using c10::DispatchKey;
+  constexpr c10::DispatchKeySet wrapped{DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                        DispatchKey::Batched, DispatchKey::Functionalize};
+  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kInt &&
+         !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.key_set().has_any(wrapped);
+}
+
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The cache and the sequences of a call with n_tok packed rows and `heads` query heads;
+// false where the Python function has to see the call.
+bool paged_of(const Tensor& like, int64_t heads, const Tensor& k, const Tensor& v, const Tensor& table,
+              const Tensor& lengths, const std::optional<Tensor>& starts, sy_paged* c) {
+  if (!ordinary() || !plain(like) || !plain(k) || !plain(v) || !whole(table) || !whole(lengths) || k.dim() != 4 ||
+      k.sizes() != v.sizes() || k.strides() != v.strides() || like.scalar_type() != k.scalar_type() ||
+      v.scalar_type() != k.scalar_type() || table.dim() != 2 || lengths.dim() != 1 ||
+      table.size(0) != lengths.size(0) || !lengths.is_contiguous() || lengths.size(0) < 1 ||
+      (table.size(1) > 1 && table.stride(1) != 1) || table.size(1) < 1)
+    return false;
+  for (const Tensor* t : {&k, &v, &table, &lengths})
+    if (t->device() != like.device()) return false;
+  const int64_t chunk_of = chunk(k), page = k.size(2), hd = k.size(3);
+  if (k.size(0) < 1 || k.size(1) < 1 || page < 1 || (page & (page - 1)) != 0 || hd < 8 || hd > 256 || hd % 8 != 0 ||
+      k.stride(3) != 1 || heads < 1 || heads % k.size(1) != 0 || heads > 0xffff || !aligned16(k) || !aligned16(v))
+    return false;
+  for (int d = 0; d < 3; ++d)
+    if (k.stride(d) < 0 || k.stride(d) % chunk_of != 0) return false;
+  const int64_t n_seq = lengths.size(0), n_tok = like.size(0);
+  if (starts.has_value()) {
+    if (!whole(*starts) || starts->dim() != 1 || starts->size(0) != n_seq + 1 || !starts->is_contiguous() ||
+        starts->device() != like.device())
+      return false;
+  } else if (n_tok % n_seq != 0) {
+    return false;
+  }
+  *c = sy_paged{k.data_ptr(), v.data_ptr(), table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(),
+                starts.has_value() ? starts->data_ptr<int32_t>() : nullptr, k.stride(0), k.stride(1), k.stride(2),
+                table.stride(0), n_seq, n_tok, k.size(0), table.size(1), (int32_t)page, (int32_t)heads,
+                (int32_t)k.size(1), (int32_t)hd, code_of(k)};
+  return true;
+}
+
+bool tracked(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// The caller's output, if it is one the kernels can write.
+bool out_ok(const std::optional<Tensor>& out, const Tensor& like, int64_t n_tok, int64_t heads, int64_t hd) {
+  return !out.has_value() ||
+         (plain(*out) && out->dim() == 3 && out->size(0) == n_tok && out->size(1) == heads && out->size(2) == hd &&
+          out->is_contiguous() && aligned16(*out) && out->scalar_type() == like.scalar_type() &&
+          out->device() == like.device() && !tracked(*out));
+}
+
+std::optional<Tensor> paged_append(const Tensor& qkv_in, const Tensor& cosv, const Tensor& sinv, const Tensor& k,
+                                   const Tensor& v, const Tensor& table, const Tensor& lengths,
+                                   const std::optional<Tensor>& starts, int64_t prefix_len,
+                                   const std::optional<Tensor>& out) {
+  sy_paged c;
+  if (qkv_in.dim() != 3 || qkv_in.size(0) < 1 || k.dim() != 4) return std::nullopt;
+  const int64_t heads = qkv_in.size(1) - 2 * k.size(1);
+  if (!paged_of(qkv_in, heads, k, v, table, lengths, starts, &c) || qkv_in.size(2) != c.hd || tracked(qkv_in) ||
+      tracked(k) || tracked(v) || prefix_len < 0 || prefix_len > 0x7fffffff ||
+      !out_ok(out, qkv_in, c.n_tok, heads, c.hd))
+    return std::nullopt;
+  for (const Tensor* t : {&cosv, &sinv})
+    if (!plain(*t) || t->scalar_type() != at::kFloat || t->device() != qkv_in.device() || !t->is_contiguous() ||
+        t->dim() < 2 || t->size(-1) * 2 != c.hd || t->numel() != t->size(0) * t->size(-1) || tracked(*t))
+      return std::nullopt;
+  if (cosv.sizes() != sinv.sizes()) return std::nullopt;
+  const c10::DeviceGuard guard(qkv_in.device());
+  const Tensor qkv = qkv_in.stride(2) == 1 && qkv_in.stride(0) >= 0 && qkv_in.stride(1) >= 0 ? qkv_in : qkv_in.contiguous();
+  Tensor q = out.has_value() ? *out : at::empty({c.n_tok, heads, c.hd}, qkv.options().requires_grad(false));
+  check(sy_paged_append(&c, qkv.data_ptr(), qkv.stride(0), qkv.stride(1), cosv.data_ptr<float>(),
+                        sinv.data_ptr<float>(), cosv.size(0), prefix_len, q.data_ptr(), out.has_value() ? 0 : 1,
+                        stream_of(qkv)),
+        "sy_paged_append");
+  changed(k);
+  changed(v);
+  if (out.has_value()) changed(q);
+  return q;
+}
+
+std::optional<Tensor> paged_attention(const Tensor& q_in, const Tensor& k, const Tensor& v, const Tensor& table,
+                                      const Tensor& lengths, const std::optional<Tensor>& starts,
+                                      const std::optional<Tensor>& prefix_pages, int64_t prefix_len, double scale,
+                                      const std::optional<Tensor>& out) {
+  sy_paged c;
+  if (q_in.dim() != 3 || q_in.size(0) < 1) return std::nullopt;
+  const int64_t heads = q_in.size(1);
+  if (!paged_of(q_in, heads, k, v, table, lengths, starts, &c) || q_in.size(2) != c.hd || tracked(q_in) ||
+      tracked(k) || tracked(v) || prefix_len < 0 || prefix_len > 0x7fffffff ||
+      !out_ok(out, q_in, c.n_tok, heads, c.hd))
+    return std::nullopt;
+  if (prefix_len > 0 && (!prefix_pages.has_value() || !whole(*prefix_pages) || prefix_pages->dim() != 1 ||
+                         !prefix_pages->is_contiguous() || prefix_pages->device() != q_in.device() ||
+                         prefix_pages->size(0) * c.page < prefix_len))
+    return std::nullopt;
+  const c10::DeviceGuard guard(q_in.device());
+  const int64_t ce = chunk(q_in);
+  const bool fits = q_in.stride(2) == 1 && q_in.stride(0) >= 0 && q_in.stride(1) >= 0 && q_in.stride(0) % ce == 0 &&
+                    q_in.stride(1) % ce == 0 && aligned16(q_in);
+  const Tensor q = fits ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
+  Tensor o = out.has_value() ? *out : at::empty({c.n_tok, heads, c.hd}, q.options().requires_grad(false));
+  const int64_t bytes = sy_paged_attention_workspace_bytes(&c, prefix_len);
+  if (bytes < 0) return std::nullopt;
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes / 4}, f32_on(q));
+  check(sy_paged_attention(&c, q.data_ptr(), q.stride(0), q.stride(1), o.data_ptr(),
+                           prefix_len > 0 ? prefix_pages->data_ptr<int32_t>() : nullptr, prefix_len, (float)scale,
+                           out.has_value() ? 0 : 1, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+        "sy_paged_attention");
+  if (out.has_value()) changed(o);
+  return o;
+}
+
+// Settings as numbers, each replaced by a tensor of one a row where that is given.
+std::optional<Tensor> sample_tokens(const Tensor& logits_in, const Tensor& u, double temperature, int64_t top_k,
+                                    double top_p, double min_p, const std::optional<Tensor>& temperatures,
+                                    const std::optional<Tensor>& top_ks, const std::optional<Tensor>& top_ps,
+                                    const std::optional<Tensor>& min_ps) {
+  if (!ordinary() || !plain(logits_in) || !plain(u) || logits_in.dim() != 2 || logits_in.numel() == 0 ||
+      logits_in.size(1) > (1 << 18) || u.dim() != 1 || u.size(0) != logits_in.size(0) ||
+      u.scalar_type() != at::kFloat || !u.is_contiguous() || u.device() != logits_in.device())
+    return std::nullopt;
+  sy_sampling how{temperature, top_p, min_p, top_k, nullptr, nullptr, nullptr, nullptr};
+  const auto row_of = [&](const std::optional<Tensor>& t, at::ScalarType dtype) {
+    return (dtype == at::kInt ? whole(*t) : plain(*t)) && t->dim() == 1 && t->size(0) == u.size(0) &&
+           t->scalar_type() == dtype && t->is_contiguous() && t->device() == u.device();
+  };
+  const std::pair<const std::optional<Tensor>*, const float**> floats[] = {
+      {&temperatures, &how.temperatures}, {&top_ps, &how.top_ps}, {&min_ps, &how.min_ps}};
+  for (const auto& [t, p] : floats)
+    if (t->has_value()) {
+      if (!row_of(*t, at::kFloat)) return std::nullopt;
+      *p = (*t)->data_ptr<float>();
+    }
+  if (top_ks.has_value()) {
+    if (!row_of(top_ks, at::kInt)) return std::nullopt;
+    how.top_ks = top_ks->data_ptr<int32_t>();
+  }
+  const c10::DeviceGuard guard(u.device());
+  const bool rows = (logits_in.stride(1) == 1 || logits_in.size(1) == 1) && logits_in.stride(0) >= 0;
+  const Tensor logits = rows ? logits_in : logits_in.contiguous();
+  Tensor tokens = at::empty({logits.size(0)}, logits.options().dtype(at::kLong).requires_grad(false));
+  check(sy_sample(logits.data_ptr(), u.data_ptr<float>(), tokens.data_ptr<int64_t>(), &how, logits.size(0),
+                  logits.size(1), logits.stride(0), code_of(logits), stream_of(logits)),
+        "sy_sample");
+  return tokens;
+}
+
 }  // namespace
 
 // The interpreter's lock is released during a call, as ctypes does.
@@ -585,4 +740,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm", &rms_norm, free_lock);
   m.def("rope_qkv", &rope_qkv, free_lock);
   m.def("swiglu", &swiglu, free_lock);
+  m.def("paged_append", &paged_append, free_lock);
+  m.def("paged_attention", &paged_attention, free_lock);
+  m.def("sample_tokens", &sample_tokens, free_lock);
 }

@@ -68,6 +68,22 @@ class Tuning(ctypes.Structure):
     ]
 
 
+class Paged(ctypes.Structure):
+    """Mirror of ``sy_paged``."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "table", "lengths", "starts")]
+                + [(n, ctypes.c_int64) for n in ("page_stride", "head_stride", "row_stride", "table_stride",
+                                                 "n_seq", "n_tok", "n_pages", "table_cols")]
+                + [(n, ctypes.c_int32) for n in ("page", "heads", "kv_heads", "hd", "dtype")])
+
+
+class Sampling(ctypes.Structure):
+    """Mirror of ``sy_sampling``."""
+
+    _fields_ = ([(n, ctypes.c_double) for n in ("temperature", "top_p", "min_p")] + [("top_k", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("temperatures", "top_ps", "min_ps", "top_ks")])
+
+
 #: Every symbol include/switchyard.h declares, with (restype, argtypes).
 SIGNATURES = {
     "sy_abi_version": (_i32, []),
@@ -113,6 +129,11 @@ SIGNATURES = {
     "sy_rope_qkv": (_i32, [_vp] * 6 + [_i64] * 4 + [_i32, _i32, _vp]),
     "sy_swiglu": (_i32, [_vp, _vp, _i64, _i64, _i32, _vp]),
     "sy_swiglu_bwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "sy_paged_append": (_i32, [ctypes.POINTER(Paged), _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "sy_paged_attention_workspace_bytes": (_i64, [ctypes.POINTER(Paged), _i64]),
+    "sy_paged_attention": (_i32, [ctypes.POINTER(Paged), _vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _i32,
+                                  _vp, _i64, _vp]),
+    "sy_sample": (_i32, [_vp, _vp, _vp, ctypes.POINTER(Sampling), _i64, _i64, _i64, _i32, _vp]),
     "sy_bw_probe": (_i32, [_i32, _vp, _vp, _i64, _vp]),
     "sy_probe_grid": (_i64, [_i64]),
     "sy_tuning_set": (_i32, [ctypes.POINTER(Tuning)]),

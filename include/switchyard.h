@@ -358,6 +358,90 @@ int sy_swiglu(const void* gate_up, void* out, int64_t n_tok, int64_t f, int dtyp
 int sy_swiglu_bwd(const void* gate_up, const void* grad_out, void* dgate_up, int64_t n_tok, int64_t f,
                   int dtype, void* stream);
 
+/* ---- Serving: a paged cache of keys and values, attention over it, sampling ----
+ *
+ * The cache of one layer holds keys and values in pages of `page` tokens (a power of
+ * two): row `slot` of kv head h of page p starts at k + p page_stride + h head_stride +
+ * slot row_stride elements, v likewise; rows are hd elements, dense, and start at
+ * 16-byte boundaries. Token j of sequence b lies in slot j % page of page
+ * table[b table_stride + j / page].
+ *
+ * A call brings new tokens of n_seq sequences, packed: sequence b has rows starts[b] to
+ * starts[b + 1] (non-decreasing, 0 <= starts <= n_tok; NULL: n_tok / n_seq rows each,
+ * in order). lengths[b] counts its tokens in the cache with the new ones, which are the
+ * last: row i of n stands at position lengths[b] - n + i. table, lengths and starts lie
+ * in device memory and are read when the kernels run, so a captured call may be replayed
+ * for other lengths. Lengths past the table's row are taken as its capacity.
+ *
+ * A prefix is shared by all sequences: prefix_len tokens in the pages that prefix_pages
+ * lists. They come before every sequence's own tokens, whose positions they shift.
+ *
+ * Rows behind the last sequence (and before the first) are left as they were, or set to
+ * zero with fill = 1. A page outside [0, n_pages) holds nothing: its tokens are not
+ * attended to, and nothing is written there. */
+typedef struct sy_paged {
+  void* k;
+  void* v;
+  const int32_t* table;    /* [n_seq][table_cols], rows table_stride apart           */
+  const int32_t* lengths;  /* [n_seq]                                                */
+  const int32_t* starts;   /* [n_seq + 1] or NULL                                    */
+  int64_t page_stride;     /* elements                                               */
+  int64_t head_stride;
+  int64_t row_stride;
+  int64_t table_stride;
+  int64_t n_seq;
+  int64_t n_tok;           /* rows of the packed tensors                             */
+  int64_t n_pages;
+  int64_t table_cols;
+  int32_t page;            /* tokens a page, a power of two                          */
+  int32_t heads;           /* query heads, a multiple of kv_heads                    */
+  int32_t kv_heads;
+  int32_t hd;              /* head width, a multiple of 8, at most 256               */
+  int32_t dtype;           /* of the cache and every packed tensor                   */
+} sy_paged;
+
+/* Rotary positions and the append: row i of qkv holds heads + 2 kv_heads heads (queries,
+ * keys, values) at qkv + i tok_stride + head head_stride. Channel c of a query's or key's
+ * first half turns with channel c of its second by cos/sin[position][c] ([n_pos][hd/2]
+ * fp32), position counted with prefix_len; queries go to q [n_tok][heads][hd], keys and
+ * values to the cache. A token with no place (a page outside the cache, a position
+ * outside the table's row or the n_pos rows) has NaN queries and is not cached. */
+int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride,
+                    const float* cosv, const float* sinv, int64_t n_pos, int64_t prefix_len, void* q,
+                    int fill, void* stream);
+
+/* out[i] = sum_j softmax_j(scale <q_i, k_j>) v_j over the keys up to row i's own position
+ * (and the whole prefix); q row i at q + i q_tok_stride + head q_head_stride (16-byte
+ * aligned), out [n_tok][heads][hd] dense. Query head h reads kv head h kv_heads / heads.
+ * Rows that see no key are zero. The workspace holds partial results of long sequences. */
+int64_t sy_paged_attention_workspace_bytes(const sy_paged* c, int64_t prefix_len);
+int sy_paged_attention(const sy_paged* c, const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                       void* out, const int32_t* prefix_pages, int64_t prefix_len, float scale, int fill,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token per row of logits [n_rows][vocab] (rows row_stride apart) from one uniform
+ * number u in [0, 1) each. The candidates, in the order of falling logits and rising
+ * index: the first top_k of them (all if < 1); of these the first ones until they hold
+ * top_p of the weight, at least one; of these those with at least min_p of the largest's
+ * weight. The token is the first candidate, in the order of indices, at which the sum of
+ * weights passes u times their total. Weights are exp((x - max) / temperature) in units
+ * of 2^-44, so that sums are exact in any order; below 2^-45 they are zero. A temperature
+ * <= 0 picks the first largest logit. NaN counts as -inf; a row without a finite or
+ * +inf logit gives -1. Each setting is a number, or with its pointer set a device array
+ * of one a row. */
+typedef struct sy_sampling {
+  double temperature;
+  double top_p;
+  double min_p;
+  int64_t top_k;
+  const float* temperatures;
+  const float* top_ps;
+  const float* min_ps;
+  const int32_t* top_ks;
+} sy_sampling;
+int sy_sample(const void* logits, const float* u, int64_t* tokens, const sy_sampling* how, int64_t n_rows,
+              int64_t vocab, int64_t row_stride, int dtype, void* stream);
+
 /* Speed-of-light ceiling: out[t] = sum_n v_n[t] with the forward's geometry and
  * bytes but no softmax. Replaces speed_of_light (src/switchyard/triton_op.py:153-191). */
 int sy_sol(const void* v, void* out, int64_t n_src, int64_t n_tok, int64_t d,
