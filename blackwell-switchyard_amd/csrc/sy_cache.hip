@@ -186,10 +186,14 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
 // fp32 ones element by element.
 //
 // The work is cut into units of one tile, ordered (kv head, sequence, row tile, key
-// tile), and every wave of a fixed grid takes an equal run of them whatever the lengths
-// are: a long sequence is shared by many waves, short ones lie many in a wave. A run
-// begins and ends inside at most one segment each, so two partial results (o, m, l) a
-// wave are enough; k_merge joins them. Nothing here depends on lengths the host knows.
+// tile), and every workgroup of a fixed grid takes an equal run of them whatever the
+// lengths are: a long sequence is shared by many workgroups, short ones lie many in one.
+// The four waves of a workgroup take the tiles of a segment in turn, each with its own
+// registers and LDS and no barrier between tiles, and join their results through LDS at
+// the segment's end. A run begins and ends inside at most one segment each, so two
+// partial results (o, m, l) a workgroup are enough; k_merge joins them. Nothing here
+// depends on lengths the host knows. Where no sequence can be longer than a few tiles a
+// wave, a workgroup takes one whole segment instead, and nothing is left to merge.
 template <class T> struct Mma;
 template <> struct Mma<BF16> {
   static __device__ __forceinline__ f32x4_t run(const i32x4_t& a, const i32x4_t& b, f32x4_t c) {
@@ -234,8 +238,8 @@ struct Cut {
   int pre;      // 1: every row over the prefix's keys
   int rt;       // rows a tile
   int kt;       // tokens a tile
-  int workers;  // waves
-  int least;    // fewest units a worker takes
+  int workers;  // workgroups
+  int least;    // fewest units a worker takes; 0: every worker takes one whole segment
   int rs;       // rows a partial result holds
   float* o;     // partial results [2 workers][rs][hd], and m, l
   float* ml;
@@ -332,36 +336,57 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
   constexpr bool kF32 = T::code == SY_F32;
   // A row's start moves by 32 (fp32: 16) bytes from row to row modulo all banks.
   constexpr int LS = HD * (int)sizeof(S) + (kF32 ? 16 : 32);
+  constexpr int OS = HD * 4 + 16;  // stride of a row of results in the same space
+  static_assert(16 * OS <= KT * LS, "results fit the values' space");
   __shared__ __align__(16) char lds[kWaves][KT * LS];
+  __shared__ float stats[kWaves][16][2];
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63;
   const int col = lane & 15, grp = lane >> 4;
-  char* const vt = lds[wave_id()];
-  const int worker = __builtin_amdgcn_readfirstlane((int)blockIdx.x * kWaves + wave_id());
+  const int wave = wave_id();
+  char* const vt = lds[wave];
+  const int worker = blockIdx.x;
   const int n_seq = u.pre ? 1 : c.n_seq;
   const int plen = (int)a.prefix_len;
   const int hd = EXACT ? HD : c.hd;
   const float sl = a.scale * 1.44269504088896340736f;
 
-  const int per_head = total_units(c, u, plen, n_seq);
-  const int64_t units = (int64_t)per_head * c.kv_heads;
-  const int64_t share = max((units + u.workers - 1) / u.workers, (int64_t)u.least);
-  const int64_t first = worker * share;
-  const int64_t end = min(first + share, units);
-
-  if (first < end) {
-    int h = (int)(first / per_head);
-    int b, base;
-    locate(c, u, plen, n_seq, (int)(first - (int64_t)h * per_head), &b, &base);
-    Seq s = pass_seq(c, u, plen, b);
-    Tiles ti = tiles_of(u, c.group, s);
-    int rtile, tile;
-    {
-      const int r = (int)(first - (int64_t)h * per_head) - base;
-      rtile = r / ti.key_tiles;
-      tile = r - rtile * ti.key_tiles;
+  int h, b, rtile, tile;
+  Seq s;
+  Tiles ti;
+  int64_t unit = 0, end = 0;
+  bool some;
+  if (u.least == 0) {
+    // Equal row tiles for every sequence: no search.
+    const int per_seq = (c.each * c.group + u.rt - 1) / u.rt;
+    h = worker / (per_seq * n_seq);
+    b = worker / per_seq - h * n_seq;
+    rtile = worker - (h * n_seq + b) * per_seq;
+    tile = 0;
+    s = pass_seq(c, u, plen, b);
+    ti = tiles_of(u, c.group, s);
+    end = ti.key_tiles;
+    some = true;
+  } else {
+    const int per_head = total_units(c, u, plen, n_seq);
+    const int64_t units = (int64_t)per_head * c.kv_heads;
+    const int64_t share = max((units + u.workers - 1) / u.workers, (int64_t)u.least);
+    unit = worker * share;
+    end = min(unit + share, units);
+    some = unit < end;
+    if (some) {
+      h = (int)(unit / per_head);
+      const int at = (int)(unit - (int64_t)h * per_head);
+      int base;
+      locate(c, u, plen, n_seq, at, &b, &base);
+      s = pass_seq(c, u, plen, b);
+      ti = tiles_of(u, c.group, s);
+      rtile = (at - base) / ti.key_tiles;
+      tile = at - base - rtile * ti.key_tiles;
     }
-    int64_t unit = first;
+  }
+
+  if (some) {
     while (true) {
       const int count = (int)min((int64_t)(ti.key_tiles - tile), end - unit);
       const bool begins = tile == 0, whole = begins && count == ti.key_tiles;
@@ -373,16 +398,15 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
       const int last = min(r0 + 16 * NT, rows) - 1;
       const int least = u.pre ? plen : past + r0 / c.group;
       const int most = u.pre ? plen : past + last / c.group;
-      int limit[NT], tok[NT], head[NT];
+      int limit[NT];
       i32x4_t q[NT][KC];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int r = min(r0 + 16 * n + col, last);  // rows past the last repeat it and are not stored
         const int t = r / c.group;
-        tok[n] = s.row0 + t;
-        head[n] = h * c.group + (r - t * c.group);
         limit[n] = u.pre ? plen : past + t;
-        const S* const qp = static_cast<const S*>(a.q) + tok[n] * a.q_tok_stride + head[n] * a.q_head_stride;
+        const S* const qp = static_cast<const S*>(a.q) + (s.row0 + t) * a.q_tok_stride +
+                            (h * c.group + (r - t * c.group)) * a.q_head_stride;
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
           const int ch = (k * 4 + grp) * CE;
@@ -409,19 +433,18 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
       bool ok[MT], okn[MT];
       i32x4_t kx[MT][KC], vx[MT][KC];
       int64_t off[MT];
+      // Ids are read whether or not a token is there (within the row): the first ones do
+      // not wait for the sequence's length.
+      const int last_page = u.pre ? (plen - 1) >> c.page_shift : (int)(c.cap >> c.page_shift) - 1;
       const auto ask_ids = [&](int t) {
 #pragma unroll
-        for (int x = 0; x < MT; ++x) {
-          const int j = t * KT + x * 16 + col;
-          id[x] = -1;
-          if (t < tiles && j < most) id[x] = pages[j >> c.page_shift];
-        }
+        for (int x = 0; x < MT; ++x) id[x] = pages[min((t * KT + x * 16 + col) >> c.page_shift, last_page)];
       };
       const auto place = [&](int t) {  // ids -> offsets; a key with no place reads the cache's first row
 #pragma unroll
         for (int x = 0; x < MT; ++x) {
           const int j = t * KT + x * 16 + col;
-          okn[x] = (unsigned)id[x] < (unsigned)c.n_pages;
+          okn[x] = (unsigned)id[x] < (unsigned)c.n_pages && j < most;
           off[x] = okn[x] ? id[x] * c.page_stride + (j & ((1 << c.page_shift) - 1)) * c.row_stride : 0;
         }
       };
@@ -434,12 +457,12 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
             dst[x][k] = *reinterpret_cast<const i32x4_t*>(base_p + off[x] + (EXACT || ch < hd ? ch : 0));
           }
       };
-      ask_ids(tile);
-      place(tile);
+      ask_ids(tile + wave);
+      place(tile + wave);
       ask(kb, kx);
       ask(vb, vx);
-      ask_ids(tile + 1);
-      for (int t = tile; t < tiles; ++t) {
+      ask_ids(tile + wave + kWaves);
+      for (int t = tile + wave; t < tiles; t += kWaves) {
 #pragma unroll
         for (int x = 0; x < MT; ++x) ok[x] = okn[x];
         bool all_ok = true;
@@ -472,8 +495,8 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
             for (int k = 0; k < KC; ++k)
               if ((k * 4 + grp) * CE >= hd) kx[x][k] = i32x4_t{0, 0, 0, 0};
         }
-        place(t + 1);
-        if (t + 1 < tiles) ask(vb, vx);
+        place(t + kWaves);
+        if (t + kWaves < tiles) ask(vb, vx);
         // S^T
         f32x4_t st[NT][MT];
 #pragma unroll
@@ -484,8 +507,8 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
 #pragma unroll
             for (int k = 0; k < KC; ++k) st[n][x] = Mma<T>::run(kx[x][k], q[n][k], st[n][x]);
           }
-        if (t + 1 < tiles) ask(kb, kx);
-        ask_ids(t + 2);
+        if (t + kWaves < tiles) ask(kb, kx);
+        ask_ids(t + 2 * kWaves);
         // softmax of the tile; a lane holds tokens 4 grp .. 4 grp + 3 of each 16
         i32x4_t p16[NT];
         float pf[NT][MT * 4];
@@ -590,46 +613,55 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
         asm volatile("" ::: "memory");
       }
 
-      // ---- results of the segment
+      // ---- results of the segment: the waves' joined, in their order
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float sum = group_sum(l[n]);
-        const int r = r0 + 16 * n + col;
-        if (r > last) continue;
-        if (whole && direct) {
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          S* const op = static_cast<S*>(a.out) + ((int64_t)tok[n] * c.heads + head[n]) * hd;
+        if (grp == 0) {
+          stats[wave][col][0] = m[n];
+          stats[wave][col][1] = sum;
+        }
 #pragma unroll
-          for (int d = 0; d < MD; ++d) {
-            const int ch = d * 16 + 4 * grp;
-            if (!EXACT && ch >= hd) continue;
+        for (int d = 0; d < MD; ++d)
+          *reinterpret_cast<f32x4_t*>(vt + col * OS + (d * 16 + 4 * grp) * 4) = o[n][d];
+        __syncthreads();
+        const int here = min(16, last + 1 - r0 - 16 * n);
+        const int per_row = hd / 4;
+        for (int i = threadIdx.x; i < here * per_row; i += kBlock) {
+          const int row = i / per_row, ch = (i - row * per_row) * 4;
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][row][0]);
+          const float mu = top == -INFINITY ? 0.0f : top;
+          float all = 0.0f;
+          f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) {
+            const float lw = stats[w][row][1];
+            const float f = lw != lw ? 1.0f : __builtin_amdgcn_exp2f(stats[w][row][0] - mu);
+            all = fmaf(lw, f, all);
+            x += f * *reinterpret_cast<const f32x4_t*>(lds[w] + row * OS + ch * 4);
+          }
+          const int r = r0 + 16 * n + row;
+          const int t = r / c.group;
+          const int64_t at = (int64_t)(s.row0 + t) * c.heads + h * c.group + (r - t * c.group);
+          if (whole && direct) {
             float f[T::ce] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = sum == 0.0f ? 0.0f : o[n][d][i] * inv;
+            for (int e = 0; e < 4; ++e) f[e] = all == 0.0f ? 0.0f : x[e] / all;
             const i32x4_t x4 = pack<T>(f);
-            __builtin_memcpy(op + ch, &x4, 4 * sizeof(S));
-          }
-        } else {
-          float *po, *pm;
-          if (whole) {
-            const int64_t row = (int64_t)tok[n] * c.heads + head[n];
-            po = row_o + row * hd;
-            pm = row_ml + row * 2;
+            __builtin_memcpy(static_cast<S*>(a.out) + at * hd + ch, &x4, 4 * sizeof(S));
           } else {
-            const int64_t slot = (2 * (int64_t)worker + (begins ? 1 : 0)) * u.rs + (r - r0);
-            po = u.o + slot * hd;
-            pm = u.ml + slot * 2;
-          }
-#pragma unroll
-          for (int d = 0; d < MD; ++d) {
-            const int ch = d * 16 + 4 * grp;
-            if (EXACT || ch < hd) *reinterpret_cast<f32x4_t*>(po + ch) = o[n][d];
-          }
-          if (grp == 0) {
-            pm[0] = m[n];
-            pm[1] = sum;
+            const int64_t slot = whole ? at : (2 * (int64_t)worker + (begins ? 1 : 0)) * u.rs + (r - r0);
+            *reinterpret_cast<f32x4_t*>((whole ? row_o : u.o) + slot * hd + ch) = x;
+            if (ch == 0) {
+              float* const pm = (whole ? row_ml : u.ml) + slot * 2;
+              pm[0] = top;
+              pm[1] = all;
+            }
           }
         }
+        __syncthreads();
       }
 
       unit += count;
@@ -661,102 +693,142 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
 
 // ---------------------------------------------------------------------- merge
 //
-// Joins the partial results of rows that several waves worked on, and those of a prefix
-// with a sequence's own: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, in the order
-// of the keys. A wave per output row. Rows that one wave finished are left alone.
+// Joins the partial results of rows that several workgroups worked on, and those of a
+// prefix with a sequence's own: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. A
+// workgroup takes some heads of one token; hd / 4 threads read a partial result, so many
+// results are read at once, and every thread's sum runs in the order of the keys. Rows
+// that one workgroup finished are left alone.
 struct Parts {
-  int first, count, rows_at;  // slots of workers first .. first + count - 1, or one whole result
-  int share_first;            // the worker in whose run the segment begins
-  int row;
+  int first, count, row;  // workers first .. first + count - 1; row of the tile
+};
+struct Shares {
+  int per_head, base;
+  int64_t share;
 };
 
-__device__ __forceinline__ Parts parts_of(const CacheArgs& c, const Cut& u, int plen, int b, const Seq& s, int h, int r) {
-  const Tiles t = tiles_of(u, c.group, s);
-  const int n_seq = u.pre ? 1 : c.n_seq;
-  const int per_head = total_units(c, u, plen, n_seq);
-  const int base = u.pre ? 0 : total_units(c, u, plen, b);
-  const int64_t units = (int64_t)per_head * c.kv_heads;
-  const int64_t share = max((units + u.workers - 1) / u.workers, (int64_t)u.least);
-  const int rtile = r / u.rt;
-  const int64_t at = (int64_t)h * per_head + base + (int64_t)rtile * t.key_tiles;
+__device__ __forceinline__ Shares shares_of(const CacheArgs& c, const Cut& u, int plen, int b) {
+  Shares x;
+  x.per_head = total_units(c, u, plen, u.pre ? 1 : c.n_seq);
+  x.base = u.pre ? 0 : total_units(c, u, plen, b);
+  const int64_t units = (int64_t)x.per_head * c.kv_heads;
+  x.share = max((units + u.workers - 1) / u.workers, (int64_t)u.least);
+  return x;
+}
+__device__ __forceinline__ Parts parts_of(const CacheArgs& c, const Cut& u, const Shares& x, const Seq& s, int h, int r) {
   Parts p;
-  p.first = (int)(at / share);
-  p.count = (int)((at + t.key_tiles - 1) / share) - p.first + 1;
+  const int rtile = r / u.rt;
   p.row = r - rtile * u.rt;
+  if (u.least == 0) {
+    p.first = 0;
+    p.count = 1;
+    return p;
+  }
+  const int k = tiles_of(u, c.group, s).key_tiles;
+  const int64_t at = (int64_t)h * x.per_head + x.base + (int64_t)rtile * k;
+  p.first = (int)(at / x.share);
+  p.count = (int)((at + k - 1) / x.share) - p.first + 1;
   return p;
 }
 
+constexpr int kMostWorkers = 1024;
+
 template <class T>
 __global__ void __launch_bounds__(kBlock)
-k_merge(const AttendArgs a, const Cut own, const Cut pre, const int has_pre, float* const row_o, float* const row_ml,
-        float* const pre_o, float* const pre_ml) {
+k_merge(const AttendArgs a, const Cut own, const Cut pre, const int has_pre, const int per_wg, float* const row_o,
+        float* const row_ml, float* const pre_o, float* const pre_ml) {
   using S = typename T::storage;
   const CacheArgs& c = a.c;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * kWaves + wave_id();
-  if (row >= (int64_t)c.n_tok * c.heads) return;
-  const int tok = (int)(row / c.heads), hq = (int)(row - (int64_t)tok * c.heads);
-  const int h = hq / c.group;
+  __shared__ float weight[2 * kMostWorkers];
+  __shared__ f32x4_t fold[kBlock];
+  __shared__ float tops[kWaves], sums[kWaves];
+  const int tid = threadIdx.x;
+  const int slices = (c.heads + per_wg - 1) / per_wg;
+  const int tok = blockIdx.x / slices, slice = blockIdx.x - tok * slices;
   const int b = find_seq(c, tok);
   if (b < 0) return;
   const Seq s = seq_of(c, b);
-  const Parts mine = parts_of(c, own, 0, b, s, h, (tok - s.row0) * c.group + hq - h * c.group);
-  if (!has_pre && mine.count == 1) return;
-  Parts front{};
+  const Shares xo = own.least == 0 ? Shares{} : shares_of(c, own, 0, b);
+  Shares xp{};
+  Seq ps{};
   if (has_pre) {
-    const Seq ps = pass_seq(c, pre, (int)a.prefix_len, 0);
-    front = parts_of(c, pre, (int)a.prefix_len, 0, ps, h, (tok - ps.row0) * c.group + hq - h * c.group);
+    ps = pass_seq(c, pre, (int)a.prefix_len, 0);
+    xp = shares_of(c, pre, (int)a.prefix_len, 0);
   }
-  // Partial result i: the prefix's come first.
-  const auto part = [&](int i, const float** po, const float** pm) {
-    const bool f = i < front.count;
-    const Cut& u = f ? pre : own;
-    const Parts& p = f ? front : mine;
-    const int k = f ? i : i - front.count;
-    int64_t at;
-    if (p.count == 1) {
-      *po = (f ? pre_o : row_o) + row * c.hd;
-      *pm = (f ? pre_ml : row_ml) + row * 2;
-      return;
+  const int lpr = c.hd / 4, groups = kBlock / lpr;
+  const int grp = tid / lpr, ch = (tid - grp * lpr) * 4;
+  for (int hq = slice * per_wg; hq < min((slice + 1) * per_wg, c.heads); ++hq) {
+    const int64_t row = (int64_t)tok * c.heads + hq;
+    const int h = hq / c.group, g = hq - h * c.group;
+    const Parts mine = parts_of(c, own, xo, s, h, (tok - s.row0) * c.group + g);
+    if (!has_pre && mine.count == 1) continue;
+    Parts front{};
+    if (has_pre) front = parts_of(c, pre, xp, ps, h, (tok - ps.row0) * c.group + g);
+    // Partial result i, the prefix's first: worker first + k's second slot where the segment
+    // begins (k = 0), its first slot otherwise, or one whole result.
+    const auto slot = [&](int i) -> int64_t {
+      const bool f = i < front.count;
+      const Parts& p = f ? front : mine;
+      if (p.count == 1) return row;
+      const int k = f ? i : i - front.count;
+      return (2 * (int64_t)(p.first + k) + (k == 0 ? 1 : 0)) * (f ? pre.rs : own.rs) + p.row;
+    };
+    const float* const fo = front.count == 1 ? pre_o : pre.o;
+    const float* const fm = front.count == 1 ? pre_ml : pre.ml;
+    const float* const mo = mine.count == 1 ? row_o : own.o;
+    const float* const mm = mine.count == 1 ? row_ml : own.ml;
+    const int n = front.count + mine.count;
+    float m = -INFINITY;
+    for (int i = tid; i < n; i += kBlock) {
+      const float x = (i < front.count ? fm : mm)[slot(i) * 2];
+      weight[i] = x;
+      m = fmaxf(m, x);
     }
-    at = (2 * (int64_t)(p.first + k) + (k == 0 ? 1 : 0)) * u.rs + p.row;
-    *po = u.o + at * c.hd;
-    *pm = u.ml + at * 2;
-  };
-  const int n = front.count + mine.count;
-  float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) {
-    const float *po, *pm;
-    part(i, &po, &pm);
-    m = fmaxf(m, pm[0]);
-  }
 #pragma unroll
-  for (int k = 32; k >= 1; k /= 2) m = fmaxf(m, __shfl_xor(m, k));
-  const float mu = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f;
-  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int ch = lane * 4;
+    for (int k = 32; k >= 1; k /= 2) m = fmaxf(m, __shfl_xor(m, k));
+    if ((tid & 63) == 0) tops[wave_id()] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+    for (int i = tid; i < n; i += kBlock) {
+      const float l = (i < front.count ? fm : mm)[slot(i) * 2 + 1];
+      // NaN scores leave no maximum, but the row is not an empty one.
+      const float w = l != l ? 1.0f : __builtin_amdgcn_exp2f(weight[i] - mu);
+      weight[i] = w;
+      sum = fmaf(l, w, sum);
+    }
+#pragma unroll
+    for (int k = 32; k >= 1; k /= 2) sum += __shfl_xor(sum, k);
+    if ((tid & 63) == 0) sums[wave_id()] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) sum += sums[w];
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (grp < groups) {
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float *po, *pm;
-    part(i, &po, &pm);
-    const float w = __builtin_amdgcn_exp2f(pm[0] - mu), li = pm[1];
-    sum = fmaf(li, li != li ? 1.0f : w, sum);  // a row of NaN scores has no maximum but is no empty one
-    if (ch < c.hd) {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(po + ch);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], li != li ? 1.0f : w, o[e]);
+      for (int i = grp; i < n; i += groups)
+        o += weight[i] * *reinterpret_cast<const f32x4_t*>((i < front.count ? fo : mo) + slot(i) * c.hd + ch);
     }
-  }
-  if (ch >= c.hd) return;
-  float f[T::ce] = {};
+    fold[tid] = o;
+    __syncthreads();
+    if (tid < lpr) {
+      for (int k = 1; k < min(groups, n); ++k) o += fold[k * lpr + tid];
+      float f[T::ce] = {};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = sum == 0.0f ? 0.0f : o[e] / sum;
-  const i32x4_t x4 = pack<T>(f);
-  __builtin_memcpy(static_cast<S*>(a.out) + row * c.hd + ch, &x4, 4 * sizeof(S));
+      for (int e = 0; e < 4; ++e) f[e] = sum == 0.0f ? 0.0f : o[e] / sum;
+      const i32x4_t x4 = pack<T>(f);
+      __builtin_memcpy(static_cast<S*>(a.out) + row * c.hd + ch, &x4, 4 * sizeof(S));
+    }
+    __syncthreads();
+  }
 }
 
 // ----------------------------------------------------------------------- host
+
+// Tiles a wave at most of a segment that is not cut.
+constexpr int kShort = 4;
 
 // Row groups of 16 that a tile takes: one where a sequence brings at most 16 rows (a
 // decoded token of up to 16 heads a kv head), else as many as the registers hold.
@@ -777,21 +849,26 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int nt, int cus, 
   u->pre = pre;
   u->kt = dtype == SY_F32 ? 16 : 32;
   u->rt = 16 * nt;
-  u->least = 2;
   const int64_t rows = (int64_t)c.n_tok * c.group;
   const int64_t keys = std::max<int64_t>(1, (len + u->kt - 1) / u->kt);
+  const bool even = !pre && c.starts == nullptr;
   int64_t tiles;  // row tiles, at most
   if (pre) tiles = (rows + u->rt - 1) / u->rt;
-  else if (c.starts == nullptr) tiles = c.n_seq * (((int64_t)c.each * c.group + u->rt - 1) / u->rt);
+  else if (even) tiles = c.n_seq * (((int64_t)c.each * c.group + u->rt - 1) / u->rt);
   else tiles = rows / u->rt + std::min<int64_t>(c.n_seq, rows);
   const int64_t most = 0x7fffffff;
-  if (rows * c.kv_heads > most || tiles > most / keys) return false;
+  if (rows * c.kv_heads > most || tiles > most / keys || tiles * keys > most / c.kv_heads) return false;
+  u->rs = (int)std::min<int64_t>(u->rt, even ? (int64_t)c.each * c.group : rows);
+  // Whole segments where the longest takes a wave few tiles.
+  if (even && keys <= kShort * kWaves) {
+    u->least = 0;
+    u->workers = (int)(tiles * c.kv_heads);
+    return true;
+  }
+  u->least = 2 * kWaves;
   const int64_t units = tiles * keys * c.kv_heads;
-  const int64_t waves = (int64_t)cus * kWaves * (nt == 1 && c.hd <= 128 ? 2 : 1);
-  int64_t w = std::min(waves, (units + u->least - 1) / u->least);
-  w = std::max<int64_t>(kWaves, (w + kWaves - 1) / kWaves * kWaves);
-  u->workers = (int)w;
-  u->rs = (int)std::min<int64_t>(u->rt, pre || c.starts != nullptr ? rows : (int64_t)c.each * c.group);
+  const int64_t full = std::min<int64_t>(kMostWorkers, (int64_t)cus * (nt == 1 && c.hd <= 128 ? 2 : 1));
+  u->workers = (int)std::max<int64_t>(1, std::min(full, (units + u->least - 1) / u->least));
   return true;
 }
 
@@ -816,7 +893,7 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
     u.o = reinterpret_cast<float*>(take(n * c.hd) * sizeof(float));
     u.ml = reinterpret_cast<float*>(take(n * 2) * sizeof(float));
   };
-  slots(p.own);
+  if (p.own.least != 0) slots(p.own);
   if (prefix_len > 0) {
     slots(p.pre);
     const int64_t n = (int64_t)c.n_tok * c.heads;
@@ -831,7 +908,7 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
 
 template <class T, int HD, int NT>
 hipError_t attend_t(const AttendArgs& a, const Cut& u, int direct, float* row_o, float* row_ml, hipStream_t s) {
-  const dim3 grid((unsigned)(u.workers / kWaves));
+  const dim3 grid((unsigned)u.workers);
   if (a.c.hd == HD)
     hipLaunchKernelGGL((k_attend<T, HD, NT, true>), grid, dim3(kBlock), 0, s, a, u, direct, row_o, row_ml);
   else
@@ -858,7 +935,7 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   Plan p = plan_attend(a.c, a.prefix_len, T::code);
   float* const ws = static_cast<float*>(a.workspace);
   const auto at = [&](float* off) { return reinterpret_cast<float*>((char*)ws + reinterpret_cast<uintptr_t>(off)); };
-  p.own.o = at(p.own.o);
+  p.own.o = at(p.own.o);  // (not used where nothing is cut)
   p.own.ml = at(p.own.ml);
   const bool pre = a.prefix_len > 0;
   if (pre) {
@@ -869,10 +946,12 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   }
   hipError_t e = attend_pass<T>(a, p.own, pre ? 0 : 1, ws + p.row_o, ws + p.row_ml, s);
   if (e != hipSuccess) return e;
-  if (!pre && a.c.cap <= p.own.kt) return hipSuccess;  // one key tile: nothing was split
-  const int64_t rows = (int64_t)a.c.n_tok * a.c.heads;
-  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)((rows + kWaves - 1) / kWaves)), dim3(kBlock), 0, s, a, p.own,
-                     p.pre, pre ? 1 : 0, ws + p.row_o, ws + p.row_ml, ws + p.pre_o, ws + p.pre_ml);
+  if (!pre && (p.own.least == 0 || a.c.cap <= p.own.kt)) return hipSuccess;  // nothing was cut
+  // Heads a workgroup: one, until there are far more tokens than fit the device at once.
+  const int per_wg = (int)std::min<int64_t>(a.c.heads, std::max<int64_t>(1, (int64_t)a.c.n_tok * a.c.heads / 8192));
+  const int64_t grid = (int64_t)a.c.n_tok * ((a.c.heads + per_wg - 1) / per_wg);
+  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)grid), dim3(kBlock), 0, s, a, p.own, p.pre, pre ? 1 : 0, per_wg,
+                     ws + p.row_o, ws + p.row_ml, ws + p.pre_o, ws + p.pre_ml);
   return hipGetLastError();
 }
 

@@ -1092,7 +1092,8 @@ static int cache_args(const sy_paged* c, CacheArgs* out) {
   if (c->page_stride % chunk != 0 || c->head_stride % chunk != 0 || c->row_stride % chunk != 0)
     return SY_ERR_STRIDE;
   if (c->n_tok == 0) return SY_OK;
-  if (!c->k || !c->v || !c->lengths || (c->table_cols != 0 && !c->table)) return SY_ERR_NULL;
+  if (c->table_cols < 1) return SY_ERR_SHAPE;
+  if (!c->k || !c->v || !c->lengths || !c->table) return SY_ERR_NULL;
   if (!al16(c->k) || !al16(c->v)) return SY_ERR_SHAPE;
   int shift = 0;
   while ((1 << shift) < c->page) ++shift;

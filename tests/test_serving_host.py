@@ -25,7 +25,7 @@ def _paged(**kw):
 
 BAD = [
     (dict(dtype=7), DTYPE), (dict(n_seq=-1), SHAPE), (dict(n_tok=-1), SHAPE), (dict(n_tok=4), SHAPE),
-    (dict(n_seq=0), SHAPE), (dict(n_pages=0), SHAPE), (dict(table_cols=-1), SHAPE), (dict(page=0), SHAPE),
+    (dict(n_seq=0), SHAPE), (dict(n_pages=0), SHAPE), (dict(table_cols=-1), SHAPE), (dict(table_cols=0), SHAPE), (dict(page=0), SHAPE),
     (dict(page=24), SHAPE), (dict(page=1 << 21), SHAPE), (dict(table_cols=1 << 28), SHAPE), (dict(heads=3), SHAPE),
     (dict(kv_heads=0), SHAPE), (dict(heads=0), SHAPE), (dict(heads=1 << 16), SHAPE), (dict(hd=0), SHAPE),
     (dict(hd=60), SHAPE), (dict(hd=264), SHAPE), (dict(n_tok=1 << 31, starts=FAKE), SHAPE), (dict(k=None), NULL),
