@@ -236,6 +236,7 @@ template <class T> constexpr int tokens_of() { return T::code == SY_F32 ? 16 : 3
 // How a pass over the keys is cut, the same for the kernel, the merge and the host.
 struct Cut {
   int pre;      // 1: every row over the prefix's keys
+  int few;      // sequences of more rows a kv head are k_flash's (none: INT_MAX)
   int rt;       // rows a tile
   int kt;       // tokens a tile
   int workers;  // workgroups
@@ -245,22 +246,23 @@ struct Cut {
   float* ml;
 };
 
-struct Tiles {
-  int row_tiles, key_tiles;
-};
-__device__ __forceinline__ Tiles tiles_of(const Cut& u, int group, const Seq& s) {
-  if (s.n == 0) return {0, 0};
-  const int k = (s.len + u.kt - 1) / u.kt;  // rows that see nothing still have to be written
-  return {(int)(((int64_t)s.n * group + u.rt - 1) / u.rt), k < 1 ? 1 : k};
-}
-
-__device__ __forceinline__ Seq pass_seq(const CacheArgs& c, const Cut& u, int prefix_len, int b) {
-  if (!u.pre) return seq_of(c, b);
+__device__ __forceinline__ Seq pass_seq(const CacheArgs& c, int pre, int prefix_len, int b) {
+  if (!pre) return seq_of(c, b);
   Seq s;
   s.row0 = c.starts != nullptr ? clamp(c.starts[0], 0, c.n_tok) : 0;
   s.n = (c.starts != nullptr ? clamp(c.starts[c.n_seq], s.row0, c.n_tok) : c.n_tok) - s.row0;
   s.len = prefix_len;
   return s;
+}
+
+struct Tiles {
+  int row_tiles, key_tiles;
+};
+__device__ __forceinline__ Tiles tiles_of(const Cut& u, int group, const Seq& s) {
+  const int rows = s.n * group;
+  if (rows == 0 || (!u.pre && rows > u.few)) return {0, 0};
+  const int k = (s.len + u.kt - 1) / u.kt;  // rows that see nothing still have to be written
+  return {(rows + u.rt - 1) / u.rt, k < 1 ? 1 : k};
 }
 
 __device__ __forceinline__ int scan_add(int x) {  // inclusive over the lanes
@@ -273,39 +275,36 @@ __device__ __forceinline__ int scan_add(int x) {  // inclusive over the lanes
   return x;
 }
 
-// The units of one kv head before sequence b (b < 0: not asked for), and of all
-// sequences; and the sequence that holds unit `unit`, with the units before it.
-struct Place {
-  int total, before, seq, base;
-};
-__device__ __forceinline__ int units_of(const CacheArgs& c, const Cut& u, int prefix_len, int b) {
-  const Tiles t = tiles_of(u, c.group, pass_seq(c, u, prefix_len, b));
-  return t.row_tiles * t.key_tiles;
-}
-__device__ __forceinline__ int total_units(const CacheArgs& c, const Cut& u, int prefix_len, int upto) {
-  const int lane = threadIdx.x & 63;
+// Sums and searches over the sequences, `count(b)` units each: every lane looks at another
+// sequence, so 64 of them cost one round of loads.
+template <class F> __device__ __forceinline__ int total_of(int upto, F count) {
   int x = 0;
-  for (int b = lane; b < upto; b += 64) x += units_of(c, u, prefix_len, b);
+  for (int b = threadIdx.x & 63; b < upto; b += 64) x += count(b);
   return __builtin_amdgcn_readlane(scan_add(x), 63);
 }
-__device__ __forceinline__ void locate(const CacheArgs& c, const Cut& u, int prefix_len, int n_seq, int unit,
-                                       int* seq, int* base) {
+// The sequence that holds a unit, and the units before it; false past the last.
+template <class F> __device__ __forceinline__ bool locate(int n_seq, int unit, F count, int* seq, int* base) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int b0 = 0; b0 < n_seq; b0 += 64) {
-    const int mine = b0 + lane < n_seq ? units_of(c, u, prefix_len, b0 + lane) : 0;
+    const int mine = b0 + lane < n_seq ? count(b0 + lane) : 0;
     const int incl = scan_add(mine);
     const uint64_t hit = __ballot(before + incl > unit);
     if (hit != 0) {
       const int l = __ffsll((unsigned long long)hit) - 1;
       *seq = b0 + l;
       *base = before + __builtin_amdgcn_readlane(incl - mine, l);
-      return;
+      return true;
     }
     before += __builtin_amdgcn_readlane(incl, 63);
   }
-  *seq = n_seq - 1;  // not reached: unit < the total
-  *base = before;
+  return false;
+}
+// Units a worker takes (the host sees to it that all numbers of units fit 31 bits).
+__device__ __forceinline__ int share_of(const Cut& u, int units) { return max((units + u.workers - 1) / u.workers, u.least); }
+__device__ __forceinline__ int units_of(const CacheArgs& c, const Cut& u, int prefix_len, int b) {
+  const Tiles t = tiles_of(u, c.group, pass_seq(c, u.pre, prefix_len, b));
+  return t.row_tiles * t.key_tiles;
 }
 
 // Whether any of a chunk's elements is an infinity or NaN.
@@ -324,9 +323,21 @@ template <class T> __device__ __forceinline__ bool nonfinite(const i32x4_t& x) {
   return bad;
 }
 
+// Rows before the first sequence and behind the last become zero.
+template <class T> __device__ __forceinline__ void zero_outside(const AttendArgs& a) {
+  using S = typename T::storage;
+  const CacheArgs& c = a.c;
+  const int lo = clamp(c.starts[0], 0, c.n_tok), hi = clamp(c.starts[c.n_seq], lo, c.n_tok);
+  const int64_t width = (int64_t)c.heads * c.hd;
+  S* const out = static_cast<S*>(a.out);
+  const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x, step = (int64_t)gridDim.x * kBlock;
+  for (int64_t i = at; i < lo * width; i += step) out[i] = S(0);
+  for (int64_t i = hi * width + at; i < c.n_tok * width; i += step) out[i] = S(0);
+}
+
 template <class T, int HD, int NT, bool EXACT>
 __global__ void __launch_bounds__(kBlock, NT == 1 && HD <= 128 ? 2 : 1)
-k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, float* const row_ml) {
+k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, float* const row_o, float* const row_ml) {
   using S = typename T::storage;
   constexpr int CE = T::ce;
   constexpr int KT = tokens_of<T>();
@@ -354,7 +365,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
   int h, b, rtile, tile;
   Seq s;
   Tiles ti;
-  int64_t unit = 0, end = 0;
+  int unit = 0, end = 0;
   bool some;
   if (u.least == 0) {
     // Equal row tiles for every sequence: no search.
@@ -363,23 +374,24 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
     b = worker / per_seq - h * n_seq;
     rtile = worker - (h * n_seq + b) * per_seq;
     tile = 0;
-    s = pass_seq(c, u, plen, b);
+    s = pass_seq(c, u.pre, plen, b);
     ti = tiles_of(u, c.group, s);
     end = ti.key_tiles;
     some = true;
   } else {
-    const int per_head = total_units(c, u, plen, n_seq);
-    const int64_t units = (int64_t)per_head * c.kv_heads;
-    const int64_t share = max((units + u.workers - 1) / u.workers, (int64_t)u.least);
+    const auto count = [&](int x) { return units_of(c, u, plen, x); };
+    const int per_head = total_of(n_seq, count);
+    const int units = per_head * c.kv_heads;
+    const int share = share_of(u, units);
     unit = worker * share;
     end = min(unit + share, units);
     some = unit < end;
     if (some) {
-      h = (int)(unit / per_head);
-      const int at = (int)(unit - (int64_t)h * per_head);
+      h = unit / per_head;
+      const int at = unit - h * per_head;
       int base;
-      locate(c, u, plen, n_seq, at, &b, &base);
-      s = pass_seq(c, u, plen, b);
+      locate(n_seq, at, count, &b, &base);
+      s = pass_seq(c, u.pre, plen, b);
       ti = tiles_of(u, c.group, s);
       rtile = (at - base) / ti.key_tiles;
       tile = at - base - rtile * ti.key_tiles;
@@ -388,7 +400,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
 
   if (some) {
     while (true) {
-      const int count = (int)min((int64_t)(ti.key_tiles - tile), end - unit);
+      const int count = min(ti.key_tiles - tile, end - unit);
       const bool begins = tile == 0, whole = begins && count == ti.key_tiles;
 
       // ---- this segment: kv head h, row tile rtile of sequence b, key tiles [tile, tile + count)
@@ -674,20 +686,354 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
             b = 0;
             ++h;
           }
-          s = pass_seq(c, u, plen, b);
-        } while (s.n == 0);
-        ti = tiles_of(u, c.group, s);
+          s = pass_seq(c, u.pre, plen, b);
+          ti = tiles_of(u, c.group, s);
+        } while (ti.row_tiles == 0);
       }
     }
   }
-  if (a.fill && !u.pre && c.starts != nullptr) {
-    const int lo = clamp(c.starts[0], 0, c.n_tok), hi = clamp(c.starts[c.n_seq], lo, c.n_tok);
-    const int64_t width = (int64_t)c.heads * hd;
-    S* const out = static_cast<S*>(a.out);
-    const int64_t step = (int64_t)gridDim.x * kBlock;
-    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < lo * width; i += step) out[i] = S(0);
-    for (int64_t i = hi * width + (int64_t)blockIdx.x * kBlock + threadIdx.x; i < c.n_tok * width; i += step)
-      out[i] = S(0);
+  if (zero) zero_outside<T>(a);
+}
+
+// ------------------------------------------------- attention of many rows (16-bit)
+//
+// The same pass where a sequence brings more rows than a tile of 16: a workgroup takes 128
+// query rows of a kv head, a wave 32 of them, and all four waves read the same tiles of 64
+// keys and values from LDS, double-buffered: tile t + 1 goes from registers to LDS and
+// tile t + 2 from memory to registers while tile t is multiplied, one barrier a tile. The
+// products run on v_mfma_f32_32x32x16 in the same transposed form; 32 rows a wave take
+// 32 KB of LDS reads for 2^20 products a tile, which LDS delivers in half the time of the
+// products. The maximum is only followed when a score passes it by more than 2^8 (weights
+// stay below 256, and the ratio to their sum is what counts), so the results are hardly
+// ever rescaled.
+//
+// Bound by the matrix cores and, next to them, by the exponentials (a quarter of the
+// vector rate): each wave's tile is 1024 cycles of products and about as many of softmax,
+// which two waves a SIMD overlap.
+struct Flash {
+  int pre;     // 1: every row over the prefix's keys
+  int virt;    // 1: the prefix's tiles come before each sequence's own
+  int few;     // sequences of at most as many rows are k_attend's
+  int tiles;   // row tiles, at most
+  int splits;  // parts that a row tile's keys are cut into
+  float* o;    // partial results [tiles][kv_heads][splits][128][hd], and m, l
+  float* ml;
+};
+constexpr int kFlashRows = 128, kFlashKeys = 64;
+
+__device__ __forceinline__ int flash_tiles(const CacheArgs& c, const Flash& f, int prefix_len, int b) {
+  const Seq s = pass_seq(c, f.pre, prefix_len, b);
+  const int rows = s.n * c.group;
+  return !f.pre && rows <= f.few ? 0 : (rows + kFlashRows - 1) / kFlashRows;
+}
+__device__ __forceinline__ int64_t flash_slot(const CacheArgs& c, const Flash& f, int tile, int h, int split) {
+  return (((int64_t)tile * c.kv_heads + h) * f.splits + split) * kFlashRows;
+}
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+template <class T> __device__ __forceinline__ f32x16_t mma32(const i32x4_t& a, const i32x4_t& b, const f32x16_t& c) {
+  if constexpr (T::code == SY_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+}
+
+template <class T, int HD, bool EXACT>
+__global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
+k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, float* const row_o, float* const row_ml) {
+  using S = typename T::storage;
+  constexpr int KT = kFlashKeys;
+  constexpr int CPR = HD / 8;          // 16-byte chunks of a row
+  constexpr int RP = kBlock / CPR;     // rows the workgroup loads at a time
+  constexpr int NP = KT / RP;
+  constexpr int KS = HD * 2 + 16, VS = HD * 2 + 32;  // strides that spread rows over the banks
+  constexpr int KC = HD / 16, MD = HD / 32;
+  __shared__ __align__(16) char kl[2][KT * KS];
+  __shared__ __align__(16) char vl[2][KT * VS];
+  __shared__ int flags[2][KT];  // 1: the key is there, 2: its value holds an infinity or NaN
+  const CacheArgs& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int col = lane & 31, half = lane >> 5;
+  const int plen = (int)a.prefix_len;
+  const int hd = EXACT ? HD : c.hd;
+  if (zero) zero_outside<T>(a);
+
+  const int h = blockIdx.x % c.kv_heads;
+  const int rest = blockIdx.x / c.kv_heads;
+  const int split = rest % f.splits, tile_id = rest / f.splits;
+  int b, base;
+  if (!locate(f.pre ? 1 : c.n_seq, tile_id, [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &base)) return;
+  const Seq s = pass_seq(c, f.pre, plen, b);
+  const int rows = s.n * c.group;
+  // A sequence's last row tile, which sees the most keys, is first in the grid.
+  const int rtile = (rows + kFlashRows - 1) / kFlashRows - 1 - (tile_id - base);
+  const int r0 = rtile * kFlashRows;
+  const int last = min(r0 + kFlashRows, rows) - 1;
+  const int past = f.pre ? plen : s.len - s.n + 1;  // keys the first token sees
+  const int most = f.pre ? plen : past + last / c.group;
+  const int pre_tiles = f.virt ? (plen + KT - 1) / KT : 0;
+  const int tiles = pre_tiles + (most > 0 ? (most + KT - 1) / KT : 0);
+  const int t0 = (int)((int64_t)tiles * split / f.splits), t1 = (int)((int64_t)tiles * (split + 1) / f.splits);
+
+  // This wave's rows, a lane's own among them.
+  const int w0 = r0 + 32 * wave;
+  const bool active = w0 <= last;
+  const int r = min(w0 + col, last);
+  const int tok = r / c.group;
+  const int limit = f.pre ? plen : past + tok;
+  const int least = f.pre ? plen : past + w0 / c.group;
+  const int wmost = f.pre ? plen : past + min(w0 + 31, last) / c.group;
+  const int64_t out_row = (int64_t)(s.row0 + tok) * c.heads + h * c.group + (r - tok * c.group);
+  i32x4_t q[KC];
+  {
+    const S* const qp = static_cast<const S*>(a.q) + (s.row0 + tok) * a.q_tok_stride +
+                        (h * c.group + (r - tok * c.group)) * a.q_head_stride;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      const int ch = (2 * k + half) * 8;
+      q[k] = i32x4_t{0, 0, 0, 0};
+      if (EXACT || ch < hd) q[k] = *reinterpret_cast<const i32x4_t*>(qp + ch);
+    }
+  }
+  // Scores in base 2; a negative scale turns the queries' signs, so that the largest
+  // product is the largest score.
+  float sl = a.scale * 1.44269504088896340736f;
+  if (sl < 0.0f) {
+    sl = -sl;
+#pragma unroll
+    for (int k = 0; k < KC; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[k][e] ^= (int)0x80008000;
+  }
+
+  // Loading: a thread's rows lr, lr + RP, ... and chunk lc of each.
+  const int lr = tid / CPR, lc = tid % CPR;
+  const bool lc_in = EXACT || lc * 8 < hd;
+  const S* const kb = static_cast<const S*>(c.k) + h * c.head_stride + (lc_in ? lc * 8 : 0);
+  const S* const vb = static_cast<const S*>(c.v) + h * c.head_stride + (lc_in ? lc * 8 : 0);
+  const int32_t* const own_pages = f.pre ? a.prefix_pages : c.table + b * c.table_stride;
+  const int own_last = f.pre ? (plen - 1) >> c.page_shift : (int)(c.cap >> c.page_shift) - 1;
+  const int wg_least = f.pre ? plen : past + r0 / c.group;
+  int id[NP];
+  i32x4_t kx[NP], vx[NP];
+  bool ok[NP];
+  const auto ask_ids = [&](int t) {
+    const bool own = t >= pre_tiles;
+    const int32_t* const pages = own ? own_pages : a.prefix_pages;
+    const int end = own ? own_last : (plen - 1) >> c.page_shift;
+    const int j0 = (own ? t - pre_tiles : t) * KT + lr;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) id[p] = pages[min((j0 + p * RP) >> c.page_shift, end)];
+  };
+  const auto ask = [&](int t) {  // keys with no place read the cache's first row
+    const bool own = t >= pre_tiles;
+    const int j0 = (own ? t - pre_tiles : t) * KT + lr;
+    const int end = own ? most : plen;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int j = j0 + p * RP;
+      ok[p] = (unsigned)id[p] < (unsigned)c.n_pages && j < end;
+      const int64_t off =
+          ok[p] ? id[p] * c.page_stride + (j & ((1 << c.page_shift) - 1)) * c.row_stride : 0;
+      kx[p] = *reinterpret_cast<const i32x4_t*>(kb + off);
+      vx[p] = *reinterpret_cast<const i32x4_t*>(vb + off);
+    }
+  };
+  const auto put = [&](int t) {
+    const int buf = (t - t0) & 1;
+    const bool edge = t >= pre_tiles && (t - pre_tiles + 1) * KT > wg_least;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int row = lr + p * RP;
+      i32x4_t x = vx[p], y = kx[p];
+      if (!ok[p]) x = i32x4_t{0, 0, 0, 0};
+      if (!EXACT && !lc_in) y = i32x4_t{0, 0, 0, 0};
+      *reinterpret_cast<i32x4_t*>(kl[buf] + row * KS + lc * 16) = y;
+      *reinterpret_cast<i32x4_t*>(vl[buf] + row * VS + lc * 16) = x;
+      uint64_t odd = 0;
+      if (edge) odd = __ballot(nonfinite<T>(x)) >> (lane - lc);
+      if (lc == 0) flags[buf][row] = (ok[p] ? 1 : 0) | ((odd & ((1ull << CPR) - 1)) != 0 ? 2 : 0);
+    }
+  };
+
+  float m = -INFINITY, l = 0.0f;
+  f32x16_t o[MD];
+#pragma unroll
+  for (int d = 0; d < MD; ++d) o[d] = f32x16_t{};
+
+  if (t0 < t1) {
+    ask_ids(t0);
+    ask(t0);
+    if (t0 + 1 < t1) ask_ids(t0 + 1);
+    put(t0);
+    if (t0 + 1 < t1) {
+      ask(t0 + 1);
+      if (t0 + 2 < t1) ask_ids(t0 + 2);
+    }
+    __syncthreads();
+  }
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const bool own = t >= pre_tiles;
+    const int j0 = (own ? t - pre_tiles : t) * KT;
+    const bool work = active && (!own || j0 < wmost);
+    f32x16_t st[2];
+    if (work) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        st[x] = f32x16_t{};
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+          const i32x4_t w = *reinterpret_cast<const i32x4_t*>(kl[buf] + (x * 32 + col) * KS + (2 * k + half) * 16);
+          st[x] = mma32<T>(w, q[k], st[x]);
+        }
+      }
+    }
+    if (t + 1 < t1) {
+      put(t + 1);
+      if (t + 2 < t1) {
+        ask(t + 2);
+        if (t + 3 < t1) ask_ids(t + 3);
+      }
+    }
+    if (work) {
+      const int flag = flags[buf][lane];
+      const uint64_t there = __ballot(flag & 1);
+      const uint64_t odd = __ballot(flag & 2);
+      const bool full = ~there == 0 && (!own || j0 + KT <= least);
+      if (!full) {
+        const int lim = own ? limit - j0 : KT;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t bits = (uint32_t)(there >> (32 * x)) >> (4 * half);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int at = 8 * (e / 4) + e % 4;
+            const bool see = ((bits >> at) & 1u) != 0 && x * 32 + at + 4 * half < lim;
+            st[x][e] = see ? st[x][e] : -INFINITY;
+          }
+        }
+      }
+      float top = fmaxf(st[0][0], st[1][0]);
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(fmaxf(top, st[0][e]), st[1][e]);
+      {
+        const uint32_t v = __float_as_uint(top);
+        const auto sw = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * sl;
+      }
+      if (__any(top > m + 8.0f)) {
+        const float mn = fmaxf(m, top);
+        const float sc = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+        m = mn;
+        l *= sc;
+#pragma unroll
+        for (int d = 0; d < MD; ++d) o[d] *= sc;
+      }
+      const float mu = m == -INFINITY ? 0.0f : m;
+      i32x4_t p16[4];
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float pf[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pf[e] = __builtin_amdgcn_exp2f(fmaf(st[k / 2][(k % 2) * 8 + e], sl, -mu));
+          sum += pf[e];
+        }
+        // Weights are rounded to the values' dtype for the product (at most half a step,
+        // independent of one another); their sum is of the unrounded ones.
+        p16[k] = pack<T>(pf);
+      }
+      l += sum;
+      if (__builtin_expect(odd == 0 || full, 1)) {
+#pragma unroll
+        for (int d = 0; d < MD; ++d) {
+          if (!EXACT && d * 32 >= hd) continue;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            i32x4_t w;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const char* const from = vl[buf] + (16 * k + 8 * x + 4 * half + ((lane & 15) >> 2)) * VS + d * 64 +
+                                       ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+              const i16x4_t v4 =
+                  __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)from);
+              const i32x2_t v2 = __builtin_bit_cast(i32x2_t, v4);
+              w[2 * x] = v2[0];
+              w[2 * x + 1] = v2[1];
+            }
+            o[d] = mma32<T>(w, p16[k], o[d]);
+          }
+        }
+      } else {
+        // Rows that do not see a token leave its value out: 0 times an infinity is none.
+#pragma unroll 1
+        for (int j = 0; j < KT; ++j) {
+          const int e = 8 * (j >> 4) + 4 * ((j >> 3) & 1) + (j & 3);  // of the 32 weights of a lane
+          int word = p16[0][0];
+#pragma unroll
+          for (int x = 1; x < 16; ++x) word = e >> 1 == x ? p16[x / 4][x % 4] : word;
+          word = __shfl(word, col + 32 * ((j >> 2) & 1));
+          const i32x4_t w4 = {word, 0, 0, 0};
+          const float pv = (e & 1) ? elem<T>(w4, 1) : elem<T>(w4, 0);
+          if (j0 + j >= limit) continue;
+#pragma unroll
+          for (int d = 0; d < MD; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              i32x4_t v4 = {0, 0, 0, 0};
+              __builtin_memcpy(&v4, vl[buf] + j * VS + d * 64 + (8 * x + 4 * half) * 2, 8);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[d][4 * x + i] = fmaf(pv, elem<T>(v4, i), o[d][4 * x + i]);
+            }
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  {
+    const uint32_t v = __float_as_uint(l);
+    const auto sw = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  if (w0 + col > last) return;
+  if (direct) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    S* const op = static_cast<S*>(a.out) + out_row * hd;
+#pragma unroll
+    for (int d = 0; d < MD; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int ch = d * 32 + 8 * x + 4 * half;
+        if (!EXACT && ch >= hd) continue;
+        float y[8] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = l == 0.0f ? 0.0f : o[d][4 * x + i] * inv;
+        const i32x4_t v4 = pack<T>(y);
+        *reinterpret_cast<i32x2_t*>(op + ch) = i32x2_t{v4[0], v4[1]};
+      }
+    return;
+  }
+  const bool whole = f.splits == 1;
+  const int64_t slot = whole ? out_row : flash_slot(c, f, base + rtile, h, split) + (w0 - r0) + col;
+  float* const po = (whole ? row_o : f.o) + slot * hd;
+#pragma unroll
+  for (int d = 0; d < MD; ++d)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int ch = d * 32 + 8 * x + 4 * half;
+      if (EXACT || ch < hd)
+        *reinterpret_cast<f32x4_t*>(po + ch) =
+            f32x4_t{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+    }
+  if (half == 0) {
+    float* const pm = (whole ? row_ml : f.ml) + slot * 2;
+    pm[0] = m;
+    pm[1] = l;
   }
 }
 
@@ -698,88 +1044,119 @@ k_attend(const AttendArgs a, const Cut u, const int direct, float* const row_o, 
 // workgroup takes some heads of one token; hd / 4 threads read a partial result, so many
 // results are read at once, and every thread's sum runs in the order of the keys. Rows
 // that one workgroup finished are left alone.
-struct Parts {
-  int first, count, row;  // workers first .. first + count - 1; row of the tile
+struct Parts {  // `count` results, number k at row at + k step (+ second at k = 0); one: the row's own
+  int count;
+  int64_t at, step, second;
 };
 struct Shares {
-  int per_head, base;
-  int64_t share;
+  int per_head, base, share;
 };
 
 __device__ __forceinline__ Shares shares_of(const CacheArgs& c, const Cut& u, int plen, int b) {
+  const auto count = [&](int x) { return units_of(c, u, plen, x); };
   Shares x;
-  x.per_head = total_units(c, u, plen, u.pre ? 1 : c.n_seq);
-  x.base = u.pre ? 0 : total_units(c, u, plen, b);
-  const int64_t units = (int64_t)x.per_head * c.kv_heads;
-  x.share = max((units + u.workers - 1) / u.workers, (int64_t)u.least);
+  x.per_head = total_of(u.pre ? 1 : c.n_seq, count);
+  x.base = u.pre ? 0 : total_of(b, count);
+  x.share = share_of(u, x.per_head * c.kv_heads);
   return x;
 }
+// Row r of sequence s and kv head h as k_attend left it: in the second slot of the worker
+// in whose run the segment begins and the first slots of the next ones, or whole.
 __device__ __forceinline__ Parts parts_of(const CacheArgs& c, const Cut& u, const Shares& x, const Seq& s, int h, int r) {
+  const int rtile = r / u.rt, k = tiles_of(u, c.group, s).key_tiles;
+  const int at = h * x.per_head + x.base + rtile * k;
+  const int first = u.least != 0 ? at / x.share : 0;
+  const int count = u.least != 0 ? (at + k - 1) / x.share - first + 1 : 1;
   Parts p;
-  const int rtile = r / u.rt;
-  p.row = r - rtile * u.rt;
-  if (u.least == 0) {
-    p.first = 0;
-    p.count = 1;
-    return p;
-  }
-  const int k = tiles_of(u, c.group, s).key_tiles;
-  const int64_t at = (int64_t)h * x.per_head + x.base + (int64_t)rtile * k;
-  p.first = (int)(at / x.share);
-  p.count = (int)((at + k - 1) / x.share) - p.first + 1;
+  p.count = __builtin_amdgcn_readfirstlane(count);
+  p.at = 2 * (int64_t)first * u.rs + (r - rtile * u.rt);
+  p.step = 2 * u.rs;
+  p.second = u.rs;
+  return p;
+}
+// The same as k_flash left it.
+__device__ __forceinline__ Parts flash_parts(const CacheArgs& c, const Flash& f, int base, int h, int r) {
+  const int rtile = r / kFlashRows;
+  Parts p;
+  p.count = f.splits;
+  p.at = flash_slot(c, f, base + rtile, h, 0) + (r - rtile * kFlashRows);
+  p.step = kFlashRows;
+  p.second = 0;
   return p;
 }
 
-constexpr int kMostWorkers = 1024;
+constexpr int kMostParts = 1024;  // of a row, of one pass
+
+// The prefix's pass is one of pre (k_attend's) and fpre (k_flash's), by which has splits.
+struct JoinArgs {
+  Cut own, pre;
+  Flash fown, fpre;
+  int has_pre;  // 0, 1: k_attend's, 2: k_flash's
+  int per_wg;   // heads a workgroup
+  int few;      // tokens a sequence to look at, where only k_attend's rows were cut; else 0
+  float *row_o, *row_ml, *pre_o, *pre_ml;
+};
 
 template <class T>
-__global__ void __launch_bounds__(kBlock)
-k_merge(const AttendArgs a, const Cut own, const Cut pre, const int has_pre, const int per_wg, float* const row_o,
-        float* const row_ml, float* const pre_o, float* const pre_ml) {
+__global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const JoinArgs g) {
   using S = typename T::storage;
   const CacheArgs& c = a.c;
-  __shared__ float weight[2 * kMostWorkers];
+  __shared__ float weight[2 * kMostParts];
   __shared__ f32x4_t fold[kBlock];
   __shared__ float tops[kWaves], sums[kWaves];
   const int tid = threadIdx.x;
-  const int slices = (c.heads + per_wg - 1) / per_wg;
-  const int tok = blockIdx.x / slices, slice = blockIdx.x - tok * slices;
-  const int b = find_seq(c, tok);
-  if (b < 0) return;
-  const Seq s = seq_of(c, b);
-  const Shares xo = own.least == 0 ? Shares{} : shares_of(c, own, 0, b);
-  Shares xp{};
-  Seq ps{};
-  if (has_pre) {
-    ps = pass_seq(c, pre, (int)a.prefix_len, 0);
-    xp = shares_of(c, pre, (int)a.prefix_len, 0);
+  const int plen = (int)a.prefix_len;
+  const int slices = (c.heads + g.per_wg - 1) / g.per_wg;
+  int tok = blockIdx.x / slices, b;
+  const int slice = blockIdx.x - tok * slices;
+  Seq s;
+  if (g.few != 0) {
+    b = tok / g.few;
+    s = seq_of(c, b);
+    const int i = tok - b * g.few;
+    if (i >= s.n || s.n * c.group > g.own.few) return;
+    tok = s.row0 + i;
+  } else {
+    b = find_seq(c, tok);
+    if (b < 0) return;
+    s = seq_of(c, b);
   }
+  const bool flash = s.n * c.group > g.own.few;
+  Shares xo{}, xp{};
+  int fbase = 0;
+  if (flash)
+    fbase = total_of(b, [&](int x) { return flash_tiles(c, g.fown, plen, x); });
+  else if (g.own.least != 0)
+    xo = shares_of(c, g.own, 0, b);
+  Seq ps{};
+  if (g.has_pre != 0) ps = pass_seq(c, 1, plen, 0);
+  if (g.has_pre == 1) xp = shares_of(c, g.pre, plen, 0);
   const int lpr = c.hd / 4, groups = kBlock / lpr;
   const int grp = tid / lpr, ch = (tid - grp * lpr) * 4;
-  for (int hq = slice * per_wg; hq < min((slice + 1) * per_wg, c.heads); ++hq) {
+  for (int hq = slice * g.per_wg; hq < min((slice + 1) * g.per_wg, c.heads); ++hq) {
     const int64_t row = (int64_t)tok * c.heads + hq;
-    const int h = hq / c.group, g = hq - h * c.group;
-    const Parts mine = parts_of(c, own, xo, s, h, (tok - s.row0) * c.group + g);
-    if (!has_pre && mine.count == 1) continue;
+    const int h = hq / c.group, gi = hq - h * c.group;
+    const int r = (tok - s.row0) * c.group + gi;
+    const Parts mine = flash ? flash_parts(c, g.fown, fbase, h, r) : parts_of(c, g.own, xo, s, h, r);
+    if (g.has_pre == 0 && mine.count == 1) continue;
     Parts front{};
-    if (has_pre) front = parts_of(c, pre, xp, ps, h, (tok - ps.row0) * c.group + g);
-    // Partial result i, the prefix's first: worker first + k's second slot where the segment
-    // begins (k = 0), its first slot otherwise, or one whole result.
-    const auto slot = [&](int i) -> int64_t {
+    const int rp = (tok - ps.row0) * c.group + gi;
+    if (g.has_pre == 1) front = parts_of(c, g.pre, xp, ps, h, rp);
+    else if (g.has_pre == 2) front = flash_parts(c, g.fpre, 0, h, rp);
+    const float* const mo = mine.count == 1 ? g.row_o : flash ? g.fown.o : g.own.o;
+    const float* const mm = mine.count == 1 ? g.row_ml : flash ? g.fown.ml : g.own.ml;
+    const float* const fo = front.count == 1 ? g.pre_o : g.has_pre == 2 ? g.fpre.o : g.pre.o;
+    const float* const fm = front.count == 1 ? g.pre_ml : g.has_pre == 2 ? g.fpre.ml : g.pre.ml;
+    const int n = front.count + mine.count;  // the prefix's first
+    const auto at = [&](int i) -> int64_t {
       const bool f = i < front.count;
-      const Parts& p = f ? front : mine;
-      if (p.count == 1) return row;
+      if ((f ? front.count : mine.count) == 1) return row;
       const int k = f ? i : i - front.count;
-      return (2 * (int64_t)(p.first + k) + (k == 0 ? 1 : 0)) * (f ? pre.rs : own.rs) + p.row;
+      return (f ? front.at : mine.at) + k * (f ? front.step : mine.step) + (k == 0 ? (f ? front.second : mine.second) : 0);
     };
-    const float* const fo = front.count == 1 ? pre_o : pre.o;
-    const float* const fm = front.count == 1 ? pre_ml : pre.ml;
-    const float* const mo = mine.count == 1 ? row_o : own.o;
-    const float* const mm = mine.count == 1 ? row_ml : own.ml;
-    const int n = front.count + mine.count;
     float m = -INFINITY;
     for (int i = tid; i < n; i += kBlock) {
-      const float x = (i < front.count ? fm : mm)[slot(i) * 2];
+      const float x = (i < front.count ? fm : mm)[at(i) * 2];
       weight[i] = x;
       m = fmaxf(m, x);
     }
@@ -792,7 +1169,7 @@ k_merge(const AttendArgs a, const Cut own, const Cut pre, const int has_pre, con
     const float mu = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f;
     for (int i = tid; i < n; i += kBlock) {
-      const float l = (i < front.count ? fm : mm)[slot(i) * 2 + 1];
+      const float l = (i < front.count ? fm : mm)[at(i) * 2 + 1];
       // NaN scores leave no maximum, but the row is not an empty one.
       const float w = l != l ? 1.0f : __builtin_amdgcn_exp2f(weight[i] - mu);
       weight[i] = w;
@@ -809,7 +1186,7 @@ k_merge(const AttendArgs a, const Cut own, const Cut pre, const int has_pre, con
     if (grp < groups) {
 #pragma unroll 4
       for (int i = grp; i < n; i += groups)
-        o += weight[i] * *reinterpret_cast<const f32x4_t*>((i < front.count ? fo : mo) + slot(i) * c.hd + ch);
+        o += weight[i] * *reinterpret_cast<const f32x4_t*>((i < front.count ? fo : mo) + at(i) * c.hd + ch);
     }
     fold[tid] = o;
     __syncthreads();
@@ -829,24 +1206,26 @@ k_merge(const AttendArgs a, const Cut own, const Cut pre, const int has_pre, con
 
 // Tiles a wave at most of a segment that is not cut.
 constexpr int kShort = 4;
+constexpr int64_t kMost = 0x7fffffff;
 
-// Row groups of 16 that a tile takes: one where a sequence brings at most 16 rows (a
-// decoded token of up to 16 heads a kv head), else as many as the registers hold.
-int row_groups(int64_t rows, int hd, int dtype) {
-  if (rows <= 16) return 1;
-  return dtype == SY_F32 ? (hd > 128 ? 1 : 2) : (hd > 128 ? 2 : 4);
-}
-
+// What a call launches: k_attend over the sequences of few rows, k_flash over the others,
+// one of them over a shared prefix, and the merge of what was cut.
 struct Plan {
-  Cut own, pre;
-  int nt_own, nt_pre;
-  int64_t bytes;
-  int64_t row_o, row_ml, pre_o, pre_ml;  // float offsets
   bool ok;
+  bool attend, flash;  // the sequences' own keys
+  int pre;             // a pass over the prefix: 0 none, 1 k_attend, 2 k_flash
+  int direct_attend, direct_flash;
+  bool merge;
+  int merge_few;
+  Cut own, cpre;
+  Flash fown, fpre;
+  int64_t bytes;
+  int64_t row_o, row_ml, pre_o, pre_ml;  // float offsets, as the o and ml of the passes
 };
 
-bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int nt, int cus, Cut* u) {
+bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int few, int nt, int cus, Cut* u) {
   u->pre = pre;
+  u->few = few;
   u->kt = dtype == SY_F32 ? 16 : 32;
   u->rt = 16 * nt;
   const int64_t rows = (int64_t)c.n_tok * c.group;
@@ -855,9 +1234,9 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int nt, int cus, 
   int64_t tiles;  // row tiles, at most
   if (pre) tiles = (rows + u->rt - 1) / u->rt;
   else if (even) tiles = c.n_seq * (((int64_t)c.each * c.group + u->rt - 1) / u->rt);
+  else if (few <= u->rt) tiles = std::min<int64_t>(c.n_seq, rows);
   else tiles = rows / u->rt + std::min<int64_t>(c.n_seq, rows);
-  const int64_t most = 0x7fffffff;
-  if (rows * c.kv_heads > most || tiles > most / keys || tiles * keys > most / c.kv_heads) return false;
+  if (tiles > kMost / 2 / keys || tiles * keys > kMost / 2 / c.kv_heads) return false;
   u->rs = (int)std::min<int64_t>(u->rt, even ? (int64_t)c.each * c.group : rows);
   // Whole segments where the longest takes a wave few tiles.
   if (even && keys <= kShort * kWaves) {
@@ -867,35 +1246,92 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int nt, int cus, 
   }
   u->least = 2 * kWaves;
   const int64_t units = tiles * keys * c.kv_heads;
-  const int64_t full = std::min<int64_t>(kMostWorkers, (int64_t)cus * (nt == 1 && c.hd <= 128 ? 2 : 1));
+  const int64_t full = std::min<int64_t>(kMostParts, (int64_t)cus * (nt == 1 && c.hd <= 128 ? 2 : 1));
   u->workers = (int)std::max<int64_t>(1, std::min(full, (units + u->least - 1) / u->least));
   return true;
+}
+
+// Parts of a row tile's keys: as many as let the workgroups fill the device's places in
+// whole rounds, where the grid alone would not; at least four tiles each.
+bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int few, int cus, Flash* f) {
+  f->pre = pre;
+  f->virt = virt;
+  f->few = few;
+  const int64_t rows = (int64_t)c.n_tok * c.group;
+  if (pre) f->tiles = (int)((rows + kFlashRows - 1) / kFlashRows);
+  else if (c.starts == nullptr)
+    f->tiles = (int)std::min<int64_t>(kMost, c.n_seq * (((int64_t)c.each * c.group + kFlashRows - 1) / kFlashRows));
+  else f->tiles = (int)(rows / kFlashRows + std::min<int64_t>(c.n_seq, rows / (few + 1)));
+  const int64_t places = (int64_t)cus * (c.hd <= 128 ? 2 : 1);
+  const int64_t grid = (int64_t)f->tiles * c.kv_heads;
+  const int64_t keys = (pre ? prefix_len : c.cap + (virt ? prefix_len : 0));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, keys / (4 * kFlashKeys)));
+  f->splits = 1;
+  double best = 1e30;
+  for (int n = 1; n <= most && grid < 4 * places; ++n) {
+    // Rounds of the grid over the device, each 1/n of the keys, and a part's own cost.
+    const double cost = (double)((grid * n + places - 1) / places) / n + 0.02 * n;
+    if (cost < best - 1e-9) {
+      best = cost;
+      f->splits = n;
+    }
+  }
+  return grid * f->splits <= kMost / kFlashRows;
 }
 
 Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
   Plan p{};
   int cus = 0;
   if (cu_count(&cus) != hipSuccess || cus < 1) cus = 1;
-  const int64_t rows = (int64_t)c.n_tok * c.group;
-  p.nt_own = row_groups((rows + c.n_seq - 1) / c.n_seq, c.hd, dtype);
-  p.nt_pre = row_groups(rows, c.hd, dtype);
-  p.ok = cut(c, dtype, false, c.cap, p.nt_own, cus, &p.own);
-  if (p.ok && prefix_len > 0) p.ok = cut(c, dtype, true, prefix_len, p.nt_pre, cus, &p.pre);
+  const int64_t rows = (int64_t)c.n_tok * c.group;  // of a kv head
+  if (rows * c.kv_heads > kMost / 2) return p;
+  const int64_t avg = (rows + c.n_seq - 1) / c.n_seq;
+  p.ok = true;
+  if (dtype == SY_F32) {
+    const int nt = avg <= 16 ? 1 : c.hd > 128 ? 1 : 2;
+    p.attend = true;
+    p.pre = prefix_len > 0 ? 1 : 0;
+    p.ok = cut(c, dtype, false, c.cap, (int)kMost, nt, cus, &p.own);
+    if (p.ok && p.pre) p.ok = cut(c, dtype, true, prefix_len, (int)kMost, rows <= 16 || c.hd > 128 ? 1 : 2, cus, &p.cpre);
+  } else {
+    // Up to 16 rows are k_attend's. A prefix has a pass of its own where sequences bring
+    // few rows, so that it is read once for all; else its keys are part of every
+    // sequence's, whose rows share them anyway.
+    const bool shared = prefix_len > 0 && avg <= 16;
+    const bool virt = prefix_len > 0 && !shared;
+    const int few = virt ? 0 : 16;
+    p.attend = !virt && (c.starts != nullptr || avg <= 16);
+    p.flash = c.starts != nullptr ? rows > few : avg > few;
+    p.own.few = few;
+    if (p.attend) p.ok = cut(c, dtype, false, c.cap, few, 1, cus, &p.own);
+    if (p.ok && p.flash) p.ok = flash_cut(c, false, virt, prefix_len, few, cus, &p.fown);
+    p.pre = !shared ? 0 : rows <= 16 ? 1 : 2;
+    if (p.ok && p.pre == 1) p.ok = cut(c, dtype, true, prefix_len, (int)kMost, 1, cus, &p.cpre);
+    if (p.ok && p.pre == 2) p.ok = flash_cut(c, true, false, prefix_len, 0, cus, &p.fpre);
+  }
   if (!p.ok) return p;
+  p.direct_attend = p.pre == 0;
+  p.direct_flash = p.pre == 0 && p.fown.splits == 1;
+  const bool cut_attend = p.attend && p.own.least != 0 && c.cap > p.own.kt;
+  p.merge = p.pre != 0 || cut_attend || (p.flash && p.fown.splits > 1);
+  p.merge_few = p.pre == 0 && !(p.flash && p.fown.splits > 1) && p.flash ? std::max(1, 16 / c.group) : 0;
   int64_t at = 0;
   const auto take = [&](int64_t n) {
     const int64_t was = at;
     at += (n + 3) / 4 * 4;
     return was;
   };
-  const auto slots = [&](Cut& u) {
-    const int64_t n = 2 * (int64_t)u.workers * u.rs;
+  const auto slots = [&](auto& u, int64_t n) {
     u.o = reinterpret_cast<float*>(take(n * c.hd) * sizeof(float));
     u.ml = reinterpret_cast<float*>(take(n * 2) * sizeof(float));
   };
-  if (p.own.least != 0) slots(p.own);
-  if (prefix_len > 0) {
-    slots(p.pre);
+  if (p.attend && p.own.least != 0) slots(p.own, 2 * (int64_t)p.own.workers * p.own.rs);
+  if (p.flash && p.fown.splits > 1)
+    slots(p.fown, (int64_t)p.fown.tiles * c.kv_heads * p.fown.splits * kFlashRows);
+  if (p.pre == 1) slots(p.cpre, 2 * (int64_t)p.cpre.workers * p.cpre.rs);
+  if (p.pre == 2 && p.fpre.splits > 1)
+    slots(p.fpre, (int64_t)p.fpre.tiles * c.kv_heads * p.fpre.splits * kFlashRows);
+  if (p.pre != 0) {
     const int64_t n = (int64_t)c.n_tok * c.heads;
     p.row_o = take(n * c.hd);
     p.row_ml = take(n * 2);
@@ -906,52 +1342,81 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
   return p;
 }
 
+struct Rows {
+  float *o, *ml;
+};
+
 template <class T, int HD, int NT>
-hipError_t attend_t(const AttendArgs& a, const Cut& u, int direct, float* row_o, float* row_ml, hipStream_t s) {
+hipError_t attend_t(const AttendArgs& a, const Cut& u, int direct, int zero, const Rows& r, hipStream_t s) {
   const dim3 grid((unsigned)u.workers);
   if (a.c.hd == HD)
-    hipLaunchKernelGGL((k_attend<T, HD, NT, true>), grid, dim3(kBlock), 0, s, a, u, direct, row_o, row_ml);
+    hipLaunchKernelGGL((k_attend<T, HD, NT, true>), grid, dim3(kBlock), 0, s, a, u, direct, zero, r.o, r.ml);
   else
-    hipLaunchKernelGGL((k_attend<T, HD, NT, false>), grid, dim3(kBlock), 0, s, a, u, direct, row_o, row_ml);
+    hipLaunchKernelGGL((k_attend<T, HD, NT, false>), grid, dim3(kBlock), 0, s, a, u, direct, zero, r.o, r.ml);
   return hipGetLastError();
 }
 
 template <class T>
-hipError_t attend_pass(const AttendArgs& a, const Cut& u, int direct, float* row_o, float* row_ml, hipStream_t s) {
-  constexpr bool f = T::code == SY_F32;
+hipError_t attend_pass(const AttendArgs& a, const Cut& u, int direct, int zero, const Rows& r, hipStream_t s) {
+  constexpr int two = T::code == SY_F32 ? 2 : 1;  // fp32 rows in two groups of 16, up to 128 wide
   const bool one = u.rt == 16;
   if (a.c.hd <= 64)
-    return one ? attend_t<T, 64, 1>(a, u, direct, row_o, row_ml, s)
-               : attend_t<T, 64, f ? 2 : 4>(a, u, direct, row_o, row_ml, s);
+    return one ? attend_t<T, 64, 1>(a, u, direct, zero, r, s) : attend_t<T, 64, two>(a, u, direct, zero, r, s);
   if (a.c.hd <= 128)
-    return one ? attend_t<T, 128, 1>(a, u, direct, row_o, row_ml, s)
-               : attend_t<T, 128, f ? 2 : 4>(a, u, direct, row_o, row_ml, s);
-  return one ? attend_t<T, 256, 1>(a, u, direct, row_o, row_ml, s)
-             : attend_t<T, 256, f ? 1 : 2>(a, u, direct, row_o, row_ml, s);
+    return one ? attend_t<T, 128, 1>(a, u, direct, zero, r, s) : attend_t<T, 128, two>(a, u, direct, zero, r, s);
+  return attend_t<T, 256, 1>(a, u, direct, zero, r, s);
+}
+
+template <class T, int HD>
+hipError_t flash_t(const AttendArgs& a, const Flash& f, int direct, int zero, const Rows& r, hipStream_t s) {
+  const dim3 grid((unsigned)(f.tiles * a.c.kv_heads * f.splits));
+  if (a.c.hd == HD)
+    hipLaunchKernelGGL((k_flash<T, HD, true>), grid, dim3(kBlock), 0, s, a, f, direct, zero, r.o, r.ml);
+  else
+    hipLaunchKernelGGL((k_flash<T, HD, false>), grid, dim3(kBlock), 0, s, a, f, direct, zero, r.o, r.ml);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t flash_pass(const AttendArgs& a, const Flash& f, int direct, int zero, const Rows& r, hipStream_t s) {
+  if constexpr (T::code == SY_F32) {
+    return hipErrorInvalidConfiguration;
+  } else {
+    if (a.c.hd <= 64) return flash_t<T, 64>(a, f, direct, zero, r, s);
+    if (a.c.hd <= 128) return flash_t<T, 128>(a, f, direct, zero, r, s);
+    return flash_t<T, 256>(a, f, direct, zero, r, s);
+  }
 }
 
 template <class T>
 hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   Plan p = plan_attend(a.c, a.prefix_len, T::code);
-  float* const ws = static_cast<float*>(a.workspace);
-  const auto at = [&](float* off) { return reinterpret_cast<float*>((char*)ws + reinterpret_cast<uintptr_t>(off)); };
-  p.own.o = at(p.own.o);  // (not used where nothing is cut)
-  p.own.ml = at(p.own.ml);
-  const bool pre = a.prefix_len > 0;
-  if (pre) {
-    p.pre.o = at(p.pre.o);
-    p.pre.ml = at(p.pre.ml);
-    const hipError_t e = attend_pass<T>(a, p.pre, 0, ws + p.pre_o, ws + p.pre_ml, s);
-    if (e != hipSuccess) return e;
-  }
-  hipError_t e = attend_pass<T>(a, p.own, pre ? 0 : 1, ws + p.row_o, ws + p.row_ml, s);
+  char* const ws = static_cast<char*>(a.workspace);
+  const auto place = [&](auto& u) {  // offsets -> addresses (unused where nothing is cut)
+    u.o = reinterpret_cast<float*>(ws + reinterpret_cast<uintptr_t>(u.o));
+    u.ml = reinterpret_cast<float*>(ws + reinterpret_cast<uintptr_t>(u.ml));
+  };
+  place(p.own);
+  place(p.cpre);
+  place(p.fown);
+  place(p.fpre);
+  float* const wf = static_cast<float*>(a.workspace);
+  const Rows own{wf + p.row_o, wf + p.row_ml}, pre{wf + p.pre_o, wf + p.pre_ml};
+  hipError_t e = hipSuccess;
+  if (p.pre == 1) e = attend_pass<T>(a, p.cpre, 0, 0, pre, s);
+  else if (p.pre == 2) e = flash_pass<T>(a, p.fpre, 0, 0, pre, s);
   if (e != hipSuccess) return e;
-  if (!pre && (p.own.least == 0 || a.c.cap <= p.own.kt)) return hipSuccess;  // nothing was cut
-  // Heads a workgroup: one, until there are far more tokens than fit the device at once.
-  const int per_wg = (int)std::min<int64_t>(a.c.heads, std::max<int64_t>(1, (int64_t)a.c.n_tok * a.c.heads / 8192));
-  const int64_t grid = (int64_t)a.c.n_tok * ((a.c.heads + per_wg - 1) / per_wg);
-  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)grid), dim3(kBlock), 0, s, a, p.own, p.pre, pre ? 1 : 0, per_wg,
-                     ws + p.row_o, ws + p.row_ml, ws + p.pre_o, ws + p.pre_ml);
+  const int zero = a.fill && a.c.starts != nullptr;
+  if (p.flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero, own, s);
+  if (e != hipSuccess) return e;
+  if (p.attend) e = attend_pass<T>(a, p.own, p.direct_attend, zero && !p.flash, own, s);
+  if (e != hipSuccess || !p.merge) return e;
+  JoinArgs g{p.own, p.cpre, p.fown, p.fpre, p.pre, 1, p.merge_few, own.o, own.ml, pre.o, pre.ml};
+  // Heads a workgroup: one, until there are far more rows than fit the device at once.
+  const int64_t toks = p.merge_few ? (int64_t)a.c.n_seq * p.merge_few : a.c.n_tok;
+  g.per_wg = (int)std::min<int64_t>(a.c.heads, std::max<int64_t>(1, toks * a.c.heads / 8192));
+  const int64_t grid = toks * ((a.c.heads + g.per_wg - 1) / g.per_wg);
+  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)grid), dim3(kBlock), 0, s, a, g);
   return hipGetLastError();
 }
 
