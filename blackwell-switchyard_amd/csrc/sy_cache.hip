@@ -59,11 +59,12 @@ __device__ __forceinline__ int find_seq(const CacheArgs& c, int row) {
   return -1;
 }
 
-// Element offset of the row of token j in the cache (head 0), or -1 where a page id names no page.
-__device__ __forceinline__ int64_t row_offset(const CacheArgs& c, const int32_t* pages, int j) {
-  const int id = pages[j >> c.page_shift];
-  if ((unsigned)id >= (unsigned)c.n_pages) return -1;
-  return id * c.page_stride + (j & ((1 << c.page_shift) - 1)) * c.row_stride;
+// Bytes from a cache's start to the row of token j (head 0) in page `id`.
+__device__ __forceinline__ uint64_t row_at(const CacheArgs& c, int id, int j) {
+  return (uint64_t)(uint32_t)id * c.page_bytes + (uint32_t)(j & ((1 << c.page_shift) - 1)) * c.row_bytes;
+}
+template <class S> __device__ __forceinline__ S* bytes_on(S* p, uint64_t n) {
+  return reinterpret_cast<S*>(reinterpret_cast<uintptr_t>(p) + n);
 }
 
 // --------------------------------------------------------------------- append
@@ -132,15 +133,20 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
     const Seq s = seq_of(c, b);
     const int j = s.len - s.n + (tok - s.row0);  // position among the sequence's own tokens
     const int64_t at = j + a.offset;
-    int64_t dst = -1;
-    if (j >= 0 && j < c.cap && at < a.n_pos) dst = row_offset(c, c.table + b * c.table_stride, j);
+    uint64_t dst = 0;
+    bool placed = j >= 0 && j < c.cap && at < a.n_pos;
+    if (placed) {
+      const int id = c.table[b * c.table_stride + (j >> c.page_shift)];
+      placed = (unsigned)id < (unsigned)c.n_pages;
+      if (placed) dst = row_at(c, id, j);
+    }
     for (int i = threadIdx.x; i < items; i += kBlock) {
       const int head = i / per_head;
       const int ch = (i - head * per_head) * VE;
       const S* const src = row + head * a.head_stride + ch;
       Chunk<T, VE> lo = ld_chunk<T, VE>(src);
       Chunk<T, VE> hi = ld_chunk<T, VE>(src + half);
-      if (head < c.heads + c.kv_heads && dst >= 0) {
+      if (head < c.heads + c.kv_heads && placed) {
         const float* const cp = a.cosv + at * half + ch;
         const float* const sp = a.sinv + at * half + ch;
 #pragma unroll
@@ -152,16 +158,16 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
       }
       S* out;
       if (head < c.heads) {
-        if (dst < 0) {
+        if (!placed) {
 #pragma unroll
           for (int e = 0; e < VE; ++e) lo.f[e] = hi.f[e] = __int_as_float(0x7fc00000);
         }
         out = q + ((int64_t)tok * c.heads + head) * c.hd + ch;
       } else {
-        if (dst < 0) continue;
+        if (!placed) continue;
         const bool key = head < c.heads + c.kv_heads;
         const int h = head - c.heads - (key ? 0 : c.kv_heads);
-        out = static_cast<S*>(key ? c.k : c.v) + dst + h * c.head_stride + ch;
+        out = bytes_on(static_cast<S*>(key ? c.k : c.v) + h * c.head_stride + ch, dst);
       }
       st_chunk<T, VE>(out, lo);
       st_chunk<T, VE>(out + half, hi);
@@ -302,6 +308,38 @@ template <class F> __device__ __forceinline__ bool locate(int n_seq, int unit, F
 }
 // Units a worker takes (the host sees to it that all numbers of units fit 31 bits).
 __device__ __forceinline__ int share_of(const Cut& u, int units) { return max((units + u.workers - 1) / u.workers, u.least); }
+// The unit-th of all units in the order of their distance from their sequence's last one
+// (the last units of all sequences, then those before them, ...): that sequence and the
+// unit's number in it. With `most` the largest number of units a sequence can have.
+template <class F> __device__ __forceinline__ bool locate_last(int n_seq, int unit, int most, F count, int* seq, int* number) {
+  const int lane = threadIdx.x & 63;
+  const auto nearer = [&](int k) {  // units at most k - 1 before their sequence's last
+    int x = 0;
+    for (int b = lane; b < n_seq; b += 64) x += min(count(b), k);
+    return __builtin_amdgcn_readlane(scan_add(x), 63);
+  };
+  if (unit >= nearer(most)) return false;
+  int lo = 0, hi = most - 1;  // the distance: the largest k with nearer(k) <= unit
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (nearer(mid) <= unit) lo = mid;
+    else hi = mid - 1;
+  }
+  int skip = unit - nearer(lo);  // sequences of more than `lo` units to pass over
+  for (int b0 = 0; b0 < n_seq; b0 += 64) {
+    const int n = b0 + lane < n_seq ? count(b0 + lane) : 0;
+    const int incl = scan_add(n > lo ? 1 : 0);
+    const uint64_t hit = __ballot(incl > skip);
+    if (hit != 0) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      *seq = b0 + l;
+      *number = __builtin_amdgcn_readlane(n, l) - 1 - lo;
+      return true;
+    }
+    skip -= __builtin_amdgcn_readlane(incl, 63);
+  }
+  return false;
+}
 __device__ __forceinline__ int units_of(const CacheArgs& c, const Cut& u, int prefix_len, int b) {
   const Tiles t = tiles_of(u, c.group, pass_seq(c, u.pre, prefix_len, b));
   return t.row_tiles * t.key_tiles;
@@ -444,7 +482,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
       int id[MT];
       bool ok[MT], okn[MT];
       i32x4_t kx[MT][KC], vx[MT][KC];
-      int64_t off[MT];
+      uint64_t off[MT];
       // Ids are read whether or not a token is there (within the row): the first ones do
       // not wait for the sequence's length.
       const int last_page = u.pre ? (plen - 1) >> c.page_shift : (int)(c.cap >> c.page_shift) - 1;
@@ -457,7 +495,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
         for (int x = 0; x < MT; ++x) {
           const int j = t * KT + x * 16 + col;
           okn[x] = (unsigned)id[x] < (unsigned)c.n_pages && j < most;
-          off[x] = okn[x] ? id[x] * c.page_stride + (j & ((1 << c.page_shift) - 1)) * c.row_stride : 0;
+          off[x] = okn[x] ? row_at(c, id[x], j) : 0;
         }
       };
       const auto ask = [&](const S* base_p, i32x4_t (&dst)[MT][KC]) {
@@ -466,7 +504,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
 #pragma unroll
           for (int k = 0; k < KC; ++k) {
             const int ch = (k * 4 + grp) * CE;
-            dst[x][k] = *reinterpret_cast<const i32x4_t*>(base_p + off[x] + (EXACT || ch < hd ? ch : 0));
+            dst[x][k] = *reinterpret_cast<const i32x4_t*>(bytes_on(base_p, off[x]) + (EXACT || ch < hd ? ch : 0));
           }
       };
       ask_ids(tile + wave);
@@ -699,8 +737,8 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
 //
 // The same pass where a sequence brings more rows than a tile of 16: a workgroup takes 128
 // query rows of a kv head, a wave 32 of them, and all four waves read the same tiles of 64
-// keys and values from LDS, double-buffered: tile t + 1 goes from registers to LDS and
-// tile t + 2 from memory to registers while tile t is multiplied, one barrier a tile. The
+// keys and values from LDS. Tile t + 1 is on its way from memory to the other half of LDS
+// while tile t is multiplied, without passing through registers; one barrier a tile. The
 // products run on v_mfma_f32_32x32x16 in the same transposed form; 32 rows a wave take
 // 32 KB of LDS reads for 2^20 products a tile, which LDS delivers in half the time of the
 // products. The maximum is only followed when a score passes it by more than 2^8 (weights
@@ -740,19 +778,33 @@ template <class T> __device__ __forceinline__ f32x16_t mma32(const i32x4_t& a, c
                                                   0, 0);
 }
 
+// 16 bytes a lane from memory to LDS, lane i's at byte `at` + 16 i of the workgroup's LDS;
+// done when vmcnt says so. (The builtin's loads are waited for before the next read of any
+// LDS, the other buffer included. There is no output register that could be reused while
+// the load is under way. The compiler does not count these loads: a wait of its own for an
+// earlier load would wait for them too, so there must be none behind them.)
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_byte(void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p;
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <class T, int HD, bool EXACT>
 __global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
 k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, float* const row_o, float* const row_ml) {
   using S = typename T::storage;
   constexpr int KT = kFlashKeys;
-  constexpr int CPR = HD / 8;          // 16-byte chunks of a row
-  constexpr int RP = kBlock / CPR;     // rows the workgroup loads at a time
-  constexpr int NP = KT / RP;
-  constexpr int KS = HD * 2 + 16, VS = HD * 2 + 32;  // strides that spread rows over the banks
+  constexpr int CPR = HD / 8;      // 16-byte chunks of a row
+  constexpr int RB = HD * 2;       // bytes of a row in LDS, without padding: chunks are swizzled instead
+  constexpr int RPI = 64 / CPR;    // rows a wave loads at a time
+  constexpr int NP = KT / (RPI * kWaves);
   constexpr int KC = HD / 16, MD = HD / 32;
-  __shared__ __align__(16) char kl[2][KT * KS];
-  __shared__ __align__(16) char vl[2][KT * VS];
-  __shared__ int flags[2][KT];  // 1: the key is there, 2: its value holds an infinity or NaN
+  __shared__ __align__(16) char kl[2][KT * RB];
+  __shared__ __align__(16) char vl[2][KT * RB];
+  __shared__ __align__(16) int whole[2][kWaves];  // all keys of a wave's rows are there
+  __shared__ int flags[KT];  // of a tile's keys: 1 it is there, 2 its value holds an infinity or NaN
   const CacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int col = lane & 31, half = lane >> 5;
@@ -763,12 +815,11 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
   const int h = blockIdx.x % c.kv_heads;
   const int rest = blockIdx.x / c.kv_heads;
   const int split = rest % f.splits, tile_id = rest / f.splits;
-  int b, base;
-  if (!locate(f.pre ? 1 : c.n_seq, tile_id, [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &base)) return;
+  int b, rtile;
+  if (!locate_last(f.pre ? 1 : c.n_seq, tile_id, f.tiles, [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &rtile))
+    return;
   const Seq s = pass_seq(c, f.pre, plen, b);
   const int rows = s.n * c.group;
-  // A sequence's last row tile, which sees the most keys, is first in the grid.
-  const int rtile = (rows + kFlashRows - 1) / kFlashRows - 1 - (tile_id - base);
   const int r0 = rtile * kFlashRows;
   const int last = min(r0 + kFlashRows, rows) - 1;
   const int past = f.pre ? plen : s.len - s.n + 1;  // keys the first token sees
@@ -808,56 +859,62 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
       for (int e = 0; e < 4; ++e) q[k][e] ^= (int)0x80008000;
   }
 
-  // Loading: a thread's rows lr, lr + RP, ... and chunk lc of each.
-  const int lr = tid / CPR, lc = tid % CPR;
-  const bool lc_in = EXACT || lc * 8 < hd;
-  const S* const kb = static_cast<const S*>(c.k) + h * c.head_stride + (lc_in ? lc * 8 : 0);
-  const S* const vb = static_cast<const S*>(c.v) + h * c.head_stride + (lc_in ? lc * 8 : 0);
+  // Loading: a wave's rows of load p are (4 p + wave) RPI + lane / CPR, a lane's place in a
+  // row lane % CPR. Chunk ch of row r lies at place ch ^ key_swizzle(r) (keys: 16 rows of
+  // one chunk then lie in 16 different groups of banks) or ch ^ value_swizzle(r) (values: 4
+  // rows of one 64-byte group in 4 different ones).
+  const auto key_swizzle = [](int r) { return HD == 64 ? (r >> 1) & 7 : r & 15; };
+  const auto value_swizzle = [](int r) { return (HD == 64 ? (r >> 1) & 1 : r & 3) << 2; };
+  const S* const kb = static_cast<const S*>(c.k) + h * c.head_stride;
+  const S* const vb = static_cast<const S*>(c.v) + h * c.head_stride;
   const int32_t* const own_pages = f.pre ? a.prefix_pages : c.table + b * c.table_stride;
   const int own_last = f.pre ? (plen - 1) >> c.page_shift : (int)(c.cap >> c.page_shift) - 1;
   const int wg_least = f.pre ? plen : past + r0 / c.group;
+  const uint32_t kl_at = lds_byte(&kl[0][0]), vl_at = lds_byte(&vl[0][0]);
   int id[NP];
-  i32x4_t kx[NP], vx[NP];
-  bool ok[NP];
   const auto ask_ids = [&](int t) {
     const bool own = t >= pre_tiles;
     const int32_t* const pages = own ? own_pages : a.prefix_pages;
     const int end = own ? own_last : (plen - 1) >> c.page_shift;
-    const int j0 = (own ? t - pre_tiles : t) * KT + lr;
+    const int j0 = (own ? t - pre_tiles : t) * KT + wave * RPI + lane / CPR;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) id[p] = pages[min((j0 + p * RP) >> c.page_shift, end)];
+    for (int p = 0; p < NP; ++p) id[p] = pages[min((j0 + p * kWaves * RPI) >> c.page_shift, end)];
   };
   const auto ask = [&](int t) {  // keys with no place read the cache's first row
-    const bool own = t >= pre_tiles;
-    const int j0 = (own ? t - pre_tiles : t) * KT + lr;
-    const int end = own ? most : plen;
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int j = j0 + p * RP;
-      ok[p] = (unsigned)id[p] < (unsigned)c.n_pages && j < end;
-      const int64_t off =
-          ok[p] ? id[p] * c.page_stride + (j & ((1 << c.page_shift) - 1)) * c.row_stride : 0;
-      kx[p] = *reinterpret_cast<const i32x4_t*>(kb + off);
-      vx[p] = *reinterpret_cast<const i32x4_t*>(vb + off);
-    }
-  };
-  const auto put = [&](int t) {
     const int buf = (t - t0) & 1;
-    const bool edge = t >= pre_tiles && (t - pre_tiles + 1) * KT > wg_least;
+    const bool own = t >= pre_tiles;
+    const int j0 = (own ? t - pre_tiles : t) * KT;
+    const int end = own ? most : plen;
+    bool all = true;
+    uint64_t off[NP];
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const int row = lr + p * RP;
-      i32x4_t x = vx[p], y = kx[p];
-      if (!ok[p]) x = i32x4_t{0, 0, 0, 0};
-      if (!EXACT && !lc_in) y = i32x4_t{0, 0, 0, 0};
-      *reinterpret_cast<i32x4_t*>(kl[buf] + row * KS + lc * 16) = y;
-      *reinterpret_cast<i32x4_t*>(vl[buf] + row * VS + lc * 16) = x;
-      uint64_t odd = 0;
-      if (edge) odd = __ballot(nonfinite<T>(x)) >> (lane - lc);
-      if (lc == 0) flags[buf][row] = (ok[p] ? 1 : 0) | ((odd & ((1ull << CPR) - 1)) != 0 ? 2 : 0);
+      asm volatile("" : "+v"(id[p]));  // its wait is here, before the first load to LDS
+      const int j = j0 + (p * kWaves + wave) * RPI + lane / CPR;
+      const bool ok = (unsigned)id[p] < (unsigned)c.n_pages && j < end;
+      all = all && ok;
+      off[p] = row_at(c, ok ? id[p] : 0, ok ? j : 0);
     }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int first = (p * kWaves + wave) * RPI, row = first + lane / CPR;
+      const int kc = (lane % CPR ^ key_swizzle(row)) * 8, vc = (lane % CPR ^ value_swizzle(row)) * 8;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(buf * (KT * RB) + first * RB);
+      load_to_lds(bytes_on(kb + (EXACT || kc < hd ? kc : 0), off[p]), kl_at + to);
+      load_to_lds(bytes_on(vb + (EXACT || vc < hd ? vc : 0), off[p]), vl_at + to);
+    }
+    all = __all(all);
+    if (lane == 0) whole[buf][wave] = all;
   };
+  // Where a lane reads: keys of row `col`, chunk 2 k + half, at key_at ^ 32 k; values of row
+  // 4 half + (lane & 15) / 4, output tile d, at value_at ^ 64 d.
+  const int key_at = col * RB + ((half ^ key_swizzle(col)) << 4);
+  const int vrow = 4 * half + ((lane & 15) >> 2);
+  const int value_at =
+      vrow * RB + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ value_swizzle(vrow)) << 4) + (lane & 1) * 8;
 
+  constexpr int kOnes = T::code == SY_BF16 ? 0x3f803f80 : 0x3c003c00;
+  const i32x4_t ones = {kOnes, kOnes, kOnes, kOnes};
   float m = -INFINITY, l = 0.0f;
   f32x16_t o[MD];
 #pragma unroll
@@ -866,44 +923,57 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
   if (t0 < t1) {
     ask_ids(t0);
     ask(t0);
-    if (t0 + 1 < t1) ask_ids(t0 + 1);
-    put(t0);
-    if (t0 + 1 < t1) {
-      ask(t0 + 1);
-      if (t0 + 2 < t1) ask_ids(t0 + 2);
-    }
-    __syncthreads();
+    ask_ids(min(t0 + 1, t1 - 1));
   }
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
     const bool own = t >= pre_tiles;
     const int j0 = (own ? t - pre_tiles : t) * KT;
-    const bool work = active && (!own || j0 < wmost);
-    f32x16_t st[2];
-    if (work) {
+    wait_loads();  // tile t, which was asked for a whole tile ago
+    __syncthreads();
+    if (t + 1 < t1) {
+      ask(t + 1);  // into the buffer that was read before the barrier
+      ask_ids(min(t + 2, t1 - 1));
+    }
+    uint64_t there = ~0ull, odd = 0;
+    const i32x4_t w4 = *reinterpret_cast<const i32x4_t*>(whole[buf]);
+    if ((w4[0] & w4[1] & w4[2] & w4[3]) == 0 || (own && j0 + KT > wg_least)) {
+      // Values of keys that are not there become zero; those that some rows must not see
+      // are looked through for infinities and NaN. Four threads a row.
+      const int row = tid / 4, j = j0 + row;
+      const int32_t* const pages = own ? own_pages : a.prefix_pages;
+      const int page = pages[min(j >> c.page_shift, own ? own_last : (plen - 1) >> c.page_shift)];
+      const bool ok = (unsigned)page < (unsigned)c.n_pages && j < (own ? most : plen);
+      bool bad = false;
+#pragma unroll
+      for (int x = 0; x < CPR / 4; ++x) {
+        i32x4_t* const at = reinterpret_cast<i32x4_t*>(vl[buf] + row * RB + (tid % 4 * (CPR / 4) + x) * 16);
+        if (ok) bad = bad || nonfinite<T>(*at);
+        else *at = i32x4_t{0, 0, 0, 0};
+      }
+      const uint64_t any = __ballot(bad);
+      if (tid % 4 == 0) flags[row] = (ok ? 1 : 0) | ((any >> lane & 15) != 0 ? 2 : 0);
+      __syncthreads();
+      const int flag = flags[lane];
+      there = __ballot(flag & 1);
+      odd = __ballot(flag & 2);
+    }
+    if (active && (!own || j0 < wmost)) {
+      f32x16_t st[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         st[x] = f32x16_t{};
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
-          const i32x4_t w = *reinterpret_cast<const i32x4_t*>(kl[buf] + (x * 32 + col) * KS + (2 * k + half) * 16);
+          if (!EXACT && k * 16 >= hd) continue;
+          i32x4_t w = *reinterpret_cast<const i32x4_t*>(kl[buf] + x * 32 * RB + (key_at ^ (k * 32)));
+          if (!EXACT && (2 * k + half) * 8 >= hd) w = i32x4_t{0, 0, 0, 0};
           st[x] = mma32<T>(w, q[k], st[x]);
         }
       }
-    }
-    if (t + 1 < t1) {
-      put(t + 1);
-      if (t + 2 < t1) {
-        ask(t + 2);
-        if (t + 3 < t1) ask_ids(t + 3);
-      }
-    }
-    if (work) {
-      const int flag = flags[buf][lane];
-      const uint64_t there = __ballot(flag & 1);
-      const uint64_t odd = __ballot(flag & 2);
       const bool full = ~there == 0 && (!own || j0 + KT <= least);
-      if (!full) {
+      if (__builtin_expect(!full, 0)) {
+        asm volatile("" ::: "memory");  // a branch: selects would cost every tile
         const int lim = own ? limit - j0 : KT;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -939,13 +1009,12 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
       for (int k = 0; k < 4; ++k) {
         float pf[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          pf[e] = __builtin_amdgcn_exp2f(fmaf(st[k / 2][(k % 2) * 8 + e], sl, -mu));
-          sum += pf[e];
-        }
+        for (int e = 0; e < 8; ++e) pf[e] = __builtin_amdgcn_exp2f(fmaf(st[k / 2][(k % 2) * 8 + e], sl, -mu));
         // Weights are rounded to the values' dtype for the product (at most half a step,
-        // independent of one another); their sum is of the unrounded ones.
+        // independent of one another), and their sum is of the rounded ones: two a
+        // v_dot2, half the additions.
         p16[k] = pack<T>(pf);
+        sum = dot<T>(p16[k], ones, sum);
       }
       l += sum;
       if (__builtin_expect(odd == 0 || full, 1)) {
@@ -957,8 +1026,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
             i32x4_t w;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const char* const from = vl[buf] + (16 * k + 8 * x + 4 * half + ((lane & 15) >> 2)) * VS + d * 64 +
-                                       ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+              char* const from = vl[buf] + (16 * k + 8 * x) * RB + (value_at ^ (d * 64));
               const i16x4_t v4 =
                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)from);
               const i32x2_t v2 = __builtin_bit_cast(i32x2_t, v4);
@@ -985,14 +1053,13 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               i32x4_t v4 = {0, 0, 0, 0};
-              __builtin_memcpy(&v4, vl[buf] + j * VS + d * 64 + (8 * x + 4 * half) * 2, 8);
+              __builtin_memcpy(&v4, vl[buf] + j * RB + ((d * 4 + x) ^ value_swizzle(j)) * 16 + half * 8, 8);
 #pragma unroll
               for (int i = 0; i < 4; ++i) o[d][4 * x + i] = fmaf(pv, elem<T>(v4, i), o[d][4 * x + i]);
             }
         }
       }
     }
-    __syncthreads();
   }
 
   {
@@ -1000,6 +1067,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
     const auto sw = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
+  const int base = f.splits == 1 || f.pre ? 0 : total_of(b, [&](int x) { return flash_tiles(c, f, plen, x); });
   if (w0 + col > last) return;
   if (direct) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1018,9 +1086,9 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
       }
     return;
   }
-  const bool whole = f.splits == 1;
-  const int64_t slot = whole ? out_row : flash_slot(c, f, base + rtile, h, split) + (w0 - r0) + col;
-  float* const po = (whole ? row_o : f.o) + slot * hd;
+  const bool uncut = f.splits == 1;
+  const int64_t slot = uncut ? out_row : flash_slot(c, f, base + rtile, h, split) + (w0 - r0) + col;
+  float* const po = (uncut ? row_o : f.o) + slot * hd;
 #pragma unroll
   for (int d = 0; d < MD; ++d)
 #pragma unroll
@@ -1031,7 +1099,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
             f32x4_t{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
     }
   if (half == 0) {
-    float* const pm = (whole ? row_ml : f.ml) + slot * 2;
+    float* const pm = (uncut ? row_ml : f.ml) + slot * 2;
     pm[0] = m;
     pm[1] = l;
   }
@@ -1251,8 +1319,9 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int few, int nt, 
   return true;
 }
 
-// Parts of a row tile's keys: as many as let the workgroups fill the device's places in
-// whole rounds, where the grid alone would not; at least four tiles each.
+// Parts of a row tile's keys: the number that promises the shortest time, as the rounds of
+// the grid over the device's places, each a part of the keys long, and the writing, reading
+// and joining of the partial results.
 bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int few, int cus, Flash* f) {
   f->pre = pre;
   f->virt = virt;
@@ -1265,13 +1334,15 @@ bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int 
   const int64_t places = (int64_t)cus * (c.hd <= 128 ? 2 : 1);
   const int64_t grid = (int64_t)f->tiles * c.kv_heads;
   const int64_t keys = (pre ? prefix_len : c.cap + (virt ? prefix_len : 0));
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, keys / (4 * kFlashKeys)));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, keys / (2 * kFlashKeys)));
+  const double tile_us = c.hd <= 64 ? 0.8 : c.hd <= 128 ? 1.3 : 2.6;  // of a full device
+  const double row_us = (double)rows * c.kv_heads * c.hd * 8 / 4e6;   // fp32 results out and in again at 4 TB/s
   f->splits = 1;
-  double best = 1e30;
-  for (int n = 1; n <= most && grid < 4 * places; ++n) {
-    // Rounds of the grid over the device, each 1/n of the keys, and a part's own cost.
-    const double cost = (double)((grid * n + places - 1) / places) / n + 0.02 * n;
-    if (cost < best - 1e-9) {
+  double best = 0.0;
+  for (int n = 1; n <= most; ++n) {
+    const double cost = (double)((grid * n + places - 1) / places) / n * keys / kFlashKeys * tile_us +
+                        (n > 1 ? 6.0 + n * row_us : 0.0);
+    if (n == 1 || cost < best) {
       best = cost;
       f->splits = n;
     }

@@ -1091,14 +1091,16 @@ static int cache_args(const sy_paged* c, CacheArgs* out) {
   if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0 || c->table_stride < 0) return SY_ERR_STRIDE;
   if (c->page_stride % chunk != 0 || c->head_stride % chunk != 0 || c->row_stride % chunk != 0)
     return SY_ERR_STRIDE;
+  const int64_t span = ((int64_t)1 << 32) / esize(c->dtype);  // of a page, and between pages
+  if (c->page_stride >= span || c->row_stride >= span / c->page) return SY_ERR_STRIDE;
   if (c->n_tok == 0) return SY_OK;
   if (c->table_cols < 1) return SY_ERR_SHAPE;
   if (!c->k || !c->v || !c->lengths || !c->table) return SY_ERR_NULL;
   if (!al16(c->k) || !al16(c->v)) return SY_ERR_SHAPE;
   int shift = 0;
   while ((1 << shift) < c->page) ++shift;
-  *out = CacheArgs{c->k, c->v, c->table, c->lengths, c->starts, c->page_stride, c->head_stride, c->row_stride,
-                   c->table_stride, (int)c->n_seq, (int)c->n_tok, (int)(c->n_tok / c->n_seq), (int)c->n_pages,
+  *out = CacheArgs{c->k, c->v, c->table, c->lengths, c->starts, c->head_stride, c->table_stride,
+                   (uint32_t)(c->page_stride * esize(c->dtype)), (uint32_t)(c->row_stride * esize(c->dtype)), (int)c->n_seq, (int)c->n_tok, (int)(c->n_tok / c->n_seq), (int)c->n_pages,
                    shift, c->heads, c->kv_heads, c->heads / c->kv_heads, c->hd, c->table_cols << shift};
   return SY_OK;
 }

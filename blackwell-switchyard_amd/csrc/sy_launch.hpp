@@ -433,7 +433,8 @@ struct CacheArgs {
   const int32_t* table;
   const int32_t* lengths;
   const int32_t* starts;  // nullptr: `each` rows a sequence
-  int64_t page_stride, head_stride, row_stride, table_stride;  // elements
+  int64_t head_stride, table_stride;  // elements
+  uint32_t page_bytes, row_bytes;     // between pages, and rows of a page
   int n_seq, n_tok, each, n_pages, page_shift, heads, kv_heads, group, hd;
   int64_t cap;  // tokens a row of the table can hold
 };

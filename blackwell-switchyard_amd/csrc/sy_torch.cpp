@@ -604,6 +604,8 @@ bool paged_of(const Tensor& like, int64_t heads, const Tensor& k, const Tensor& 
     return false;
   for (int d = 0; d < 3; ++d)
     if (k.stride(d) < 0 || k.stride(d) % chunk_of != 0) return false;
+  const int64_t span = ((int64_t)1 << 32) / (int64_t)k.element_size();
+  if (k.stride(0) >= span || k.stride(2) >= span / page) return false;
   const int64_t n_seq = lengths.size(0), n_tok = like.size(0);
   if (starts.has_value()) {
     if (!whole(*starts) || starts->dim() != 1 || starts->size(0) != n_seq + 1 || !starts->is_contiguous() ||

@@ -72,6 +72,8 @@ def _validate_cache(rows, heads: int, what: str, k, v, page_table, lengths, star
     _need(k.stride(3) == 1 and all(s >= 0 and s % chunk == 0 for s in k.stride()[:3])
           and k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0,
           "the caches' rows must be dense and start at 16-byte boundaries")
+    span = 2**32 // k.element_size()
+    _need(k.stride(0) < span and k.stride(2) * page < span, "a page must span less than 4 GiB, and so pages apart")
     _need(0 <= prefix_len <= 0x7FFFFFFF, "prefix_len must not be negative")
     _need(rows.is_cuda, f"{what} must be on a CUDA device")
     return _lib.Paged(k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),

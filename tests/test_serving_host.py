@@ -30,7 +30,7 @@ BAD = [
     (dict(kv_heads=0), SHAPE), (dict(heads=0), SHAPE), (dict(heads=1 << 16), SHAPE), (dict(hd=0), SHAPE),
     (dict(hd=60), SHAPE), (dict(hd=264), SHAPE), (dict(n_tok=1 << 31, starts=FAKE), SHAPE), (dict(k=None), NULL),
     (dict(v=None), NULL), (dict(table=None), NULL), (dict(lengths=None), NULL), (dict(k=FAKE + 8), SHAPE),
-    (dict(page_stride=-16), STRIDE), (dict(row_stride=65), STRIDE), (dict(head_stride=12), STRIDE),
+    (dict(page_stride=-16), STRIDE), (dict(row_stride=65), STRIDE), (dict(head_stride=12), STRIDE), (dict(page_stride=1 << 31), STRIDE), (dict(row_stride=1 << 27), STRIDE),
 ]
 
 
