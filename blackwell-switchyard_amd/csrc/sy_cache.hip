@@ -913,6 +913,9 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
   const int value_at =
       vrow * RB + (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ value_swizzle(vrow)) << 4) + (lane & 1) * 8;
 
+  // The queries' waits are here: inside the loop they would wait for its loads.
+#pragma unroll
+  for (int k = 0; k < KC; ++k) asm volatile("" : "+v"(q[k]));
   constexpr int kOnes = T::code == SY_BF16 ? 0x3f803f80 : 0x3c003c00;
   const i32x4_t ones = {kOnes, kOnes, kOnes, kOnes};
   float m = -INFINITY, l = 0.0f;
@@ -938,34 +941,35 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
     uint64_t there = ~0ull, odd = 0;
     const i32x4_t w4 = *reinterpret_cast<const i32x4_t*>(whole[buf]);
     if ((w4[0] & w4[1] & w4[2] & w4[3]) == 0 || (own && j0 + KT > wg_least)) {
-      // Values of keys that are not there become zero; those that some rows must not see
-      // are looked through for infinities and NaN. Four threads a row.
+      // Values of keys that are not there become zero, and so do those that some rows must
+      // not see and that hold an infinity or NaN (0 times one is none): the rows that see
+      // them add them on their own. Four threads a row.
       const int row = tid / 4, j = j0 + row;
       const int32_t* const pages = own ? own_pages : a.prefix_pages;
       const int page = pages[min(j >> c.page_shift, own ? own_last : (plen - 1) >> c.page_shift)];
       const bool ok = (unsigned)page < (unsigned)c.n_pages && j < (own ? most : plen);
+      i32x4_t* const at = reinterpret_cast<i32x4_t*>(vl[buf] + row * RB + tid % 4 * (RB / 4));
       bool bad = false;
 #pragma unroll
-      for (int x = 0; x < CPR / 4; ++x) {
-        i32x4_t* const at = reinterpret_cast<i32x4_t*>(vl[buf] + row * RB + (tid % 4 * (CPR / 4) + x) * 16);
-        if (ok) bad = bad || nonfinite<T>(*at);
-        else *at = i32x4_t{0, 0, 0, 0};
+      for (int x = 0; x < CPR / 4; ++x) bad = bad || nonfinite<T>(at[x]);
+      bad = (__ballot(bad) >> (lane & ~3) & 15) != 0;
+      if (bad || !ok) {
+#pragma unroll
+        for (int x = 0; x < CPR / 4; ++x) at[x] = i32x4_t{0, 0, 0, 0};
       }
-      const uint64_t any = __ballot(bad);
-      if (tid % 4 == 0) flags[row] = (ok ? 1 : 0) | ((any >> lane & 15) != 0 ? 2 : 0);
+      if (tid % 4 == 0) flags[row] = (ok ? 1 : 0) | (ok && bad ? 2 : 0);
       __syncthreads();
       const int flag = flags[lane];
       there = __ballot(flag & 1);
       odd = __ballot(flag & 2);
     }
     if (active && (!own || j0 < wmost)) {
-      f32x16_t st[2];
+      f32x16_t st[2] = {f32x16_t{}, f32x16_t{}};
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        st[x] = f32x16_t{};
+      for (int k = 0; k < KC; ++k) {
+        if (!EXACT && k * 16 >= hd) continue;
 #pragma unroll
-        for (int k = 0; k < KC; ++k) {
-          if (!EXACT && k * 16 >= hd) continue;
+        for (int x = 0; x < 2; ++x) {
           i32x4_t w = *reinterpret_cast<const i32x4_t*>(kl[buf] + x * 32 * RB + (key_at ^ (k * 32)));
           if (!EXACT && (2 * k + half) * 8 >= hd) w = i32x4_t{0, 0, 0, 0};
           st[x] = mma32<T>(w, q[k], st[x]);
@@ -1017,29 +1021,11 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
         sum = dot<T>(p16[k], ones, sum);
       }
       l += sum;
-      if (__builtin_expect(odd == 0 || full, 1)) {
-#pragma unroll
-        for (int d = 0; d < MD; ++d) {
-          if (!EXACT && d * 32 >= hd) continue;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            i32x4_t w;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              char* const from = vl[buf] + (16 * k + 8 * x) * RB + (value_at ^ (d * 64));
-              const i16x4_t v4 =
-                  __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)from);
-              const i32x2_t v2 = __builtin_bit_cast(i32x2_t, v4);
-              w[2 * x] = v2[0];
-              w[2 * x + 1] = v2[1];
-            }
-            o[d] = mma32<T>(w, p16[k], o[d]);
-          }
-        }
-      } else {
-        // Rows that do not see a token leave its value out: 0 times an infinity is none.
+      if (__builtin_expect(odd != 0, 0)) {
+        asm volatile("" ::: "memory");
 #pragma unroll 1
         for (int j = 0; j < KT; ++j) {
+          if ((odd >> j & 1) == 0) continue;
           const int e = 8 * (j >> 4) + 4 * ((j >> 3) & 1) + (j & 3);  // of the 32 weights of a lane
           int word = p16[0][0];
 #pragma unroll
@@ -1047,18 +1033,39 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
           word = __shfl(word, col + 32 * ((j >> 2) & 1));
           const i32x4_t w4 = {word, 0, 0, 0};
           const float pv = (e & 1) ? elem<T>(w4, 1) : elem<T>(w4, 0);
-          if (j0 + j >= limit) continue;
+          const int id = (own ? own_pages : a.prefix_pages)[(j0 + j) >> c.page_shift];
+          const S* const vr = bytes_on(vb, row_at(c, id, j0 + j));
+          if (own && j0 + j >= limit) continue;
 #pragma unroll
           for (int d = 0; d < MD; ++d)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
+              const int ch = d * 32 + 8 * x + 4 * half;
+              if (!EXACT && ch >= hd) continue;
               i32x4_t v4 = {0, 0, 0, 0};
-              __builtin_memcpy(&v4, vl[buf] + j * RB + ((d * 4 + x) ^ value_swizzle(j)) * 16 + half * 8, 8);
+              __builtin_memcpy(&v4, vr + ch, 8);
 #pragma unroll
               for (int i = 0; i < 4; ++i) o[d][4 * x + i] = fmaf(pv, elem<T>(v4, i), o[d][4 * x + i]);
             }
         }
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int d = 0; d < MD; ++d) {
+          if (!EXACT && d * 32 >= hd) continue;
+          i32x4_t w;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            char* const from = vl[buf] + (16 * k + 8 * x) * RB + (value_at ^ (d * 64));
+            const i16x4_t v4 =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)from);
+            const i32x2_t v2 = __builtin_bit_cast(i32x2_t, v4);
+            w[2 * x] = v2[0];
+            w[2 * x + 1] = v2[1];
+          }
+          o[d] = mma32<T>(w, p16[k], o[d]);
+        }
     }
   }
 
