@@ -310,15 +310,21 @@ template <class F> __device__ __forceinline__ bool locate(int n_seq, int unit, F
 __device__ __forceinline__ int share_of(const Cut& u, int units) { return max((units + u.workers - 1) / u.workers, u.least); }
 // The unit-th of all units in the order of their distance from their sequence's last one
 // (the last units of all sequences, then those before them, ...): that sequence and the
-// unit's number in it. With `most` the largest number of units a sequence can have.
-template <class F> __device__ __forceinline__ bool locate_last(int n_seq, int unit, int most, F count, int* seq, int* number) {
+// unit's number in it. With `most` the largest number of units a sequence can have. The
+// second `fold` units are taken in reverse: workgroups are handed out to one place of every
+// CU, then to the next, so a CU's second one is the shorter the longer its first.
+template <class F>
+__device__ __forceinline__ bool locate_last(int n_seq, int unit, int most, int fold, F count, int* seq, int* number) {
   const int lane = threadIdx.x & 63;
+  const int mine = lane < n_seq ? count(lane) : 0;  // (up to 64 sequences are asked once)
   const auto nearer = [&](int k) {  // units at most k - 1 before their sequence's last
-    int x = 0;
-    for (int b = lane; b < n_seq; b += 64) x += min(count(b), k);
+    int x = min(mine, k);
+    for (int b = lane + 64; b < n_seq; b += 64) x += min(count(b), k);
     return __builtin_amdgcn_readlane(scan_add(x), 63);
   };
-  if (unit >= nearer(most)) return false;
+  const int total = nearer(most);
+  if (unit >= total) return false;
+  if (unit >= fold && unit < 2 * fold) unit = min(2 * fold, total) - 1 - (unit - fold);
   int lo = 0, hi = most - 1;  // the distance: the largest k with nearer(k) <= unit
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
@@ -327,7 +333,7 @@ template <class F> __device__ __forceinline__ bool locate_last(int n_seq, int un
   }
   int skip = unit - nearer(lo);  // sequences of more than `lo` units to pass over
   for (int b0 = 0; b0 < n_seq; b0 += 64) {
-    const int n = b0 + lane < n_seq ? count(b0 + lane) : 0;
+    const int n = b0 == 0 ? mine : b0 + lane < n_seq ? count(b0 + lane) : 0;
     const int incl = scan_add(n > lo ? 1 : 0);
     const uint64_t hit = __ballot(incl > skip);
     if (hit != 0) {
@@ -373,9 +379,18 @@ template <class T> __device__ __forceinline__ void zero_outside(const AttendArgs
   for (int64_t i = hi * width + at; i < c.n_tok * width; i += step) out[i] = S(0);
 }
 
+// LDS of a workgroup: a piece a wave, then the statistics of a segment's results.
+template <class T, int HD> constexpr int value_stride() {
+  // A row's start moves by 32 (fp32: 16) bytes from row to row modulo all banks.
+  return HD * (int)sizeof(typename T::storage) + (T::code == SY_F32 ? 16 : 32);
+}
+template <class T, int HD> constexpr int attend_lds() {
+  return kWaves * tokens_of<T>() * value_stride<T, HD>() + kWaves * 16 * 2 * 4;
+}
+
 template <class T, int HD, int NT, bool EXACT>
-__global__ void __launch_bounds__(kBlock, NT == 1 && HD <= 128 ? 2 : 1)
-k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, float* const row_o, float* const row_ml) {
+__device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const int direct, float* const row_o,
+                                       float* const row_ml, const int worker, char* const shared) {
   using S = typename T::storage;
   constexpr int CE = T::ce;
   constexpr int KT = tokens_of<T>();
@@ -383,18 +398,15 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
   constexpr int KC = HD / (4 * CE);  // chunks a lane holds of a row
   constexpr int MD = HD / 16;        // output tiles
   constexpr bool kF32 = T::code == SY_F32;
-  // A row's start moves by 32 (fp32: 16) bytes from row to row modulo all banks.
-  constexpr int LS = HD * (int)sizeof(S) + (kF32 ? 16 : 32);
+  constexpr int LS = value_stride<T, HD>();
   constexpr int OS = HD * 4 + 16;  // stride of a row of results in the same space
   static_assert(16 * OS <= KT * LS, "results fit the values' space");
-  __shared__ __align__(16) char lds[kWaves][KT * LS];
-  __shared__ float stats[kWaves][16][2];
+  const auto stats = reinterpret_cast<float (*)[16][2]>(shared + kWaves * KT * LS);
   const CacheArgs& c = a.c;
   const int lane = threadIdx.x & 63;
   const int col = lane & 15, grp = lane >> 4;
   const int wave = wave_id();
-  char* const vt = lds[wave];
-  const int worker = blockIdx.x;
+  char* const vt = shared + wave * (KT * LS);
   const int n_seq = u.pre ? 1 : c.n_seq;
   const int plen = (int)a.prefix_len;
   const int hd = EXACT ? HD : c.hd;
@@ -690,7 +702,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
             const float lw = stats[w][row][1];
             const float f = lw != lw ? 1.0f : __builtin_amdgcn_exp2f(stats[w][row][0] - mu);
             all = fmaf(lw, f, all);
-            x += f * *reinterpret_cast<const f32x4_t*>(lds[w] + row * OS + ch * 4);
+            x += f * *reinterpret_cast<const f32x4_t*>(shared + w * (KT * LS) + row * OS + ch * 4);
           }
           const int r = r0 + 16 * n + row;
           const int t = r / c.group;
@@ -730,6 +742,13 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
       }
     }
   }
+}
+
+template <class T, int HD, int NT, bool EXACT>
+__global__ void __launch_bounds__(kBlock, NT == 1 && HD <= 128 ? 2 : 1)
+k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, float* const row_o, float* const row_ml) {
+  __shared__ __align__(16) char shared[attend_lds<T, HD>()];
+  attend<T, HD, NT, EXACT>(a, u, direct, row_o, row_ml, blockIdx.x, shared);
   if (zero) zero_outside<T>(a);
 }
 
@@ -754,6 +773,7 @@ struct Flash {
   int few;     // sequences of at most as many rows are k_attend's
   int tiles;   // row tiles, at most
   int splits;  // parts that a row tile's keys are cut into
+  int fold;    // row tiles whose workgroups take one place on every CU
   float* o;    // partial results [tiles][kv_heads][splits][128][hd], and m, l
   float* ml;
 };
@@ -791,9 +811,13 @@ __device__ __forceinline__ uint32_t lds_byte(void* p) {
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// LDS: two tiles of keys, two of values; whether all keys of a wave's rows are there, of
+// either tile; and of an edge tile's keys, 1 it is there, 2 its value holds an infinity or NaN.
+template <int HD> constexpr int flash_lds() { return 4 * kFlashKeys * HD * 2 + 2 * kWaves * 4 + kFlashKeys * 4; }
+
 template <class T, int HD, bool EXACT>
-__global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
-k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, float* const row_o, float* const row_ml) {
+__device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const int direct, float* const row_o,
+                                      float* const row_ml, const int block, char* const shared) {
   using S = typename T::storage;
   constexpr int KT = kFlashKeys;
   constexpr int CPR = HD / 8;      // 16-byte chunks of a row
@@ -801,22 +825,21 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
   constexpr int RPI = 64 / CPR;    // rows a wave loads at a time
   constexpr int NP = KT / (RPI * kWaves);
   constexpr int KC = HD / 16, MD = HD / 32;
-  __shared__ __align__(16) char kl[2][KT * RB];
-  __shared__ __align__(16) char vl[2][KT * RB];
-  __shared__ __align__(16) int whole[2][kWaves];  // all keys of a wave's rows are there
-  __shared__ int flags[KT];  // of a tile's keys: 1 it is there, 2 its value holds an infinity or NaN
+  char* const kl = shared;
+  char* const vl = kl + 2 * KT * RB;
+  const auto whole = reinterpret_cast<int (*)[kWaves]>(vl + 2 * KT * RB);
+  int* const flags = reinterpret_cast<int*>(whole + 2);
   const CacheArgs& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int col = lane & 31, half = lane >> 5;
   const int plen = (int)a.prefix_len;
   const int hd = EXACT ? HD : c.hd;
-  if (zero) zero_outside<T>(a);
 
-  const int h = blockIdx.x % c.kv_heads;
-  const int rest = blockIdx.x / c.kv_heads;
+  const int h = block % c.kv_heads;
+  const int rest = block / c.kv_heads;
   const int split = rest % f.splits, tile_id = rest / f.splits;
   int b, rtile;
-  if (!locate_last(f.pre ? 1 : c.n_seq, tile_id, f.tiles, [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &rtile))
+  if (!locate_last(f.pre ? 1 : c.n_seq, tile_id, f.tiles, f.fold, [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &rtile))
     return;
   const Seq s = pass_seq(c, f.pre, plen, b);
   const int rows = s.n * c.group;
@@ -870,7 +893,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
   const int32_t* const own_pages = f.pre ? a.prefix_pages : c.table + b * c.table_stride;
   const int own_last = f.pre ? (plen - 1) >> c.page_shift : (int)(c.cap >> c.page_shift) - 1;
   const int wg_least = f.pre ? plen : past + r0 / c.group;
-  const uint32_t kl_at = lds_byte(&kl[0][0]), vl_at = lds_byte(&vl[0][0]);
+  const uint32_t kl_at = lds_byte(kl), vl_at = lds_byte(vl);
   int id[NP];
   const auto ask_ids = [&](int t) {
     const bool own = t >= pre_tiles;
@@ -948,7 +971,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
       const int32_t* const pages = own ? own_pages : a.prefix_pages;
       const int page = pages[min(j >> c.page_shift, own ? own_last : (plen - 1) >> c.page_shift)];
       const bool ok = (unsigned)page < (unsigned)c.n_pages && j < (own ? most : plen);
-      i32x4_t* const at = reinterpret_cast<i32x4_t*>(vl[buf] + row * RB + tid % 4 * (RB / 4));
+      i32x4_t* const at = reinterpret_cast<i32x4_t*>(vl + buf * (KT * RB) + row * RB + tid % 4 * (RB / 4));
       bool bad = false;
 #pragma unroll
       for (int x = 0; x < CPR / 4; ++x) bad = bad || nonfinite<T>(at[x]);
@@ -970,7 +993,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
         if (!EXACT && k * 16 >= hd) continue;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          i32x4_t w = *reinterpret_cast<const i32x4_t*>(kl[buf] + x * 32 * RB + (key_at ^ (k * 32)));
+          i32x4_t w = *reinterpret_cast<const i32x4_t*>(kl + buf * (KT * RB) + x * 32 * RB + (key_at ^ (k * 32)));
           if (!EXACT && (2 * k + half) * 8 >= hd) w = i32x4_t{0, 0, 0, 0};
           st[x] = mma32<T>(w, q[k], st[x]);
         }
@@ -1057,7 +1080,7 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
           i32x4_t w;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            char* const from = vl[buf] + (16 * k + 8 * x) * RB + (value_at ^ (d * 64));
+            char* const from = vl + buf * (KT * RB) + (16 * k + 8 * x) * RB + (value_at ^ (d * 64));
             const i16x4_t v4 =
                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)from);
             const i32x2_t v2 = __builtin_bit_cast(i32x2_t, v4);
@@ -1110,6 +1133,29 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
     pm[0] = m;
     pm[1] = l;
   }
+}
+
+template <class T, int HD, bool EXACT>
+__global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
+k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, float* const row_o, float* const row_ml) {
+  __shared__ __align__(16) char shared[flash_lds<HD>()];
+  flash<T, HD, EXACT>(a, f, direct, row_o, row_ml, blockIdx.x, shared);
+  if (zero) zero_outside<T>(a);
+}
+
+// Both in one launch, where a call may bring sequences of either kind: the many rows' long
+// workgroups first, the equal runs of the few rows fill up behind them.
+template <class T, int HD, bool EXACT>
+__global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
+k_both(const AttendArgs a, const Cut u, const Flash f, const int direct_u, const int direct_f, const int zero,
+       float* const row_o, float* const row_ml) {
+  __shared__ __align__(16) char shared[flash_lds<HD>() > attend_lds<T, HD>() ? flash_lds<HD>() : attend_lds<T, HD>()];
+  const int many = f.tiles * a.c.kv_heads * f.splits;
+  if ((int)blockIdx.x < many)
+    flash<T, HD, EXACT>(a, f, direct_f, row_o, row_ml, blockIdx.x, shared);
+  else
+    attend<T, HD, 1, EXACT>(a, u, direct_u, row_o, row_ml, blockIdx.x - many, shared);
+  if (zero) zero_outside<T>(a);
 }
 
 // ---------------------------------------------------------------------- merge
@@ -1168,7 +1214,7 @@ struct JoinArgs {
   Flash fown, fpre;
   int has_pre;  // 0, 1: k_attend's, 2: k_flash's
   int per_wg;   // heads a workgroup
-  int few;      // tokens a sequence to look at, where only k_attend's rows were cut; else 0
+  int few;      // tokens a sequence to look at, where only k_attend's rows are left; else 0
   float *row_o, *row_ml, *pre_o, *pre_ml;
 };
 
@@ -1277,6 +1323,47 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
   }
 }
 
+// The same for k_flash's cut rows where there is no prefix to join: a workgroup takes the 128
+// rows of a tile and kv head, hd / 4 threads one row's few results, without LDS or barriers.
+// Bound by reading the partial results once.
+template <class T>
+__global__ void __launch_bounds__(kBlock) k_merge_flash(const AttendArgs a, const Flash f) {
+  using S = typename T::storage;
+  const CacheArgs& c = a.c;
+  const int h = blockIdx.x % c.kv_heads, tile = blockIdx.x / c.kv_heads;
+  int b, base;
+  if (!locate(c.n_seq, tile, [&](int x) { return flash_tiles(c, f, 0, x); }, &b, &base)) return;
+  const Seq s = seq_of(c, b);
+  const int r0 = (tile - base) * kFlashRows;
+  const int rows = min(kFlashRows, s.n * c.group - r0);
+  const int64_t slot = flash_slot(c, f, tile, h, 0);
+  const int lpr = c.hd / 4, groups = kBlock / lpr;
+  const int grp = threadIdx.x / lpr, ch = (threadIdx.x - grp * lpr) * 4;
+  if (grp >= groups) return;
+  for (int i = grp; i < rows; i += groups) {
+    const float* const ml = f.ml + (slot + i) * 2;
+    float m = -INFINITY;
+    for (int k = 0; k < f.splits; ++k) m = fmaxf(m, ml[k * (2 * kFlashRows)]);
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f;
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k = 0; k < f.splits; ++k) {
+      const float l = ml[k * (2 * kFlashRows) + 1];
+      const float w = l != l ? 1.0f : __builtin_amdgcn_exp2f(ml[k * (2 * kFlashRows)] - mu);
+      sum = fmaf(l, w, sum);
+      o += w * *reinterpret_cast<const f32x4_t*>(f.o + (slot + i + (int64_t)k * kFlashRows) * c.hd + ch);
+    }
+    const int r = r0 + i, t = r / c.group;
+    const int64_t row = (int64_t)(s.row0 + t) * c.heads + h * c.group + (r - t * c.group);
+    float y[T::ce] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = sum == 0.0f ? 0.0f : o[e] / sum;
+    const i32x4_t x4 = pack<T>(y);
+    __builtin_memcpy(static_cast<S*>(a.out) + row * c.hd + ch, &x4, 4 * sizeof(S));
+  }
+}
+
 // ----------------------------------------------------------------------- host
 
 // Tiles a wave at most of a segment that is not cut.
@@ -1290,7 +1377,7 @@ struct Plan {
   bool attend, flash;  // the sequences' own keys
   int pre;             // a pass over the prefix: 0 none, 1 k_attend, 2 k_flash
   int direct_attend, direct_flash;
-  bool merge;
+  bool merge, merge_flash;
   int merge_few;
   Cut own, cpre;
   Flash fown, fpre;
@@ -1326,9 +1413,11 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int few, int nt, 
   return true;
 }
 
-// Parts of a row tile's keys: the number that promises the shortest time, as the rounds of
-// the grid over the device's places, each a part of the keys long, and the writing, reading
-// and joining of the partial results.
+// Parts of a row tile's keys: the number that promises the shortest time. A CU works
+// through its workgroups' tiles at a rate (measured: 1.45 us a tile of 64 keys and 128 rows
+// of 128, 0.72 of 64, 3.2 of 256), a workgroup alone no faster than 1.2 us a tile; the last
+// workgroups leave CUs idle for part of their time; cut rows are written, read and joined.
+// Prompts see half of their own tokens on average, and sequences are rarely of one length.
 bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int few, int cus, Flash* f) {
   f->pre = pre;
   f->virt = virt;
@@ -1338,22 +1427,25 @@ bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int 
   else if (c.starts == nullptr)
     f->tiles = (int)std::min<int64_t>(kMost, c.n_seq * (((int64_t)c.each * c.group + kFlashRows - 1) / kFlashRows));
   else f->tiles = (int)(rows / kFlashRows + std::min<int64_t>(c.n_seq, rows / (few + 1)));
-  const int64_t places = (int64_t)cus * (c.hd <= 128 ? 2 : 1);
   const int64_t grid = (int64_t)f->tiles * c.kv_heads;
   const int64_t keys = (pre ? prefix_len : c.cap + (virt ? prefix_len : 0));
+  const double longest = (double)keys / kFlashKeys;
+  const double mean = pre ? longest : 0.8 * std::max(longest / 2, longest - 0.5 * c.n_tok / c.n_seq / kFlashKeys);
+  const int places = c.hd <= 64 ? 3 : c.hd <= 128 ? 2 : 1;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, keys / (2 * kFlashKeys)));
-  const double tile_us = c.hd <= 64 ? 0.8 : c.hd <= 128 ? 1.3 : 2.6;  // of a full device
-  const double row_us = (double)rows * c.kv_heads * c.hd * 8 / 4e6;   // fp32 results out and in again at 4 TB/s
+  const double tile_us = c.hd <= 64 ? 0.72 : c.hd <= 128 ? 1.45 : 3.2;
+  const double row_us = (double)rows * c.kv_heads * c.hd * 8 / 4e6;  // fp32 results out and in again at 4 TB/s
   f->splits = 1;
   double best = 0.0;
   for (int n = 1; n <= most; ++n) {
-    const double cost = (double)((grid * n + places - 1) / places) / n * keys / kFlashKeys * tile_us +
-                        (n > 1 ? 6.0 + n * row_us : 0.0);
+    const double cost = std::max(grid * mean * tile_us / cus, longest / n * 1.2) +
+                        0.25 * longest / n * tile_us * places + (n > 1 ? 6.0 + n * row_us : 0.0);
     if (n == 1 || cost < best) {
       best = cost;
       f->splits = n;
     }
   }
+  f->fold = cus / (c.kv_heads * f->splits);
   return grid * f->splits <= kMost / kFlashRows;
 }
 
@@ -1391,8 +1483,9 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
   p.direct_attend = p.pre == 0;
   p.direct_flash = p.pre == 0 && p.fown.splits == 1;
   const bool cut_attend = p.attend && p.own.least != 0 && c.cap > p.own.kt;
-  p.merge = p.pre != 0 || cut_attend || (p.flash && p.fown.splits > 1);
-  p.merge_few = p.pre == 0 && !(p.flash && p.fown.splits > 1) && p.flash ? std::max(1, 16 / c.group) : 0;
+  p.merge = p.pre != 0 || cut_attend;
+  p.merge_flash = p.pre == 0 && p.flash && p.fown.splits > 1;
+  p.merge_few = p.pre == 0 && p.flash ? std::max(1, 16 / c.group) : 0;
   int64_t at = 0;
   const auto take = [&](int64_t n) {
     const int64_t was = at;
@@ -1466,6 +1559,29 @@ hipError_t flash_pass(const AttendArgs& a, const Flash& f, int direct, int zero,
   }
 }
 
+template <class T, int HD>
+hipError_t both_t(const AttendArgs& a, const Plan& p, int zero, const Rows& r, hipStream_t s) {
+  const dim3 grid((unsigned)(p.own.workers + p.fown.tiles * a.c.kv_heads * p.fown.splits));
+  if (a.c.hd == HD)
+    hipLaunchKernelGGL((k_both<T, HD, true>), grid, dim3(kBlock), 0, s, a, p.own, p.fown, p.direct_attend,
+                       p.direct_flash, zero, r.o, r.ml);
+  else
+    hipLaunchKernelGGL((k_both<T, HD, false>), grid, dim3(kBlock), 0, s, a, p.own, p.fown, p.direct_attend,
+                       p.direct_flash, zero, r.o, r.ml);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t both_pass(const AttendArgs& a, const Plan& p, int zero, const Rows& r, hipStream_t s) {
+  if constexpr (T::code == SY_F32) {
+    return hipErrorInvalidConfiguration;
+  } else {
+    if (a.c.hd <= 64) return both_t<T, 64>(a, p, zero, r, s);
+    if (a.c.hd <= 128) return both_t<T, 128>(a, p, zero, r, s);
+    return both_t<T, 256>(a, p, zero, r, s);
+  }
+}
+
 template <class T>
 hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   Plan p = plan_attend(a.c, a.prefix_len, T::code);
@@ -1485,10 +1601,16 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   else if (p.pre == 2) e = flash_pass<T>(a, p.fpre, 0, 0, pre, s);
   if (e != hipSuccess) return e;
   const int zero = a.fill && a.c.starts != nullptr;
-  if (p.flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero, own, s);
+  if (p.flash && p.attend) e = both_pass<T>(a, p, zero, own, s);
+  else if (p.flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero, own, s);
+  else e = attend_pass<T>(a, p.own, p.direct_attend, zero, own, s);
   if (e != hipSuccess) return e;
-  if (p.attend) e = attend_pass<T>(a, p.own, p.direct_attend, zero && !p.flash, own, s);
-  if (e != hipSuccess || !p.merge) return e;
+  if (p.merge_flash) {
+    hipLaunchKernelGGL((k_merge_flash<T>), dim3((unsigned)(p.fown.tiles * a.c.kv_heads)), dim3(kBlock), 0, s, a,
+                       p.fown);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  if (!p.merge) return e;
   JoinArgs g{p.own, p.cpre, p.fown, p.fpre, p.pre, 1, p.merge_few, own.o, own.ml, pre.o, pre.ml};
   // Heads a workgroup: one, until there are far more rows than fit the device at once.
   const int64_t toks = p.merge_few ? (int64_t)a.c.n_seq * p.merge_few : a.c.n_tok;
