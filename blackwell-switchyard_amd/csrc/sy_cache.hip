@@ -1143,18 +1143,24 @@ k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, flo
   if (zero) zero_outside<T>(a);
 }
 
-// Both in one launch, where a call may bring sequences of either kind: the many rows' long
-// workgroups first, the equal runs of the few rows fill up behind them.
+// Where whole results of rows go that are yet to be joined: [n_tok][heads][hd], and m, l.
+struct Rows {
+  float *o, *ml;
+};
+
+// Both in one launch, where a call may bring sequences of either kind, or the pass over a
+// shared prefix goes with that over the sequences' own keys: the many rows' long workgroups
+// first, the equal runs of the few rows fill up behind them.
 template <class T, int HD, bool EXACT>
 __global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
 k_both(const AttendArgs a, const Cut u, const Flash f, const int direct_u, const int direct_f, const int zero,
-       float* const row_o, float* const row_ml) {
+       const Rows ru, const Rows rf) {
   __shared__ __align__(16) char shared[flash_lds<HD>() > attend_lds<T, HD>() ? flash_lds<HD>() : attend_lds<T, HD>()];
   const int many = f.tiles * a.c.kv_heads * f.splits;
   if ((int)blockIdx.x < many)
-    flash<T, HD, EXACT>(a, f, direct_f, row_o, row_ml, blockIdx.x, shared);
+    flash<T, HD, EXACT>(a, f, direct_f, rf.o, rf.ml, blockIdx.x, shared);
   else
-    attend<T, HD, 1, EXACT>(a, u, direct_u, row_o, row_ml, blockIdx.x - many, shared);
+    attend<T, HD, 1, EXACT>(a, u, direct_u, ru.o, ru.ml, blockIdx.x - many, shared);
   if (zero) zero_outside<T>(a);
 }
 
@@ -1513,10 +1519,6 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
   return p;
 }
 
-struct Rows {
-  float *o, *ml;
-};
-
 template <class T, int HD, int NT>
 hipError_t attend_t(const AttendArgs& a, const Cut& u, int direct, int zero, const Rows& r, hipStream_t s) {
   const dim3 grid((unsigned)u.workers);
@@ -1559,26 +1561,34 @@ hipError_t flash_pass(const AttendArgs& a, const Flash& f, int direct, int zero,
   }
 }
 
+// k_attend's pass u and k_flash's pass f.
+struct Both {
+  const Cut& u;
+  const Flash& f;
+  int direct_u, direct_f, zero;
+  Rows ru, rf;
+};
+
 template <class T, int HD>
-hipError_t both_t(const AttendArgs& a, const Plan& p, int zero, const Rows& r, hipStream_t s) {
-  const dim3 grid((unsigned)(p.own.workers + p.fown.tiles * a.c.kv_heads * p.fown.splits));
+hipError_t both_t(const AttendArgs& a, const Both& b, hipStream_t s) {
+  const dim3 grid((unsigned)(b.u.workers + b.f.tiles * a.c.kv_heads * b.f.splits));
   if (a.c.hd == HD)
-    hipLaunchKernelGGL((k_both<T, HD, true>), grid, dim3(kBlock), 0, s, a, p.own, p.fown, p.direct_attend,
-                       p.direct_flash, zero, r.o, r.ml);
+    hipLaunchKernelGGL((k_both<T, HD, true>), grid, dim3(kBlock), 0, s, a, b.u, b.f, b.direct_u, b.direct_f, b.zero,
+                       b.ru, b.rf);
   else
-    hipLaunchKernelGGL((k_both<T, HD, false>), grid, dim3(kBlock), 0, s, a, p.own, p.fown, p.direct_attend,
-                       p.direct_flash, zero, r.o, r.ml);
+    hipLaunchKernelGGL((k_both<T, HD, false>), grid, dim3(kBlock), 0, s, a, b.u, b.f, b.direct_u, b.direct_f, b.zero,
+                       b.ru, b.rf);
   return hipGetLastError();
 }
 
 template <class T>
-hipError_t both_pass(const AttendArgs& a, const Plan& p, int zero, const Rows& r, hipStream_t s) {
+hipError_t both_pass(const AttendArgs& a, const Both& b, hipStream_t s) {
   if constexpr (T::code == SY_F32) {
     return hipErrorInvalidConfiguration;
   } else {
-    if (a.c.hd <= 64) return both_t<T, 64>(a, p, zero, r, s);
-    if (a.c.hd <= 128) return both_t<T, 128>(a, p, zero, r, s);
-    return both_t<T, 256>(a, p, zero, r, s);
+    if (a.c.hd <= 64) return both_t<T, 64>(a, b, s);
+    if (a.c.hd <= 128) return both_t<T, 128>(a, b, s);
+    return both_t<T, 256>(a, b, s);
   }
 }
 
@@ -1597,13 +1607,18 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   float* const wf = static_cast<float*>(a.workspace);
   const Rows own{wf + p.row_o, wf + p.row_ml}, pre{wf + p.pre_o, wf + p.pre_ml};
   hipError_t e = hipSuccess;
-  if (p.pre == 1) e = attend_pass<T>(a, p.cpre, 0, 0, pre, s);
-  else if (p.pre == 2) e = flash_pass<T>(a, p.fpre, 0, 0, pre, s);
-  if (e != hipSuccess) return e;
   const int zero = a.fill && a.c.starts != nullptr;
-  if (p.flash && p.attend) e = both_pass<T>(a, p, zero, own, s);
-  else if (p.flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero, own, s);
-  else e = attend_pass<T>(a, p.own, p.direct_attend, zero, own, s);
+  bool attend = p.attend, flash = p.flash;
+  if (p.pre == 1) {
+    e = attend_pass<T>(a, p.cpre, 0, 0, pre, s);
+  } else if (p.pre == 2) {
+    e = both_pass<T>(a, Both{p.own, p.fpre, p.direct_attend, 0, zero, own, pre}, s);
+    attend = false;
+  }
+  if (e == hipSuccess && attend && flash)
+    e = both_pass<T>(a, Both{p.own, p.fown, p.direct_attend, p.direct_flash, zero, own, own}, s), attend = flash = false;
+  if (e == hipSuccess && flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero && !p.attend, own, s);
+  if (e == hipSuccess && attend) e = attend_pass<T>(a, p.own, p.direct_attend, zero, own, s);
   if (e != hipSuccess) return e;
   if (p.merge_flash) {
     hipLaunchKernelGGL((k_merge_flash<T>), dim3((unsigned)(p.fown.tiles * a.c.kv_heads)), dim3(kBlock), 0, s, a,
