@@ -8,12 +8,15 @@
 // counts, weights per bin and the running sums of the draw need no fixed order, and the
 // token is the same on every run.
 //
-// A workgroup of 16 waves per row; a wave owns a contiguous run of the row, read once
-// into registers (longer rows are read again, from L2). A cut is found without sorting:
-// a histogram over 2048 equal steps of the logits' range (counts or weights, LDS
+// A workgroup of 16 waves per row, which is read from memory once into LDS (rows that do
+// not fit are read again, from L2); a wave owns a contiguous run of it. The passes over the
+// row are short loops: unrolled over registers they were bound by fetching their own code,
+// which each workgroup runs once (8 rows of 32000 bf16 72 us, 256 of 50257 fp32 230). A cut is found without
+// sorting: a histogram over 2048 equal steps of the logits' range (counts or weights, LDS
 // atomics) gives the step in which it falls, and the few candidates of that step are
 // ranked against one another in LDS. Steps with more candidates than fit (rows of equal
-// logits) are bisected instead.
+// logits) are bisected instead. What is kept is gathered, weighed once more and summed by
+// 256 runs of indices; the one that holds the random number's place is ranked by index.
 #include <algorithm>
 
 #include "sy_launch.hpp"
@@ -25,7 +28,9 @@ namespace {
 constexpr int kBlock = 1024;
 constexpr int kWaves = kBlock / 64;
 constexpr int kBins = 2048;
-constexpr int kList = 1024;
+constexpr int kRanked = kBlock;  // candidates that are ranked against one another
+constexpr int kList = 4096;      // candidates that are gathered
+constexpr int kRuns = 256;       // of a row's indices
 constexpr double kOne = 17592186044416.0;  // 2^44
 
 typedef unsigned long long u64;
@@ -66,7 +71,7 @@ __device__ __forceinline__ double exp2_of(double z) {
   p = fma(p, y, 0.5);
   p = fma(p, y, 1.0);
   p = fma(p, y, 1.0);
-  return ldexp(p, (int)n);
+  return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
 }
 
 // A token's weight as a fraction of the largest (e) and in units of 2^-44.
@@ -101,30 +106,33 @@ __device__ __forceinline__ float float_of(uint32_t k) {
 }
 
 struct Shared {
-  u64 mass[kBins];
-  uint32_t count[kBins];
+  u64 mass[kBins];  // weights (or counts) of the steps, then of the ranked
   float lx[kList];
   int li[kList];
-  u64 lw[kList];
-  u64 sums[kWaves + 1];
-  float fmax_[kWaves], fmin_[kWaves];
+  u64 run[kRuns];
+  u64 sums[kWaves];
+  float tops[kWaves], lows[kWaves];
   int n, bin, rank, tok;
-  u64 before;
+  u64 before, total;
   Last last;
 };
 
-// NCH chunks of a row a lane in registers; 0: as many as the row needs, read each time.
-template <class T, int NCH>
+// A row, in LDS (`held`) or read from memory each time. A wave has nch chunks a lane of it.
+template <class T>
 struct Row {
   using S = typename T::storage;
   static constexpr int CE = T::ce;
   const S* p;
-  int vocab, nch, start;  // chunks a lane, first element of the wave
-  i32x4_t x[NCH ? NCH : 1];
+  const char* held;
+  int vocab, nch, start;
 
   __device__ __forceinline__ int index(int j) const { return start + (j * 64 + (int)(threadIdx.x & 63)) * CE; }
   __device__ __forceinline__ i32x4_t load(int j) const {
     const int at = index(j);
+    if (held != nullptr) return *reinterpret_cast<const i32x4_t*>(held + (int64_t)at * (int)sizeof(S));
+    return fetch(at);
+  }
+  __device__ __forceinline__ i32x4_t fetch(int at) const {
     i32x4_t v;
     if (at + CE <= vocab) {
       __builtin_memcpy(&v, p + at, 16);  // rows start anywhere
@@ -136,16 +144,6 @@ struct Row {
     }
     return v;
   }
-  __device__ __forceinline__ void init(const S* row, int n) {
-    p = row;
-    vocab = n;
-    nch = NCH ? NCH : (n + kBlock * CE - 1) / (kBlock * CE);
-    start = wave_id() * nch * 64 * CE;
-    if constexpr (NCH != 0) {
-#pragma unroll
-      for (int j = 0; j < NCH; ++j) x[j] = load(j);
-    }
-  }
   // f(logit, index) over the chunk's elements; NaN as -inf, -0 as 0, past the row -inf.
   template <class F> __device__ __forceinline__ void chunk(const i32x4_t& v, int at, F f) const {
 #pragma unroll
@@ -156,12 +154,8 @@ struct Row {
     }
   }
   template <class F> __device__ __forceinline__ void each(F f) const {
-    if constexpr (NCH != 0) {
-#pragma unroll
-      for (int j = 0; j < NCH; ++j) chunk(x[j], index(j), f);
-    } else {
-      for (int j = 0; j < nch; ++j) chunk(load(j), index(j), f);
-    }
+#pragma unroll 1
+    for (int j = 0; j < nch; ++j) chunk(load(j), index(j), f);
   }
 };
 
@@ -180,7 +174,7 @@ __device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
 // The last of the candidates up to `from` that a cut keeps. COUNT: the first `k` of them;
 // else those before whose own place less than p of the total weight lies, at least one.
 template <bool COUNT, class R>
-__device__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last& from, float low, u64 k, double p) {
+__device__ __forceinline__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last& from, float low, u64 k, double p) {
   const int tid = threadIdx.x;
   const float span = wt.top - low;
   const float step = wt.top == INFINITY ? 1.0f : span > 0.0f ? (float)kBins / span : 0.0f;
@@ -188,21 +182,19 @@ __device__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last
     return x == wt.top ? 0 : (int)fminf((wt.top - x) * step, (float)(kBins - 1));
   };
   __syncthreads();
-  for (int b = tid; b < kBins; b += kBlock) {
-    sh.mass[b] = 0;
-    sh.count[b] = 0;
-  }
+  for (int b = tid; b < kBins; b += kBlock) sh.mass[b] = 0;
   if (tid == 0) {
     sh.n = 0;
     sh.bin = -1;
     sh.rank = -1;
   }
   __syncthreads();
+  uint32_t* const count = reinterpret_cast<uint32_t*>(sh.mass);
   row.each([&](float x, int i) {
     if (x == -INFINITY || !from.keeps(x, i)) return;
     const int b = bin_of(x);
     if constexpr (COUNT) {
-      atomicAdd(&sh.count[b], 1u);
+      atomicAdd(&count[b], 1u);
     } else {
       const u64 w = wt.w(x);
       if (w != 0) atomicAdd(&sh.mass[b], w);
@@ -210,8 +202,8 @@ __device__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last
   });
   __syncthreads();
   // Sums before each bin; a thread has two.
-  const u64 a0 = COUNT ? sh.count[2 * tid] : sh.mass[2 * tid];
-  const u64 a1 = COUNT ? sh.count[2 * tid + 1] : sh.mass[2 * tid + 1];
+  const u64 a0 = COUNT ? count[2 * tid] : sh.mass[2 * tid];
+  const u64 a1 = COUNT ? count[2 * tid + 1] : sh.mass[2 * tid + 1];
   const u64 incl = scan64(a0 + a1);
   if ((tid & 63) == 63) sh.sums[wave_id()] = incl;
   __syncthreads();
@@ -241,24 +233,25 @@ __device__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last
   row.each([&](float x, int i) {
     if (!in(x, i)) return;
     const int at = atomicAdd(&sh.n, 1);
-    if (at < kList) {
+    if (at < kRanked) {
       sh.lx[at] = x;
       sh.li[at] = i;
-      sh.lw[at] = COUNT ? 1 : wt.w(x);
+      sh.mass[at] = COUNT ? 1 : wt.w(x);
     }
   });
   __syncthreads();
   const int n = sh.n;
-  if (n <= kList) {
+  if (n <= kRanked) {
     int rank = 0;
     u64 b = base;
     const bool mine = tid < n;
     const float x = mine ? sh.lx[tid] : 0.0f;
     const int i = mine ? sh.li[tid] : 0;
+#pragma unroll 4
     for (int q = 0; q < n; ++q) {
       const bool ahead = sh.lx[q] > x || (sh.lx[q] == x && sh.li[q] < i);
       rank += ahead ? 1 : 0;
-      b += ahead ? sh.lw[q] : 0;
+      b += ahead ? sh.mass[q] : 0;
     }
     const bool keep = mine && kept(b);
     if (keep) atomicMax(&sh.rank, rank);
@@ -295,33 +288,45 @@ __device__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last
   return Last{xt, first};
 }
 
-template <class T, int NCH>
+template <class T, int HELD>  // bytes of LDS for the row
 __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
   __shared__ Shared sh;
+  __shared__ __align__(16) char held[HELD ? HELD : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int64_t r = blockIdx.x;
-  Row<T, NCH> row;
-  row.init(static_cast<const typename T::storage*>(a.logits) + r * a.row_stride, a.vocab);
+  constexpr int CE = T::ce;
+  Row<T> row;
+  row.p = static_cast<const typename T::storage*>(a.logits) + r * a.row_stride;
+  row.held = HELD ? held : nullptr;
+  row.vocab = a.vocab;
+  row.nch = (a.vocab + kBlock * CE - 1) / (kBlock * CE);
+  row.start = wave * row.nch * 64 * CE;
   float top = -INFINITY, low = INFINITY;
-  row.each([&](float x, int) {
-    top = fmaxf(top, x);
-    low = x == -INFINITY ? low : fminf(low, x);
-  });
+#pragma unroll 4
+  for (int j = 0; j < row.nch; ++j) {
+    const int at = row.index(j);
+    const i32x4_t v = row.fetch(at);
+    if constexpr (HELD != 0) *reinterpret_cast<i32x4_t*>(held + at * (int)sizeof(typename T::storage)) = v;
+    row.chunk(v, at, [&](float x, int) {
+      top = fmaxf(top, x);
+      low = x == -INFINITY ? low : fminf(low, x);
+    });
+  }
 #pragma unroll
   for (int k = 32; k >= 1; k /= 2) {
     top = fmaxf(top, __shfl_xor(top, k));
     low = fminf(low, __shfl_xor(low, k));
   }
   if (lane == 0) {
-    sh.fmax_[wave] = top;
-    sh.fmin_[wave] = low;
+    sh.tops[wave] = top;
+    sh.lows[wave] = low;
   }
   if (tid == 0) sh.tok = 0x7fffffff;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) {
-    top = fmaxf(top, sh.fmax_[k]);
-    low = fminf(low, sh.fmin_[k]);
+    top = fmaxf(top, sh.tops[k]);
+    low = fminf(low, sh.lows[k]);
   }
   if (top == -INFINITY) {
     if (tid == 0) a.tokens[r] = -1;
@@ -347,21 +352,42 @@ __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
     const float zero = top - (float)fmin(31.3 * t, 3.0e38);
     last = find_cut<false>(sh, row, wt, last, fmaxf(low, zero), 0, top_p);
   }
-  // The draw. A wave's run of the row is contiguous, so sums of waves are in index order.
-  const auto weight = [&](float x, int i) -> u64 {
-    if (x == -INFINITY || !last.keeps(x, i)) return 0;
+  // The draw. What is kept, weighed and summed by runs of indices.
+  __syncthreads();
+  if (tid == 0) sh.n = 0;
+  if (tid < kRuns) sh.run[tid] = 0;
+  __syncthreads();
+  row.each([&](float x, int i) {
+    if (x == -INFINITY || !last.keeps(x, i)) return;
+    const int at = atomicAdd(&sh.n, 1);
+    if (at < kList) {
+      sh.lx[at] = x;
+      sh.li[at] = i;
+    }
+  });
+  __syncthreads();
+  const int n = sh.n;
+  const int len = (a.vocab + kRuns - 1) / kRuns;
+  const auto weight = [&](float x) -> u64 {
     const double e = wt.e(x);
     return e >= min_p ? Weigher::units(e) : 0;
   };
-  u64 mine = 0;
-  row.each([&](float x, int i) { mine += weight(x, i); });
+  if (n <= kList) {
+    for (int q = tid; q < n; q += kBlock) atomicAdd(&sh.run[sh.li[q] / len], weight(sh.lx[q]));
+  } else {
+    row.each([&](float x, int i) {
+      if (x != -INFINITY && last.keeps(x, i)) atomicAdd(&sh.run[i / len], weight(x));
+    });
+  }
+  __syncthreads();
+  const u64 mine = tid < kRuns ? sh.run[tid] : 0;
   const u64 incl = scan64(mine);
-  __syncthreads();
   if (lane == 63) sh.sums[wave] = incl;
+  if (tid == 0) sh.n = 0;
   __syncthreads();
-  u64 before = 0, total = 0;
+  u64 before = incl - mine, total = 0;
 #pragma unroll
-  for (int k = 0; k < kWaves; ++k) {
+  for (int k = 0; k < kRuns / 64; ++k) {
     const u64 s = sh.sums[k];
     before += k < wave ? s : 0;
     total += s;
@@ -369,46 +395,44 @@ __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
   const double u = (double)a.u[r];
   u64 goal = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
   goal = min(goal, total - 1);
-  if (goal < before || goal >= before + sh.sums[wave]) return;
-  goal -= before;
-  for (int j = 0; j < row.nch; ++j) {
-    u64 s = 0;
-    const i32x4_t v = row.load(j);
-    const int at = row.index(j);
-    row.chunk(v, at, [&](float x, int i) { s += weight(x, i); });
-    const u64 in = scan64(s);
-    const u64 all = shfl64(in, 63);
-    if (goal >= all) {
-      goal -= all;
-      continue;
-    }
-    if (goal >= in - s && goal < in) {
-      u64 cum = in - s;
-      int tok = -1;
-      row.chunk(v, at, [&](float x, int i) {
-        cum += weight(x, i);
-        if (tok < 0 && cum > goal) tok = i;
-      });
-      a.tokens[r] = tok;
-    }
-    return;
+  if (tid < kRuns && goal >= before && goal < before + mine) {
+    sh.bin = tid;
+    sh.before = before;
   }
+  __syncthreads();
+  // The run that holds the goal: at most 1024 tokens, a thread each, in the order of indices.
+  const int i = sh.bin * len + tid;
+  u64 w = 0;
+  if (tid < len && i < a.vocab) {
+    i32x4_t v = {0, 0, 0, 0};
+    __builtin_memcpy(&v, row.p + i, sizeof(typename T::storage));
+    float x = elem<T>(v, 0);
+    x = x == x ? x + 0.0f : -INFINITY;
+    if (x != -INFINITY && last.keeps(x, i)) w = weight(x);
+  }
+  u64 in = scan64(w);
+  if (lane == 63) sh.sums[wave] = in;
+  __syncthreads();
+  in += sh.before;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) in += k < wave ? sh.sums[k] : 0;
+  if (goal >= in - w && goal < in) a.tokens[r] = i;
 }
 
-template <class T, int NCH>
+template <class T, int HELD>
 hipError_t sample_n(const SampleArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_sample<T, NCH>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, s, a);
+  hipLaunchKernelGGL((k_sample<T, HELD>), dim3((unsigned)a.n_rows), dim3(kBlock), 0, s, a);
   return hipGetLastError();
 }
 
 template <class T>
 hipError_t sample_t(const SampleArgs& a, hipStream_t s) {
-  const int n = (a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce);
-  if (n <= 1) return sample_n<T, 1>(a, s);
-  if (n <= 2) return sample_n<T, 2>(a, s);
-  if (n <= 4) return sample_n<T, 4>(a, s);
-  if (n <= 8) return sample_n<T, 8>(a, s);
-  if (T::ce == 4 && n <= 16) return sample_n<T, T::ce == 4 ? 16 : 0>(a, s);
+  // Whole chunks of every lane, which is what the kernel stores. Short rows leave room for
+  // a second workgroup on a CU.
+  const int64_t chunks = (a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce);
+  const int64_t bytes = chunks * kBlock * 16;
+  if (bytes <= 16384) return sample_n<T, 16384>(a, s);
+  if (bytes <= 98304) return sample_n<T, 98304>(a, s);
   return sample_n<T, 0>(a, s);
 }
 
