@@ -271,22 +271,12 @@ __device__ __forceinline__ Tiles tiles_of(const Cut& u, int group, const Seq& s)
   return {(rows + u.rt - 1) / u.rt, k < 1 ? 1 : k};
 }
 
-__device__ __forceinline__ int scan_add(int x) {  // inclusive over the lanes
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) {
-    const int y = __shfl_up(x, k);
-    if (lane >= k) x += y;
-  }
-  return x;
-}
-
 // Sums and searches over the sequences, `count(b)` units each: every lane looks at another
 // sequence, so 64 of them cost one round of loads.
 template <class F> __device__ __forceinline__ int total_of(int upto, F count) {
   int x = 0;
   for (int b = threadIdx.x & 63; b < upto; b += 64) x += count(b);
-  return __builtin_amdgcn_readlane(scan_add(x), 63);
+  return __builtin_amdgcn_readlane((int)wave_scan<uint32_t>(x), 63);
 }
 // The sequence that holds a unit, and the units before it; false past the last.
 template <class F> __device__ __forceinline__ bool locate(int n_seq, int unit, F count, int* seq, int* base) {
@@ -294,7 +284,7 @@ template <class F> __device__ __forceinline__ bool locate(int n_seq, int unit, F
   int before = 0;
   for (int b0 = 0; b0 < n_seq; b0 += 64) {
     const int mine = b0 + lane < n_seq ? count(b0 + lane) : 0;
-    const int incl = scan_add(mine);
+    const int incl = (int)wave_scan<uint32_t>(mine);
     const uint64_t hit = __ballot(before + incl > unit);
     if (hit != 0) {
       const int l = __ffsll((unsigned long long)hit) - 1;
@@ -320,7 +310,7 @@ __device__ __forceinline__ bool locate_last(int n_seq, int unit, int most, int f
   const auto nearer = [&](int k) {  // units at most k - 1 before their sequence's last
     int x = min(mine, k);
     for (int b = lane + 64; b < n_seq; b += 64) x += min(count(b), k);
-    return __builtin_amdgcn_readlane(scan_add(x), 63);
+    return __builtin_amdgcn_readlane((int)wave_scan<uint32_t>(x), 63);
   };
   const int total = nearer(most);
   if (unit >= total) return false;
@@ -334,7 +324,7 @@ __device__ __forceinline__ bool locate_last(int n_seq, int unit, int most, int f
   int skip = unit - nearer(lo);  // sequences of more than `lo` units to pass over
   for (int b0 = 0; b0 < n_seq; b0 += 64) {
     const int n = b0 == 0 ? mine : b0 + lane < n_seq ? count(b0 + lane) : 0;
-    const int incl = scan_add(n > lo ? 1 : 0);
+    const int incl = (int)wave_scan<uint32_t>(n > lo ? 1 : 0);
     const uint64_t hit = __ballot(incl > skip);
     if (hit != 0) {
       const int l = __ffsll((unsigned long long)hit) - 1;

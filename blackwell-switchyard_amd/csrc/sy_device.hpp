@@ -601,6 +601,25 @@ __device__ __forceinline__ float wave_sum(float x) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
+// Inclusive sums over the lanes of whole numbers, without LDS.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <class U, int CTRL, int ROWS = 0xf> __device__ __forceinline__ U dpp_whole(U x) {
+  if constexpr (sizeof(U) == 4) return (U)dpp_u32<CTRL, ROWS>((uint32_t)x);
+  else return ((U)dpp_u32<CTRL, ROWS>((uint32_t)(x >> 32)) << 32) | dpp_u32<CTRL, ROWS>((uint32_t)x);
+}
+template <class U> __device__ __forceinline__ U wave_scan(U x) {
+  x += dpp_whole<U, 0x111>(x);       // row_shr:1, 2, 4, 8
+  x += dpp_whole<U, 0x112>(x);
+  x += dpp_whole<U, 0x114>(x);
+  x += dpp_whole<U, 0x118>(x);
+  x += dpp_whole<U, 0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x += dpp_whole<U, 0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 // Sums of P per-lane values over the 64 lanes, transposed (P = 2, 4, ..., 32):
 // lane l ends up with the total of v[tsum_row<P>(l)]. Each step halves the
 // values a lane carries: gfx950's permlane32/permlane16 swaps pair the halves

@@ -29,59 +29,53 @@ constexpr int kBlock = 1024;
 constexpr int kWaves = kBlock / 64;
 constexpr int kBins = 2048;
 constexpr int kRanked = kBlock;  // candidates that are ranked against one another
-constexpr int kList = 4096;      // candidates that are gathered
 constexpr int kRuns = 256;       // of a row's indices
+constexpr int kGroup = 4;        // chunks that are read from memory together
 constexpr double kOne = 17592186044416.0;  // 2^44
 
 typedef unsigned long long u64;
 
-__device__ __forceinline__ u64 shfl_up64(u64 x, int k) {
-  const uint32_t lo = __shfl_up((uint32_t)x, k), hi = __shfl_up((uint32_t)(x >> 32), k);
-  return ((u64)hi << 32) | lo;
-}
-__device__ __forceinline__ u64 shfl64(u64 x, int l) {
-  const uint32_t lo = __shfl((uint32_t)x, l), hi = __shfl((uint32_t)(x >> 32), l);
-  return ((u64)hi << 32) | lo;
-}
-__device__ __forceinline__ u64 scan64(u64 x) {  // inclusive over the lanes
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) {
-    const u64 y = shfl_up64(x, k);
-    if (lane >= k) x += y;
-  }
+__device__ __forceinline__ u64 scan64(u64 x) { return wave_scan<u64>(x); }  // inclusive over the lanes
+
+// Sums over the 16 lanes of a row, in its last lane.
+template <class U> __device__ __forceinline__ U row16_sum(U x) {
+  x += dpp_whole<U, 0x111>(x);
+  x += dpp_whole<U, 0x112>(x);
+  x += dpp_whole<U, 0x114>(x);
+  x += dpp_whole<U, 0x118>(x);
   return x;
 }
 
-// exp2(z) for -46 < z <= 0 in double: 2^n times the series of exp over |y| <= ln(2)/2,
-// whose first term left out is y^13/13! < 2e-16.
-__device__ __forceinline__ double exp2_of(double z) {
-  const double n = rint(z);
-  const double y = (z - n) * 0.693147180559945309417;
-  double p = 1.0 / 479001600.0;
-  p = fma(p, y, 1.0 / 39916800.0);
-  p = fma(p, y, 1.0 / 3628800.0);
-  p = fma(p, y, 1.0 / 362880.0);
-  p = fma(p, y, 1.0 / 40320.0);
-  p = fma(p, y, 1.0 / 5040.0);
-  p = fma(p, y, 1.0 / 720.0);
-  p = fma(p, y, 1.0 / 120.0);
-  p = fma(p, y, 1.0 / 24.0);
-  p = fma(p, y, 1.0 / 6.0);
-  p = fma(p, y, 0.5);
-  p = fma(p, y, 1.0);
-  p = fma(p, y, 1.0);
-  return __longlong_as_double(__double_as_longlong(p) + ((long long)(int)n << 52));
+// 2^y for |y| <= 1/2: the series of exp(y ln 2), whose first term left out is below 2e-16.
+// (The coefficients are ln(2)^k / k!.)
+__device__ __forceinline__ double exp2_near(double y) {
+  constexpr double l = 0.693147180559945309417;
+  constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
+                   c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11, c12 = c11 * l / 12;
+  double p = fma(c12, y, c11);
+  p = fma(p, y, c10);
+  p = fma(p, y, c9);
+  p = fma(p, y, c8);
+  p = fma(p, y, c7);
+  p = fma(p, y, c6);
+  p = fma(p, y, c5);
+  p = fma(p, y, c4);
+  p = fma(p, y, c3);
+  p = fma(p, y, c2);
+  p = fma(p, y, l);
+  return fma(p, y, 1.0);
 }
 
-// A token's weight as a fraction of the largest (e) and in units of 2^-44.
+// A token's weight as a fraction of the largest (e) and in units of 2^-44. Far below the
+// largest, and for -inf, e is 2^-60, whose weight is zero.
 struct Weigher {
   float top;
-  double c;  // log2(e) / T
+  double c;  // log2(e) / T, finite
   __device__ __forceinline__ double e(float x) const {
-    if (x == top) return 1.0;
-    const double z = ((double)x - (double)top) * c;
-    return x > -INFINITY && z > -46.0 ? exp2_of(z) : 0.0;
+    if (top == INFINITY) return x == top ? 1.0 : 0.0;
+    const double z = fmax(((double)x - (double)top) * c, -60.0);  // (0 times -inf: -60 too)
+    const double n = rint(z);
+    return ldexp(exp2_near(z - n), (int)n);
   }
   // rint(e 2^44): 2^52 + w has the whole number in its mantissa
   static __device__ __forceinline__ u64 units(double e) {
@@ -105,33 +99,35 @@ __device__ __forceinline__ float float_of(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
+template <int LIST>  // candidates that are gathered
 struct Shared {
+  static constexpr int kList = LIST;
   u64 mass[kBins];  // weights (or counts) of the steps, then of the ranked
-  float lx[kList];
-  int li[kList];
+  float lx[LIST];  // gathered candidates
+  int li[LIST];
+  float rx[kRanked];  // ranked ones
+  int ri[kRanked];
   u64 run[kRuns];
   u64 sums[kWaves];
   float tops[kWaves], lows[kWaves];
-  int n, bin, rank, tok;
+  int n, bin, rank, tok, listed;
   u64 before, total;
   Last last;
 };
 
-// A row, in LDS (`held`) or read from memory each time. A wave has nch chunks a lane of it.
-template <class T>
+// The candidates: a row, in LDS (HELD: NaN there as -inf, and past the row) or read from
+// memory each time; or what was gathered of it. A wave has nch chunks a lane of a row.
+template <class T, bool HELD, class Shared>
 struct Row {
   using S = typename T::storage;
   static constexpr int CE = T::ce;
   const S* p;
-  const char* held;
+  char* held;
+  Shared* sh;
   int vocab, nch, start;
+  int listed;  // gathered candidates, or -1
 
   __device__ __forceinline__ int index(int j) const { return start + (j * 64 + (int)(threadIdx.x & 63)) * CE; }
-  __device__ __forceinline__ i32x4_t load(int j) const {
-    const int at = index(j);
-    if (held != nullptr) return *reinterpret_cast<const i32x4_t*>(held + (int64_t)at * (int)sizeof(S));
-    return fetch(at);
-  }
   __device__ __forceinline__ i32x4_t fetch(int at) const {
     i32x4_t v;
     if (at + CE <= vocab) {
@@ -144,23 +140,88 @@ struct Row {
     }
     return v;
   }
-  // f(logit, index) over the chunk's elements; NaN as -inf, -0 as 0, past the row -inf.
-  template <class F> __device__ __forceinline__ void chunk(const i32x4_t& v, int at, F f) const {
+  // A chunk's logits: NaN as -inf, -0 as 0, past the row -inf.
+  __device__ __forceinline__ void clean(const i32x4_t& v, int at, float (&y)[CE]) const {
 #pragma unroll
     for (int e = 0; e < CE; ++e) {
-      float y = elem<T>(v, e);
-      y = at + e < vocab && y == y ? y + 0.0f : -INFINITY;
-      f(y, at + e);
+      const float x = elem<T>(v, e);
+      y[e] = at + e < vocab && x == x ? x + 0.0f : -INFINITY;
     }
   }
-  template <class F> __device__ __forceinline__ void each(F f) const {
+  // f(logits, index of the first) of every chunk of the row.
+  template <class F> __device__ __forceinline__ void chunks(F f) const {
+    float y[CE];
+    if constexpr (HELD) {
 #pragma unroll 1
-    for (int j = 0; j < nch; ++j) chunk(load(j), index(j), f);
+      for (int j = 0; j < nch; ++j) {
+        const int at = index(j);
+        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(held + at * (int)sizeof(S));
+#pragma unroll
+        for (int e = 0; e < CE; ++e) y[e] = elem<T>(v, e);
+        f(y, at);
+      }
+    } else {
+      // Four chunks are on their way while the four before them are worked on.
+      i32x4_t next[kGroup];
+#pragma unroll
+      for (int q = 0; q < kGroup; ++q) next[q] = fetch(index(q));
+#pragma unroll 1
+      for (int j = 0; j < nch; j += kGroup) {
+        i32x4_t v[kGroup];
+#pragma unroll
+        for (int q = 0; q < kGroup; ++q) v[q] = next[q];
+        if (j + kGroup < nch) {
+#pragma unroll
+          for (int q = 0; q < kGroup; ++q) next[q] = fetch(index(j + kGroup + q));
+        }
+#pragma unroll
+        for (int q = 0; q < kGroup; ++q) {
+          const int at = index(j + q);
+          clean(v[q], at, y);
+          f(y, at);
+        }
+      }
+    }
+  }
+  // f(logit, index) of every candidate.
+  template <class F> __device__ __forceinline__ void each(F f) const {
+    if (listed >= 0) {
+      for (int q = threadIdx.x; q < listed; q += kBlock) f(sh->lx[q], sh->li[q]);
+    } else {
+      chunks([&](const float (&y)[CE], int at) {
+#pragma unroll
+        for (int e = 0; e < CE; ++e) f(y[e], at + e);
+      });
+    }
+  }
+  // Gathers the row's logits above `over`, if there is room: a place for a wave's at a time.
+  __device__ __forceinline__ void gather(float over) {
+    chunks([&](const float (&y)[CE], int at) {
+      uint32_t mask = 0;
+#pragma unroll
+      for (int e = 0; e < CE; ++e) mask |= y[e] > over ? 1u << e : 0u;
+      if (!__any(mask)) return;
+      const uint32_t n = __popc(mask), incl = wave_scan<uint32_t>(n);
+      int base = 0;
+      if ((threadIdx.x & 63) == 63) base = atomicAdd(&sh->listed, (int)incl);
+      int to = __builtin_amdgcn_readlane(base, 63) + (int)(incl - n);
+#pragma unroll
+      for (int e = 0; e < CE; ++e) {
+        if ((mask >> e & 1) == 0) continue;
+        if (to < Shared::kList) {
+          sh->lx[to] = y[e];
+          sh->li[to] = at + e;
+        }
+        ++to;
+      }
+    });
+    __syncthreads();
+    if (sh->listed <= Shared::kList) listed = sh->listed;
   }
 };
 
 // Sum over the workgroup, known to every thread.
-__device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
+template <class Shared> __device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
   const u64 t = scan64(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) sh.sums[wave_id()] = t;
@@ -173,90 +234,127 @@ __device__ __forceinline__ u64 block_sum(Shared& sh, u64 x) {
 
 // The last of the candidates up to `from` that a cut keeps. COUNT: the first `k` of them;
 // else those before whose own place less than p of the total weight lies, at least one.
-template <bool COUNT, class R>
-__device__ __forceinline__ Last find_cut(Shared& sh, const R& row, const Weigher& wt, const Last& from, float low, u64 k, double p) {
+// Leaves the candidates that can still be kept gathered, if there is room for them.
+// OPEN: nothing is cut yet (`from` keeps all).
+template <bool COUNT, bool OPEN, class Shared, class R>
+__device__ __forceinline__ Last find_cut(Shared& sh, R& row, const Weigher& wt, const Last& from, float low, u64 k,
+                                         double p) {
   const int tid = threadIdx.x;
+  const bool few = !OPEN && row.listed >= 0 && row.listed <= kRanked / 2;  // all of them are ranked
   const float span = wt.top - low;
-  const float step = wt.top == INFINITY ? 1.0f : span > 0.0f ? (float)kBins / span : 0.0f;
+  const float step = span > 0.0f ? (float)kBins / span : 0.0f;
   const auto bin_of = [&](float x) {  // falls with x; anything past the range in the last
-    return x == wt.top ? 0 : (int)fminf((wt.top - x) * step, (float)(kBins - 1));
+    if (few) return 0;
+    if (wt.top == INFINITY) return x == wt.top ? 0 : kBins - 1;
+    return (int)fminf((wt.top - x) * step, (float)(kBins - 1));
   };
+  const auto left = [&](float x, int i) { return x != -INFINITY && (OPEN || from.keeps(x, i)); };
   __syncthreads();
-  for (int b = tid; b < kBins; b += kBlock) sh.mass[b] = 0;
   if (tid == 0) {
     sh.n = 0;
     sh.bin = -1;
     sh.rank = -1;
+    sh.listed = 0;
   }
-  __syncthreads();
-  uint32_t* const count = reinterpret_cast<uint32_t*>(sh.mass);
-  row.each([&](float x, int i) {
-    if (x == -INFINITY || !from.keeps(x, i)) return;
-    const int b = bin_of(x);
-    if constexpr (COUNT) {
-      atomicAdd(&count[b], 1u);
-    } else {
-      const u64 w = wt.w(x);
-      if (w != 0) atomicAdd(&sh.mass[b], w);
-    }
-  });
-  __syncthreads();
-  // Sums before each bin; a thread has two.
-  const u64 a0 = COUNT ? count[2 * tid] : sh.mass[2 * tid];
-  const u64 a1 = COUNT ? count[2 * tid + 1] : sh.mass[2 * tid + 1];
-  const u64 incl = scan64(a0 + a1);
-  if ((tid & 63) == 63) sh.sums[wave_id()] = incl;
-  __syncthreads();
-  u64 before = incl - (a0 + a1), total = 0;
-#pragma unroll
-  for (int q = 0; q < kWaves; ++q) {
-    const u64 s = sh.sums[q];
-    before += q < wave_id() ? s : 0;
-    total += s;
-  }
-  // A place is kept where less than the goal lies before it.
-  const double goal = COUNT ? (double)k : fmax(p * (double)total, 0.5);
+  int bin = 0;
+  u64 base = 0;
+  double goal;  // a place is kept where less than the goal lies before it
   const auto kept = [&](u64 b) { return (double)b < goal; };
-  if (a0 != 0 && kept(before) && !kept(before + a0)) {
-    sh.bin = 2 * tid;
-    sh.before = before;
+  if (few) {
+    u64 mine = 0;
+    row.each([&](float x, int i) {
+      if (left(x, i)) mine += COUNT ? 1 : wt.w(x);
+    });
+    const u64 total = block_sum(sh, mine);
+    goal = COUNT ? (double)k : fmax(p * (double)total, 0.5);
+    if (kept(total)) return from;
+  } else {
+    for (int b = tid; b < kBins; b += kBlock) sh.mass[b] = 0;
+    __syncthreads();
+    uint32_t* const count = reinterpret_cast<uint32_t*>(sh.mass);
+    row.each([&](float x, int i) {
+      if (!left(x, i)) return;
+      const int b = bin_of(x);
+      if constexpr (COUNT) {
+        atomicAdd(&count[b], 1u);
+      } else {
+        const u64 w = wt.w(x);
+        if (w != 0) atomicAdd(&sh.mass[b], w);
+      }
+    });
+    __syncthreads();
+    // Sums before each bin; a thread has two.
+    const u64 a0 = COUNT ? count[2 * tid] : sh.mass[2 * tid];
+    const u64 a1 = COUNT ? count[2 * tid + 1] : sh.mass[2 * tid + 1];
+    const u64 incl = scan64(a0 + a1);
+    if ((tid & 63) == 63) sh.sums[wave_id()] = incl;
+    __syncthreads();
+    u64 before = incl - (a0 + a1), total = 0;
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) {
+      const u64 s = sh.sums[q];
+      before += q < wave_id() ? s : 0;
+      total += s;
+    }
+    goal = COUNT ? (double)k : fmax(p * (double)total, 0.5);
+    if (a0 != 0 && kept(before) && !kept(before + a0)) {
+      sh.bin = 2 * tid;
+      sh.before = before;
+    }
+    if (a1 != 0 && kept(before + a0) && !kept(before + a0 + a1)) {
+      sh.bin = 2 * tid + 1;
+      sh.before = before + a0;
+    }
+    __syncthreads();
+    bin = sh.bin;
+    if (bin < 0) return from;  // the goal is never reached: nothing is cut
+    base = sh.before;
   }
-  if (a1 != 0 && kept(before + a0) && !kept(before + a0 + a1)) {
-    sh.bin = 2 * tid + 1;
-    sh.before = before + a0;
+  // The goal's bin and those before it are gathered, the ones in it ranked.
+  if (row.listed < 0) {
+    // A little below the bin's lower edge, whatever the roundings of bin_of.
+    const float down = (float)(bin + 1) / step * 1.00001f;
+    const bool edge = bin < kBins - 1 && step > 0.0f && wt.top != INFINITY;
+    row.gather(edge ? wt.top - down - (fabsf(wt.top) + down) * 1e-6f : -INFINITY);
   }
-  __syncthreads();
-  const int bin = sh.bin;
-  if (bin < 0) return from;  // the goal is never reached: nothing is cut
-  const u64 base = sh.before;
-  const auto in = [&](float x, int i) { return x != -INFINITY && bin_of(x) == bin && from.keeps(x, i); };
   row.each([&](float x, int i) {
-    if (!in(x, i)) return;
+    if (!left(x, i) || bin_of(x) != bin) return;
     const int at = atomicAdd(&sh.n, 1);
     if (at < kRanked) {
-      sh.lx[at] = x;
-      sh.li[at] = i;
+      sh.rx[at] = x;
+      sh.ri[at] = i;
       sh.mass[at] = COUNT ? 1 : wt.w(x);
     }
   });
   __syncthreads();
+  const auto in = [&](float x, int i) { return left(x, i) && bin_of(x) == bin; };
   const int n = sh.n;
   if (n <= kRanked) {
-    int rank = 0;
-    u64 b = base;
-    const bool mine = tid < n;
-    const float x = mine ? sh.lx[tid] : 0.0f;
-    const int i = mine ? sh.li[tid] : 0;
-#pragma unroll 4
-    for (int q = 0; q < n; ++q) {
-      const bool ahead = sh.lx[q] > x || (sh.lx[q] == x && sh.li[q] < i);
-      rank += ahead ? 1 : 0;
-      b += ahead ? sh.mass[q] : 0;
+    // Sixteen lanes count what is ahead of one candidate; the last of them has the sums.
+    int best = -1;
+    Last mine{};
+    for (int at = tid / 16; at < n; at += kBlock / 16) {
+      const float x = sh.rx[at];
+      const int i = sh.ri[at];
+      uint32_t rank = 0;
+      u64 b = 0;
+      for (int q = tid % 16; q < n; q += 16) {
+        const float y = sh.rx[q];
+        const u64 m = sh.mass[q];
+        const bool ahead = y > x || (y == x && sh.ri[q] < i);
+        rank += ahead ? 1 : 0;
+        b += ahead ? m : 0;
+      }
+      rank = row16_sum(rank);
+      b = row16_sum(b);
+      if (tid % 16 == 15 && kept(base + b) && (int)rank > best) {
+        best = (int)rank;
+        mine = Last{x, i};
+      }
     }
-    const bool keep = mine && kept(b);
-    if (keep) atomicMax(&sh.rank, rank);
+    if (best >= 0) atomicMax(&sh.rank, best);
     __syncthreads();
-    if (keep && rank == sh.rank) sh.last = Last{x, i};
+    if (best >= 0 && best == sh.rank) sh.last = mine;
     __syncthreads();
     return sh.last;
   }
@@ -290,33 +388,42 @@ __device__ __forceinline__ Last find_cut(Shared& sh, const R& row, const Weigher
 
 template <class T, int HELD>  // bytes of LDS for the row
 __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
-  __shared__ Shared sh;
+  using Sh = Shared<HELD == 0 ? 16384 : 4096>;
+  __shared__ Sh sh;
   __shared__ __align__(16) char held[HELD ? HELD : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int64_t r = blockIdx.x;
   constexpr int CE = T::ce;
-  Row<T> row;
+  Row<T, HELD != 0, Sh> row;
   row.p = static_cast<const typename T::storage*>(a.logits) + r * a.row_stride;
-  row.held = HELD ? held : nullptr;
+  row.held = held;
+  row.sh = &sh;
   row.vocab = a.vocab;
   row.nch = (a.vocab + kBlock * CE - 1) / (kBlock * CE);
+  if (HELD == 0) row.nch = (row.nch + kGroup - 1) / kGroup * kGroup;
   row.start = wave * row.nch * 64 * CE;
+  row.listed = -1;
+  // (Asked for before the row, not when they are needed.)
+  const double t = a.how.temperatures != nullptr ? (double)a.how.temperatures[r] : a.how.temperature;
+  const double top_p = a.how.top_ps != nullptr ? (double)a.how.top_ps[r] : a.how.top_p;
+  const double min_p = fmin(a.how.min_ps != nullptr ? (double)a.how.min_ps[r] : a.how.min_p, 1.0);
+  const int64_t top_k = a.how.top_ks != nullptr ? a.how.top_ks[r] : a.how.top_k;
+  const double u = (double)a.u[r];
   float top = -INFINITY, low = INFINITY;
 #pragma unroll 4
   for (int j = 0; j < row.nch; ++j) {
     const int at = row.index(j);
-    const i32x4_t v = row.fetch(at);
-    if constexpr (HELD != 0) *reinterpret_cast<i32x4_t*>(held + at * (int)sizeof(typename T::storage)) = v;
-    row.chunk(v, at, [&](float x, int) {
-      top = fmaxf(top, x);
-      low = x == -INFINITY ? low : fminf(low, x);
-    });
-  }
+    float y[CE];
+    row.clean(row.fetch(at), at, y);
 #pragma unroll
-  for (int k = 32; k >= 1; k /= 2) {
-    top = fmaxf(top, __shfl_xor(top, k));
-    low = fminf(low, __shfl_xor(low, k));
+    for (int e = 0; e < CE; ++e) {
+      top = fmaxf(top, y[e]);
+      low = y[e] == -INFINITY ? low : fminf(low, y[e]);
+    }
+    if constexpr (HELD != 0) *reinterpret_cast<i32x4_t*>(held + at * (int)sizeof(typename T::storage)) = pack<T>(y);
   }
+  top = wave_max(top);
+  low = -wave_max(-low);
   if (lane == 0) {
     sh.tops[wave] = top;
     sh.lows[wave] = low;
@@ -332,7 +439,6 @@ __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
     if (tid == 0) a.tokens[r] = -1;
     return;
   }
-  const double t = a.how.temperatures != nullptr ? (double)a.how.temperatures[r] : a.how.temperature;
   if (!(t > 0.0)) {
     int at = 0x7fffffff;
     row.each([&](float x, int i) { at = x == top ? min(at, i) : at; });
@@ -341,49 +447,33 @@ __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
     if (tid == 0) a.tokens[r] = sh.tok;
     return;
   }
-  const double top_p = a.how.top_ps != nullptr ? (double)a.how.top_ps[r] : a.how.top_p;
-  const double min_p = fmin(a.how.min_ps != nullptr ? (double)a.how.min_ps[r] : a.how.min_p, 1.0);
-  const int64_t top_k = a.how.top_ks != nullptr ? a.how.top_ks[r] : a.how.top_k;
-  const Weigher wt{top, 1.44269504088896340736 / t};
+  const Weigher wt{top, fmin(1.44269504088896340736 / t, 1e200)};
   Last last{-INFINITY, 0x7fffffff};
-  if (top_k >= 1 && top_k < a.vocab) last = find_cut<true>(sh, row, wt, last, low, (u64)top_k, 0.0);
+  if (top_k >= 1 && top_k < a.vocab) last = find_cut<true, true>(sh, row, wt, last, low, (u64)top_k, 0.0);
   if (top_p < 1.0) {
     // Weights are zero from 45 ln 2 = 31.2 temperatures below the largest on.
     const float zero = top - (float)fmin(31.3 * t, 3.0e38);
-    last = find_cut<false>(sh, row, wt, last, fmaxf(low, zero), 0, top_p);
+    if (last.x == -INFINITY)
+      last = find_cut<false, true>(sh, row, wt, last, fmaxf(low, zero), 0, top_p);
+    else
+      last = find_cut<false, false>(sh, row, wt, last, fmaxf(low, zero), 0, top_p);
   }
-  // The draw. What is kept, weighed and summed by runs of indices.
+  // The draw: what is kept, summed by runs of indices.
   __syncthreads();
-  if (tid == 0) sh.n = 0;
   if (tid < kRuns) sh.run[tid] = 0;
   __syncthreads();
-  row.each([&](float x, int i) {
-    if (x == -INFINITY || !last.keeps(x, i)) return;
-    const int at = atomicAdd(&sh.n, 1);
-    if (at < kList) {
-      sh.lx[at] = x;
-      sh.li[at] = i;
-    }
-  });
-  __syncthreads();
-  const int n = sh.n;
   const int len = (a.vocab + kRuns - 1) / kRuns;
   const auto weight = [&](float x) -> u64 {
     const double e = wt.e(x);
     return e >= min_p ? Weigher::units(e) : 0;
   };
-  if (n <= kList) {
-    for (int q = tid; q < n; q += kBlock) atomicAdd(&sh.run[sh.li[q] / len], weight(sh.lx[q]));
-  } else {
-    row.each([&](float x, int i) {
-      if (x != -INFINITY && last.keeps(x, i)) atomicAdd(&sh.run[i / len], weight(x));
-    });
-  }
+  row.each([&](float x, int i) {
+    if (x != -INFINITY && last.keeps(x, i)) atomicAdd(&sh.run[i / len], weight(x));
+  });
   __syncthreads();
   const u64 mine = tid < kRuns ? sh.run[tid] : 0;
   const u64 incl = scan64(mine);
   if (lane == 63) sh.sums[wave] = incl;
-  if (tid == 0) sh.n = 0;
   __syncthreads();
   u64 before = incl - mine, total = 0;
 #pragma unroll
@@ -392,7 +482,6 @@ __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
     before += k < wave ? s : 0;
     total += s;
   }
-  const double u = (double)a.u[r];
   u64 goal = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
   goal = min(goal, total - 1);
   if (tid < kRuns && goal >= before && goal < before + mine) {
