@@ -16,7 +16,7 @@
 // atomics) gives the step in which it falls, and the few candidates of that step are
 // ranked against one another in LDS. Steps with more candidates than fit (rows of equal
 // logits) are bisected instead. What is kept is gathered, weighed once more and summed by
-// 256 runs of indices; the one that holds the random number's place is ranked by index.
+// runs of 64 chunks of the row; the run that holds the random number's place is scanned.
 #include <algorithm>
 
 #include "sy_launch.hpp"
@@ -29,7 +29,7 @@ constexpr int kBlock = 1024;
 constexpr int kWaves = kBlock / 64;
 constexpr int kBins = 2048;
 constexpr int kRanked = kBlock;  // candidates that are ranked against one another
-constexpr int kRuns = 256;       // of a row's indices
+constexpr int kRuns = kBlock;    // of a row's indices, a wave's chunk each
 constexpr int kGroup = 4;        // chunks that are read from memory together
 constexpr double kOne = 17592186044416.0;  // 2^44
 
@@ -388,7 +388,7 @@ __device__ __forceinline__ Last find_cut(Shared& sh, R& row, const Weigher& wt, 
 
 template <class T, int HELD>  // bytes of LDS for the row
 __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
-  using Sh = Shared<HELD == 0 ? 16384 : 4096>;
+  using Sh = Shared<HELD == 0 ? 14336 : 4096>;
   __shared__ Sh sh;
   __shared__ __align__(16) char held[HELD ? HELD : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
@@ -458,46 +458,57 @@ __global__ void __launch_bounds__(kBlock) k_sample(const SampleArgs a) {
     else
       last = find_cut<false, false>(sh, row, wt, last, fmaxf(low, zero), 0, top_p);
   }
-  // The draw: what is kept, summed by runs of indices.
+  // The draw: what is kept, summed by runs of indices, which are a wave's chunk each.
+  constexpr int kLen = 64 * CE;
   __syncthreads();
-  if (tid < kRuns) sh.run[tid] = 0;
+  sh.run[tid] = 0;
   __syncthreads();
-  const int len = (a.vocab + kRuns - 1) / kRuns;
-  const auto weight = [&](float x) -> u64 {
+  const auto weight = [&](float x, int i) -> u64 {
+    if (x == -INFINITY || !last.keeps(x, i)) return 0;
     const double e = wt.e(x);
     return e >= min_p ? Weigher::units(e) : 0;
   };
-  row.each([&](float x, int i) {
-    if (x != -INFINITY && last.keeps(x, i)) atomicAdd(&sh.run[i / len], weight(x));
-  });
+  if (row.listed >= 0) {
+    for (int q = tid; q < row.listed; q += kBlock) {
+      const int i = sh.li[q];
+      atomicAdd(&sh.run[i / kLen], weight(sh.lx[q], i));
+    }
+  } else {
+    row.chunks([&](const float (&y)[CE], int at) {
+      u64 w = 0;
+#pragma unroll
+      for (int e = 0; e < CE; ++e) w += weight(y[e], at + e);
+      w = scan64(w);
+      if (lane == 63 && at < kRuns * kLen) sh.run[at / kLen] = w;
+    });
+  }
   __syncthreads();
-  const u64 mine = tid < kRuns ? sh.run[tid] : 0;
+  const u64 mine = sh.run[tid];
   const u64 incl = scan64(mine);
   if (lane == 63) sh.sums[wave] = incl;
   __syncthreads();
   u64 before = incl - mine, total = 0;
 #pragma unroll
-  for (int k = 0; k < kRuns / 64; ++k) {
+  for (int k = 0; k < kWaves; ++k) {
     const u64 s = sh.sums[k];
     before += k < wave ? s : 0;
     total += s;
   }
   u64 goal = u > 0.0 ? (u64)fmin(u * (double)total, 9.0e18) : 0;
   goal = min(goal, total - 1);
-  if (tid < kRuns && goal >= before && goal < before + mine) {
+  if (goal >= before && goal < before + mine) {
     sh.bin = tid;
     sh.before = before;
   }
   __syncthreads();
-  // The run that holds the goal: at most 1024 tokens, a thread each, in the order of indices.
-  const int i = sh.bin * len + tid;
+  // The run that holds the goal, a thread a token, in the order of indices.
+  const int i = sh.bin * kLen + tid;
   u64 w = 0;
-  if (tid < len && i < a.vocab) {
+  if (tid < kLen && i < a.vocab) {
     i32x4_t v = {0, 0, 0, 0};
     __builtin_memcpy(&v, row.p + i, sizeof(typename T::storage));
-    float x = elem<T>(v, 0);
-    x = x == x ? x + 0.0f : -INFINITY;
-    if (x != -INFINITY && last.keeps(x, i)) w = weight(x);
+    const float x = elem<T>(v, 0);
+    w = weight(x == x ? x + 0.0f : -INFINITY, i);
   }
   u64 in = scan64(w);
   if (lane == 63) sh.sums[wave] = in;
@@ -521,7 +532,7 @@ hipError_t sample_t(const SampleArgs& a, hipStream_t s) {
   const int64_t chunks = (a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce);
   const int64_t bytes = chunks * kBlock * 16;
   if (bytes <= 16384) return sample_n<T, 16384>(a, s);
-  if (bytes <= 98304) return sample_n<T, 98304>(a, s);
+  if (bytes <= 81920) return sample_n<T, 81920>(a, s);
   return sample_n<T, 0>(a, s);
 }
 
