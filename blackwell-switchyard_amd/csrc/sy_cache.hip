@@ -19,10 +19,11 @@ constexpr int kWaves = kBlock / 64;
 
 // ------------------------------------------------------------------ sequences
 
-// One sequence's rows of the packed tensors and its keys. The prefix pass takes every
-// row as one sequence over the prefix's keys.
+// One sequence's rows of the packed tensors, its length, and how many of its tokens the
+// cache can hold: later ones are not there. The prefix pass takes every row as one sequence
+// over the prefix's keys.
 struct Seq {
-  int row0, n, len;
+  int row0, n, len, keys;
 };
 
 __device__ __forceinline__ int clamp(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
@@ -36,7 +37,8 @@ __device__ __forceinline__ Seq seq_of(const CacheArgs& c, int b) {
     s.row0 = b * c.each;
     s.n = c.each;
   }
-  s.len = (int)clamp(c.lengths[b], 0, (int)c.cap);
+  s.len = clamp(c.lengths[b], 0, 1 << 30);
+  s.keys = min(s.len, (int)c.cap);
   return s;
 }
 
@@ -257,7 +259,7 @@ __device__ __forceinline__ Seq pass_seq(const CacheArgs& c, int pre, int prefix_
   Seq s;
   s.row0 = c.starts != nullptr ? clamp(c.starts[0], 0, c.n_tok) : 0;
   s.n = (c.starts != nullptr ? clamp(c.starts[c.n_seq], s.row0, c.n_tok) : c.n_tok) - s.row0;
-  s.len = prefix_len;
+  s.len = s.keys = prefix_len;
   return s;
 }
 
@@ -267,7 +269,7 @@ struct Tiles {
 __device__ __forceinline__ Tiles tiles_of(const Cut& u, int group, const Seq& s) {
   const int rows = s.n * group;
   if (rows == 0 || (!u.pre && rows > u.few)) return {0, 0};
-  const int k = (s.len + u.kt - 1) / u.kt;  // rows that see nothing still have to be written
+  const int k = (s.keys + u.kt - 1) / u.kt;  // rows that see nothing still have to be written
   return {(rows + u.rt - 1) / u.rt, k < 1 ? 1 : k};
 }
 
@@ -448,15 +450,15 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
       const int r0 = rtile * 16 * NT;
       const int past = u.pre ? plen : s.len - s.n + 1;  // keys the first token sees
       const int last = min(r0 + 16 * NT, rows) - 1;
-      const int least = u.pre ? plen : past + r0 / c.group;
-      const int most = u.pre ? plen : past + last / c.group;
+      const int least = u.pre ? plen : min(past + r0 / c.group, s.keys);
+      const int most = u.pre ? plen : min(past + last / c.group, s.keys);
       int limit[NT];
       i32x4_t q[NT][KC];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int r = min(r0 + 16 * n + col, last);  // rows past the last repeat it and are not stored
         const int t = r / c.group;
-        limit[n] = u.pre ? plen : past + t;
+        limit[n] = u.pre ? plen : min(past + t, s.keys);
         const S* const qp = static_cast<const S*>(a.q) + (s.row0 + t) * a.q_tok_stride +
                             (h * c.group + (r - t * c.group)) * a.q_head_stride;
 #pragma unroll
@@ -836,7 +838,7 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
   const int r0 = rtile * kFlashRows;
   const int last = min(r0 + kFlashRows, rows) - 1;
   const int past = f.pre ? plen : s.len - s.n + 1;  // keys the first token sees
-  const int most = f.pre ? plen : past + last / c.group;
+  const int most = f.pre ? plen : min(past + last / c.group, s.keys);
   const int pre_tiles = f.virt ? (plen + KT - 1) / KT : 0;
   const int tiles = pre_tiles + (most > 0 ? (most + KT - 1) / KT : 0);
   const int t0 = (int)((int64_t)tiles * split / f.splits), t1 = (int)((int64_t)tiles * (split + 1) / f.splits);
@@ -846,9 +848,9 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
   const bool active = w0 <= last;
   const int r = min(w0 + col, last);
   const int tok = r / c.group;
-  const int limit = f.pre ? plen : past + tok;
-  const int least = f.pre ? plen : past + w0 / c.group;
-  const int wmost = f.pre ? plen : past + min(w0 + 31, last) / c.group;
+  const int limit = f.pre ? plen : min(past + tok, s.keys);
+  const int least = f.pre ? plen : min(past + w0 / c.group, s.keys);
+  const int wmost = f.pre ? plen : min(past + min(w0 + 31, last) / c.group, s.keys);
   const int64_t out_row = (int64_t)(s.row0 + tok) * c.heads + h * c.group + (r - tok * c.group);
   i32x4_t q[KC];
   {
@@ -882,7 +884,7 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
   const S* const vb = static_cast<const S*>(c.v) + h * c.head_stride;
   const int32_t* const own_pages = f.pre ? a.prefix_pages : c.table + b * c.table_stride;
   const int own_last = f.pre ? (plen - 1) >> c.page_shift : (int)(c.cap >> c.page_shift) - 1;
-  const int wg_least = f.pre ? plen : past + r0 / c.group;
+  const int wg_least = f.pre ? plen : min(past + r0 / c.group, s.keys);
   const uint32_t kl_at = lds_byte(kl), vl_at = lds_byte(vl);
   int id[NP];
   const auto ask_ids = [&](int t) {

@@ -20,8 +20,7 @@ Not checked, as it would mean to wait for the device: ``starts`` out of order, a
 rows of the table with the same page, are the caller's mistakes (results are then those
 of some order). Pages outside the cache hold nothing: a token that would go there is not
 cached and its queries are NaN, and attention leaves its position out. The same goes for
-positions past the rotary tables or the table's row. A length past the table's row counts
-as its capacity. Rows that belong to no sequence are zero, or keep their content in a
+positions past the rotary tables or the table's row. Rows that belong to no sequence are zero, or keep their content in a
 given ``out``.
 
 There is no backward: under autograd the functions raise.

@@ -65,8 +65,10 @@ from torch import Tensor
 
 from . import _lib
 from .baselines import folded_form
+from .cache_op import paged_append, paged_attention
 from .hip_op import block_attn_res_hip
 from .reference import DEFAULT_EPS, BlockAttnRes
+from .sample_op import sample_tokens
 
 __all__ = [
     "ModelConfig",
@@ -75,6 +77,7 @@ __all__ = [
     "SOURCE_MODES",
     "source_count_schedule",
     "slab_copies",
+    "DecodeState",
 ]
 
 RESIDUAL_MODES = ("standard", "attnres", "switchyard")
@@ -239,6 +242,8 @@ class Attention(nn.Module):
         self.out = nn.Linear(cfg.d_model, cfg.d_model, bias=False)
 
     def forward(self, x: Tensor, rotary: Rotary) -> Tensor:
+        if isinstance(rotary, _CacheStep):
+            return rotary.attend(self, x)
         b, t, d = x.shape
         qkv = self.qkv(x).view(b, t, 3, self.heads, self.hd)
         split = None
@@ -286,6 +291,73 @@ class DecoderLayer(nn.Module):
     def sublayers(self):
         yield self.attn_norm, self.attn
         yield self.mlp_norm, self.mlp
+
+
+# --------------------------------------------------------------------------
+# Generation
+# --------------------------------------------------------------------------
+
+
+class DecodeState:
+    """The keys and values of ``batch`` sequences that a model is generating, every layer's
+    in pages of its own (``cache_op``), and how many tokens each sequence has.
+
+    ``max_len`` tokens a sequence, ``prefix_len`` more that all of them share (the prefix is
+    filled by ``Transformer.decode(..., to_prefix=True)``, before anything else)."""
+
+    def __init__(self, model: Transformer, batch: int, max_len: int, *, page: int = 64, prefix_len: int = 0) -> None:
+        cfg, w = model.cfg, model.embed.weight
+        if batch < 1 or max_len < 1 or prefix_len < 0:
+            raise ValueError(f"a state needs sequences of at least one token, got {batch} of {max_len} "
+                             f"behind {prefix_len}")
+        if prefix_len + max_len > cfg.max_seq_len:
+            raise ValueError(f"sequence length {prefix_len + max_len} exceeds max_seq_len {cfg.max_seq_len}")
+        if cfg.head_dim % 8 != 0 or cfg.head_dim > 256:
+            raise ValueError(f"generation needs heads of a multiple of 8 up to 256, got {cfg.head_dim}")
+        if not w.is_cuda:
+            raise ValueError("generation needs the model on a CUDA device")
+        dev, ints = w.device, dict(device=w.device, dtype=torch.int32)
+        self.batch, self.max_len, self.prefix_len = batch, max_len, prefix_len
+        shared, own = -(-prefix_len // page), -(-max_len // page)
+        shape = (cfg.n_layers, shared + batch * own, cfg.n_heads, page, cfg.head_dim)
+        self.k = torch.zeros(shape, device=dev, dtype=w.dtype)
+        self.v = torch.zeros(shape, device=dev, dtype=w.dtype)
+        self.prefix_pages = torch.arange(shared, **ints)
+        self.page_table = torch.arange(shared, shared + batch * own, **ints).view(batch, own)
+        self.lengths = torch.zeros(batch, **ints)
+        # The kernels take fp32 tables; a model cast as a whole has rounded ones, as its training has.
+        self.cos, self.sin = model.rotary.cos.float(), model.rotary.sin.float()
+        self._prefix_filled = prefix_len == 0
+
+    def reset(self) -> None:
+        """Forget the sequences' own tokens; the prefix stays."""
+        self.lengths.zero_()
+
+
+class _CacheStep:
+    """What the attention sublayers of one pass over new tokens are given in place of the
+    rotary: where their keys and values go, layer by layer."""
+
+    def __init__(self, state: DecodeState, starts: Tensor | None, to_prefix: bool) -> None:
+        self.state, self.starts, self.layer = state, starts, 0
+        if to_prefix:
+            self.table = state.prefix_pages[None]
+            self.lengths = torch.full((1,), state.prefix_len, device=state.k.device, dtype=torch.int32)
+            self.more, self.prefix_len = {}, 0
+        else:
+            self.table, self.lengths, self.prefix_len = state.page_table, state.lengths, state.prefix_len
+            self.more = {"prefix_pages": state.prefix_pages, "prefix_len": state.prefix_len} if state.prefix_len else {}
+
+    def attend(self, attn: Attention, x: Tensor) -> Tensor:
+        """``x [1, n_tok, D]``, the packed new tokens of all sequences."""
+        st, layer = self.state, self.layer
+        self.layer += 1
+        n_tok, d = x.shape[1:]
+        qkv = attn.qkv(x).view(n_tok, 3 * attn.heads, attn.hd)
+        q = paged_append(qkv, st.cos, st.sin, st.k[layer], st.v[layer], self.table, self.lengths, self.starts,
+                         prefix_len=self.prefix_len)
+        y = paged_attention(q, st.k[layer], st.v[layer], self.table, self.lengths, self.starts, **self.more)
+        return attn.out(y.view(1, n_tok, d))
 
 
 # --------------------------------------------------------------------------
@@ -534,21 +606,92 @@ class Transformer(nn.Module):
         weight per source in ``last_alphas`` (a diagnostic; it costs time)."""
         if idx.shape[1] > self.cfg.max_seq_len:
             raise ValueError(f"sequence length {idx.shape[1]} exceeds max_seq_len {self.cfg.max_seq_len}")
-        x = self.embed(idx)
         self.last_alphas = []
-        if self.cfg.uses_attnres:
-            h = self._attnres_stream(x, collect_alphas)
-        else:
-            for norm, fn in self._sublayers():
-                x = x + fn(norm(x), self.rotary)
-            self.last_source_counts = []
-            h = x
-        logits = self.lm_head(self.final_norm(h))
+        logits = self.lm_head(self.final_norm(self._stream(self.embed(idx), self.rotary, collect_alphas)))
         if targets is None:
             return logits
         return logits, F.cross_entropy(logits.float().flatten(0, 1), targets.flatten())
 
-    def _attnres_stream(self, x0: Tensor, collect_alphas: bool) -> Tensor:
+    def _stream(self, x: Tensor, rotary, collect_alphas: bool) -> Tensor:
+        if self.cfg.uses_attnres:
+            return self._attnres_stream(x, rotary, collect_alphas)
+        for norm, fn in self._sublayers():
+            x = x + fn(norm(x), rotary)
+        self.last_source_counts = []
+        return x
+
+    @torch.no_grad()
+    def decode(self, tokens: Tensor, state: DecodeState, starts: Tensor | None = None, *,
+               to_prefix: bool = False) -> Tensor:
+        """Append new tokens to a state's sequences and return the logits behind each
+        sequence's last one, ``[batch, V]``.
+
+        ``tokens`` is ``[batch, n]``, or ``[n_tok]`` with ``starts [batch + 1]`` (int32 on the
+        device) where sequences bring different numbers: sequence ``b`` has
+        ``starts[b] .. starts[b + 1]``, at least one each (the logits of one without tokens
+        mean nothing). With ``to_prefix`` the tokens ``[prefix_len]`` are the state's shared
+        prefix. Lengths are counted on the device and not checked against ``max_len``: what
+        does not fit is not cached, and its logits are NaN."""
+        if to_prefix:
+            if tokens.shape != (state.prefix_len,) or starts is not None or state.prefix_len == 0:
+                raise ValueError(f"the prefix must be [{state.prefix_len}] tokens, got {tuple(tokens.shape)}")
+        elif not state._prefix_filled:
+            raise ValueError("the state's prefix has to be filled first (to_prefix=True)")
+        elif starts is None:
+            if tokens.ndim != 2 or tokens.shape[0] != state.batch or tokens.shape[1] == 0:
+                raise ValueError(f"tokens must be [{state.batch}, n], got {tuple(tokens.shape)}")
+            state.lengths += tokens.shape[1]
+        else:
+            if tokens.ndim != 1 or tokens.numel() == 0 or starts.shape != (state.batch + 1,):
+                raise ValueError(f"tokens must be [n_tok] and starts [{state.batch + 1}], got "
+                                 f"{tuple(tokens.shape)} and {tuple(starts.shape)}")
+            state.lengths += starts.diff()
+        step = _CacheStep(state, starts, to_prefix)
+        h = self._stream(self.embed(tokens.reshape(1, -1)), step, False)[0]
+        if to_prefix:
+            state._prefix_filled = True
+            h = h[-1:]
+        elif starts is None:
+            h = h.view(state.batch, -1, h.shape[-1])[:, -1]
+        else:
+            h = h[(starts[1:] - 1).clamp(min=0).long()]
+        return self.lm_head(self.final_norm(h.contiguous()))
+
+    @torch.no_grad()
+    def generate(self, prompts, n_new: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 prefix: Tensor | None = None, u: Tensor | None = None, generator=None, page: int = 64) -> Tensor:
+        """``n_new`` tokens behind each prompt, ``[batch, n_new]`` (int64).
+
+        ``prompts`` is ``[batch, T]`` or a list of 1-D tensors of any lengths of at least one;
+        ``prefix`` a 1-D tensor of tokens that come before all of them, computed once. The
+        settings are those of ``sample_op.sample_tokens``; its uniform numbers are ``u
+        [n_new, batch]`` or drawn from ``generator``."""
+        rows = list(prompts)
+        if not rows or any(r.ndim != 1 or r.numel() == 0 for r in rows):
+            raise ValueError("prompts must be 1-D tensors of at least one token each")
+        if n_new < 1:
+            raise ValueError(f"n_new must be at least 1, got {n_new}")
+        dev, lens = self.embed.weight.device, [r.numel() for r in rows]
+        shared = 0 if prefix is None else prefix.numel()
+        state = DecodeState(self, len(rows), max(lens) + n_new - 1, page=page, prefix_len=shared)
+        if u is None:
+            u = torch.rand(n_new, len(rows), device=dev, generator=generator)
+        elif u.shape != (n_new, len(rows)):
+            raise ValueError(f"u must be [{n_new}, {len(rows)}], got {tuple(u.shape)}")
+        u = u.to(device=dev, dtype=torch.float32)
+        if shared:
+            self.decode(prefix.to(dev), state, to_prefix=True)
+        starts = torch.tensor([0, *lens], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
+        logits = self.decode(torch.cat([r.to(dev) for r in rows]), state, starts)
+        out = torch.empty(len(rows), n_new, device=dev, dtype=torch.int64)
+        for i in range(n_new):
+            tokens = sample_tokens(logits, u[i], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            out[:, i] = tokens
+            if i + 1 < n_new:
+                logits = self.decode(tokens[:, None], state)
+        return out
+
+    def _attnres_stream(self, x0: Tensor, rotary, collect_alphas: bool) -> Tensor:
         cfg = self.cfg
         with self._region("attnres_stage"):
             stream = _Stream(x0, cfg.n_blocks, arena=cfg.sources == "arena")
@@ -559,7 +702,7 @@ class Transformer(nn.Module):
                 stream.close_block()
             h = self._site(i, stream, collect_alphas, queries)
             counts.append(stream.count())
-            y = fn(norm(h), self.rotary)
+            y = fn(norm(h), rotary)
             stream.accumulate(y, lambda: self._region("attnres_stage"))
         stream.close_block()
         counts.append(stream.count())

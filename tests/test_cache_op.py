@@ -198,11 +198,36 @@ def test_bad_pages_and_lengths_hold_nothing():
         k, v = (c.rows(x, b, int(c.lengths[b]))[keep].transpose(0, 1) for x in (c.k, c.v))
         p = torch.softmax(c.q[b].double().view(2, 2, 64) @ k.transpose(1, 2) / 8, -1)
         assert ((p @ v).view(4, 64) - got[b].double()).abs().max() <= 2 * 2.0**-8 * 4
-    # a length past the table's row is its capacity
+    # a length past the table's row: all that the row holds is seen
     c.lengths = torch.tensor([1 << 30, 41], dtype=torch.int32)
     big = c.call().cpu()
     c.lengths = torch.tensor([64, 41], dtype=torch.int32)
     assert torch.equal(big, c.call().cpu()) and torch.equal(big[1], whole[1])
+
+
+@pytest.mark.parametrize("n", [3, 30])
+def test_tokens_past_the_capacity(n):
+    """The last new tokens have no room: they are not cached, and a row sees what is there."""
+    c = Case([n, n], [64 - n, 10], kv=2, group=2, hd=64, page=16, dtype=BF, seed=27)
+    cos, sin = _tables(128, 64)
+    qkv = torch.randn(2 * n, 8, 64, generator=_gen(28)).to(BF).to(DEV)
+    c.lengths[0] = 66  # two more than the row of the table holds
+    k, v = c.k.to(DEV), c.v.to(DEV)
+    q = paged_append(qkv, cos, sin, k, v, c.table.to(DEV), c.lengths.to(DEV))
+    lost = torch.zeros(2 * n, dtype=torch.bool)
+    lost[n - 2:n] = True
+    assert torch.equal(torch.isnan(q).any(-1).any(-1).cpu(), lost)
+    want = qkv[:n, 6:].cpu()
+    for i in range(n - 2):  # positions 66 - n + i
+        j = 66 - n + i
+        assert torch.equal(v[c.table[0, j // 16], :, j % 16].cpu(), want[i])
+    c.k, c.v, c.q = k.cpu(), v.cpu(), torch.nan_to_num(q).cpu()
+    got = c.call().cpu().double()
+    for i in range(n):
+        see = min(66 - n + i + 1, 64)
+        kk, vv = (c.rows(x, 0, 64)[:see].transpose(0, 1) for x in (c.k, c.v))
+        p = torch.softmax(c.q[i].double().view(2, 2, 64) @ kk.transpose(1, 2) / 8, -1)
+        assert ((p @ vv).view(4, 64) - got[i]).abs().max() <= 2 * 2.0**-8 * 4
 
 
 @pytest.mark.parametrize("op", ["attend", "prefix"])
