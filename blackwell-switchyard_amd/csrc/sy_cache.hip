@@ -564,7 +564,7 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
         if (t + kWaves < tiles) ask(kb, kx);
         ask_ids(t + 2 * kWaves);
         // softmax of the tile; a lane holds tokens 4 grp .. 4 grp + 3 of each 16
-        i32x4_t p16[NT];
+        i32x4_t p16[NT], p16r[NT];
         float pf[NT][MT * 4];
         bool any_new = false;
         float scale_o[NT];
@@ -602,9 +602,17 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
             sum += pf[n][e];
           }
           l[n] = fmaf(l[n], scale_o[n], sum);
-          // The weights are rounded to the values' dtype for the product (at most half a
-          // step each, independent of one another; the sum keeps them unrounded).
-          if constexpr (!kF32) p16[n] = pack<T>(pf[n]);
+          // The second product takes a weight as two numbers of the values' dtype, the
+          // rounded weight and what it lacks: rounded once the weights alone would put 0.7 of
+          // the output's own rounding on top of it (bf16 relative error 1.9e-3, so 1.7e-3),
+          // and this kernel waits for memory, not for products.
+          if constexpr (!kF32) {
+            p16[n] = pack<T>(pf[n]);
+            float rest[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rest[e] = pf[n][e] - elem<T>(p16[n], e);
+            p16r[n] = pack<T>(rest);
+          }
         }
         if (__any(any_new)) {
 #pragma unroll
@@ -638,7 +646,7 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
                 w[2 * x + 1] = r2[1];
               }
 #pragma unroll
-              for (int n = 0; n < NT; ++n) o[n][d] = Mma<T>::run(w, p16[n], o[n][d]);
+              for (int n = 0; n < NT; ++n) o[n][d] = Mma<T>::run(w, p16r[n], Mma<T>::run(w, p16[n], o[n][d]));
             }
           }
         } else {
@@ -1364,8 +1372,13 @@ __global__ void __launch_bounds__(kBlock) k_merge_flash(const AttendArgs a, cons
 
 // ----------------------------------------------------------------------- host
 
-// Tiles a wave at most of a segment that is not cut.
-constexpr int kShort = 4;
+// Tokens at most of a sequence that one workgroup reads whole, by the number of workgroups
+// that gives. One alone takes 8 us for 256 tokens, 12 for 512, 19 for 1024 and 33 for 2048;
+// shared out, 16 for any of them, 8 of which are the second launch. Many of them hide each
+// other's latency: 128 over 1024 tokens 19.4 us whole, 22 shared out, over 2048 33 and 31;
+// 1024 over 2048 tokens 183 and 190 (16 kv heads), 184 and 203 (8, of 32 heads).
+int whole_tokens(int64_t workgroups) { return workgroups >= 1024 ? 2048 : workgroups >= 128 ? 1024 : 512; }
+
 constexpr int64_t kMost = 0x7fffffff;
 
 // What a call launches: k_attend over the sequences of few rows, k_flash over the others,
@@ -1398,8 +1411,7 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int few, int nt, 
   else tiles = rows / u->rt + std::min<int64_t>(c.n_seq, rows);
   if (tiles > kMost / 2 / keys || tiles * keys > kMost / 2 / c.kv_heads) return false;
   u->rs = (int)std::min<int64_t>(u->rt, even ? (int64_t)c.each * c.group : rows);
-  // Whole segments where the longest takes a wave few tiles.
-  if (even && keys <= kShort * kWaves) {
+  if (even && keys * u->kt <= whole_tokens(tiles * c.kv_heads)) {
     u->least = 0;
     u->workers = (int)(tiles * c.kv_heads);
     return true;
