@@ -314,6 +314,8 @@ class DecodeState:
             raise ValueError(f"sequence length {prefix_len + max_len} exceeds max_seq_len {cfg.max_seq_len}")
         if cfg.head_dim % 8 != 0 or cfg.head_dim > 256:
             raise ValueError(f"generation needs heads of a multiple of 8 up to 256, got {cfg.head_dim}")
+        if page < 1 or page & (page - 1) != 0:
+            raise ValueError(f"a page must hold a power of two tokens, got {page}")
         if not w.is_cuda:
             raise ValueError("generation needs the model on a CUDA device")
         dev, ints = w.device, dict(device=w.device, dtype=torch.int32)
@@ -338,14 +340,12 @@ class _CacheStep:
     """What the attention sublayers of one pass over new tokens are given in place of the
     rotary: where their keys and values go, layer by layer."""
 
-    def __init__(self, state: DecodeState, starts: Tensor | None, to_prefix: bool) -> None:
-        self.state, self.starts, self.layer = state, starts, 0
+    def __init__(self, state: DecodeState, lengths: Tensor, starts: Tensor | None, to_prefix: bool) -> None:
+        self.state, self.lengths, self.starts, self.layer = state, lengths, starts, 0
         if to_prefix:
-            self.table = state.prefix_pages[None]
-            self.lengths = torch.full((1,), state.prefix_len, device=state.k.device, dtype=torch.int32)
-            self.more, self.prefix_len = {}, 0
+            self.table, self.more, self.prefix_len = state.prefix_pages[None], {}, 0
         else:
-            self.table, self.lengths, self.prefix_len = state.page_table, state.lengths, state.prefix_len
+            self.table, self.prefix_len = state.page_table, state.prefix_len
             self.more = {"prefix_pages": state.prefix_pages, "prefix_len": state.prefix_len} if state.prefix_len else {}
 
     def attend(self, attn: Attention, x: Tensor) -> Tensor:
@@ -635,27 +635,34 @@ class Transformer(nn.Module):
         if to_prefix:
             if tokens.shape != (state.prefix_len,) or starts is not None or state.prefix_len == 0:
                 raise ValueError(f"the prefix must be [{state.prefix_len}] tokens, got {tuple(tokens.shape)}")
+            lengths = torch.full((1,), state.prefix_len, device=state.k.device, dtype=torch.int32)
         elif not state._prefix_filled:
             raise ValueError("the state's prefix has to be filled first (to_prefix=True)")
         elif starts is None:
             if tokens.ndim != 2 or tokens.shape[0] != state.batch or tokens.shape[1] == 0:
                 raise ValueError(f"tokens must be [{state.batch}, n], got {tuple(tokens.shape)}")
-            state.lengths += tokens.shape[1]
+            lengths = state.lengths + tokens.shape[1]
         else:
             if tokens.ndim != 1 or tokens.numel() == 0 or starts.shape != (state.batch + 1,):
                 raise ValueError(f"tokens must be [n_tok] and starts [{state.batch + 1}], got "
                                  f"{tuple(tokens.shape)} and {tuple(starts.shape)}")
-            state.lengths += starts.diff()
-        step = _CacheStep(state, starts, to_prefix)
+            if starts.dtype != torch.int32 or starts.device != state.lengths.device:
+                raise ValueError(f"starts must be int32 on {state.lengths.device}")
+            lengths = state.lengths + starts.diff()
+        step = _CacheStep(state, lengths, starts, to_prefix)
         h = self._stream(self.embed(tokens.reshape(1, -1)), step, False)[0]
         if to_prefix:
-            state._prefix_filled = True
             h = h[-1:]
         elif starts is None:
             h = h.view(state.batch, -1, h.shape[-1])[:, -1]
         else:
-            h = h[(starts[1:] - 1).clamp(min=0).long()]
-        return self.lm_head(self.final_norm(h.contiguous()))
+            h = h[(starts[1:] - 1).clamp(0, h.shape[0] - 1).long()]
+        logits = self.lm_head(self.final_norm(h.contiguous()))
+        if to_prefix:
+            state._prefix_filled = True
+        else:
+            state.lengths.copy_(lengths)  # (a call that raised has added nothing)
+        return logits
 
     @torch.no_grad()
     def generate(self, prompts, n_new: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -665,7 +672,8 @@ class Transformer(nn.Module):
         ``prompts`` is ``[batch, T]`` or a list of 1-D tensors of any lengths of at least one;
         ``prefix`` a 1-D tensor of tokens that come before all of them, computed once. The
         settings are those of ``sample_op.sample_tokens``; its uniform numbers are ``u
-        [n_new, batch]`` or drawn from ``generator``."""
+        [n_new, batch]`` or drawn from ``generator``. Where a model's logits are all NaN the
+        tokens are -1 (and the model goes on from token 0)."""
         rows = list(prompts)
         if not rows or any(r.ndim != 1 or r.numel() == 0 for r in rows):
             raise ValueError("prompts must be 1-D tensors of at least one token each")
@@ -688,7 +696,7 @@ class Transformer(nn.Module):
             tokens = sample_tokens(logits, u[i], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
             out[:, i] = tokens
             if i + 1 < n_new:
-                logits = self.decode(tokens[:, None], state)
+                logits = self.decode(tokens.clamp(min=0)[:, None], state)
         return out
 
     def _attnres_stream(self, x0: Tensor, rotary, collect_alphas: bool) -> Tensor:

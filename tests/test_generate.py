@@ -151,6 +151,29 @@ def test_what_does_not_fit_is_nan():
     assert torch.isnan(m.decode(_tokens(2, 1).cuda(), state)).all()
 
 
+@gpu
+@needs
+def test_a_model_of_nan():
+    """Rows without a logit give -1, which is no token that the model could go on from."""
+    m = _model("standard")
+    with torch.no_grad():
+        m.lm_head.weight.fill_(float("nan"))
+    assert (m.generate(_tokens(2, 5), 3) == -1).all()
+    assert torch.isnan(m(_tokens(1, 4).cuda())).all()
+
+
+@gpu
+@needs
+def test_starts_past_the_tokens():
+    """The logits of a sequence that ends past the tokens are some row's, not a read behind them."""
+    m = _model("standard")
+    state = DecodeState(m, 2, 16, page=16)
+    starts = torch.tensor([0, 3, 90], dtype=torch.int32, device="cuda")
+    idx = _tokens(8).cuda()
+    got = m.decode(idx, state, starts)
+    _close(got[:1], m(idx[None, :3])[:, -1])
+
+
 def test_refusals():
     m = _model(dev="cpu")
     with pytest.raises(ValueError, match="CUDA"):
@@ -159,6 +182,8 @@ def test_refusals():
         DecodeState(m, 2, 100, prefix_len=29)
     with pytest.raises(ValueError, match="at least one token"):
         DecodeState(m, 0, 16)
+    with pytest.raises(ValueError, match="power of two"):
+        DecodeState(m, 2, 16, page=24)
     with pytest.raises(ValueError, match="multiple of 8"):
         DecodeState(_model(dev="cpu", d_model=120, n_heads=10), 2, 16)
     with pytest.raises(ValueError, match="at least one token"):
@@ -181,3 +206,9 @@ def test_refusals_of_a_state():
         m.decode(_tokens(3).cuda(), state, torch.zeros(2, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError, match=r"u must be"):
         m.generate(_tokens(2, 4), 3, u=torch.zeros(2, 2))
+    before = state.lengths.tolist()
+    with pytest.raises(ValueError, match="int32"):
+        m.decode(_tokens(3).cuda(), state, torch.tensor([0, 1, 3], device="cuda"))
+    with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(ValueError, match="same dtype"):
+        m.decode(_tokens(2, 3).cuda(), state)
+    assert state.lengths.tolist() == before  # a refused call adds nothing
