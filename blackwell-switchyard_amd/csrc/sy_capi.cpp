@@ -1100,8 +1100,9 @@ static int cache_args(const sy_paged* c, CacheArgs* out) {
   int shift = 0;
   while ((1 << shift) < c->page) ++shift;
   *out = CacheArgs{c->k, c->v, c->table, c->lengths, c->starts, c->head_stride, c->table_stride,
-                   (uint32_t)(c->page_stride * esize(c->dtype)), (uint32_t)(c->row_stride * esize(c->dtype)), (int)c->n_seq, (int)c->n_tok, (int)(c->n_tok / c->n_seq), (int)c->n_pages,
-                   shift, c->heads, c->kv_heads, c->heads / c->kv_heads, c->hd, c->table_cols << shift};
+                   (uint32_t)(c->page_stride * esize(c->dtype)), (uint32_t)(c->row_stride * esize(c->dtype)),
+                   (int)c->n_seq, (int)c->n_tok, (int)(c->n_tok / c->n_seq), (int)c->n_pages, shift, c->heads,
+                   c->kv_heads, c->heads / c->kv_heads, c->hd, c->table_cols << shift};
   return SY_OK;
 }
 
@@ -1220,7 +1221,7 @@ const char* sy_strerror(int code) {
     case SY_ERR_SHAPE: return "switchyard: a size is out of range";
     case SY_ERR_DTYPE: return "switchyard: unsupported dtype";
     case SY_ERR_WORKSPACE: return "switchyard: backward workspace missing or too small";
-    case SY_ERR_STRIDE: return "switchyard: source stride smaller than n_tok * D";
+    case SY_ERR_STRIDE: return "switchyard: source stride smaller than n_tok * D, or a stride out of range";
     case SY_ERR_DEVICE: return "switchyard: no usable HIP device";
     case SY_ERR_OP: return "switchyard: unknown operation";
     default: break;

@@ -11,12 +11,18 @@
 // A workgroup of 16 waves per row, which is read from memory once into LDS (rows that do
 // not fit are read again, from L2); a wave owns a contiguous run of it. The passes over the
 // row are short loops: unrolled over registers they were bound by fetching their own code,
-// which each workgroup runs once (8 rows of 32000 bf16 72 us, 256 of 50257 fp32 230). A cut is found without
-// sorting: a histogram over 2048 equal steps of the logits' range (counts or weights, LDS
-// atomics) gives the step in which it falls, and the few candidates of that step are
-// ranked against one another in LDS. Steps with more candidates than fit (rows of equal
-// logits) are bisected instead. What is kept is gathered, weighed once more and summed by
-// runs of 64 chunks of the row; the run that holds the random number's place is scanned.
+// which each workgroup runs once. A cut is found without sorting: a histogram over 2048
+// equal steps of the logits' range (counts or weights, LDS atomics) gives the step in which
+// it falls, and the few candidates of that step are ranked against one another in LDS.
+// Steps with more candidates than fit (rows of equal logits) are bisected instead. What is
+// kept is gathered, weighed once more and summed by runs of 64 chunks of the row; the run
+// that holds the random number's place is scanned.
+//
+// 8 rows of 32000 bf16 with top-k and top-p take 17.7 us (72 with the rows in registers):
+// one workgroup a CU, bound by the latency of its passes one after another. 256 rows of
+// 50257 fp32 with top-p take 82 us (230): the row's 201 KB are read four times from the
+// last cache, and of a workgroup's time 42 % go into the histogram with its double exp, 19 %
+// into gathering, 14 % into the maximum, 8 % into the ranking and 12 % into the draw.
 #include <algorithm>
 
 #include "sy_launch.hpp"
@@ -111,7 +117,7 @@ struct Shared {
   u64 sums[kWaves];
   float tops[kWaves], lows[kWaves];
   int n, bin, rank, tok, listed;
-  u64 before, total;
+  u64 before;
   Last last;
 };
 

@@ -16,12 +16,12 @@ Sequences that continue one prompt share its pages: ``prefix_len`` tokens in the
 that ``prefix_pages`` lists come before every sequence's own tokens. Where every sequence
 brings few rows, attention reads the prefix once for all of them.
 
-Not checked, as it would mean to wait for the device: ``starts`` out of order, and two
-rows of the table with the same page, are the caller's mistakes (results are then those
-of some order). Pages outside the cache hold nothing: a token that would go there is not
+Not checked, as it would mean to wait for the device: ``starts`` out of order (results
+are then undefined), and two new tokens whose places are the same one (which of them is
+kept is). Pages outside the cache hold nothing: a token that would go there is not
 cached and its queries are NaN, and attention leaves its position out. The same goes for
-positions past the rotary tables or the table's row. Rows that belong to no sequence are zero, or keep their content in a
-given ``out``.
+positions past the rotary tables or the table's row. Rows that belong to no sequence are
+zero, or keep their content in a given ``out``, which may be the queries themselves.
 
 There is no backward: under autograd the functions raise.
 """
@@ -85,6 +85,10 @@ def _validate_out(out, like, shape) -> None:
           and out.data_ptr() % 16 == 0, f"out must be a dense {list(shape)} tensor of the inputs' dtype and device")
 
 
+def _given(*tensors) -> list:
+    return [t for t in tensors if t is not None]
+
+
 def _no_backward(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward; run it under torch.no_grad() for inference")
@@ -101,7 +105,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
     ``cos``, ``sin`` are fp32 ``[positions, head_dim / 2]`` (``[positions, 1, ...]`` as
     the decoder's). Row ``i`` of ``n`` new ones stands at ``lengths[b] - n + i``, behind
     ``prefix_len``. Arithmetic is fp32, every output rounded once."""
-    if _lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths) and (
+    if _lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths, *_given(starts, out)) and (
             qkv.is_cuda and type(prefix_len) is int):
         q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out)
         if q is not None:
@@ -139,8 +143,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     each row sees its own position and every earlier one, and the whole prefix. Query head
     ``h`` reads kv head ``h * kv_heads // heads``; ``scale`` is ``head_dim**-0.5`` by
     default. A row that sees nothing is zero. Scores, softmax statistics and sums are
-    fp32; 16-bit caches have the weights rounded to their dtype for the second product."""
-    if _lib.ordinary(q, k_cache, v_cache, page_table, lengths) and q.is_cuda and type(prefix_len) is int:
+    fp32. Where a sequence brings more than 16 rows a kv head to a 16-bit cache, or the rows
+    that share a prefix are more than 16, the weights are rounded to its dtype for the second
+    product (relative error 2.0e-3 in bf16, of which the output's own rounding is 1.7e-3);
+    where there are fewer they are not."""
+    if _lib.ordinary(q, k_cache, v_cache, page_table, lengths, *_given(starts, prefix_pages, out)) and (
+            q.is_cuda and type(prefix_len) is int):
         o = _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, starts, prefix_pages, prefix_len,
                                           q.shape[-1] ** -0.5 if scale is None else scale, out)
         if o is not None:

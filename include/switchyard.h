@@ -363,8 +363,8 @@ int sy_swiglu_bwd(const void* gate_up, const void* grad_out, void* dgate_up, int
  * The cache of one layer holds keys and values in pages of `page` tokens (a power of
  * two): row `slot` of kv head h of page p starts at k + p page_stride + h head_stride +
  * slot row_stride elements, v likewise; rows are hd elements, dense, and start at
- * 16-byte boundaries; page_stride and page row_stride are below 2^32 bytes. Token j of sequence b lies in slot j % page of page
- * table[b table_stride + j / page].
+ * 16-byte boundaries; page_stride and page row_stride are below 2^32 bytes. Token j of
+ * sequence b lies in slot j % page of page table[b table_stride + j / page].
  *
  * A call brings new tokens of n_seq sequences, packed: sequence b has rows starts[b] to
  * starts[b + 1] (non-decreasing, 0 <= starts <= n_tok; NULL: n_tok / n_seq rows each,

@@ -244,6 +244,19 @@ def test_rows_behind_the_last_sequence(op):
     assert torch.equal(out[1:6], got[1:6]) and (out[0] == 3).all() and (out[6:] == 3).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("prefix", [0, 40])
+@pytest.mark.parametrize("new", [[1] * 3, [5] * 70, [70, 3, 1], [200, 130, 1]])
+def test_the_queries_as_out(new, prefix, dtype):
+    past = [(900, 33, 0, 5)[i % 4] for i in range(len(new))]
+    c = Case(new, past, kv=2, group=2, hd=64, page=16, dtype=dtype, prefix=prefix, seed=9)
+    q = c.q.to(DEV)
+    got = c.call(q=q, out=q)
+    assert got is q
+    assert torch.equal(got, c.call())
+    c.check(got=got)
+
+
 def test_strides_and_orders_of_the_caches_and_queries():
     c = Case([1, 4], [50, 9], kv=2, group=2, hd=64, page=16, dtype=HF, seed=8)
     want = c.call()
