@@ -1170,7 +1170,8 @@ k_both(const AttendArgs a, const Cut u, const Flash f, const int direct_u, const
 // prefix with a sequence's own: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. A
 // workgroup takes some heads of one token; hd / 4 threads read a partial result, so many
 // results are read at once, and every thread's sum runs in the order of the keys. Rows
-// that one workgroup finished are left alone.
+// that one workgroup finished are left alone. Bound by latency: lengths, statistics and
+// the first results are three loads one after another. MERGE_FIGURES
 struct Parts {  // `count` results, number k at row at + k step (+ second at k = 0); one: the row's own
   int count;
   int64_t at, step, second;
@@ -1221,21 +1222,22 @@ struct JoinArgs {
   int has_pre;  // 0, 1: k_attend's, 2: k_flash's
   int per_wg;   // heads a workgroup
   int few;      // tokens a sequence to look at, where only k_attend's rows are left; else 0
+  int many;     // workgroups for k_flash's cut rows, where there is no prefix to join
   float *row_o, *row_ml, *pre_o, *pre_ml;
 };
 
 template <class T>
-__global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const JoinArgs g) {
+__device__ __forceinline__ void merge(const AttendArgs& a, const JoinArgs& g, const int block) {
   using S = typename T::storage;
   const CacheArgs& c = a.c;
-  __shared__ float weight[2 * kMostParts];
+  __shared__ float weight[2 * kMostParts], mass[2 * kMostParts];
   __shared__ f32x4_t fold[kBlock];
   __shared__ float tops[kWaves], sums[kWaves];
   const int tid = threadIdx.x;
   const int plen = (int)a.prefix_len;
   const int slices = (c.heads + g.per_wg - 1) / g.per_wg;
-  int tok = blockIdx.x / slices, b;
-  const int slice = blockIdx.x - tok * slices;
+  int tok = block / slices, b;
+  const int slice = block - tok * slices;
   Seq s;
   if (g.few != 0) {
     b = tok / g.few;
@@ -1281,11 +1283,19 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
       const int k = f ? i : i - front.count;
       return (f ? front.at : mine.at) + k * (f ? front.step : mine.step) + (k == 0 ? (f ? front.second : mine.second) : 0);
     };
+    // The first result is on its way while its weight is worked out.
+    const auto part = [&](int i) {
+      return *reinterpret_cast<const f32x4_t*>((i < front.count ? fo : mo) + at(i) * c.hd + ch);
+    };
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool mine_too = grp < groups && grp < n;
+    if (mine_too) o = part(grp);
     float m = -INFINITY;
     for (int i = tid; i < n; i += kBlock) {
-      const float x = (i < front.count ? fm : mm)[at(i) * 2];
-      weight[i] = x;
-      m = fmaxf(m, x);
+      const float* const x = (i < front.count ? fm : mm) + at(i) * 2;
+      weight[i] = x[0];
+      mass[i] = x[1];
+      m = fmaxf(m, x[0]);
     }
 #pragma unroll
     for (int k = 32; k >= 1; k /= 2) m = fmaxf(m, __shfl_xor(m, k));
@@ -1296,7 +1306,7 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
     const float mu = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f;
     for (int i = tid; i < n; i += kBlock) {
-      const float l = (i < front.count ? fm : mm)[at(i) * 2 + 1];
+      const float l = mass[i];
       // NaN scores leave no maximum, but the row is not an empty one.
       const float w = l != l ? 1.0f : __builtin_amdgcn_exp2f(weight[i] - mu);
       weight[i] = w;
@@ -1309,11 +1319,10 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
     sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += sums[w];
-    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (grp < groups) {
+    if (mine_too) {
+      o *= weight[grp];
 #pragma unroll 4
-      for (int i = grp; i < n; i += groups)
-        o += weight[i] * *reinterpret_cast<const f32x4_t*>((i < front.count ? fo : mo) + at(i) * c.hd + ch);
+      for (int i = grp + groups; i < n; i += groups) o += weight[i] * part(i);
     }
     fold[tid] = o;
     __syncthreads();
@@ -1329,14 +1338,18 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
   }
 }
 
-// The same for k_flash's cut rows where there is no prefix to join: a workgroup takes the 128
+// The same for k_flash's cut rows where there is no prefix to join: a workgroup takes 32
 // rows of a tile and kv head, hd / 4 threads one row's few results, without LDS or barriers.
-// Bound by reading the partial results once.
+// Bound by reading the partial results once, with enough workgroups to hide that the
+// statistics come first (all 128 rows of a tile in one: 27 us where this takes FLASH_MERGE).
+constexpr int kMergeRows = 32;
 template <class T>
-__global__ void __launch_bounds__(kBlock) k_merge_flash(const AttendArgs a, const Flash f) {
+__device__ __forceinline__ void merge_flash(const AttendArgs& a, const Flash& f, const int block) {
   using S = typename T::storage;
   const CacheArgs& c = a.c;
-  const int h = blockIdx.x % c.kv_heads, tile = blockIdx.x / c.kv_heads;
+  constexpr int kParts = kFlashRows / kMergeRows;
+  const int i0 = block % kParts * kMergeRows, rest = block / kParts;
+  const int h = rest % c.kv_heads, tile = rest / c.kv_heads;
   int b, base;
   if (!locate(c.n_seq, tile, [&](int x) { return flash_tiles(c, f, 0, x); }, &b, &base)) return;
   const Seq s = seq_of(c, b);
@@ -1346,7 +1359,7 @@ __global__ void __launch_bounds__(kBlock) k_merge_flash(const AttendArgs a, cons
   const int lpr = c.hd / 4, groups = kBlock / lpr;
   const int grp = threadIdx.x / lpr, ch = (threadIdx.x - grp * lpr) * 4;
   if (grp >= groups) return;
-  for (int i = grp; i < rows; i += groups) {
+  for (int i = i0 + grp; i < min(rows, i0 + kMergeRows); i += groups) {
     const float* const ml = f.ml + (slot + i) * 2;
     float m = -INFINITY;
     for (int k = 0; k < f.splits; ++k) m = fmaxf(m, ml[k * (2 * kFlashRows)]);
@@ -1370,14 +1383,24 @@ __global__ void __launch_bounds__(kBlock) k_merge_flash(const AttendArgs a, cons
   }
 }
 
+template <class T>
+__global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const JoinArgs g) {
+  if ((int)blockIdx.x < g.many) merge_flash<T>(a, g.fown, blockIdx.x);
+  else merge<T>(a, g, (int)blockIdx.x - g.many);
+}
+
 // ----------------------------------------------------------------------- host
 
 // Tokens at most of a sequence that one workgroup reads whole, by the number of workgroups
 // that gives. One alone takes 8 us for 256 tokens, 12 for 512, 19 for 1024 and 33 for 2048;
 // shared out, 16 for any of them, 8 of which are the second launch. Many of them hide each
 // other's latency: 128 over 1024 tokens 19.4 us whole, 22 shared out, over 2048 33 and 31;
-// 1024 over 2048 tokens 183 and 190 (16 kv heads), 184 and 203 (8, of 32 heads).
-int whole_tokens(int64_t workgroups) { return workgroups >= 1024 ? 2048 : workgroups >= 128 ? 1024 : 512; }
+// 1024 over 2048 tokens 183 and 190 (16 kv heads), 184 and 203 (8, of 32 heads). Next to a
+// prefix's pass they start behind it, and what starts last must not be long: 128 over 1024
+// tokens behind 30011 shared ones 57.8 us whole, PREFIX_FIGURE shared out.
+int whole_tokens(int64_t workgroups, bool beside) {
+  return beside ? 512 : workgroups >= 1024 ? 2048 : workgroups >= 128 ? 1024 : 512;
+}
 
 constexpr int64_t kMost = 0x7fffffff;
 
@@ -1396,7 +1419,7 @@ struct Plan {
   int64_t row_o, row_ml, pre_o, pre_ml;  // float offsets, as the o and ml of the passes
 };
 
-bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int few, int nt, int cus, Cut* u) {
+bool cut(const CacheArgs& c, int dtype, bool pre, bool beside, int64_t len, int few, int nt, int cus, Cut* u) {
   u->pre = pre;
   u->few = few;
   u->kt = dtype == SY_F32 ? 16 : 32;
@@ -1411,7 +1434,7 @@ bool cut(const CacheArgs& c, int dtype, bool pre, int64_t len, int few, int nt, 
   else tiles = rows / u->rt + std::min<int64_t>(c.n_seq, rows);
   if (tiles > kMost / 2 / keys || tiles * keys > kMost / 2 / c.kv_heads) return false;
   u->rs = (int)std::min<int64_t>(u->rt, even ? (int64_t)c.each * c.group : rows);
-  if (even && keys * u->kt <= whole_tokens(tiles * c.kv_heads)) {
+  if (even && keys * u->kt <= whole_tokens(tiles * c.kv_heads, beside)) {
     u->least = 0;
     u->workers = (int)(tiles * c.kv_heads);
     return true;
@@ -1456,7 +1479,7 @@ bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int 
     }
   }
   f->fold = cus / (c.kv_heads * f->splits);
-  return grid * f->splits <= kMost / kFlashRows;
+  return grid * f->splits <= kMost / kFlashRows;  // (of rows, and so of the merge's workgroups)
 }
 
 Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
@@ -1471,8 +1494,8 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
     const int nt = avg <= 16 ? 1 : c.hd > 128 ? 1 : 2;
     p.attend = true;
     p.pre = prefix_len > 0 ? 1 : 0;
-    p.ok = cut(c, dtype, false, c.cap, (int)kMost, nt, cus, &p.own);
-    if (p.ok && p.pre) p.ok = cut(c, dtype, true, prefix_len, (int)kMost, rows <= 16 || c.hd > 128 ? 1 : 2, cus, &p.cpre);
+    p.ok = cut(c, dtype, false, false, c.cap, (int)kMost, nt, cus, &p.own);
+    if (p.ok && p.pre) p.ok = cut(c, dtype, true, false, prefix_len, (int)kMost, rows <= 16 || c.hd > 128 ? 1 : 2, cus, &p.cpre);
   } else {
     // Up to 16 rows are k_attend's. A prefix has a pass of its own where sequences bring
     // few rows, so that it is read once for all; else its keys are part of every
@@ -1483,10 +1506,10 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
     p.attend = !virt && (c.starts != nullptr || avg <= 16);
     p.flash = c.starts != nullptr ? rows > few : avg > few;
     p.own.few = few;
-    if (p.attend) p.ok = cut(c, dtype, false, c.cap, few, 1, cus, &p.own);
+    if (p.attend) p.ok = cut(c, dtype, false, shared && rows > 16, c.cap, few, 1, cus, &p.own);
     if (p.ok && p.flash) p.ok = flash_cut(c, false, virt, prefix_len, few, cus, &p.fown);
     p.pre = !shared ? 0 : rows <= 16 ? 1 : 2;
-    if (p.ok && p.pre == 1) p.ok = cut(c, dtype, true, prefix_len, (int)kMost, 1, cus, &p.cpre);
+    if (p.ok && p.pre == 1) p.ok = cut(c, dtype, true, false, prefix_len, (int)kMost, 1, cus, &p.cpre);
     if (p.ok && p.pre == 2) p.ok = flash_cut(c, true, false, prefix_len, 0, cus, &p.fpre);
   }
   if (!p.ok) return p;
@@ -1624,18 +1647,15 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   if (e == hipSuccess && flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero && !p.attend, own, s);
   if (e == hipSuccess && attend) e = attend_pass<T>(a, p.own, p.direct_attend, zero, own, s);
   if (e != hipSuccess) return e;
-  if (p.merge_flash) {
-    hipLaunchKernelGGL((k_merge_flash<T>), dim3((unsigned)(p.fown.tiles * a.c.kv_heads)), dim3(kBlock), 0, s, a,
-                       p.fown);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-  }
-  if (!p.merge) return e;
-  JoinArgs g{p.own, p.cpre, p.fown, p.fpre, p.pre, 1, p.merge_few, own.o, own.ml, pre.o, pre.ml};
+  if (!p.merge && !p.merge_flash) return e;
+  const int many = p.merge_flash ? p.fown.tiles * a.c.kv_heads * (kFlashRows / kMergeRows) : 0;
+  JoinArgs g{p.own, p.cpre, p.fown, p.fpre, p.pre, 1, p.merge_few, many, own.o, own.ml, pre.o, pre.ml};
   // Heads a workgroup: one, until there are far more rows than fit the device at once.
   const int64_t toks = p.merge_few ? (int64_t)a.c.n_seq * p.merge_few : a.c.n_tok;
   g.per_wg = (int)std::min<int64_t>(a.c.heads, std::max<int64_t>(1, toks * a.c.heads / 8192));
-  const int64_t grid = toks * ((a.c.heads + g.per_wg - 1) / g.per_wg);
-  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)grid), dim3(kBlock), 0, s, a, g);
+  const int64_t grid = p.merge ? toks * ((a.c.heads + g.per_wg - 1) / g.per_wg) : 0;
+  if (grid > kMost - many) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)(many + grid)), dim3(kBlock), 0, s, a, g);
   return hipGetLastError();
 }
 
