@@ -72,9 +72,10 @@ template <class S> __device__ __forceinline__ S* bytes_on(S* p, uint64_t n) {
 // --------------------------------------------------------------------- append
 //
 // A workgroup per token, a thread per two chunks of VE elements that turn together
-// (channel i of a head's first half with channel i of its second). Bound by memory:
-// every byte is read once and written once. The projection's chunks and the tables' are
-// asked for before the token's sequence is looked up.
+// (channel i of a head's first half with channel i of its second). Every byte is read once
+// and written once. Prompts are bound by memory: 5754 tokens of 16 heads of 128 in bf16, 144
+// MB, take 31 us at 4.7 TB/s; a large copy runs at 5.2. One token each of 8 sequences is bound
+// by latency: starts or lengths, the table's entry and the row, 4 us of the 6.6 a call takes.
 template <class T, int VE>
 struct Chunk {
   float f[VE];
@@ -198,7 +199,11 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
 // lengths are: a long sequence is shared by many workgroups, short ones lie many in one.
 // The four waves of a workgroup take the tiles of a segment in turn, each with its own
 // registers and LDS and no barrier between tiles, and join their results through LDS at
-// the segment's end. A run begins and ends inside at most one segment each, so two
+// the segment's end. Bound by memory: 32 sequences of any lengths up to 4096, 16 heads of
+// 128 in bf16, read 567 MB in 111 us with the merge (5.1 TB/s; 5.9 where nothing is merged;
+// a plain read of as much runs at 6.5), two of 131000 tokens and 4 kv heads 469 MB in 94.
+// Single tokens over a few hundred are bound by latency: lengths, page ids, keys and the
+// fold through LDS one after another, 10 us. A run begins and ends inside at most one segment each, so two
 // partial results (o, m, l) a workgroup are enough; k_merge joins them. Nothing here
 // depends on lengths the host knows. Where no sequence can be longer than a few tiles a
 // wave, a workgroup takes one whole segment instead, and nothing is left to merge.
@@ -758,15 +763,16 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
 // query rows of a kv head, a wave 32 of them, and all four waves read the same tiles of 64
 // keys and values from LDS. Tile t + 1 is on its way from memory to the other half of LDS
 // while tile t is multiplied, without passing through registers; one barrier a tile. The
-// products run on v_mfma_f32_32x32x16 in the same transposed form; 32 rows a wave take
-// 32 KB of LDS reads for 2^20 products a tile, which LDS delivers in half the time of the
-// products. The maximum is only followed when a score passes it by more than 2^8 (weights
+// products run on v_mfma_f32_32x32x16 in the same transposed form. The maximum is only followed when a score passes it by more than 2^8 (weights
 // stay below 256, and the ratio to their sum is what counts), so the results are hardly
 // ever rescaled.
 //
 // Bound by the matrix cores and, next to them, by the exponentials (a quarter of the
-// vector rate): each wave's tile is 1024 cycles of products and about as many of softmax,
-// which two waves a SIMD overlap.
+// vector rate): a wave's tile of heads of 128 is 1024 cycles of products and about as many of
+// softmax, which two waves a SIMD overlap. Long even sequences run at 760 TFLOP/s (heads of
+// 128, 16 of each kind), 930 (32 that share 8), 745 (heads of 64) and 480 (256, one workgroup
+// a CU); four prompts of up to 2048 tokens at 530, as the causal triangles' ends leave CUs
+// idle. A large bf16 product of the library runs at 1070.
 struct Flash {
   int pre;     // 1: every row over the prefix's keys
   int virt;    // 1: the prefix's tiles come before each sequence's own
@@ -1171,7 +1177,8 @@ k_both(const AttendArgs a, const Cut u, const Flash f, const int direct_u, const
 // workgroup takes some heads of one token; hd / 4 threads read a partial result, so many
 // results are read at once, and every thread's sum runs in the order of the keys. Rows
 // that one workgroup finished are left alone. Bound by latency: lengths, statistics and
-// the first results are three loads one after another. MERGE_FIGURES
+// the first results are loads one after another (32 tokens of 16 heads, one to three results
+// each, 6.4 us, of 7.3 with the sums and results asked for one by one).
 struct Parts {  // `count` results, number k at row at + k step (+ second at k = 0); one: the row's own
   int count;
   int64_t at, step, second;
@@ -1341,7 +1348,8 @@ __device__ __forceinline__ void merge(const AttendArgs& a, const JoinArgs& g, co
 // The same for k_flash's cut rows where there is no prefix to join: a workgroup takes 32
 // rows of a tile and kv head, hd / 4 threads one row's few results, without LDS or barriers.
 // Bound by reading the partial results once, with enough workgroups to hide that the
-// statistics come first (all 128 rows of a tile in one: 27 us where this takes FLASH_MERGE).
+// statistics come first (64 tiles of 8 kv heads, all 128 rows in one workgroup and the few
+// rows' merge in a launch of its own: 36 us; together in this one 18).
 constexpr int kMergeRows = 32;
 template <class T>
 __device__ __forceinline__ void merge_flash(const AttendArgs& a, const Flash& f, const int block) {
@@ -1397,7 +1405,7 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
 // other's latency: 128 over 1024 tokens 19.4 us whole, 22 shared out, over 2048 33 and 31;
 // 1024 over 2048 tokens 183 and 190 (16 kv heads), 184 and 203 (8, of 32 heads). Next to a
 // prefix's pass they start behind it, and what starts last must not be long: 128 over 1024
-// tokens behind 30011 shared ones 57.8 us whole, PREFIX_FIGURE shared out.
+// tokens behind 30011 shared ones 57.8 us whole, 52.0 shared out.
 int whole_tokens(int64_t workgroups, bool beside) {
   return beside ? 512 : workgroups >= 1024 ? 2048 : workgroups >= 128 ? 1024 : 512;
 }
