@@ -808,9 +808,10 @@ template <class T> __device__ __forceinline__ f32x16_t mma32(const i32x4_t& a, c
 // done when vmcnt says so. (The builtin's loads are waited for before the next read of any
 // LDS, the other buffer included. There is no output register that could be reused while
 // the load is under way. The compiler does not count these loads: a wait of its own for an
-// earlier load would wait for them too, so there must be none behind them.)
+// earlier load would wait for them too, so there must be none behind them. m0 is a reserved
+// register, set where it is used: the compiler keeps nothing in it.)
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t lds_byte(void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p;
@@ -1459,6 +1460,9 @@ bool cut(const CacheArgs& c, int dtype, bool pre, bool beside, int64_t len, int 
 // of 128, 0.72 of 64, 3.2 of 256), a workgroup alone no faster than 1.2 us a tile; the last
 // workgroups leave CUs idle for part of their time; cut rows are written, read and joined.
 // Prompts see half of their own tokens on average, and sequences are rarely of one length.
+// A prefix's parts are all as long, and the sequences' own keys fill what they leave idle:
+// there the CU with the most of them counts (30011 tokens behind 8 kv heads: 32 parts, one a
+// CU, 47.6 us; 48, two on half of the CUs, 52.1).
 bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int few, int cus, Flash* f) {
   f->pre = pre;
   f->virt = virt;
@@ -1471,7 +1475,7 @@ bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int 
   const int64_t grid = (int64_t)f->tiles * c.kv_heads;
   const int64_t keys = (pre ? prefix_len : c.cap + (virt ? prefix_len : 0));
   const double longest = (double)keys / kFlashKeys;
-  const double mean = pre ? longest : 0.8 * std::max(longest / 2, longest - 0.5 * c.n_tok / c.n_seq / kFlashKeys);
+  const double mean = 0.8 * std::max(longest / 2, longest - 0.5 * c.n_tok / c.n_seq / kFlashKeys);
   const int places = c.hd <= 64 ? 3 : c.hd <= 128 ? 2 : 1;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, keys / (2 * kFlashKeys)));
   const double tile_us = c.hd <= 64 ? 0.72 : c.hd <= 128 ? 1.45 : 3.2;
@@ -1479,8 +1483,10 @@ bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int 
   f->splits = 1;
   double best = 0.0;
   for (int n = 1; n <= most; ++n) {
-    const double cost = std::max(grid * mean * tile_us / cus, longest / n * 1.2) +
-                        0.25 * longest / n * tile_us * places + (n > 1 ? 6.0 + n * row_us : 0.0);
+    const double work = pre ? (double)((grid * n + cus - 1) / cus) * longest / n * tile_us
+                            : std::max(grid * mean * tile_us / cus, longest / n * 1.2) +
+                                  0.25 * longest / n * tile_us * places;
+    const double cost = work + (n > 1 ? 6.0 + n * row_us : 0.0);
     if (n == 1 || cost < best) {
       best = cost;
       f->splits = n;
