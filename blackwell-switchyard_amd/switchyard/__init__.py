@@ -5,7 +5,9 @@ Submodules (imported directly, as in the reference):
   ``switchyard.triton_op``  import-compatible alias of the reference's module
   ``switchyard.reference``  DEFAULT_EPS, BlockAttnRes parameters, byte model
   ``switchyard.baselines``  eager PyTorch formulations (comparators)
-  ``switchyard.model``      decoder Transformer with a source arena
+  ``switchyard.model``      decoder Transformer with a source arena; generation
+  ``switchyard.cache_op``   paged cache of keys and values, attention over it
+  ``switchyard.sample_op``  sampling tokens from logits
   ``switchyard.harness``    measurement primitives
 """
 

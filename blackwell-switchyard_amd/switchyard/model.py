@@ -50,6 +50,9 @@ value they read. Two mechanisms handle that:
     site's output through the running sum), so the restored value is never
     needed elsewhere. Saved-tensor hooks also bypass autograd's storage-wide
     version check, which the slot writes would otherwise trip.
+
+Generation. ``Transformer.decode`` appends new tokens to a ``DecodeState`` (paged keys and
+values of every layer) and returns the next logits; ``generate`` samples from them.
 """
 
 from __future__ import annotations
