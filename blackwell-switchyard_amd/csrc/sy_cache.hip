@@ -1401,14 +1401,15 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
 // ----------------------------------------------------------------------- host
 
 // Tokens at most of a sequence that one workgroup reads whole, by the number of workgroups
-// that gives. One alone takes 8 us for 256 tokens, 12 for 512, 19 for 1024 and 33 for 2048;
-// shared out, 16 for any of them, 8 of which are the second launch. Many of them hide each
-// other's latency: 128 over 1024 tokens 19.4 us whole, 22 shared out, over 2048 33 and 31;
-// 1024 over 2048 tokens 183 and 190 (16 kv heads), 184 and 203 (8, of 32 heads). Next to a
-// prefix's pass they start behind it, and what starts last must not be long: 128 over 1024
-// tokens behind 30011 shared ones 57.8 us whole, 52.0 shared out.
+// that gives. One takes 8 us for 256 tokens, 12 for 512, 19 for 1024 and 33 for 2048 (37
+// GB/s, which is what a CU's loads reach: eight waves take as long as four); shared out, 16
+// for any of them, 8 of which are the second launch. More of them share memory's rate: 128
+// over 1024 tokens 19.4 us whole, 22 shared out, over 2048 33 and 31; 256 over 2048 tokens
+// 43 and 49 to 53; 1024 over 2048 tokens 180 and 190 (16 kv heads), 183 and 204 (8). Next
+// to a prefix's pass they start behind it, and what starts last must not be long: 128 over
+// 1024 tokens behind 30011 shared ones 57.8 us whole, 52.0 shared out.
 int whole_tokens(int64_t workgroups, bool beside) {
-  return beside ? 512 : workgroups >= 1024 ? 2048 : workgroups >= 128 ? 1024 : 512;
+  return beside ? 512 : workgroups >= 256 ? 2048 : workgroups >= 128 ? 1024 : 512;
 }
 
 constexpr int64_t kMost = 0x7fffffff;
