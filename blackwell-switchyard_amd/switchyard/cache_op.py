@@ -85,10 +85,6 @@ def _validate_out(out, like, shape) -> None:
           and out.data_ptr() % 16 == 0, f"out must be a dense {list(shape)} tensor of the inputs' dtype and device")
 
 
-def _given(*tensors) -> list:
-    return [t for t in tensors if t is not None]
-
-
 def _no_backward(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward; run it under torch.no_grad() for inference")
@@ -105,8 +101,9 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
     ``cos``, ``sin`` are fp32 ``[positions, head_dim / 2]`` (``[positions, 1, ...]`` as
     the decoder's). Row ``i`` of ``n`` new ones stands at ``lengths[b] - n + i``, behind
     ``prefix_len``. Arithmetic is fp32, every output rounded once."""
-    if _lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths, *_given(starts, out)) and (
-            qkv.is_cuda and type(prefix_len) is int):
+    if (_lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths) and qkv.is_cuda
+            and type(prefix_len) is int and (starts is None or _lib.ordinary(starts))
+            and (out is None or _lib.ordinary(out))):
         q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out)
         if q is not None:
             return q
@@ -147,8 +144,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     that share a prefix are more than 16, the weights are rounded to its dtype for the second
     product (relative error 2.0e-3 in bf16, of which the output's own rounding is 1.7e-3);
     where there are fewer they are not."""
-    if _lib.ordinary(q, k_cache, v_cache, page_table, lengths, *_given(starts, prefix_pages, out)) and (
-            q.is_cuda and type(prefix_len) is int):
+    if (_lib.ordinary(q, k_cache, v_cache, page_table, lengths) and q.is_cuda and type(prefix_len) is int
+            and (starts is None or _lib.ordinary(starts)) and (out is None or _lib.ordinary(out))
+            and (prefix_pages is None or _lib.ordinary(prefix_pages))):
         o = _lib.native().paged_attention(q, k_cache, v_cache, page_table, lengths, starts, prefix_pages, prefix_len,
                                           q.shape[-1] ** -0.5 if scale is None else scale, out)
         if o is not None:

@@ -54,7 +54,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     k, ks = _split("top_k", top_k, integer=True)
     p, ps = _split("top_p", top_p)
     m, ms = _split("min_p", min_p)
-    if _lib.ordinary(logits, u, *(x for x in (ts, ks, ps, ms) if x is not None)) and logits.is_cuda:
+    if _lib.ordinary(logits, u) and logits.is_cuda and all(x is None or _lib.ordinary(x) for x in (ts, ks, ps, ms)):
         tokens = _lib.native().sample_tokens(logits, u, t, k, p, m, ts, ks, ps, ms)
         if tokens is not None:
             return tokens

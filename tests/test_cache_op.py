@@ -433,6 +433,39 @@ def test_a_captured_step_follows_lengths_and_tables():
             assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_a_captured_ragged_call_follows_starts(prefix, dtype):
+    """How the packed rows divide among the sequences is read when the call is replayed: many
+    rows of one, few of all, none of some, rows of no sequence."""
+    c = Case([60, 37, 3, 40], [100, 0, 900, 33], kv=2, group=2, hd=64, page=16, dtype=dtype, prefix=prefix, seed=21)
+    q, k, v, table = c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), c.table.to(DEV)
+    starts, lengths = c.starts.to(DEV), c.lengths.to(DEV)
+    more = dict(prefix_pages=torch.tensor(c.prefix_ids, dtype=torch.int32, device=DEV), prefix_len=prefix)
+    out = torch.zeros_like(q)
+
+    def call(to=None):
+        return paged_attention(q, k, v, table, lengths, starts, out=to, **(more if prefix else {}))
+
+    call(out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out)
+    for new, lens in (([60, 37, 3, 40], None), ([1, 1, 1, 137], [160, 1, 903, 139]), ([0, 0, 140, 0], [1, 0, 903, 2]),
+                      ([8, 8, 8, 8], [160, 37, 8, 64]), ([30, 0, 2, 90], [31, 5, 800, 73])):
+        starts.copy_(torch.tensor([0, *new], dtype=torch.int32).cumsum(0, dtype=torch.int32))
+        lengths.copy_(c.lengths if lens is None else torch.tensor(lens, dtype=torch.int32))
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want = call()
+        rows = sum(new)
+        assert torch.equal(out[:rows], want[:rows]) and (out[rows:] == 7).all() and (want[rows:] == 0).all()
+        if lens is None:
+            c.check(got=want)
+
+
 def test_calls_on_two_streams_at_once():
     c = Case([1] * 8, [500 * i for i in range(8)], kv=2, group=2, hd=128, page=64, dtype=BF, seed=22)
     d = Case([40, 30], [800, 20], kv=2, group=2, hd=128, page=64, dtype=BF, seed=23)

@@ -144,6 +144,23 @@ def test_a_captured_token_step():
 
 @gpu
 @needs
+@pytest.mark.parametrize("residual", ["standard", "switchyard"])
+def test_inference_mode_and_another_stream(residual):
+    m = _model(residual)
+    idx, u = _tokens(2, 9), torch.rand(4, 2, generator=torch.Generator().manual_seed(3))
+    want = m.generate(idx, 4, u=u, top_p=0.9)
+    with torch.inference_mode():
+        assert torch.equal(m.generate(idx, 4, u=u, top_p=0.9), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = m.generate(idx, 4, u=u, top_p=0.9)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+@gpu
+@needs
 def test_what_does_not_fit_is_nan():
     m = _model("standard")
     state = DecodeState(m, 2, 16, page=16)
