@@ -304,7 +304,9 @@ template <class F> __device__ __forceinline__ bool locate(int n_seq, int unit, F
   return false;
 }
 // Units a worker takes (the host sees to it that all numbers of units fit 31 bits).
-__device__ __forceinline__ int share_of(const Cut& u, int units) { return max((units + u.workers - 1) / u.workers, u.least); }
+__device__ __forceinline__ int share_of(const Cut& u, int units) {
+  return max((units + u.workers - 1) / u.workers, u.least);
+}
 // The unit-th of all units in the order of their distance from their sequence's last one
 // (the last units of all sequences, then those before them, ...): that sequence and the
 // unit's number in it. With `most` the largest number of units a sequence can have. The
@@ -432,12 +434,14 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
     const int share = share_of(u, units);
     unit = worker * share;
     end = min(unit + share, units);
-    some = unit < end;
+    int at = 0, base = 0;
+    some = unit < end && per_head > 0;  // (overlapping sequences can have more units than fit)
     if (some) {
       h = unit / per_head;
-      const int at = unit - h * per_head;
-      int base;
-      locate(n_seq, at, count, &b, &base);
+      at = unit - h * per_head;
+      some = locate(n_seq, at, count, &b, &base);
+    }
+    if (some) {
       s = pass_seq(c, u.pre, plen, b);
       ti = tiles_of(u, c.group, s);
       rtile = (at - base) / ti.key_tiles;
@@ -763,9 +767,9 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
 // query rows of a kv head, a wave 32 of them, and all four waves read the same tiles of 64
 // keys and values from LDS. Tile t + 1 is on its way from memory to the other half of LDS
 // while tile t is multiplied, without passing through registers; one barrier a tile. The
-// products run on v_mfma_f32_32x32x16 in the same transposed form. The maximum is only followed when a score passes it by more than 2^8 (weights
-// stay below 256, and the ratio to their sum is what counts), so the results are hardly
-// ever rescaled.
+// products run on v_mfma_f32_32x32x16 in the same transposed form. The maximum is only
+// followed when a score passes it by more than 2^8 (weights stay below 256, and the ratio to
+// their sum is what counts), so the results are hardly ever rescaled.
 //
 // Bound by the matrix cores and, next to them, by the exponentials (a quarter of the
 // vector rate): a wave's tile of heads of 128 is 1024 cycles of products and about as many of
@@ -846,7 +850,8 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
   const int rest = block / c.kv_heads;
   const int split = rest % f.splits, tile_id = rest / f.splits;
   int b, rtile;
-  if (!locate_last(f.pre ? 1 : c.n_seq, tile_id, f.tiles, f.fold, [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &rtile))
+  if (!locate_last(f.pre ? 1 : c.n_seq, tile_id, f.tiles, f.fold,
+                   [&](int x) { return flash_tiles(c, f, plen, x); }, &b, &rtile))
     return;
   const Seq s = pass_seq(c, f.pre, plen, b);
   const int rows = s.n * c.group;
@@ -1106,6 +1111,8 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
   }
   const int base = f.splits == 1 || f.pre ? 0 : total_of(b, [&](int x) { return flash_tiles(c, f, plen, x); });
   if (w0 + col > last) return;
+  // Sequences that overlap have more tiles than there are places for.
+  if (f.splits > 1 && base + rtile >= f.tiles) return;
   if (direct) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     S* const op = static_cast<S*>(a.out) + out_row * hd;
@@ -1198,11 +1205,14 @@ __device__ __forceinline__ Shares shares_of(const CacheArgs& c, const Cut& u, in
 }
 // Row r of sequence s and kv head h as k_attend left it: in the second slot of the worker
 // in whose run the segment begins and the first slots of the next ones, or whole.
-__device__ __forceinline__ Parts parts_of(const CacheArgs& c, const Cut& u, const Shares& x, const Seq& s, int h, int r) {
+// (Workers past the last are those of sequences that overlap, whose numbers of units may be
+// past all bounds: then results are some numbers, but read from where there are any.)
+__device__ __forceinline__ Parts parts_of(const CacheArgs& c, const Cut& u, const Shares& x, const Seq& s, int h,
+                                          int r) {
   const int rtile = r / u.rt, k = tiles_of(u, c.group, s).key_tiles;
   const int at = h * x.per_head + x.base + rtile * k;
-  const int first = u.least != 0 ? at / x.share : 0;
-  const int count = u.least != 0 ? (at + k - 1) / x.share - first + 1 : 1;
+  const int first = u.least != 0 ? clamp(at / x.share, 0, u.workers - 1) : 0;
+  const int count = u.least != 0 ? clamp((at + k - 1) / x.share - first + 1, 1, u.workers - first) : 1;
   Parts p;
   p.count = __builtin_amdgcn_readfirstlane(count);
   p.at = 2 * (int64_t)first * u.rs + (r - rtile * u.rt);
@@ -1276,6 +1286,7 @@ __device__ __forceinline__ void merge(const AttendArgs& a, const JoinArgs& g, co
     const int r = (tok - s.row0) * c.group + gi;
     const Parts mine = flash ? flash_parts(c, g.fown, fbase, h, r) : parts_of(c, g.own, xo, s, h, r);
     if (g.has_pre == 0 && mine.count == 1) continue;
+    if (flash && g.fown.splits > 1 && fbase + r / kFlashRows >= g.fown.tiles) continue;
     Parts front{};
     const int rp = (tok - ps.row0) * c.group + gi;
     if (g.has_pre == 1) front = parts_of(c, g.pre, xp, ps, h, rp);
@@ -1289,7 +1300,8 @@ __device__ __forceinline__ void merge(const AttendArgs& a, const JoinArgs& g, co
       const bool f = i < front.count;
       if ((f ? front.count : mine.count) == 1) return row;
       const int k = f ? i : i - front.count;
-      return (f ? front.at : mine.at) + k * (f ? front.step : mine.step) + (k == 0 ? (f ? front.second : mine.second) : 0);
+      return (f ? front.at : mine.at) + k * (f ? front.step : mine.step) +
+             (k == 0 ? (f ? front.second : mine.second) : 0);
     };
     // The first result is on its way while its weight is worked out.
     const auto part = [&](int i) {
@@ -1510,7 +1522,8 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
     p.attend = true;
     p.pre = prefix_len > 0 ? 1 : 0;
     p.ok = cut(c, dtype, false, false, c.cap, (int)kMost, nt, cus, &p.own);
-    if (p.ok && p.pre) p.ok = cut(c, dtype, true, false, prefix_len, (int)kMost, rows <= 16 || c.hd > 128 ? 1 : 2, cus, &p.cpre);
+    const int nt_pre = rows <= 16 || c.hd > 128 ? 1 : 2;
+    if (p.ok && p.pre) p.ok = cut(c, dtype, true, false, prefix_len, (int)kMost, nt_pre, cus, &p.cpre);
   } else {
     // Up to 16 rows are k_attend's. A prefix has a pass of its own where sequences bring
     // few rows, so that it is read once for all; else its keys are part of every

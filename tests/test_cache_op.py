@@ -276,6 +276,20 @@ def test_strides_and_orders_of_the_caches_and_queries():
     assert torch.equal(paged_attention(c.q.to(DEV), c.k.to(DEV), c.v.to(DEV), c.table.to(DEV), *rest, scale=0.125), want)
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("prefix", [0, 100])
+@pytest.mark.parametrize("new", [[30, 10, 30, 10, 20, 40], [3, 1, 3, 1, 2, 4], [200, 1, 3, 1, 2, 4]])
+def test_starts_out_of_order(new, prefix, dtype):
+    """Results are then undefined; the caches stay as they are, and so does the call after."""
+    c = Case(new, [900] * 6, kv=2, group=1, hd=64, page=16, dtype=dtype, prefix=prefix, seed=22)
+    k, v, q = c.k.to(DEV), c.v.to(DEV), c.q.to(DEV)
+    more = dict(prefix_pages=torch.tensor(c.prefix_ids, dtype=torch.int32, device=DEV), prefix_len=prefix)
+    bad = torch.tensor([0, c.n_tok] * 3 + [0], dtype=torch.int32, device=DEV)
+    paged_attention(q, k, v, c.table.to(DEV), c.lengths.to(DEV), bad, **(more if prefix else {}))
+    assert torch.equal(k.cpu(), c.k) and torch.equal(v.cpu(), c.v) and torch.equal(q.cpu(), c.q)
+    c.check()
+
+
 def test_a_cache_past_32_bit_offsets():
     """Pages whose elements lie behind 2^32 bytes and 2^31 elements."""
     pages, kv, page, hd = 140000, 2, 64, 128
