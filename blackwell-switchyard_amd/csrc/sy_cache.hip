@@ -1417,11 +1417,13 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
 // GB/s, which is what a CU's loads reach: eight waves take as long as four); shared out, 16
 // for any of them, 8 of which are the second launch. More of them share memory's rate: 128
 // over 1024 tokens 19.4 us whole, 22 shared out, over 2048 33 and 31; 256 over 2048 tokens
-// 43 and 49 to 53; 1024 over 2048 tokens 180 and 190 (16 kv heads), 183 and 204 (8). Next
-// to a prefix's pass they start behind it, and what starts last must not be long: 128 over
-// 1024 tokens behind 30011 shared ones 57.8 us whole, 52.0 shared out.
+// 43 and 49 to 53, over any lengths up to 2048 34 and 36, or 35 and 41 (8 kv heads of 32).
+// With more than two a CU the long ones among sequences of any lengths may start last: 1024
+// over up to 2048 tokens 130 us whole, 116 shared out (180 and 190 where all are as long),
+// 2048 over up to 1024 125 and 129. Next to a prefix's pass they start behind it anyway: 128
+// over 1024 tokens behind 30011 shared ones 57.8 us whole, 52.0 shared out.
 int whole_tokens(int64_t workgroups, bool beside) {
-  return beside ? 512 : workgroups >= 256 ? 2048 : workgroups >= 128 ? 1024 : 512;
+  return beside || workgroups < 128 ? 512 : workgroups >= 256 && workgroups < 512 ? 2048 : 1024;
 }
 
 constexpr int64_t kMost = 0x7fffffff;
