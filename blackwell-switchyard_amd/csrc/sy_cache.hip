@@ -37,7 +37,7 @@ __device__ __forceinline__ Seq seq_of(const CacheArgs& c, int b) {
     s.row0 = b * c.each;
     s.n = c.each;
   }
-  s.len = clamp(c.lengths[b], 0, 1 << 30);
+  s.len = clamp(c.lengths[b], 0, 0x7fffff00);  // (with room for a tile's rows)
   s.keys = min(s.len, (int)c.cap);
   return s;
 }

@@ -1076,6 +1076,10 @@ int64_t sy_probe_grid(int64_t bytes) {
   return g < 1 ? 1 : (g > 32768 ? 32768 : g);
 }
 
+// Tokens at most in a sequence's pages, and in a prefix: the kernels count positions in 32
+// bits and look some tiles ahead of the last one.
+constexpr int64_t kMostTokens = (int64_t)1 << 30;
+
 // The cache's sizes and strides, into *out; nothing here reads device memory.
 static int cache_args(const sy_paged* c, CacheArgs* out) {
   if (!c) return SY_ERR_NULL;
@@ -1083,7 +1087,7 @@ static int cache_args(const sy_paged* c, CacheArgs* out) {
   const int64_t big = 0x7fffffff;
   if (c->n_seq < 0 || c->n_tok < 0 || c->n_seq > big / 2 || c->n_tok > big / 2 || c->n_pages < 1 ||
       c->n_pages > big || c->table_cols < 0 || c->page < 1 || (c->page & (c->page - 1)) != 0 ||
-      c->page > (1 << 20) || c->table_cols > big / c->page || c->kv_heads < 1 || c->heads < c->kv_heads ||
+      c->page > (1 << 20) || c->table_cols > kMostTokens / c->page || c->kv_heads < 1 || c->heads < c->kv_heads ||
       c->heads % c->kv_heads != 0 || c->heads > 0xffff || c->hd < 8 || c->hd > 256 || c->hd % 8 != 0)
     return SY_ERR_SHAPE;
   if (c->n_tok != 0 && (c->n_seq == 0 || (!c->starts && c->n_tok % c->n_seq != 0))) return SY_ERR_SHAPE;
@@ -1112,7 +1116,7 @@ int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int6
   AppendArgs a{};
   const int rc = cache_args(c, &a.c);
   if (rc != SY_OK) return rc;
-  if (n_pos < 0 || prefix_len < 0 || prefix_len > 0x7fffffff || (fill != 0 && fill != 1)) return SY_ERR_SHAPE;
+  if (n_pos < 0 || prefix_len < 0 || prefix_len > kMostTokens || (fill != 0 && fill != 1)) return SY_ERR_SHAPE;
   if (tok_stride < 0 || head_stride < 0) return SY_ERR_STRIDE;
   if (c->n_tok == 0) return SY_OK;
   if (!qkv || !q || (n_pos != 0 && (!cosv || !sinv))) return SY_ERR_NULL;
@@ -1133,7 +1137,7 @@ int64_t sy_paged_attention_workspace_bytes(const sy_paged* c, int64_t prefix_len
   CacheArgs a{};
   const int rc = cache_args(c, &a);
   if (rc != SY_OK) return rc;
-  if (prefix_len < 0 || prefix_len > 0x7fffffff) return SY_ERR_SHAPE;
+  if (prefix_len < 0 || prefix_len > kMostTokens) return SY_ERR_SHAPE;
   if (c->n_tok == 0) return 0;
   const int64_t bytes = attend_workspace(a, prefix_len, c->dtype);
   return bytes < 0 ? SY_ERR_SHAPE : bytes;
@@ -1145,7 +1149,7 @@ int sy_paged_attention(const sy_paged* c, const void* q, int64_t q_tok_stride, i
   AttendArgs a{};
   const int rc = cache_args(c, &a.c);
   if (rc != SY_OK) return rc;
-  if (prefix_len < 0 || prefix_len > 0x7fffffff || (fill != 0 && fill != 1)) return SY_ERR_SHAPE;
+  if (prefix_len < 0 || prefix_len > kMostTokens || (fill != 0 && fill != 1)) return SY_ERR_SHAPE;
   const int64_t chunk = 16 / esize(c->dtype);
   if (q_tok_stride < 0 || q_head_stride < 0 || q_tok_stride % chunk != 0 || q_head_stride % chunk != 0)
     return SY_ERR_STRIDE;

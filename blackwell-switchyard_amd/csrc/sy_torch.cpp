@@ -586,6 +586,8 @@ void changed(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+constexpr int64_t kMostTokens = (int64_t)1 << 30;  // in a sequence's pages, and in a prefix
+
 // The cache and the sequences of a call with n_tok packed rows and `heads` query heads;
 // false where the Python function has to see the call.
 bool paged_of(const Tensor& like, int64_t heads, const Tensor& k, const Tensor& v, const Tensor& table,
@@ -594,7 +596,8 @@ bool paged_of(const Tensor& like, int64_t heads, const Tensor& k, const Tensor& 
       k.sizes() != v.sizes() || k.strides() != v.strides() || like.scalar_type() != k.scalar_type() ||
       v.scalar_type() != k.scalar_type() || table.dim() != 2 || lengths.dim() != 1 ||
       table.size(0) != lengths.size(0) || !lengths.is_contiguous() || lengths.size(0) < 1 ||
-      (table.size(1) > 1 && table.stride(1) != 1) || table.size(1) < 1)
+      (table.size(1) > 1 && table.stride(1) != 1) || table.size(1) < 1 || k.size(2) < 1 ||
+      table.size(1) > kMostTokens / k.size(2))
     return false;
   for (const Tensor* t : {&k, &v, &table, &lengths})
     if (t->device() != like.device()) return false;
@@ -639,7 +642,7 @@ std::optional<Tensor> paged_append(const Tensor& qkv_in, const Tensor& cosv, con
   if (qkv_in.dim() != 3 || qkv_in.size(0) < 1 || k.dim() != 4) return std::nullopt;
   const int64_t heads = qkv_in.size(1) - 2 * k.size(1);
   if (!paged_of(qkv_in, heads, k, v, table, lengths, starts, &c) || qkv_in.size(2) != c.hd || tracked(qkv_in) ||
-      tracked(k) || tracked(v) || prefix_len < 0 || prefix_len > 0x7fffffff ||
+      tracked(k) || tracked(v) || prefix_len < 0 || prefix_len > kMostTokens ||
       !out_ok(out, qkv_in, c.n_tok, heads, c.hd))
     return std::nullopt;
   for (const Tensor* t : {&cosv, &sinv})
@@ -668,7 +671,7 @@ std::optional<Tensor> paged_attention(const Tensor& q_in, const Tensor& k, const
   if (q_in.dim() != 3 || q_in.size(0) < 1) return std::nullopt;
   const int64_t heads = q_in.size(1);
   if (!paged_of(q_in, heads, k, v, table, lengths, starts, &c) || q_in.size(2) != c.hd || tracked(q_in) ||
-      tracked(k) || tracked(v) || prefix_len < 0 || prefix_len > 0x7fffffff ||
+      tracked(k) || tracked(v) || prefix_len < 0 || prefix_len > kMostTokens ||
       !out_ok(out, q_in, c.n_tok, heads, c.hd))
     return std::nullopt;
   if (prefix_len > 0 && (!prefix_pages.has_value() || !whole(*prefix_pages) || prefix_pages->dim() != 1 ||

@@ -3,7 +3,8 @@
 What generating with the decoder needs between its projections. The cache of a layer is a
 pair of tensors ``k_cache``, ``v_cache`` ``[n_pages, kv_heads, page, head_dim]`` (any
 strides with dense rows, the same for both); a sequence's tokens lie in the pages that
-its row of ``page_table`` ``[B, columns]`` lists, ``page`` of them each, in order.
+its row of ``page_table`` ``[B, columns]`` lists, ``page`` of them each, in order, at most
+2^30 in all.
 
 A call brings the new tokens of ``B`` sequences packed into one tensor: sequence ``b``
 has the rows ``starts[b]`` to ``starts[b + 1]``; without ``starts`` every sequence has
@@ -36,6 +37,9 @@ from . import _lib
 from .hip_op import _ptr
 
 __all__ = ["paged_append", "paged_attention"]
+
+#: Tokens at most in a row of the page table, and in a prefix.
+_MOST_TOKENS = 1 << 30
 
 
 def _need(ok: bool, message: str) -> None:
@@ -73,7 +77,8 @@ def _validate_cache(rows, heads: int, what: str, k, v, page_table, lengths, star
           "the caches' rows must be dense and start at 16-byte boundaries")
     span = 2**32 // k.element_size()
     _need(k.stride(0) < span and k.stride(2) * page < span, "a page must span less than 4 GiB, and so pages apart")
-    _need(0 <= prefix_len <= 0x7FFFFFFF, "prefix_len must not be negative")
+    _need(0 <= prefix_len <= _MOST_TOKENS, "prefix_len must not be negative, and at most 2^30")
+    _need(page_table.shape[1] * page <= _MOST_TOKENS, "a row of page_table must hold at most 2^30 tokens")
     _need(rows.is_cuda, f"{what} must be on a CUDA device")
     return _lib.Paged(k.data_ptr(), v.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
                       None if starts is None else starts.data_ptr(), k.stride(0), k.stride(1), k.stride(2),

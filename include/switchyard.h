@@ -371,7 +371,8 @@ int sy_swiglu_bwd(const void* gate_up, const void* grad_out, void* dgate_up, int
  * in order). lengths[b] counts its tokens in the cache with the new ones, which are the
  * last: row i of n stands at position lengths[b] - n + i. table, lengths and starts lie
  * in device memory and are read when the kernels run, so a captured call may be replayed
- * for other lengths. Tokens past the capacity of the table's row are not there.
+ * for other lengths. Tokens past the capacity of the table's row are not there; a row, and
+ * a prefix, hold at most 2^30 tokens.
  *
  * A prefix is shared by all sequences: prefix_len tokens in the pages that prefix_pages
  * lists. They come before every sequence's own tokens, whose positions they shift.
