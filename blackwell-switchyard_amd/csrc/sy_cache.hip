@@ -884,9 +884,19 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
     }
   }
   // Scores in base 2; a negative scale turns the queries' signs, so that the largest
-  // product is the largest score.
+  // product is the largest score. A scale of zero goes into the queries (those of infinities
+  // and NaN become NaN, as their products would): hidden scores are -inf before the scale.
   float sl = a.scale * 1.44269504088896340736f;
-  if (sl < 0.0f) {
+  if (sl == 0.0f) {
+    sl = 1.0f;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = 0.0f * elem<T>(q[k], e);
+      q[k] = pack<T>(z);
+    }
+  } else if (sl < 0.0f) {
     sl = -sl;
 #pragma unroll
     for (int k = 0; k < KC; ++k)

@@ -11,6 +11,8 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover
     pytest.skip("needs a HIP device", allow_module_level=True)
 
+from test_cache_op import Case  # noqa: E402
+
 from switchyard.cache_op import paged_append  # noqa: E402
 
 DEV = "cuda"
@@ -31,3 +33,44 @@ def test_a_length_past_the_longest_row():
     q = paged_append(qkv, turn, turn, k, v, table, lengths)
     assert torch.equal(torch.isnan(q).all(-1)[:, 0], torch.arange(n, device=DEV) >= 5)
     assert torch.equal(v[0, 0, -5:], qkv[:5, 2]) and (v[0, 0, :-5] == 0).all() and (k[0, 0, :-5] == 0).all()
+
+
+def scaled(c, scale, **more):
+    """``paged_attention`` with a scale, checked; a negative one is a positive one of turned queries."""
+    got = c.call(scale=scale, **more).cpu().double()
+    q = c.q
+    c.q = q if scale >= 0 else -q
+    want, tol = c.expected(abs(scale))
+    c.q = q
+    assert torch.isfinite(got).all()
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol.clamp_min(1e-30)).max().item()
+
+
+SCALES = [
+    # new, past, kv, group, hd, page, prefix
+    ([1, 1, 3], [5, 70, 300], 2, 2, 64, 16, 0),  # few rows
+    ([65, 129], [0, 77], 1, 1, 128, 64, 0),  # many
+    ([17, 1, 40], [15, 0, 130], 2, 2, 80, 16, 0),  # both, of a padded width
+    ([1] * 20, list(range(20)), 1, 3, 64, 32, 200),  # a prefix's pass of many rows
+    ([1, 1], [9, 40], 2, 2, 128, 16, 333),  # and of few
+    ([90, 41], [0, 7], 1, 2, 64, 16, 100),  # a prefix before many rows of each
+]
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-42, -0.2, 0.5, -0.0])
+@pytest.mark.parametrize("shape", SCALES, ids=[str(i) for i in range(len(SCALES))])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_scales(dtype, shape, scale):
+    """Any scale: none gives the mean of what a row sees."""
+    new, past, kv, group, hd, page, prefix = shape
+    scaled(Case(new, past, kv=kv, group=group, hd=hd, page=page, dtype=dtype, prefix=prefix, seed=31), scale)
+
+
+def test_a_query_of_nan_without_a_scale():
+    """Only its own row is NaN."""
+    c = Case([65, 40], [0, 30], kv=1, group=2, hd=64, page=16, dtype=BF, seed=32)
+    c.q[50, 1, 3] = float("nan")
+    bad = torch.zeros(105, 2, dtype=torch.bool)
+    bad[50, 1] = True
+    assert torch.equal(torch.isnan(c.call(scale=0.0).cpu()).all(-1), bad)
+    assert torch.equal(torch.isnan(c.call(scale=0.0).cpu()).any(-1), bad)
