@@ -812,11 +812,16 @@ template <class T> __device__ __forceinline__ f32x16_t mma32(const i32x4_t& a, c
 // done when vmcnt says so. (The builtin's loads are waited for before the next read of any
 // LDS, the other buffer included. There is no output register that could be reused while
 // the load is under way. The compiler does not count these loads: a wait of its own for an
-// earlier load would wait for them too, so there must be none behind them. m0 is a reserved
-// register, set where it is used: the compiler keeps nothing in it.)
+// earlier load would wait for them too, so there must be none behind them. m0 is declared as
+// written, so that the compiler's own uses of it, in indexed registers and LDS, set it anew; its
+// warning that the register is a reserved one is of no use here.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const void* from, uint32_t at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from)
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ uint32_t lds_byte(void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p;
 }
