@@ -24,7 +24,7 @@ cached and its queries are NaN, and attention leaves its position out. The same 
 positions past the rotary tables or the table's row. Rows that belong to no sequence are
 zero, or keep their content in a given ``out``, which may be the queries themselves.
 
-There is no backward: under autograd the functions raise.
+There is no derivative: under autograd, and on tensors with tangents, the functions raise.
 """
 
 from __future__ import annotations
@@ -32,6 +32,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .hip_op import _ptr
@@ -93,6 +94,8 @@ def _validate_out(out, like, shape) -> None:
 def _no_backward(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no backward; run it under torch.no_grad() for inference")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no derivative; run it on tensors without tangents")
 
 
 def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,
@@ -112,6 +115,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
         q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out)
         if q is not None:
             return q
+    _no_backward("paged_append", qkv, cos, sin, k_cache, v_cache, out)
     _need(qkv.ndim == 3, f"qkv must be [n_tok, heads + 2 kv_heads, head_dim], got {tuple(qkv.shape)}")
     _need(k_cache.ndim == 4, "k_cache must be [n_pages, kv_heads, page, head_dim]")
     heads = qkv.shape[1] - 2 * k_cache.shape[1]
@@ -122,7 +126,6 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
         _need(t.dtype == torch.float32 and t.device == qkv.device and t.is_contiguous() and t.ndim >= 2
               and t.shape[-1] * 2 == c.hd and t.numel() == t.shape[0] * t.shape[-1] and t.shape == cos.shape,
               f"{name} must be a dense fp32 [positions, {c.hd // 2}] tensor on the same CUDA device")
-    _no_backward("paged_append", qkv, cos, sin, k_cache, v_cache, out)
     shape = (c.n_tok, heads, c.hd)
     if out is not None:
         _validate_out(out, qkv, shape)
@@ -156,6 +159,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                           q.shape[-1] ** -0.5 if scale is None else scale, out)
         if o is not None:
             return o
+    _no_backward("paged_attention", q, k_cache, v_cache, out)
     _need(q.ndim == 3, f"q must be [n_tok, heads, head_dim], got {tuple(q.shape)}")
     prefix_len = int(prefix_len)
     heads = q.shape[1]
@@ -167,7 +171,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
               "prefix_pages must be a dense int32 [pages] tensor on the same CUDA device")
         _need(prefix_pages.shape[0] * c.page >= prefix_len,
               f"{prefix_pages.shape[0]} prefix pages of {c.page} do not hold {prefix_len} tokens")
-    _no_backward("paged_attention", q, k_cache, v_cache, out)
     if out is not None:
         _validate_out(out, q, (c.n_tok, heads, c.hd))
     chunk = 16 // q.element_size()

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -13,7 +14,7 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 from test_cache_op import Case  # noqa: E402
 
-from switchyard.cache_op import paged_append  # noqa: E402
+from switchyard.cache_op import paged_append, paged_attention  # noqa: E402
 
 DEV = "cuda"
 BF, HF, F = torch.bfloat16, torch.float16, torch.float32
@@ -74,3 +75,39 @@ def test_a_query_of_nan_without_a_scale():
     bad[50, 1] = True
     assert torch.equal(torch.isnan(c.call(scale=0.0).cpu()).all(-1), bad)
     assert torch.equal(torch.isnan(c.call(scale=0.0).cpu()).any(-1), bad)
+
+
+def _serving(seed):
+    """A case's tensors for both functions: (append's arguments, attention's), by name."""
+    c = Case([1, 2], [5, 20], kv=1, group=2, hd=64, page=16, dtype=F, seed=seed)
+    d = dict(qkv=torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(seed)).to(DEV),
+             cos=torch.ones(64, 32, device=DEV), sin=torch.zeros(64, 32, device=DEV), q=c.q.to(DEV), k=c.k.to(DEV),
+             v=c.v.to(DEV))
+    rest = (c.table.to(DEV), c.lengths.to(DEV), c.starts.to(DEV))
+    return d, rest
+
+
+def _both(d, rest, out=None):
+    q = paged_append(d["qkv"], d["cos"], d["sin"], d["k"], d["v"], *rest, out=out)
+    return q, paged_attention(d["q"], d["k"], d["v"], *rest, out=out)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", ["qkv", "cos", "sin", "q", "k", "v"])
+def test_tangents_are_refused(name, grad):
+    """A tangent must not get lost: no_grad does not switch forward mode off."""
+    d, rest = _serving(41)
+    _both(d, rest)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        dual = {**d, name: forward_ad.make_dual(d[name], torch.ones_like(d[name]))}
+        with pytest.raises(RuntimeError, match="no derivative"):
+            _both(dual, rest)
+    def one(x):  # the function that takes it, inside a transform
+        e = {**d, name: x}
+        if name in ("qkv", "cos", "sin"):
+            return paged_append(e["qkv"], e["cos"], e["sin"], e["k"], e["v"], *rest)
+        return paged_attention(e["q"], e["k"], e["v"], *rest)
+
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.func.jvp(one, (d[name],), (torch.ones_like(d[name]),))
+    _both(d, rest)
