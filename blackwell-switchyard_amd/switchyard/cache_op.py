@@ -33,6 +33,7 @@ import ctypes
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .hip_op import _ptr
@@ -98,6 +99,13 @@ def _no_backward(name: str, *tensors) -> None:
         raise RuntimeError(f"{name} has no derivative; run it on tensors without tangents")
 
 
+def _changed(*tensors) -> None:
+    """Tell autograd that the kernels wrote into these."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            increment_version(t)
+
+
 def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,
                  v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                  starts: torch.Tensor | None = None, *, prefix_len: int = 0,
@@ -137,6 +145,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
                                         cos.shape[0], prefix_len, _ptr(q), int(out is None),
                                         _lib.stream_ptr(qkv.device))
     _lib.check(rc, "sy_paged_append")
+    _changed(k_cache, v_cache, out)
     return q
 
 
@@ -188,4 +197,5 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                     q.shape[-1] ** -0.5 if scale is None else float(scale), int(out is None),
                                     _ptr(ws), ws.numel() * 4, _lib.stream_ptr(q.device))
     _lib.check(rc, "sy_paged_attention")
+    _changed(out)
     return o

@@ -3,9 +3,12 @@
 
 from __future__ import annotations
 
+import contextlib
+
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.overrides import TorchFunctionMode
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +114,27 @@ def test_tangents_are_refused(name, grad):
     with pytest.raises(RuntimeError, match="no derivative"):
         torch.func.jvp(one, (d[name],), (torch.ones_like(d[name]),))
     _both(d, rest)
+
+
+class _Mode(TorchFunctionMode):
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("mode", [contextlib.nullcontext, _Mode], ids=["native", "python"])
+def test_autograd_notices_what_is_written(mode):
+    """A tensor that a backward saved and a call then overwrote."""
+    d, rest = _serving(42)
+    w = torch.randn((), device=DEV, requires_grad=True)
+    out = torch.zeros(3, 2, 64, device=DEV)
+    for name, t in (("k", d["k"]), ("v", d["v"]), ("out", out)):
+        loss = (w * t).sum()
+        with torch.no_grad(), mode():
+            before = t._version
+            _both(d, rest, out=out if name == "out" else None)
+            assert t._version == before + (2 if name == "out" else 1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode(), mode():  # such tensors have no version
+        e, rest = _serving(42)
+        _both(e, rest, out=torch.zeros(3, 2, 64, device=DEV))
