@@ -244,6 +244,18 @@ __device__ __forceinline__ float group_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// What a pass takes the exponentials relative to: the largest score, or a little below it.
+// fp16 ends at 2^-14 (2^-24 with fewer bits), and a context of 10^5 faint tokens behind one
+// strong one has weights below both that make up a percent of a row together. Their sum is
+// what the row is divided by, so the second product must not lose them: weights start at
+// 2^LIFT instead of 1. A weight is then off by its own rounding or 2^-(25 + LIFT) of the
+// largest, whichever is more. Scores from 2^22 on are whole steps apart in fp32, and with
+// them the difference would be: they keep their place. bf16 and fp32 reach down to 2^-126.
+template <class T, int LIFT> __device__ __forceinline__ float reference_of(float top) {
+  if constexpr (T::code == SY_F16) return fabsf(top) < 4194304.0f ? top - (float)LIFT : top;
+  else return top;
+}
+
 template <class T> constexpr int tokens_of() { return T::code == SY_F32 ? 16 : 32; }
 
 // How a pass over the keys is cut, the same for the kernel, the merge and the host.
@@ -599,7 +611,7 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
           float top = y[0];
 #pragma unroll
           for (int e = 1; e < MT * 4; ++e) top = fmaxf(top, y[e]);
-          const float mn = fmaxf(m[n], group_max(top));
+          const float mn = fmaxf(m[n], reference_of<T, 15>(group_max(top)));  // weights of at most 2^15.2
           const float mu = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet
           scale_o[n] = __builtin_amdgcn_exp2f(m[n] - mu);
           any_new = any_new || mn != m[n];
@@ -614,7 +626,8 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
           // The second product takes a weight as two numbers of the values' dtype, the
           // rounded weight and what it lacks: rounded once the weights alone would put 0.7 of
           // the output's own rounding on top of it (bf16 relative error 1.9e-3, so 1.7e-3),
-          // and this kernel waits for memory, not for products.
+          // and this kernel waits for memory, not for products. (fp16: a weight is off by
+          // 2^-22 of itself or 2^-40 of the largest.)
           if constexpr (!kF32) {
             p16[n] = pack<T>(pf[n]);
             float rest[8];
@@ -768,8 +781,9 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
 // keys and values from LDS. Tile t + 1 is on its way from memory to the other half of LDS
 // while tile t is multiplied, without passing through registers; one barrier a tile. The
 // products run on v_mfma_f32_32x32x16 in the same transposed form. The maximum is only
-// followed when a score passes it by more than 2^8 (weights stay below 256, and the ratio to
-// their sum is what counts), so the results are hardly ever rescaled.
+// followed when a score passes it by more than 2^8 (weights stay below 256, fp16's lifted
+// ones below 2^15.4, and the ratio to their sum is what counts), so the results are hardly
+// ever rescaled.
 //
 // Bound by the matrix cores and, next to them, by the exponentials (a quarter of the
 // vector rate): a wave's tile of heads of 128 is 1024 cycles of products and about as many of
@@ -967,6 +981,7 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
 #pragma unroll
   for (int k = 0; k < KC; ++k) asm volatile("" : "+v"(q[k]));
   constexpr int kOnes = T::code == SY_BF16 ? 0x3f803f80 : 0x3c003c00;
+  constexpr float kLag = T::code == SY_F16 ? 15.0f : 8.0f;  // of the reference behind the maximum: 7 and 8
   const i32x4_t ones = {kOnes, kOnes, kOnes, kOnes};
   float m = -INFINITY, l = 0.0f;
   f32x16_t o[MD];
@@ -1048,8 +1063,8 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
         const auto sw = __builtin_amdgcn_permlane32_swap(v, v, false, false);
         top = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * sl;
       }
-      if (__any(top > m + 8.0f)) {
-        const float mn = fmaxf(m, top);
+      if (__any(top > m + kLag)) {
+        const float mn = fmaxf(m, reference_of<T, 7>(top));
         const float sc = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
         m = mn;
         l *= sc;

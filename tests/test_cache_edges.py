@@ -1,5 +1,11 @@
 """Edges of the paged cache's operators on the GPU, against float64 with the bounds of
-``test_cache_op``."""
+``test_cache_op``.
+
+fp16 ends where bf16 goes on: its steps are 2^-24 below 2^-14. A weight (relative to the
+largest) is therefore off by at most half of such a step over what the kernels lift weights
+by, 2^-25 2^-15 where a sequence has up to 16 rows and 2^-25 2^-7 where it has more, if that is
+more than its own rounding. Over n keys that is n step / l (max|v| + |o|) of the result, with
+l the sum of the weights."""
 
 from __future__ import annotations
 
@@ -138,3 +144,37 @@ def test_autograd_notices_what_is_written(mode):
     with torch.inference_mode(), mode():  # such tensors have no version
         e, rest = _serving(42)
         _both(e, rest, out=torch.zeros(3, 2, 64, device=DEV))
+
+
+FAINT = [
+    # new, past, kv, group, prefix, what a weight may be off by
+    ([1, 1], [3000, 40], 2, 2, 0, 2.0**-40),  # whole sequences in one workgroup
+    ([1, 3], [20000, 64], 1, 1, 0, 2.0**-40),  # one shared out
+    ([65, 30], [3000, 100], 1, 2, 0, 2.0**-32),
+    ([1] * 20, list(range(20)), 1, 2, 3000, 2.0**-32),  # a prefix's pass
+    ([1, 1], [9, 40], 2, 2, 3000, 2.0**-40),
+    ([40, 20], [0, 7], 1, 2, 3000, 2.0**-32),
+]
+
+
+@pytest.mark.parametrize("below", [14.0, 20.0, 24.5])
+@pytest.mark.parametrize("shape", FAINT, ids=[str(i) for i in range(len(FAINT))])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_many_faint_tokens(dtype, shape, below):
+    """Every 32nd token is strong and has no value; all the others are 2^-below and fainter,
+    and are the result."""
+    new, past, kv, group, prefix, step = shape
+    c = Case(new, past, kv=kv, group=group, hd=64, page=32, dtype=dtype, prefix=prefix, seed=51)
+    g = torch.Generator().manual_seed(52)
+    c.q.zero_()
+    c.q[..., 0] = 8.0  # (the scale is 1/8)
+    c.k.zero_()
+    c.k[..., 0] = -(below + 3 * torch.rand(c.k.shape[:3], generator=g)) * 0.6931
+    c.v.copy_(512 * (1 + 0.25 * torch.randn(c.v.shape, generator=g)))
+    c.k[:, :, 0], c.v[:, :, 0] = 0.0, 0.0
+    want, tol = c.expected()
+    got = c.call().cpu().double()
+    assert (want > 0).any()
+    if dtype == HF:
+        tol = tol + 2.0**-25 + 32 * step * (c.v.double().abs().max() + want)  # (l is at least n / 32)
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol.clamp_min(1e-30)).max().item()
