@@ -251,8 +251,14 @@ __device__ __forceinline__ float group_max(float x) {
 // 2^LIFT instead of 1. A weight is then off by its own rounding or 2^-(25 + LIFT) of the
 // largest, whichever is more. Scores from 2^22 on are whole steps apart in fp32, and with
 // them the difference would be: they keep their place. bf16 and fp32 reach down to 2^-126.
+constexpr float kWholeScores = 4194304.0f;
+// x y, rounded (never part of a fused operation).
+__device__ __forceinline__ float product(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
+}
 template <class T, int LIFT> __device__ __forceinline__ float reference_of(float top) {
-  if constexpr (T::code == SY_F16) return fabsf(top) < 4194304.0f ? top - (float)LIFT : top;
+  if constexpr (T::code == SY_F16) return fabsf(top) < kWholeScores ? top - (float)LIFT : top;
   else return top;
 }
 
@@ -1072,13 +1078,29 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
         for (int d = 0; d < MD; ++d) o[d] *= sc;
       }
       const float mu = m == -INFINITY ? 0.0f : m;
+      // A product that is not rounded before the reference is taken off it may pass a rounded
+      // one: by an eighth where that is below 2^22, by more than the weights' room above.
+      // (The branch costs nothing at widths of 64 and 128 and 1 to 2 % at 256. Padded widths
+      // round every product instead, 2 to 4 %: the branch's registers cost 72 to 248 20 to 50 %.)
+      float sx = sl;
+      if (EXACT && __builtin_expect(__any(fabsf(mu) >= kWholeScores), 0)) {
+        asm volatile("" ::: "memory");
+        sx = 1.0f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[x][e] *= sl;
+      }
       i32x4_t p16[4];
       float sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float pf[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pf[e] = __builtin_amdgcn_exp2f(fmaf(st[k / 2][(k % 2) * 8 + e], sl, -mu));
+        for (int e = 0; e < 8; ++e) {
+          const float x = st[k / 2][(k % 2) * 8 + e];
+          pf[e] = __builtin_amdgcn_exp2f(EXACT ? fmaf(x, sx, -mu) : product(x, sl) - mu);
+        }
         // Weights are rounded to the values' dtype for the product (at most half a step,
         // independent of one another), and their sum is of the rounded ones: two a
         // v_dot2, half the additions.

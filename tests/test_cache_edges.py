@@ -178,3 +178,26 @@ def test_many_faint_tokens(dtype, shape, below):
     if dtype == HF:
         tol = tol + 2.0**-25 + 32 * step * (c.v.double().abs().max() + want)  # (l is at least n / 32)
     assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol.clamp_min(1e-30)).max().item()
+
+
+@pytest.mark.parametrize("q", [300.0, 3000.0, 60000.0, -300.0, -3000.0, -60000.0])
+@pytest.mark.parametrize("shape", FAINT, ids=[str(i) for i in range(len(FAINT))])
+@pytest.mark.parametrize("dtype,times", [(HF, 1.0), (BF, 1.0), (BF, 1e12), (F, 1.0)])
+@pytest.mark.parametrize("hd", [64, 80])
+def test_scores_past_every_step(hd, dtype, times, shape, q):
+    """Scores of 2^21 to 2^29 (bf16 to 2^109) of either sign: the nearest other is thousands
+    below the largest, so that the result is its value to the bit."""
+    new, past, kv, group, prefix, _ = shape
+    c = Case(new, past, kv=kv, group=group, hd=hd, page=32, dtype=dtype, prefix=prefix, seed=53)
+    g = torch.Generator().manual_seed(54)
+    c.q.zero_()
+    c.q[..., 0] = q * times
+    c.k.zero_()
+    c.k[..., 0] = times * (55000 + 10000 * torch.rand(c.k.shape[:3], generator=g) * (1 if q < 0 else -5))
+    want, at = torch.zeros(c.n_tok, c.heads, hd, dtype=dtype), 0
+    for b, n in enumerate(new):
+        first = c.prefix_ids[0] if prefix else int(c.table[b, 0])
+        c.k[first, :, 0, 0] = times * (50000.0 if q < 0 else 60000.0)
+        want[at:at + n] = c.v[first, :, 0].repeat_interleave(group, 0)
+        at += n
+    assert torch.equal(c.call().cpu(), want)
