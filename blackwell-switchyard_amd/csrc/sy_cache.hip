@@ -851,7 +851,7 @@ __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)"
 // either tile; and of an edge tile's keys, 1 it is there, 2 its value holds an infinity or NaN.
 template <int HD> constexpr int flash_lds() { return 4 * kFlashKeys * HD * 2 + 2 * kWaves * 4 + kFlashKeys * 4; }
 
-template <class T, int HD, bool EXACT>
+template <class T, int HD, bool EXACT, bool TWO>
 __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const int direct, float* const row_o,
                                       float* const row_ml, const int block, char* const shared) {
   using S = typename T::storage;
@@ -1092,6 +1092,7 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
           for (int e = 0; e < 16; ++e) st[x][e] *= sl;
       }
       i32x4_t p16[4];
+      [[maybe_unused]] i32x4_t p16r[4];
       float sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -1103,9 +1104,25 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
         }
         // Weights are rounded to the values' dtype for the product (at most half a step,
         // independent of one another), and their sum is of the rounded ones: two a
-        // v_dot2, half the additions.
+        // v_dot2, half the additions. As two numbers (TWO) they would make three products
+        // of the two that bound this kernel: error 2.0e-3 or 1.64e-3 in bf16, 2.9e-4 or
+        // 2.1e-4 in fp16, and prompts 76 or 93 us, pieces of them 198 or 272. A prefix's
+        // pass, whose rows are few, takes them as k_attend does: there the products wait
+        // for memory (64 rows behind 4096 tokens 38.1 and 39.0 us, 16 of 4 heads each
+        // behind 30011 47.4 and 50.9), and a token's result does not depend on how many
+        // others share the prefix.
         p16[k] = pack<T>(pf);
-        sum = dot<T>(p16[k], ones, sum);
+        if constexpr (TWO) {
+          float rest[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            rest[e] = pf[e] - elem<T>(p16[k], e);
+            sum += pf[e];
+          }
+          p16r[k] = pack<T>(rest);
+        } else {
+          sum = dot<T>(p16[k], ones, sum);
+        }
       }
       l += sum;
       if (__builtin_expect(odd != 0, 0)) {
@@ -1114,12 +1131,16 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
         for (int j = 0; j < KT; ++j) {
           if ((odd >> j & 1) == 0) continue;
           const int e = 8 * (j >> 4) + 4 * ((j >> 3) & 1) + (j & 3);  // of the 32 weights of a lane
-          int word = p16[0][0];
+          const auto weight = [&](const i32x4_t (&p)[4]) {
+            int word = p[0][0];
 #pragma unroll
-          for (int x = 1; x < 16; ++x) word = e >> 1 == x ? p16[x / 4][x % 4] : word;
-          word = __shfl(word, col + 32 * ((j >> 2) & 1));
-          const i32x4_t w4 = {word, 0, 0, 0};
-          const float pv = (e & 1) ? elem<T>(w4, 1) : elem<T>(w4, 0);
+            for (int x = 1; x < 16; ++x) word = e >> 1 == x ? p[x / 4][x % 4] : word;
+            word = __shfl(word, col + 32 * ((j >> 2) & 1));
+            const i32x4_t w4 = {word, 0, 0, 0};
+            return (e & 1) ? elem<T>(w4, 1) : elem<T>(w4, 0);
+          };
+          float pv = weight(p16);
+          if constexpr (TWO) pv += weight(p16r);
           const int id = (own ? own_pages : a.prefix_pages)[(j0 + j) >> c.page_shift];
           const S* const vr = bytes_on(vb, row_at(c, id, j0 + j));
           if (own && j0 + j >= limit) continue;
@@ -1137,22 +1158,30 @@ __device__ __forceinline__ void flash(const AttendArgs& a, const Flash& f, const
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        i32x4_t w[MD];
 #pragma unroll
         for (int d = 0; d < MD; ++d) {
           if (!EXACT && d * 32 >= hd) continue;
-          i32x4_t w;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             char* const from = vl + buf * (KT * RB) + (16 * k + 8 * x) * RB + (value_at ^ (d * 64));
             const i16x4_t v4 =
                 __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t*)from);
             const i32x2_t v2 = __builtin_bit_cast(i32x2_t, v4);
-            w[2 * x] = v2[0];
-            w[2 * x + 1] = v2[1];
+            w[d][2 * x] = v2[0];
+            w[d][2 * x + 1] = v2[1];
           }
-          o[d] = mma32<T>(w, p16[k], o[d]);
+          o[d] = mma32<T>(w[d], p16[k], o[d]);
         }
+        if constexpr (TWO) {  // (no product next to the one whose sum it adds to)
+#pragma unroll
+          for (int d = 0; d < MD; ++d) {
+            if (!EXACT && d * 32 >= hd) continue;
+            o[d] = mma32<T>(w[d], p16r[k], o[d]);
+          }
+        }
+      }
     }
   }
 
@@ -1205,7 +1234,7 @@ template <class T, int HD, bool EXACT>
 __global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
 k_flash(const AttendArgs a, const Flash f, const int direct, const int zero, float* const row_o, float* const row_ml) {
   __shared__ __align__(16) char shared[flash_lds<HD>()];
-  flash<T, HD, EXACT>(a, f, direct, row_o, row_ml, blockIdx.x, shared);
+  flash<T, HD, EXACT, false>(a, f, direct, row_o, row_ml, blockIdx.x, shared);
   if (zero) zero_outside<T>(a);
 }
 
@@ -1215,16 +1244,16 @@ struct Rows {
 };
 
 // Both in one launch, where a call may bring sequences of either kind, or the pass over a
-// shared prefix goes with that over the sequences' own keys: the many rows' long workgroups
-// first, the equal runs of the few rows fill up behind them.
-template <class T, int HD, bool EXACT>
+// shared prefix goes with that over the sequences' own keys (PRE): the many rows' long
+// workgroups first, the equal runs of the few rows fill up behind them.
+template <class T, int HD, bool EXACT, bool PRE>
 __global__ void __launch_bounds__(kBlock, HD <= 128 ? 2 : 1)
 k_both(const AttendArgs a, const Cut u, const Flash f, const int direct_u, const int direct_f, const int zero,
        const Rows ru, const Rows rf) {
   __shared__ __align__(16) char shared[flash_lds<HD>() > attend_lds<T, HD>() ? flash_lds<HD>() : attend_lds<T, HD>()];
   const int many = f.tiles * a.c.kv_heads * f.splits;
   if ((int)blockIdx.x < many)
-    flash<T, HD, EXACT>(a, f, direct_f, rf.o, rf.ml, blockIdx.x, shared);
+    flash<T, HD, EXACT, PRE>(a, f, direct_f, rf.o, rf.ml, blockIdx.x, shared);
   else
     attend<T, HD, 1, EXACT>(a, u, direct_u, ru.o, ru.ml, blockIdx.x - many, shared);
   if (zero) zero_outside<T>(a);
@@ -1678,26 +1707,26 @@ struct Both {
   Rows ru, rf;
 };
 
-template <class T, int HD>
+template <class T, int HD, bool PRE>
 hipError_t both_t(const AttendArgs& a, const Both& b, hipStream_t s) {
   const dim3 grid((unsigned)(b.u.workers + b.f.tiles * a.c.kv_heads * b.f.splits));
   if (a.c.hd == HD)
-    hipLaunchKernelGGL((k_both<T, HD, true>), grid, dim3(kBlock), 0, s, a, b.u, b.f, b.direct_u, b.direct_f, b.zero,
+    hipLaunchKernelGGL((k_both<T, HD, true, PRE>), grid, dim3(kBlock), 0, s, a, b.u, b.f, b.direct_u, b.direct_f, b.zero,
                        b.ru, b.rf);
   else
-    hipLaunchKernelGGL((k_both<T, HD, false>), grid, dim3(kBlock), 0, s, a, b.u, b.f, b.direct_u, b.direct_f, b.zero,
+    hipLaunchKernelGGL((k_both<T, HD, false, PRE>), grid, dim3(kBlock), 0, s, a, b.u, b.f, b.direct_u, b.direct_f, b.zero,
                        b.ru, b.rf);
   return hipGetLastError();
 }
 
-template <class T>
+template <class T, bool PRE>
 hipError_t both_pass(const AttendArgs& a, const Both& b, hipStream_t s) {
   if constexpr (T::code == SY_F32) {
     return hipErrorInvalidConfiguration;
   } else {
-    if (a.c.hd <= 64) return both_t<T, 64>(a, b, s);
-    if (a.c.hd <= 128) return both_t<T, 128>(a, b, s);
-    return both_t<T, 256>(a, b, s);
+    if (a.c.hd <= 64) return both_t<T, 64, PRE>(a, b, s);
+    if (a.c.hd <= 128) return both_t<T, 128, PRE>(a, b, s);
+    return both_t<T, 256, PRE>(a, b, s);
   }
 }
 
@@ -1721,11 +1750,11 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   if (p.pre == 1) {
     e = attend_pass<T>(a, p.cpre, 0, 0, pre, s);
   } else if (p.pre == 2) {
-    e = both_pass<T>(a, Both{p.own, p.fpre, p.direct_attend, 0, zero, own, pre}, s);
+    e = both_pass<T, true>(a, Both{p.own, p.fpre, p.direct_attend, 0, zero, own, pre}, s);
     attend = false;
   }
   if (e == hipSuccess && attend && flash)
-    e = both_pass<T>(a, Both{p.own, p.fown, p.direct_attend, p.direct_flash, zero, own, own}, s), attend = flash = false;
+    e = both_pass<T, false>(a, Both{p.own, p.fown, p.direct_attend, p.direct_flash, zero, own, own}, s), attend = flash = false;
   if (e == hipSuccess && flash) e = flash_pass<T>(a, p.fown, p.direct_flash, zero && !p.attend, own, s);
   if (e == hipSuccess && attend) e = attend_pass<T>(a, p.own, p.direct_attend, zero, own, s);
   if (e != hipSuccess) return e;

@@ -156,14 +156,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of the new tokens' queries ``q [n_tok, heads, head_dim]`` over the cache:
     each row sees its own position and every earlier one, and the whole prefix. Query head
     ``h`` reads kv head ``h * kv_heads // heads``; ``scale`` is ``head_dim**-0.5`` by
-    default. A row that sees nothing is zero. Scores, softmax statistics and sums are
-    fp32. Where a sequence brings more than 16 rows a kv head to a 16-bit cache, or the rows
-    that share a prefix are more than 16, the weights are rounded to its dtype for the second
-    product (relative error 2.0e-3 in bf16, of which the output's own rounding is 1.7e-3):
-    a token's result behind a prefix so depends, within that, on how many share it. Where there
-    are fewer the product takes a weight as two numbers, the rounded one and what it lacks.
-    fp16 weights below 2^-21 of the largest (as two numbers 2^-18) are off by up to 2^-32
-    (2^-40) of it."""
+    default. A row that sees nothing is zero; an infinite value that a row sees makes its
+    channel infinite or NaN, one that it does not see changes nothing.
+
+    Scores, softmax statistics and sums are fp32. Where a sequence brings more than 16 rows a
+    kv head to a 16-bit cache, the weights are rounded to its dtype for the second product
+    (relative error 2.0e-3 in bf16, of which the output's own rounding is 1.7e-3); so they are
+    for all sequences behind a prefix that bring more than 16 on average. Where there are fewer
+    the product takes a weight as two numbers, the rounded one and what it lacks. fp16 weights
+    below 2^-21 of the largest (as two numbers 2^-18) are off by up to 2^-32 (2^-40) of it."""
     if (_lib.ordinary(q, k_cache, v_cache, page_table, lengths) and q.is_cuda and type(prefix_len) is int
             and (starts is None or _lib.ordinary(starts)) and (out is None or _lib.ordinary(out))
             and (prefix_pages is None or _lib.ordinary(prefix_pages))):
