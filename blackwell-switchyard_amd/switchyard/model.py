@@ -306,7 +306,8 @@ class DecodeState:
     in pages of its own (``cache_op``), and how many tokens each sequence has.
 
     ``max_len`` tokens a sequence, ``prefix_len`` more that all of them share (the prefix is
-    filled by ``Transformer.decode(..., to_prefix=True)``, before anything else)."""
+    filled by ``Transformer.decode(..., to_prefix=True)``, before anything else; another one
+    may take its place when ``reset`` has forgotten the tokens behind it)."""
 
     def __init__(self, model: Transformer, batch: int, max_len: int, *, page: int = 64, prefix_len: int = 0) -> None:
         cfg, w = model.cfg, model.embed.weight
@@ -333,10 +334,12 @@ class DecodeState:
         # The kernels take fp32 tables; a model cast as a whole has rounded ones, as its training has.
         self.cos, self.sin = model.rotary.cos.float(), model.rotary.sin.float()
         self._prefix_filled = prefix_len == 0
+        self._begun = False  # a sequence has tokens of its own
 
     def reset(self) -> None:
         """Forget the sequences' own tokens; the prefix stays."""
         self.lengths.zero_()
+        self._begun = False
 
 
 class _CacheStep:
@@ -638,6 +641,8 @@ class Transformer(nn.Module):
         if to_prefix:
             if tokens.shape != (state.prefix_len,) or starts is not None or state.prefix_len == 0:
                 raise ValueError(f"the prefix must be [{state.prefix_len}] tokens, got {tuple(tokens.shape)}")
+            if state._begun:
+                raise ValueError("the sequences' tokens stand behind the present prefix; reset() forgets them")
             lengths = torch.full((1,), state.prefix_len, device=state.k.device, dtype=torch.int32)
         elif not state._prefix_filled:
             raise ValueError("the state's prefix has to be filled first (to_prefix=True)")
@@ -665,6 +670,7 @@ class Transformer(nn.Module):
             state._prefix_filled = True
         else:
             state.lengths.copy_(lengths)  # (a call that raised has added nothing)
+            state._begun = True
         return logits
 
     @torch.no_grad()
