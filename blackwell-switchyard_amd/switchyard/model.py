@@ -643,6 +643,7 @@ class Transformer(nn.Module):
                 raise ValueError(f"the prefix must be [{state.prefix_len}] tokens, got {tuple(tokens.shape)}")
             if state._begun:
                 raise ValueError("the sequences' tokens stand behind the present prefix; reset() forgets them")
+            state._prefix_filled = False  # (until all layers have it)
             lengths = torch.full((1,), state.prefix_len, device=state.k.device, dtype=torch.int32)
         elif not state._prefix_filled:
             raise ValueError("the state's prefix has to be filled first (to_prefix=True)")

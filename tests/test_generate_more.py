@@ -30,3 +30,15 @@ def test_another_prefix_needs_a_reset():
     state.reset()
     m.decode(second, state, to_prefix=True)
     _close(m.decode(idx, state), m(torch.cat((second.expand(2, -1), idx), 1))[:, -1].detach())
+
+
+def test_a_prefix_that_failed_is_no_prefix():
+    m = _model()
+    state = DecodeState(m, 2, 16, page=16, prefix_len=7)
+    m.decode(_tokens(7).cuda(), state, to_prefix=True)
+    hook = m.layers[1].mlp.register_forward_pre_hook(lambda *_: (_ for _ in ()).throw(RuntimeError("stop")))
+    with pytest.raises(RuntimeError, match="stop"):
+        m.decode(_tokens(7, seed=2).cuda(), state, to_prefix=True)
+    hook.remove()
+    with pytest.raises(ValueError, match="filled first"):
+        m.decode(_tokens(2, 3).cuda(), state)
