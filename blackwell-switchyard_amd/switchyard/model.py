@@ -307,7 +307,9 @@ class DecodeState:
 
     ``max_len`` tokens a sequence, ``prefix_len`` more that all of them share (the prefix is
     filled by ``Transformer.decode(..., to_prefix=True)``, before anything else; another one
-    may take its place when ``reset`` has forgotten the tokens behind it)."""
+    may take its place when ``reset`` has forgotten the tokens behind it). Under autocast the
+    pages have its dtype, as the projections have: a state goes with the calls of the setting
+    it was made in."""
 
     def __init__(self, model: Transformer, batch: int, max_len: int, *, page: int = 64, prefix_len: int = 0) -> None:
         cfg, w = model.cfg, model.embed.weight
@@ -326,8 +328,9 @@ class DecodeState:
         self.batch, self.max_len, self.prefix_len = batch, max_len, prefix_len
         shared, own = -(-prefix_len // page), -(-max_len // page)
         shape = (cfg.n_layers, shared + batch * own, cfg.n_heads, page, cfg.head_dim)
-        self.k = torch.zeros(shape, device=dev, dtype=w.dtype)
-        self.v = torch.zeros(shape, device=dev, dtype=w.dtype)
+        dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else w.dtype
+        self.k = torch.zeros(shape, device=dev, dtype=dtype)
+        self.v = torch.zeros(shape, device=dev, dtype=dtype)
         self.prefix_pages = torch.arange(shared, **ints)
         self.page_table = torch.arange(shared, shared + batch * own, **ints).view(batch, own)
         self.lengths = torch.zeros(batch, **ints)

@@ -42,3 +42,25 @@ def test_a_prefix_that_failed_is_no_prefix():
     hook.remove()
     with pytest.raises(ValueError, match="filled first"):
         m.decode(_tokens(2, 3).cuda(), state)
+
+
+@pytest.mark.parametrize("residual", ["standard", "attnres", "switchyard"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast(dtype, residual):
+    """fp32 weights under autocast, as the forward takes them: no further from the fp32 logits
+    than twice the forward is."""
+    m = _model(residual)
+    idx, prefix = _tokens(3, 33).cuda(), _tokens(20, seed=2).cuda()
+    seq = torch.cat((prefix.expand(3, -1), idx), 1)
+    with torch.no_grad():
+        exact = m(seq)[:, [-2, -1]]
+        with torch.autocast("cuda", dtype=dtype):
+            near = m(seq)[:, [-2, -1]]
+            state = DecodeState(m, 3, 40, page=16, prefix_len=20)
+            m.decode(prefix, state, to_prefix=True)
+            got = torch.stack((m.decode(idx[:, :-1], state), m.decode(idx[:, -1:], state)), 1)
+            assert state.k.dtype == dtype and got.dtype == near.dtype
+            assert (m.generate(idx, 4, prefix=prefix) >= 0).all()
+        assert (got.float() - exact).norm() <= 2 * (near.float() - exact).norm()
+        with pytest.raises(ValueError, match="same dtype"):  # a state of the other setting
+            m.decode(idx[:, -1:], state)
