@@ -533,11 +533,10 @@ hipError_t sample_n(const SampleArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t sample_t(const SampleArgs& a, hipStream_t s) {
-  // Whole chunks of every lane, which is what the kernel stores. Short rows leave room for
-  // a second workgroup on a CU.
+  // Whole chunks of every lane, which is what the kernel stores. (Less LDS for short rows
+  // would put no second workgroup on a CU: sixteen waves of 90 registers fill it.)
   const int64_t chunks = (a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce);
   const int64_t bytes = chunks * kBlock * 16;
-  if (bytes <= 16384) return sample_n<T, 16384>(a, s);
   if (bytes <= 81920) return sample_n<T, 81920>(a, s);
   return sample_n<T, 0>(a, s);
 }
