@@ -532,13 +532,36 @@ hipError_t sample_n(const SampleArgs& a, hipStream_t s) {
 }
 
 template <class T>
-hipError_t sample_t(const SampleArgs& a, hipStream_t s) {
+hipError_t sample_rows(const SampleArgs& a, hipStream_t s) {
   // Whole chunks of every lane, which is what the kernel stores. (Less LDS for short rows
   // would put no second workgroup on a CU: sixteen waves of 90 registers fill it.)
   const int64_t chunks = (a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce);
   const int64_t bytes = chunks * kBlock * 16;
   if (bytes <= 81920) return sample_n<T, 81920>(a, s);
   return sample_n<T, 0>(a, s);
+}
+
+// A launch has less than 2^32 threads: 2^21 rows at a time.
+template <class T>
+hipError_t sample_t(const SampleArgs& a, hipStream_t s) {
+  constexpr int64_t kMost = 1 << 21;
+  hipError_t e = hipSuccess;
+  for (int64_t r = 0; r < a.n_rows && e == hipSuccess; r += kMost) {
+    SampleArgs b = a;
+    const auto from = [&](auto& p) {
+      if (p != nullptr) p += r;
+    };
+    b.logits = static_cast<const typename T::storage*>(a.logits) + r * a.row_stride;
+    from(b.u);
+    from(b.tokens);
+    from(b.how.temperatures);
+    from(b.how.top_ps);
+    from(b.how.min_ps);
+    from(b.how.top_ks);
+    b.n_rows = std::min(a.n_rows - r, kMost);
+    e = sample_rows<T>(b, s);
+  }
+  return e;
 }
 
 }  // namespace
