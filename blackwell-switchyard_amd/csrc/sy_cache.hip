@@ -1508,6 +1508,7 @@ int whole_tokens(int64_t workgroups, bool beside) {
 }
 
 constexpr int64_t kMost = 0x7fffffff;
+constexpr int64_t kMostGroups = 0xffffff;  // workgroups of a launch, which has less than 2^32 threads
 
 // What a call launches: k_attend over the sequences of few rows, k_flash over the others,
 // one of them over a shared prefix, and the merge of what was cut.
@@ -1592,6 +1593,16 @@ bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int 
   return grid * f->splits <= kMost / kFlashRows;  // (of rows, and so of the merge's workgroups)
 }
 
+// Workgroups of the merge's launch, and the heads that one of them takes: one, until there
+// are far more rows than fit the device at once.
+int64_t merge_groups(const CacheArgs& c, const Plan& p, int* per_wg) {
+  const int64_t toks = p.merge_few ? (int64_t)c.n_seq * p.merge_few : c.n_tok;
+  const int heads = (int)std::min<int64_t>(c.heads, std::max<int64_t>(1, toks * c.heads / 8192));
+  if (per_wg != nullptr) *per_wg = heads;
+  return (p.merge_flash ? (int64_t)p.fown.tiles * c.kv_heads * (kFlashRows / kMergeRows) : 0) +
+         (p.merge ? toks * ((c.heads + heads - 1) / heads) : 0);
+}
+
 Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
   Plan p{};
   int cus = 0;
@@ -1630,6 +1641,11 @@ Plan plan_attend(const CacheArgs& c, int64_t prefix_len, int dtype) {
   p.merge = p.pre != 0 || cut_attend;
   p.merge_flash = p.pre == 0 && p.flash && p.fown.splits > 1;
   p.merge_few = p.pre == 0 && p.flash ? std::max(1, 16 / c.group) : 0;
+  const auto flash_groups = [&](const Flash& f) { return (int64_t)f.tiles * c.kv_heads * f.splits; };
+  const int64_t own_groups = p.attend ? p.own.workers : 0;
+  p.ok = own_groups + std::max(p.flash ? flash_groups(p.fown) : 0, p.pre == 2 ? flash_groups(p.fpre) : 0) <= kMostGroups &&
+         (int64_t)p.cpre.workers <= kMostGroups && merge_groups(c, p, nullptr) <= kMostGroups;
+  if (!p.ok) return p;
   int64_t at = 0;
   const auto take = [&](int64_t n) {
     const int64_t was = at;
@@ -1761,12 +1777,8 @@ hipError_t attend_dt(const AttendArgs& a, hipStream_t s) {
   if (!p.merge && !p.merge_flash) return e;
   const int many = p.merge_flash ? p.fown.tiles * a.c.kv_heads * (kFlashRows / kMergeRows) : 0;
   JoinArgs g{p.own, p.cpre, p.fown, p.fpre, p.pre, 1, p.merge_few, many, own.o, own.ml, pre.o, pre.ml};
-  // Heads a workgroup: one, until there are far more rows than fit the device at once.
-  const int64_t toks = p.merge_few ? (int64_t)a.c.n_seq * p.merge_few : a.c.n_tok;
-  g.per_wg = (int)std::min<int64_t>(a.c.heads, std::max<int64_t>(1, toks * a.c.heads / 8192));
-  const int64_t grid = p.merge ? toks * ((a.c.heads + g.per_wg - 1) / g.per_wg) : 0;
-  if (grid > kMost - many) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((k_merge<T>), dim3((unsigned)(many + grid)), dim3(kBlock), 0, s, a, g);
+  const unsigned grid = (unsigned)merge_groups(a.c, p, &g.per_wg);
+  hipLaunchKernelGGL((k_merge<T>), dim3(grid), dim3(kBlock), 0, s, a, g);
   return hipGetLastError();
 }
 

@@ -52,3 +52,14 @@ def test_the_functions_refuse_them_too(fn):
         fn(*head, k, k, torch.zeros(1, 4, dtype=torch.int32), lengths, prefix_len=(1 << 30) + 1)
     with pytest.raises(ValueError, match="page_table"):
         fn(*head, k, k, torch.zeros(1, 1025, dtype=torch.int32), lengths)
+
+
+def test_launches_of_2_to_32_threads_are_refused():
+    """A workgroup of 256 threads for every token of 2^24 sequences, or for its merge."""
+    lib = _lib.lib()
+    more = dict(page=1, page_stride=8, head_stride=8, table_cols=1, table_stride=1)
+    for n, prefix, rc in ((1 << 24, 0, SHAPE), ((1 << 24) - 1, 0, OK), (1 << 24, 100, SHAPE), (1 << 23, 100, OK)):
+        need = lib.sy_paged_attention_workspace_bytes(ctypes.byref(_paged(n_seq=n, n_tok=n, **more)), prefix)
+        assert need == rc if rc else need >= 0, (n, prefix, need)
+    wide = ctypes.byref(_paged(n_seq=1 << 21, n_tok=1 << 21, heads=8, kv_heads=8, **more))
+    assert lib.sy_paged_attention_workspace_bytes(wide, 0) == SHAPE
