@@ -236,3 +236,22 @@ def test_infinities_around_a_prefixs_end(new, dtype):
     u = torch.finfo(dtype).eps / 2
     ref = want.double()
     assert ((got.double() - ref).abs() <= 2 * u * ref.abs() + (2 * u if dtype != F else 2.0**-15) * 4).all()
+
+
+WIDTHS = [
+    # new, past, kv, group, page, prefix
+    ([1, 1, 1], [5, 0, 70], 2, 2, 16, 333),  # a prefix for few rows
+    ([1] * 40, list(range(40)), 1, 3, 32, 333),  # its pass for many, next to each sequence's own
+    ([90, 41], [0, 7], 1, 2, 16, 100),  # before many rows of each
+    ([20], [5000], 1, 1, 64, 0),  # a row tile's keys in parts, joined
+    ([40, 3, 1], [2500, 4000, 900], 2, 1, 16, 0),  # next to sequences of few rows
+    ([1] * 24, list(range(24)), 1, 1, 32, 3000),  # a prefix's keys in parts
+]
+
+
+@pytest.mark.parametrize("hd", [8, 40, 64, 80, 96, 128, 136, 256])
+@pytest.mark.parametrize("shape", WIDTHS, ids=[str(i) for i in range(len(WIDTHS))])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_widths_behind_prefixes_and_in_parts(dtype, shape, hd):
+    new, past, kv, group, page, prefix = shape
+    Case(new, past, kv=kv, group=group, hd=hd, page=page, dtype=dtype, prefix=prefix, seed=71).check()
