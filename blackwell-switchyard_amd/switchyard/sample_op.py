@@ -50,6 +50,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     """One token (int64) for each row of ``logits [B, V]`` from the uniform numbers ``u [B]``
     (fp32, in ``[0, 1)``). Every setting is a number, or a tensor ``[B]`` of one a row
     (fp32; ``top_k`` int32) that is read on the device."""
+    if torch.compiler.is_compiling():
+        return _untraced(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     t, ts = _split("temperature", temperature)
     k, ks = _split("top_k", top_k, integer=True)
     p, ps = _split("top_p", top_p)
@@ -82,3 +84,6 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
                                   _lib.stream_ptr(logits.device))
     _lib.check(rc, "sy_sample")
     return tokens
+
+
+_untraced = torch.compiler.disable(sample_tokens)  # what a compiler's trace calls

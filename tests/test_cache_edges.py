@@ -24,6 +24,7 @@ if not torch.cuda.is_available():  # pragma: no cover
 from test_cache_op import Case  # noqa: E402
 
 from switchyard.cache_op import paged_append, paged_attention  # noqa: E402
+from switchyard.sample_op import sample_tokens  # noqa: E402
 
 DEV = "cuda"
 BF, HF, F = torch.bfloat16, torch.float16, torch.float32
@@ -255,3 +256,26 @@ WIDTHS = [
 def test_widths_behind_prefixes_and_in_parts(dtype, shape, hd):
     new, past, kv, group, page, prefix = shape
     Case(new, past, kv=kv, group=group, hd=hd, page=page, dtype=dtype, prefix=prefix, seed=71).check()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_a_compiled_caller(dtype):
+    """A compiler's trace steps around the functions: same results, same writes, every time."""
+    c = Case([1, 2], [5, 20], kv=1, group=2, hd=64, page=16, dtype=dtype, prefix=20, seed=72)
+    cos, sin = torch.ones(64, 32, device=DEV), torch.zeros(64, 32, device=DEV)
+    qkv = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(73)).to(dtype).to(DEV)
+    more = dict(prefix_pages=torch.tensor(c.prefix_ids, dtype=torch.int32, device=DEV), prefix_len=20)
+    u = torch.rand(3, generator=torch.Generator().manual_seed(74)).to(DEV)
+
+    def step(qkv, k, v, table, lengths, starts):
+        q = paged_append(qkv * 2, cos, sin, k, v, table, lengths, starts, prefix_len=20)
+        o = paged_attention(q, k, v, table, lengths, starts, **more) + 1
+        return o, sample_tokens(o.flatten(1), u, temperature=0.7, top_k=5) * 2
+
+    got = []
+    compiled = torch.compile(step, backend="eager")
+    for fn in (step, compiled, compiled):
+        k, v = c.k.to(DEV), c.v.to(DEV)
+        with torch.no_grad():
+            got.append((*fn(qkv, k, v, c.table.to(DEV), c.lengths.to(DEV), c.starts.to(DEV)), k, v))
+    assert all(torch.equal(a, b) for some in zip(*got) for a, b in zip(some, some[1:]))
