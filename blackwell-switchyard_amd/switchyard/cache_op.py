@@ -117,15 +117,15 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
     ``cos``, ``sin`` are fp32 ``[positions, head_dim / 2]`` (``[positions, 1, ...]`` as
     the decoder's). Row ``i`` of ``n`` new ones stands at ``lengths[b] - n + i``, behind
     ``prefix_len``. Arithmetic is fp32, every output rounded once."""
-    if torch.compiler.is_compiling():
-        return _append_untraced(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len=prefix_len,
-                                out=out)
     if (_lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths) and qkv.is_cuda
             and type(prefix_len) is int and (starts is None or _lib.ordinary(starts))
             and (out is None or _lib.ordinary(out))):
         q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out)
         if q is not None:
             return q
+    if torch.compiler.is_compiling():
+        return _append_untraced(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len=prefix_len,
+                                out=out)
     _no_backward("paged_append", qkv, cos, sin, k_cache, v_cache, out)
     _need(qkv.ndim == 3, f"qkv must be [n_tok, heads + 2 kv_heads, head_dim], got {tuple(qkv.shape)}")
     _need(k_cache.ndim == 4, "k_cache must be [n_pages, kv_heads, page, head_dim]")
@@ -168,9 +168,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     for all sequences behind a prefix that bring more than 16 on average. Where there are fewer
     the product takes a weight as two numbers, the rounded one and what it lacks. fp16 weights
     below 2^-21 of the largest (as two numbers 2^-18) are off by up to 2^-32 (2^-40) of it."""
-    if torch.compiler.is_compiling():
-        return _attention_untraced(q, k_cache, v_cache, page_table, lengths, starts, prefix_pages=prefix_pages,
-                                   prefix_len=prefix_len, scale=scale, out=out)
     if (_lib.ordinary(q, k_cache, v_cache, page_table, lengths) and q.is_cuda and type(prefix_len) is int
             and (starts is None or _lib.ordinary(starts)) and (out is None or _lib.ordinary(out))
             and (prefix_pages is None or _lib.ordinary(prefix_pages))):
@@ -178,6 +175,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                           q.shape[-1] ** -0.5 if scale is None else scale, out)
         if o is not None:
             return o
+    if torch.compiler.is_compiling():
+        return _attention_untraced(q, k_cache, v_cache, page_table, lengths, starts, prefix_pages=prefix_pages,
+                                   prefix_len=prefix_len, scale=scale, out=out)
     _no_backward("paged_attention", q, k_cache, v_cache, out)
     _need(q.ndim == 3, f"q must be [n_tok, heads, head_dim], got {tuple(q.shape)}")
     prefix_len = int(prefix_len)

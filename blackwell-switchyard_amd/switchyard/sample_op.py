@@ -50,8 +50,6 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     """One token (int64) for each row of ``logits [B, V]`` from the uniform numbers ``u [B]``
     (fp32, in ``[0, 1)``). Every setting is a number, or a tensor ``[B]`` of one a row
     (fp32; ``top_k`` int32) that is read on the device."""
-    if torch.compiler.is_compiling():
-        return _untraced(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     t, ts = _split("temperature", temperature)
     k, ks = _split("top_k", top_k, integer=True)
     p, ps = _split("top_p", top_p)
@@ -60,6 +58,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
         tokens = _lib.native().sample_tokens(logits, u, t, k, p, m, ts, ks, ps, ms)
         if tokens is not None:
             return tokens
+    if torch.compiler.is_compiling():
+        return _untraced(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     if logits.ndim != 2:
         raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
     b, v = logits.shape
