@@ -279,3 +279,38 @@ def test_a_compiled_caller(dtype):
         with torch.no_grad():
             got.append((*fn(qkv, k, v, c.table.to(DEV), c.lengths.to(DEV), c.starts.to(DEV)), k, v))
     assert all(torch.equal(a, b) for some in zip(*got) for a, b in zip(some, some[1:]))
+
+
+def _many(dtype, new, past, **kw):
+    return Case(new, past, kv=1, group=1, hd=64, page=16, dtype=dtype, seed=81, **kw)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_more_sequences_than_lanes(dtype):
+    """Of many rows each, evenly and raggedly; and thousands of single tokens, shared out."""
+    _many(dtype, [20] * 70, [3 * i for i in range(70)]).check()
+    _many(dtype, [20, 1, 33, 0, 130] * 30, [i for i in range(150)]).check()
+    _many(dtype, [20, 1, 33, 0, 130] * 15, [i for i in range(75)], prefix=50).check()
+    c = _many(dtype, [1] * 3000, [i % 60 for i in range(3000)])
+    want = c.call()
+    c.check(want)
+    c.check(c.call(packed=True))
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("prefix", [0, 50])
+@pytest.mark.parametrize("rows", [3, 200])
+def test_rows_of_no_sequence_at_all(rows, prefix, dtype):
+    c = _many(dtype, [rows, 0, 0], [40, 3, 900], prefix=prefix)
+    q = c.q.to(DEV)
+    for at in (0, 1, rows):
+        c.starts = torch.full((4,), at, dtype=torch.int32)
+        assert (c.call() == 0).all()
+        out = torch.full_like(q, 3.0)
+        c.call(out=out)
+        assert (out == 3).all()
+    k, v = c.k.to(DEV), c.v.to(DEV)
+    ones = torch.ones(1000, 32, device=DEV)
+    qkv = torch.randn(rows, 3, 64, device=DEV).to(dtype)
+    got = paged_append(qkv, ones, ones, k, v, c.table.to(DEV), c.lengths.to(DEV), c.starts.to(DEV))
+    assert (got == 0).all() and torch.equal(k.cpu(), c.k) and torch.equal(v.cpu(), c.v)
