@@ -794,7 +794,7 @@ k_attend(const AttendArgs a, const Cut u, const int direct, const int zero, floa
 // Bound by the matrix cores and, next to them, by the exponentials (a quarter of the
 // vector rate): a wave's tile of heads of 128 is 1024 cycles of products and about as many of
 // softmax, which two waves a SIMD overlap. Long even sequences run at 760 TFLOP/s (heads of
-// 128, 16 of each kind), 930 (32 that share 8), 745 (heads of 64) and 480 (256, one workgroup
+// 128, 16 of each kind), 930 (32 that share 8), 750 (heads of 64) and 465 (256, one workgroup
 // a CU); four prompts of up to 2048 tokens at 530, as the causal triangles' ends leave CUs
 // idle. A large bf16 product of the library runs at 1070.
 struct Flash {
@@ -1502,7 +1502,7 @@ __global__ void __launch_bounds__(kBlock) k_merge(const AttendArgs a, const Join
 // With more than two a CU the long ones among sequences of any lengths may start last: 1024
 // over up to 2048 tokens 130 us whole, 116 shared out (180 and 190 where all are as long),
 // 2048 over up to 1024 125 and 129. Next to a prefix's pass they start behind it anyway: 128
-// over 1024 tokens behind 30011 shared ones 57.8 us whole, 52.0 shared out.
+// over up to 1024 tokens behind 30011 shared ones 52.0 us whole, 51.3 shared out.
 int whole_tokens(int64_t workgroups, bool beside) {
   return beside || workgroups < 128 ? 512 : workgroups >= 256 && workgroups < 512 ? 2048 : 1024;
 }
@@ -1559,7 +1559,7 @@ bool cut(const CacheArgs& c, int dtype, bool pre, bool beside, int64_t len, int 
 // Prompts see half of their own tokens on average, and sequences are rarely of one length.
 // A prefix's parts are all as long, and the sequences' own keys fill what they leave idle:
 // there the CU with the most of them counts (30011 tokens behind 8 kv heads: 32 parts, one a
-// CU, 47.6 us; 48, two on half of the CUs, 52.1).
+// CU, 53.3 us; 24 58.0; 48, two on half of the CUs, 54.8).
 bool flash_cut(const CacheArgs& c, bool pre, bool virt, int64_t prefix_len, int few, int cus, Flash* f) {
   f->pre = pre;
   f->virt = virt;

@@ -21,8 +21,8 @@
 // 8 rows of 32000 bf16 with top-k and top-p take 17.7 us (72 with the rows in registers):
 // one workgroup a CU, bound by the latency of its passes one after another. 256 rows of
 // 50257 fp32 with top-p take 82 us (230): the row's 201 KB are read four times from the
-// last cache, and of a workgroup's time 42 % go into the histogram with its double exp, 19 %
-// into gathering, 14 % into the maximum, 8 % into the ranking and 12 % into the draw.
+// last cache, and of a workgroup's time 42 % go into the histogram with its double exp, 18 %
+// into gathering, 14 % into the maximum, 7 % into the ranking and 19 % into the draw.
 #include <algorithm>
 
 #include "sy_launch.hpp"
