@@ -244,6 +244,12 @@ __device__ __forceinline__ float group_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// x y, rounded (never part of a fused operation).
+__device__ __forceinline__ float product(float x, float y) {
+#pragma clang fp contract(off)
+  return x * y;
+}
+
 // What a pass takes the exponentials relative to: the largest score, or a little below it.
 // fp16 ends at 2^-14 (2^-24 with fewer bits), and a context of 10^5 faint tokens behind one
 // strong one has weights below both that make up a percent of a row together. Their sum is
@@ -252,11 +258,6 @@ __device__ __forceinline__ float group_max(float x) {
 // largest, whichever is more. Scores from 2^22 on are whole steps apart in fp32, and with
 // them the difference would be: they keep their place. bf16 and fp32 reach down to 2^-126.
 constexpr float kWholeScores = 4194304.0f;
-// x y, rounded (never part of a fused operation).
-__device__ __forceinline__ float product(float x, float y) {
-#pragma clang fp contract(off)
-  return x * y;
-}
 template <class T, int LIFT> __device__ __forceinline__ float reference_of(float top) {
   if constexpr (T::code == SY_F16) return fabsf(top) < kWholeScores ? top - (float)LIFT : top;
   else return top;
@@ -601,7 +602,7 @@ __device__ __forceinline__ void attend(const AttendArgs& a, const Cut& u, const 
 #pragma unroll
           for (int x = 0; x < MT; ++x)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[x * 4 + e] = st[n][x][e] * sl;
+            for (int e = 0; e < 4; ++e) y[x * 4 + e] = product(st[n][x][e], sl);  // as the maximum is
           if (!full) {
 #pragma unroll
             for (int x = 0; x < MT; ++x) {
