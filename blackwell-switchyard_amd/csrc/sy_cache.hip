@@ -178,6 +178,81 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
   }
 }
 
+// The same behind a norm of every query and key head, u = x r g with r = 1 / sqrt(mean(x^2) +
+// eps): L lanes a head, a power of two, of which the ones past it do nothing, each with two
+// chunks of VE elements that turn together; the sum of squares stays among them.
+template <class T, int VE, int L>
+__global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a) {
+  using S = typename T::storage;
+  const CacheArgs& c = a.c;
+  const int half = c.hd / 2, part = threadIdx.x % L, ch = part * VE;
+  const int rows = c.heads + 2 * c.kv_heads;
+  const float inv_hd = 1.0f / (float)c.hd;
+  const bool in_head = ch < half;
+  S* const q = static_cast<S*>(a.q);
+  for (int tok = blockIdx.x; tok < c.n_tok; tok += gridDim.x) {
+    const S* const from = static_cast<const S*>(a.qkv) + tok * a.tok_stride;
+    const int b = find_seq(c, tok);
+    if (b < 0) {
+      if (a.fill && outside(c, tok)) {
+        const Chunk<T, VE> zero{};
+        for (int i = threadIdx.x; i < c.heads * c.hd / VE; i += kBlock)
+          st_chunk<T, VE>(q + (int64_t)tok * c.heads * c.hd + i * VE, zero);
+      }
+      continue;
+    }
+    const Seq s = seq_of(c, b);
+    const int j = s.len - s.n + (tok - s.row0);  // position among the sequence's own tokens
+    const int64_t at = j + a.offset;
+    uint64_t dst = 0;
+    bool placed = j >= 0 && j < c.cap && at < a.n_pos;
+    if (placed) {
+      const int id = c.table[b * c.table_stride + (j >> c.page_shift)];
+      placed = (unsigned)id < (unsigned)c.n_pages;
+      if (placed) dst = row_at(c, id, j);
+    }
+    // (Whole waves go round together: their lanes add up their squares.)
+    for (int head0 = 0; head0 < rows; head0 += kBlock / L) {
+      const int head = head0 + threadIdx.x / L;
+      const bool live = in_head && head < rows;
+      Chunk<T, VE> lo{}, hi{};
+      if (live) {
+        const S* const src = from + head * a.head_stride + ch;
+        lo = ld_chunk<T, VE>(src);
+        hi = ld_chunk<T, VE>(src + half);
+      }
+      const float r = head_rinv<VE, L>(lo.f, hi.f, inv_hd, a.eps);
+      if (!live) continue;
+      if (head < c.heads + c.kv_heads && placed) {
+        const float* const cp = a.cosv + at * half + ch;
+        const float* const sp = a.sinv + at * half + ch;
+        const void* const g = head < c.heads ? a.q_gain : a.k_gain;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          lo.f[e] *= r * load_elem(g, ch + e, a.gain_dtype);
+          hi.f[e] *= r * load_elem(g, half + ch + e, a.gain_dtype);
+          turn(lo.f[e], hi.f[e], cp[e], sp[e]);
+        }
+      }
+      S* out;
+      if (head < c.heads) {
+        if (!placed) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) lo.f[e] = hi.f[e] = __int_as_float(0x7fc00000);
+        }
+        out = q + ((int64_t)tok * c.heads + head) * c.hd + ch;
+      } else {
+        if (!placed) continue;
+        const bool key = head < c.heads + c.kv_heads;
+        const int h = head - c.heads - (key ? 0 : c.kv_heads);
+        out = bytes_on(static_cast<S*>(key ? c.k : c.v) + h * c.head_stride + ch, dst);
+      }
+      st_chunk<T, VE>(out, lo);
+      st_chunk<T, VE>(out + half, hi);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ attention
 //
 // One pass over the keys with the running maximum m and sum l of a softmax:
@@ -1790,6 +1865,28 @@ hipError_t append_t(const AppendArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <class T, int VE, int L>
+hipError_t append_norm_t(const AppendArgs& a, hipStream_t s) {
+  const unsigned grid = (unsigned)std::min(a.c.n_tok, 1 << 20);
+  hipLaunchKernelGGL((k_append_norm<T, VE, L>), dim3(grid), dim3(kBlock), 0, s, a);
+  return hipGetLastError();
+}
+
+template <class T, int VE>
+hipError_t append_norm_lanes(const AppendArgs& a, hipStream_t s) {
+  int lanes = 1;
+  while (lanes * VE < a.c.hd / 2) lanes *= 2;
+  switch (lanes) {
+    case 1: return append_norm_t<T, VE, 1>(a, s);
+    case 2: return append_norm_t<T, VE, 2>(a, s);
+    case 4: return append_norm_t<T, VE, 4>(a, s);
+    case 8: return append_norm_t<T, VE, 8>(a, s);
+    case 16: return append_norm_t<T, VE, 16>(a, s);
+    case 32: return append_norm_t<T, VE, 32>(a, s);
+    default: return hipErrorInvalidConfiguration;
+  }
+}
+
 template <class T>
 hipError_t append_dt(const AppendArgs& a, hipStream_t s) {
   // The widest access that the projection's rows and half a head allow.
@@ -1800,6 +1897,12 @@ hipError_t append_dt(const AppendArgs& a, hipStream_t s) {
     return (uintptr_t)a.qkv % w == 0 && a.tok_stride * es % w == 0 && a.head_stride * es % w == 0 &&
            a.c.hd / 2 % ve == 0;
   };
+  if (a.q_gain != nullptr) {  // (the checks have seen that four elements fit)
+    if constexpr (CE == 8) {
+      if (!fits(8)) return append_norm_lanes<T, 4>(a, s);
+    }
+    return append_norm_lanes<T, CE>(a, s);
+  }
   if (fits(CE)) return append_t<T, CE>(a, s);
   if (CE == 8 && fits(4)) return append_t<T, 4>(a, s);
   return append_t<T, 1>(a, s);

@@ -1068,6 +1068,89 @@ int sy_swiglu_bwd(const void* gate_up, const void* grad_out, void* dgate_up, int
   return status(launch_swiglu(gate_up, grad_out, dgate_up, n_tok, (int)f, dtype, (hipStream_t)stream));
 }
 
+// The sizes of a head norm, into *out; nothing here looks at pointers.
+static int head_norm_args(int64_t n_tok, int64_t seq, int64_t heads, int64_t kv_heads, int64_t hd, int dtype,
+                          int gain_dtype, HeadNormArgs* out) {
+  if (!valid_dtype(dtype) || (gain_dtype != dtype && gain_dtype != SY_F32)) return SY_ERR_DTYPE;
+  if (n_tok < 0 || n_tok > ((int64_t)1 << 40) || seq < 1 || seq > 0x7fffffff || n_tok % seq != 0 || heads < 1 ||
+      kv_heads < 1 || heads > 0xffff || kv_heads > 0xffff || hd < 8 || hd > 256 || hd % 8 != 0)
+    return SY_ERR_SHAPE;
+  out->gain_dtype = gain_dtype;
+  out->n_tok = n_tok;
+  out->seq = (int)seq;
+  out->heads = (int)heads;
+  out->kv_heads = (int)kv_heads;
+  out->hd = (int)hd;
+  return SY_OK;
+}
+
+int sy_qk_norm_rope(const void* qkv, const void* q_gain, const void* k_gain, const float* cosv, const float* sinv,
+                    void* q, void* k, void* v, int64_t n_tok, int64_t seq, int64_t heads, int64_t kv_heads,
+                    int64_t hd, int dtype, int gain_dtype, float eps, void* stream) {
+  HeadNormArgs a{};
+  const int rc = head_norm_args(n_tok, seq, heads, kv_heads, hd, dtype, gain_dtype, &a);
+  if (rc != SY_OK || n_tok == 0) return rc;
+  if (!qkv || !q_gain || !k_gain || !cosv || !sinv || !q || !k || !v) return SY_ERR_NULL;
+  if (!al16(qkv) || !al16(q) || !al16(k) || !al16(v)) return SY_ERR_SHAPE;
+  a.qkv = qkv;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  for (int i = 0; i < 3; ++i) {
+    a.strides[i][0] = (i == 0 ? heads : kv_heads) * seq * hd;
+    a.strides[i][1] = seq * hd;
+    a.strides[i][2] = hd;
+  }
+  a.q_gain = q_gain;
+  a.k_gain = k_gain;
+  a.cosv = cosv;
+  a.sinv = sinv;
+  a.eps = eps;
+  return status(launch_head_norm(a, dtype, (hipStream_t)stream));
+}
+
+int64_t sy_qk_norm_rope_bwd_bytes(int64_t n_tok, int64_t heads, int64_t kv_heads, int64_t hd, int dtype) {
+  HeadNormArgs a{};
+  const int rc = head_norm_args(n_tok, 1, heads, kv_heads, hd, dtype, dtype, &a);
+  if (rc != SY_OK) return rc;
+  return n_tok == 0 ? 0 : 8 * hd * head_norm_rows(a, dtype);
+}
+
+int sy_qk_norm_rope_bwd(const void* qkv, const void* q_gain, const void* k_gain, const float* cosv,
+                        const float* sinv, const void* dq, const void* dk, const void* dv,
+                        const int64_t strides[9], void* dqkv, void* dq_gain, void* dk_gain, void* workspace,
+                        int64_t workspace_bytes, int64_t n_tok, int64_t seq, int64_t heads, int64_t kv_heads,
+                        int64_t hd, int dtype, int gain_dtype, float eps, void* stream) {
+  HeadNormArgs a{};
+  const int rc = head_norm_args(n_tok, seq, heads, kv_heads, hd, dtype, gain_dtype, &a);
+  if (rc != SY_OK) return rc;
+  if (n_tok == 0) return SY_OK;
+  if (!qkv || !q_gain || !k_gain || !cosv || !sinv || !dq || !dk || !dv || !strides || !dqkv || !dq_gain || !dk_gain)
+    return SY_ERR_NULL;
+  if (!al16(qkv) || !al16(dq) || !al16(dk) || !al16(dv) || !al16(dqkv)) return SY_ERR_SHAPE;
+  const int64_t chunk = 16 / esize(dtype);
+  for (int i = 0; i < 9; ++i) {
+    if (strides[i] < 0 || strides[i] % chunk != 0) return SY_ERR_STRIDE;
+    a.strides[i / 3][i % 3] = strides[i];
+  }
+  a.rows = head_norm_rows(a, dtype);
+  if (!workspace || workspace_bytes < 8 * hd * (int64_t)a.rows) return SY_ERR_WORKSPACE;
+  a.qkv = qkv;
+  a.q = const_cast<void*>(dq);
+  a.k = const_cast<void*>(dk);
+  a.v = const_cast<void*>(dv);
+  a.q_gain = q_gain;
+  a.k_gain = k_gain;
+  a.cosv = cosv;
+  a.sinv = sinv;
+  a.dqkv = dqkv;
+  a.partial = static_cast<float*>(workspace);
+  a.eps = eps;
+  const hipError_t e = launch_head_norm(a, dtype, (hipStream_t)stream);
+  if (e != hipSuccess) return status(e);
+  return status(launch_head_norm_gains(a, dq_gain, dk_gain, (hipStream_t)stream));
+}
+
 int64_t sy_probe_grid(int64_t bytes) {
   // 256 threads x 4 chunks in flight per workgroup; up to 32768 workgroups
   // (the grid that reached the highest read bandwidth on MI355X).
@@ -1110,9 +1193,10 @@ static int cache_args(const sy_paged* c, CacheArgs* out) {
   return SY_OK;
 }
 
-int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride,
-                    const float* cosv, const float* sinv, int64_t n_pos, int64_t prefix_len, void* q,
-                    int fill, void* stream) {
+// `norm`: with gains, and the arguments that go with them.
+static int append(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride, bool norm,
+                  const void* q_gain, const void* k_gain, int gain_dtype, float eps, const float* cosv,
+                  const float* sinv, int64_t n_pos, int64_t prefix_len, void* q, int fill, void* stream) {
   AppendArgs a{};
   const int rc = cache_args(c, &a.c);
   if (rc != SY_OK) return rc;
@@ -1121,6 +1205,16 @@ int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int6
   if (c->n_tok == 0) return SY_OK;
   if (!qkv || !q || (n_pos != 0 && (!cosv || !sinv))) return SY_ERR_NULL;
   if (!al16(q)) return SY_ERR_SHAPE;
+  if (norm) {
+    if (!q_gain || !k_gain) return SY_ERR_NULL;
+    const int64_t four = 4 * esize(c->dtype);
+    if (reinterpret_cast<uintptr_t>(qkv) % four != 0) return SY_ERR_SHAPE;
+    if (tok_stride % 4 != 0 || head_stride % 4 != 0) return SY_ERR_STRIDE;
+    a.q_gain = q_gain;
+    a.k_gain = k_gain;
+    a.gain_dtype = gain_dtype;
+    a.eps = eps;
+  }
   a.qkv = qkv;
   a.tok_stride = tok_stride;
   a.head_stride = head_stride;
@@ -1131,6 +1225,21 @@ int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int6
   a.q = q;
   a.fill = fill;
   return status(launch_append(a, c->dtype, (hipStream_t)stream));
+}
+
+int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride,
+                    const float* cosv, const float* sinv, int64_t n_pos, int64_t prefix_len, void* q,
+                    int fill, void* stream) {
+  return append(c, qkv, tok_stride, head_stride, false, nullptr, nullptr, 0, 0.0f, cosv, sinv, n_pos, prefix_len, q,
+                fill, stream);
+}
+
+int sy_paged_append_norm(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride,
+                         const void* q_gain, const void* k_gain, int gain_dtype, float eps, const float* cosv,
+                         const float* sinv, int64_t n_pos, int64_t prefix_len, void* q, int fill, void* stream) {
+  if (c && valid_dtype(c->dtype) && gain_dtype != c->dtype && gain_dtype != SY_F32) return SY_ERR_DTYPE;
+  return append(c, qkv, tok_stride, head_stride, true, q_gain, k_gain, gain_dtype, eps, cosv, sinv, n_pos, prefix_len,
+                q, fill, stream);
 }
 
 int64_t sy_paged_attention_workspace_bytes(const sy_paged* c, int64_t prefix_len) {
@@ -1181,6 +1290,91 @@ int sy_sample(const void* logits, const float* u, int64_t* tokens, const sy_samp
   if (!logits || !u || !tokens) return SY_ERR_NULL;
   const SampleArgs a{logits, u, tokens, *how, n_rows, row_stride, (int)vocab};
   return status(launch_sample(a, dtype, (hipStream_t)stream));
+}
+
+int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_rows, int64_t vocab,
+              int64_t row_stride, int64_t out_stride, int dtype, void* stream) {
+  if (!how) return SY_ERR_NULL;
+  if (!valid_dtype(dtype)) return SY_ERR_DTYPE;
+  if (how->bias && how->bias_dtype != dtype && how->bias_dtype != SY_F32) return SY_ERR_DTYPE;
+  if (n_rows < 0 || n_rows > 0x7fffffff || vocab < 1 || vocab > (1 << 30) || how->n_tokens < 0 ||
+      how->n_tokens > 0x7fffffff || (how->tokens_bytes != 4 && how->tokens_bytes != 8) || how->mask_kind < 0 ||
+      how->mask_kind > 2)
+    return SY_ERR_SHAPE;
+  if (row_stride < 0 || out_stride < 0 || (n_rows > 1 && out_stride < vocab) || how->tokens_stride < 0 ||
+      how->bias_stride < 0 || how->mask_stride < 0)
+    return SY_ERR_STRIDE;
+  if (n_rows == 0) return SY_OK;
+  if (!logits || !out || (how->mask_kind != 0 && !how->mask) || (how->n_tokens != 0 && !how->tokens)) return SY_ERR_NULL;
+  AdjustArgs a{};
+  a.logits = logits;
+  a.out = out;
+  a.row_stride = row_stride;
+  a.out_stride = out_stride;
+  a.tokens = how->n_tokens != 0 ? how->tokens : nullptr;
+  a.tokens_stride = how->tokens_stride;
+  a.n_tokens = how->n_tokens;
+  a.lengths = how->lengths;
+  a.prompts = how->prompt_lengths;
+  a.repetition = how->repetition;
+  a.presence = how->presence;
+  a.frequency = how->frequency;
+  a.repetitions = how->repetitions;
+  a.presences = how->presences;
+  a.frequencies = how->frequencies;
+  a.bias = how->bias;
+  a.bias_stride = how->bias_stride;
+  a.bias_f32 = how->bias_dtype == SY_F32;
+  a.mask = how->mask_kind != 0 ? how->mask : nullptr;
+  a.mask_stride = how->mask_stride;
+  a.mask_bytes = how->mask_kind == 2;
+  a.n_rows = n_rows;
+  a.vocab = (int)vocab;
+  a.tokens64 = how->tokens_bytes == 8;
+  return status(launch_adjust(a, dtype, (hipStream_t)stream));
+}
+
+// Sizes of 4-bit weights.
+static int quant_sizes(int64_t n, int64_t k, int64_t group, int dtype) {
+  if (!valid_dtype(dtype)) return SY_ERR_DTYPE;
+  if (n < 1 || n > (1 << 24) || k < 1 || k > (1 << 24) || (group != 32 && group != 64 && group != 128))
+    return SY_ERR_SHAPE;
+  return SY_OK;
+}
+
+int sy_quantize4(const void* w, int64_t row_stride, uint8_t* codes, void* scales, uint8_t* zeros, int64_t n,
+                 int64_t k, int64_t group, int dtype, void* stream) {
+  const int rc = quant_sizes(n, k, group, dtype);
+  if (rc != SY_OK) return rc;
+  if (row_stride < 0) return SY_ERR_STRIDE;
+  if (!w || !codes || !scales) return SY_ERR_NULL;
+  const QuantizeArgs a{w, row_stride, codes, scales, zeros, n, k, (int)group};
+  return status(launch_quantize4(a, dtype, (hipStream_t)stream));
+}
+
+int sy_pack4(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* tiles, void* tile_scales,
+             uint8_t* tile_zeros, int64_t n, int64_t k, int64_t group, int dtype, void* stream) {
+  const int rc = quant_sizes(n, k, group, dtype);
+  if (rc != SY_OK) return rc;
+  if (!codes || !scales || !tiles || !tile_scales || !zeros != !tile_zeros) return SY_ERR_NULL;
+  if (!al16(tiles)) return SY_ERR_SHAPE;
+  const PackArgs a{codes, scales, zeros, static_cast<uint32_t*>(tiles), tile_scales, tile_zeros, n, k, (int)group,
+                   (int)esize(dtype)};
+  return status(launch_pack4(a, (hipStream_t)stream));
+}
+
+int sy_linear4(const void* x, int64_t x_stride, const void* tiles, const void* tile_scales, const uint8_t* tile_zeros,
+               void* out, int64_t m, int64_t n, int64_t k, int64_t group, int dtype, void* stream) {
+  const int rc = quant_sizes(n, k, group, dtype);
+  if (rc != SY_OK) return rc;
+  if (m < 0 || m > 0x7fffffff) return SY_ERR_SHAPE;
+  if (x_stride < 0) return SY_ERR_STRIDE;
+  if (m == 0) return SY_OK;
+  if (!x || !tiles || !tile_scales || !out) return SY_ERR_NULL;
+  if (!al16(tiles)) return SY_ERR_SHAPE;
+  const Linear4Args a{x, x_stride, static_cast<const uint32_t*>(tiles), tile_scales, tile_zeros, out, m, n, (int)k,
+                      (int)group};
+  return status(launch_linear4(a, dtype, (hipStream_t)stream));
 }
 
 int sy_bw_probe(int kind, const void* src, void* dst, int64_t bytes, void* stream) {

@@ -705,6 +705,32 @@ __device__ __forceinline__ float tsum(const float (&v)[P], int lane) {
 __device__ __forceinline__ int tsum32_row(int lane) { return tsum_row<32>(lane); }
 __device__ __forceinline__ float tsum32(const float (&v)[32], int lane) { return tsum<32>(v, lane); }
 
+// Sum over groups of L neighbouring lanes, the same bits in each of them.
+template <int L>
+__device__ __forceinline__ float lane_sum(float x) {
+  if constexpr (L >= 2) x += dpp<0xB1>(x);   // quad_perm [1,0,3,2]
+  if constexpr (L >= 4) x += dpp<0x4E>(x);   // quad_perm [2,3,0,1]
+  if constexpr (L >= 8) x += dpp<0x141>(x);  // row_half_mirror
+  if constexpr (L >= 16) x += dpp<0x140>(x);  // row_mirror
+  if constexpr (L >= 32) x += __shfl_xor(x, 16);
+  return x;
+}
+
+// 1 / sqrt(mean(x^2) + eps) of a head that L lanes hold, VE channels of each half a lane, and
+// the rotation of a pair. The contractions are written out, so that every kernel rounds alike.
+template <int VE, int L>
+__device__ __forceinline__ float head_rinv(const float (&lo)[VE], const float (&hi)[VE], float inv_hd, float eps) {
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < VE; ++e) ss = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], ss));
+  return rsqrtf(fmaf(lane_sum<L>(ss), inv_hd, eps));
+}
+__device__ __forceinline__ void turn(float& lo, float& hi, float co, float si) {
+  const float x = lo, y = hi;
+  lo = fmaf(x, co, -__fmul_rn(y, si));
+  hi = fmaf(x, si, __fmul_rn(y, co));
+}
+
 // Smallest power of two >= x (x >= 1), for sizing a tsum.
 __host__ __device__ constexpr int pow2_at_least(int x) { return x <= 1 ? 1 : 2 * pow2_at_least((x + 1) / 2); }
 

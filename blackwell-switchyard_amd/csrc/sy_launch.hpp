@@ -447,6 +447,10 @@ struct AppendArgs {
   int64_t n_pos, offset;
   void* q;
   int fill;
+  const void* q_gain;  // nullptr: heads are not normalised
+  const void* k_gain;
+  int gain_dtype;
+  float eps;
 };
 struct AttendArgs {
   CacheArgs c;
@@ -474,6 +478,90 @@ struct SampleArgs {
   int vocab;
 };
 hipError_t launch_sample(const SampleArgs& a, int dtype, hipStream_t s);
+
+// What is done to logits before sampling (sy_logits.hip).
+struct AdjustArgs {
+  const void* logits;
+  void* out;
+  int64_t row_stride, out_stride;
+  const void* tokens;  // [n_rows][n_tokens] or nullptr
+  int64_t tokens_stride, n_tokens;
+  const int32_t* lengths;  // [n_rows] or nullptr: all n_tokens
+  const int32_t* prompts;  // [n_rows] or nullptr: none
+  double repetition, presence, frequency;
+  const float* repetitions;  // [n_rows] each, or nullptr
+  const float* presences;
+  const float* frequencies;
+  const void* bias;
+  int64_t bias_stride;
+  const void* mask;
+  int64_t mask_stride;
+  int64_t n_rows;
+  int vocab;
+  bool tokens64, bias_f32, mask_bytes;
+};
+hipError_t launch_adjust(const AdjustArgs& a, int dtype, hipStream_t s);
+
+// Head norms with the rotation (sy_rope.hip): qkv [n_tok][heads + 2 kv_heads][hd]. Forward
+// writes q, k, v (dense, [n_tok / seq][heads][seq][hd]); backward reads their gradients
+// (rows of hd at these strides, in elements, for batch, head and token) and writes dqkv and
+// partial sums of the gains' gradients, [2][rows][hd].
+struct HeadNormArgs {
+  const void* qkv;
+  void* q;
+  void* k;
+  void* v;
+  int64_t strides[3][3];
+  const void* q_gain;
+  const void* k_gain;
+  int gain_dtype;
+  const float* cosv;
+  const float* sinv;
+  void* dqkv;  // nullptr: forward
+  float* partial;
+  int rows;
+  int64_t n_tok;
+  int seq, heads, kv_heads, hd;
+  float eps;
+};
+int head_norm_rows(const HeadNormArgs& a, int dtype);
+hipError_t launch_head_norm(const HeadNormArgs& a, int dtype, hipStream_t s);
+// Sums of the partials to the gains' gradients, of the gains' dtype.
+hipError_t launch_head_norm_gains(const HeadNormArgs& a, void* dq_gain, void* dk_gain, hipStream_t s);
+
+// Projections with 4-bit weights (sy_quant.hip).
+struct PackArgs {
+  const uint8_t* codes;  // [n][(k + 1) / 2]
+  const void* scales;    // [n][groups]
+  const uint8_t* zeros;  // [n][groups] or nullptr
+  uint32_t* tiles;
+  void* scales_out;
+  uint8_t* zeros_out;
+  int64_t n, k;
+  int group, esize;
+};
+struct QuantizeArgs {
+  const void* w;
+  int64_t row_stride;
+  uint8_t* codes;
+  void* scales;
+  uint8_t* zeros;  // nullptr: symmetric
+  int64_t n, k;
+  int group;
+};
+struct Linear4Args {
+  const void* x;
+  int64_t x_stride;
+  const uint32_t* tiles;
+  const void* scales;
+  const uint8_t* zeros;
+  void* out;
+  int64_t m, n;
+  int k, group;
+};
+hipError_t launch_pack4(const PackArgs& a, hipStream_t s);
+hipError_t launch_quantize4(const QuantizeArgs& a, int dtype, hipStream_t s);
+hipError_t launch_linear4(const Linear4Args& a, int dtype, hipStream_t s);
 
 // Generic kernels, the dw reduction and the probes (sy_generic.hip).
 hipError_t launch_fwd_generic(const FwdArgs& a, hipStream_t s);

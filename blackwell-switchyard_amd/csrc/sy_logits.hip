@@ -1,0 +1,182 @@
+// What is done to logits before a token is drawn from them: penalties for tokens that were
+// there before, biases, and a mask of the tokens that are allowed.
+//
+//   y = x                                   token not among the row's `length` first ones
+//   y = (x > 0 ? x / r : x r) - f n - p [n > 0]  else; n counts it behind the prompt
+//   out = y + bias, or -inf where the token is not allowed
+#include <algorithm>
+
+#include "sy_launch.hpp"
+
+namespace sy {
+
+namespace {
+
+typedef int i32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any_t __attribute__((ext_vector_type(2), aligned(1)));
+
+constexpr int kBlock = 256;
+constexpr uint32_t kPrompt = 0x80000000u;  // of a token's count: it was in the prompt
+
+// Which of CE tokens from v on are allowed, a bit each.
+template <int CE>
+__device__ __forceinline__ uint32_t allowed(const AdjustArgs& a, int64_t row, int v, bool full) {
+  constexpr uint32_t all = (1u << CE) - 1u;
+  if (a.mask == nullptr) return all;
+  if (a.mask_bytes) {
+    const uint8_t* const m = static_cast<const uint8_t*>(a.mask) + row * a.mask_stride + v;
+    uint32_t r = 0;
+    if (full) {
+      uint32_t w[2] = {0, 0};
+      if constexpr (CE == 8) {
+        const u32x2_any_t x = *reinterpret_cast<const u32x2_any_t*>(m);
+        w[0] = x[0], w[1] = x[1];
+      } else {
+        __builtin_memcpy(w, m, 4);
+      }
+#pragma unroll
+      for (int e = 0; e < CE; ++e) r |= (w[e / 4] >> (8 * (e % 4)) & 0xffu ? 1u : 0u) << e;
+    } else {
+#pragma unroll
+      for (int e = 0; e < CE; ++e)
+        if (v + e < a.vocab && m[e] != 0) r |= 1u << e;
+    }
+    return r;
+  }
+  return static_cast<const uint32_t*>(a.mask)[row * a.mask_stride + (v >> 5)] >> (v & 31) & all;
+}
+
+__device__ __forceinline__ void count(uint32_t* seen, int64_t token, int lo, int n, bool said) {
+  const int64_t at = token - lo;
+  if ((uint64_t)at >= (uint64_t)n) return;
+  if (said) atomicAdd(&seen[at], 1u);
+  else atomicOr(&seen[at], kPrompt);
+}
+
+// A workgroup takes a slice of one row. It reads the row's whole history and counts in LDS
+// what falls into its slice, in whole numbers, so in any order; then one pass over the
+// logits. Chunks that stay as they are in place are not touched, and those with nothing
+// allowed are not read.
+template <class T>
+__global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice, int slices) {
+  using S = typename T::storage;
+  constexpr int CE = T::ce;
+  extern __shared__ uint32_t seen[];
+  const int64_t row = blockIdx.x / slices;
+  const int lo = (int)(blockIdx.x % slices) * slice, n = min(slice, a.vocab - lo);
+  const double r = a.repetitions != nullptr ? a.repetitions[row] : a.repetition;
+  const double p = a.presences != nullptr ? a.presences[row] : a.presence;
+  const double f = a.frequencies != nullptr ? a.frequencies[row] : a.frequency;
+  const bool counted = a.tokens != nullptr && (r != 1.0 || p != 0.0 || f != 0.0);
+  if (counted) {
+    for (int i = threadIdx.x; i < slice; i += kBlock) seen[i] = 0;
+    __syncthreads();
+    const int64_t len = a.lengths != nullptr ? min(max((int64_t)a.lengths[row], (int64_t)0), a.n_tokens) : a.n_tokens;
+    const int64_t prompt = a.prompts != nullptr ? a.prompts[row] : 0;
+    if (a.tokens64) {
+      const int64_t* const t = static_cast<const int64_t*>(a.tokens) + row * a.tokens_stride;
+      for (int64_t i = threadIdx.x; i < len; i += kBlock) count(seen, t[i], lo, n, i >= prompt);
+    } else {
+      const int32_t* const t = static_cast<const int32_t*>(a.tokens) + row * a.tokens_stride;
+      for (int64_t i = threadIdx.x; i < len; i += kBlock) count(seen, t[i], lo, n, i >= prompt);
+    }
+    __syncthreads();
+  }
+  const S* const x = static_cast<const S*>(a.logits) + row * a.row_stride + lo;
+  S* const y = static_cast<S*>(a.out) + row * a.out_stride + lo;
+  const bool in_place = static_cast<const void*>(x) == static_cast<const void*>(y);
+  for (int c = threadIdx.x * CE; c < n; c += kBlock * CE) {
+    const bool full = c + CE <= n;
+    const uint32_t keep = allowed<CE>(a, row, lo + c, full);
+    uint32_t cnt[CE], any = 0;
+#pragma unroll
+    for (int e = 0; e < CE; ++e) cnt[e] = 0;
+    if (counted) {
+#pragma unroll
+      for (int q = 0; q < CE / 4; ++q) {
+        const i32x4_t w = *reinterpret_cast<const i32x4_t*>(seen + c + 4 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) cnt[4 * q + e] = (uint32_t)w[e], any |= (uint32_t)w[e];
+      }
+    }
+    if (in_place && a.bias == nullptr && any == 0 && keep == (1u << CE) - 1u) continue;
+    float v[CE];
+#pragma unroll
+    for (int e = 0; e < CE; ++e) v[e] = 0.0f;
+    if (keep != 0) {
+      if (full) {
+        const i32x4_t w = *reinterpret_cast<const i32x4_any_t*>(x + c);
+#pragma unroll
+        for (int e = 0; e < CE; ++e) v[e] = elem<T>(w, e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < CE; ++e)
+          if (c + e < n) v[e] = load_elem(x, c + e, T::code);
+      }
+      if (any != 0) {
+#pragma unroll
+        for (int e = 0; e < CE; ++e) {
+          if (cnt[e] == 0) continue;
+          const uint32_t said = cnt[e] & ~kPrompt;
+          const double z = v[e];
+          v[e] = (float)((z > 0.0 ? z / r : z * r) - (said != 0 ? f * said + p : 0.0));
+        }
+      }
+      if (a.bias != nullptr) {
+        const int64_t at = row * a.bias_stride + lo + c;
+#pragma unroll
+        for (int e = 0; e < CE; ++e)
+          if (c + e < n) v[e] += load_elem(a.bias, at + e, a.bias_f32 ? F32::code : T::code);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < CE; ++e)
+      if ((keep >> e & 1u) == 0) v[e] = -__builtin_inff();
+    const i32x4_t w = pack<T>(v);
+    if (full) {
+      *reinterpret_cast<i32x4_any_t*>(y + c) = w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < CE; ++e)
+        if (c + e < n) store_elem(y, c + e, v[e], T::code);
+    }
+  }
+}
+
+template <class T>
+hipError_t adjust_t(const AdjustArgs& a, hipStream_t s) {
+  int slice = 4096;
+  while (slice > 1024 && a.n_rows * ((a.vocab + slice - 1) / slice) < 1024) slice /= 2;
+  const int slices = (a.vocab + slice - 1) / slice;
+  const int64_t rows = std::max<int64_t>(1, (1 << 22) / slices);  // of a launch: 2^30 threads
+  for (int64_t r0 = 0; r0 < a.n_rows; r0 += rows) {
+    AdjustArgs part = a;
+    part.n_rows = std::min(rows, a.n_rows - r0);
+    const int64_t es = sizeof(typename T::storage);
+    part.logits = static_cast<const char*>(a.logits) + r0 * a.row_stride * es;
+    part.out = static_cast<char*>(a.out) + r0 * a.out_stride * es;
+    if (a.tokens) part.tokens = static_cast<const char*>(a.tokens) + r0 * a.tokens_stride * (a.tokens64 ? 8 : 4);
+    if (a.lengths) part.lengths += r0;
+    if (a.prompts) part.prompts += r0;
+    if (a.repetitions) part.repetitions += r0;
+    if (a.presences) part.presences += r0;
+    if (a.frequencies) part.frequencies += r0;
+    if (a.bias) part.bias = static_cast<const char*>(a.bias) + r0 * a.bias_stride * (a.bias_f32 ? 4 : es);
+    if (a.mask) part.mask = static_cast<const char*>(a.mask) + r0 * a.mask_stride * (a.mask_bytes ? 1 : 4);
+    hipLaunchKernelGGL((k_adjust<T>), dim3((unsigned)(part.n_rows * slices)), dim3(kBlock),
+                       a.tokens ? slice * sizeof(uint32_t) : 0, s, part, slice, slices);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_adjust(const AdjustArgs& a, int dtype, hipStream_t s) {
+  if (dtype == SY_BF16) return adjust_t<BF16>(a, s);
+  if (dtype == SY_F16) return adjust_t<F16>(a, s);
+  return adjust_t<F32>(a, s);
+}
+
+}  // namespace sy

@@ -1,0 +1,385 @@
+// Projections with 4-bit weights, and what lays such weights out.
+//
+//   out[m][n] = sum_k x[m][k] w[n][k],   w[n][k] = s[n][g] (c[n][k] - z[n][g]),   g = k / group
+//
+// with whole codes c in 0..15 and, without zero points, z = 8.
+#include <algorithm>
+
+#include "sy_launch.hpp"
+
+namespace sy {
+
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------- layout
+//
+// Tiles of 16 features by 128 columns, 1 KiB each, a feature tile's tiles one after another
+// over the columns. Lane l of a wave reads 16 bytes of a tile: word j holds feature l % 16
+// at columns 32 j + 8 (l / 16) + (0..7), which is what the lane brings to the matrix
+// instruction over columns 32 j .. 32 j + 31. The nibble of column c of a word lies at bits
+// 4 p + 3, p = c / 2 + 4 (c % 2), so one mask leaves a pair of columns in the two halves.
+// Scales and zero points are [feature tile][group][16], with the groups of whole tiles.
+constexpr int kTileK = 128;
+
+__host__ __device__ constexpr int64_t tiles_of(int64_t n) { return (n + 15) / 16; }
+__host__ __device__ constexpr int64_t steps_of(int64_t k) { return (k + kTileK - 1) / kTileK; }
+
+__global__ void __launch_bounds__(256) k_pack4(const PackArgs a) {
+  const int64_t words = tiles_of(a.n) * steps_of(a.k) * 256;
+  const int64_t row_bytes = (a.k + 1) / 2;
+  const int steps = (int)steps_of(a.k);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
+    const int j = (int)(i & 3), lane = (int)(i >> 2) & 63;
+    const int64_t tile = i >> 8;
+    const int64_t n = tile / steps * 16 + (lane & 15);
+    const int64_t k = tile % steps * kTileK + 32 * j + 8 * (lane >> 4);
+    uint32_t w = 0;
+    if (n < a.n) {
+      const uint8_t* const row = a.codes + n * row_bytes;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int64_t at = k / 2 + b;
+        const uint32_t two = at < row_bytes ? row[at] : 0u;
+        w |= (two & 15u) << (4 * b) | (two >> 4) << (4 * b + 16);
+      }
+    }
+    a.tiles[i] = w << 3 | w >> 29;
+  }
+  // Groups that only pad a tile have scale zero.
+  const int64_t groups = (a.k + a.group - 1) / a.group, padded = (int64_t)steps * (kTileK / a.group);
+  const int64_t cells = tiles_of(a.n) * padded * 16;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / (padded * 16) * 16 + (i & 15), g = (i >> 4) % padded;
+    const bool in = n < a.n && g < groups;
+    if (a.esize == 4)
+      static_cast<uint32_t*>(a.scales_out)[i] = in ? static_cast<const uint32_t*>(a.scales)[n * groups + g] : 0u;
+    else
+      static_cast<uint16_t*>(a.scales_out)[i] = in ? static_cast<const uint16_t*>(a.scales)[n * groups + g] : (uint16_t)0;
+    if (a.zeros != nullptr) a.zeros_out[i] = in ? a.zeros[n * groups + g] : (uint8_t)0;
+  }
+}
+
+// Rounding to codes: sixteen lanes a group, each with group / 16 neighbours. Symmetric: s =
+// max |w| / 7, c = round(w / s) + 8 (1 to 15); with zero points s = (max - min) / 15 over a
+// range that holds zero, z = round(-min / s), c = round(w / s) + z. s is rounded to the
+// weights' type first, so the codes fit the scale that is kept; a group of zeros has s = 0.
+template <class T, int E>
+__global__ void __launch_bounds__(256) k_quantize4(const QuantizeArgs a) {
+  using S = typename T::storage;
+  const int64_t groups = (a.k + a.group - 1) / a.group, items = a.n * groups;
+  const int sub = threadIdx.x & 15;
+  for (int64_t i0 = (int64_t)blockIdx.x * 16; i0 < items; i0 += (int64_t)gridDim.x * 16) {
+    const int64_t i = i0 + (threadIdx.x >> 4);
+    const bool live = i < items;
+    const int64_t n = live ? i / groups : 0, g = live ? i % groups : 0;
+    const int64_t k0 = g * a.group + sub * E;
+    const S* const row = static_cast<const S*>(a.w) + n * a.row_stride;
+    float w[E], lo = 0.0f, hi = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      w[e] = live && k0 + e < a.k ? load_elem(row, k0 + e, T::code) : 0.0f;
+      lo = fminf(lo, w[e]);
+      hi = fmaxf(hi, w[e]);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+      lo = fminf(lo, __shfl_xor(lo, d, 16));
+      hi = fmaxf(hi, __shfl_xor(hi, d, 16));
+    }
+    float f[T::ce] = {a.zeros != nullptr ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f};
+    const i32x4_t kept = pack<T>(f);
+    const float s = elem<T>(kept, 0);
+    const auto steps_in = [s](float x) { return s > 0.0f ? rintf(x / s) : 0.0f; };
+    const float z = a.zeros != nullptr ? fminf(fmaxf(steps_in(-lo), 0.0f), 15.0f) : 8.0f;
+    if (!live) continue;
+    if (sub == 0) {
+      __builtin_memcpy(static_cast<S*>(a.scales) + i, &kept, sizeof(S));
+      if (a.zeros != nullptr) a.zeros[i] = (uint8_t)z;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      if (k0 + e >= a.k) break;
+      uint32_t c[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) c[h] = (uint32_t)fminf(fmaxf(steps_in(w[e + h]) + z, 0.0f), 15.0f);
+      a.codes[n * ((a.k + 1) / 2) + (k0 + e) / 2] = (uint8_t)(c[0] | c[1] << 4);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ product
+//
+// Products run on v_mfma_f32_16x16x32 with sixteen rows of x against sixteen features. A code
+// becomes 1 + c / 16 in x's type by putting its four bits at the top of the mantissa of 1.0: a
+// shift, a mask and an or for two weights, and exact. So is every product with x, and
+//
+//   sum_k x (c - z) / 16 = sum_k x (1 + c / 16) - (1 + z / 16) sum_k x
+//
+// over a group; the last sum comes from the same instruction against a constant, and is what
+// the accumulator starts from. Group sums are scaled and added in fp32: nothing is rounded to
+// fewer bits before the output.
+//
+// fp32 rows are taken as three bf16 numbers of eight bits each, which hold all 24.
+template <class T> struct Mma;
+template <> struct Mma<BF16> {
+  static constexpr int planes = 1;
+  static constexpr uint32_t one = 0x3f803f80u, mask = 0x00780078u;
+  static __device__ __forceinline__ f32x4_t run(const i32x4_t& a, const i32x4_t& b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+};
+template <> struct Mma<F16> {
+  static constexpr int planes = 1;
+  static constexpr uint32_t one = 0x3c003c00u, mask = 0x03c003c0u;
+  static __device__ __forceinline__ f32x4_t run(const i32x4_t& a, const i32x4_t& b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0,
+                                                  0, 0);
+  }
+};
+template <> struct Mma<F32> : Mma<BF16> {
+  static constexpr int planes = 3;
+};
+
+__device__ __forceinline__ uint32_t ror(uint32_t x, int n) { return __builtin_amdgcn_alignbit(x, x, n); }
+
+// The eight weights of a word as 1 + c / 16.
+template <class T> __device__ __forceinline__ i32x4_t codes_of(uint32_t w) {
+  constexpr uint32_t M = Mma<T>::mask, B = Mma<T>::one;
+  i32x4_t r;
+  if constexpr (T::code == F16::code) {
+    r[0] = (int)((w << 3 & M) | B);
+    r[1] = (int)((w >> 1 & M) | B);
+    r[2] = (int)((w >> 5 & M) | B);
+    r[3] = (int)((ror(w, 9) & M) | B);
+  } else {
+    r[0] = (int)((w & M) | B);
+    r[1] = (int)((w >> 4 & M) | B);
+    r[2] = (int)((w >> 8 & M) | B);
+    r[3] = (int)((ror(w, 12) & M) | B);
+  }
+  return r;
+}
+
+// -1, or -1.5 = -(1 + 8 / 16), in every element: what the sum over x is taken against.
+template <class T, bool ZEROS> __device__ __forceinline__ i32x4_t minus() {
+  constexpr uint32_t x = 0x80008000u | Mma<T>::one | (ZEROS ? 0u : T::code == F16::code ? 0x02000200u : 0x00400040u);
+  return i32x4_t{(int)x, (int)x, (int)x, (int)x};
+}
+
+typedef int i32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// Eight elements of a row from column k on, as Mma<T>::planes fragments; zero behind the row
+// and where the lane has no row. Rows start anywhere.
+template <class T>
+__device__ __forceinline__ void ld_x(const typename T::storage* row, bool live, int k, int k_end,
+                                     i32x4_t (&f)[Mma<T>::planes]) {
+  using S = typename T::storage;
+  constexpr int W = 8 * sizeof(S) / 16;
+  i32x4_t raw[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) raw[i] = i32x4_t{0, 0, 0, 0};
+  if (live && k + 8 <= k_end) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) raw[i] = *reinterpret_cast<const i32x4_any_t*>(row + k + i * (8 / W));
+  } else if (live) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (k + e >= k_end) continue;
+      if constexpr (sizeof(S) == 4) raw[e / 4][e % 4] = __float_as_int(row[k + e]);
+      else raw[0][e / 2] |= (int)((uint32_t)row[k + e] << (16 * (e % 2)));
+    }
+  }
+  if constexpr (W == 1) {
+    f[0] = raw[0];
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[h] = __int_as_float(raw[(2 * r + h) / 4][(2 * r + h) % 4]);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]);
+        f[p][r] = (int)((b & 0xffff0000u) | a >> 16);
+        x[0] -= __uint_as_float(a & 0xffff0000u);
+        x[1] -= __uint_as_float(b & 0xffff0000u);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float scale_of(const void* p, int64_t i, int dtype) { return load_elem(p, i, dtype); }
+
+// Few rows: a workgroup has NT feature tiles and 16 MT rows, its waves share the columns out
+// tile by tile and fold their sums in LDS in their order. GS: 32-column pieces of a group.
+template <class T, int MT, int NT, int GS, bool ZEROS>
+__global__ void __launch_bounds__(512) k_linear4(const Linear4Args a) {
+  using S = typename T::storage;
+  constexpr int P = Mma<T>::planes, NG = 4 / GS;
+  extern __shared__ float fold[];
+  const int lane = threadIdx.x & 63, wave = wave_id(), waves = blockDim.x >> 6;
+  const int col = lane & 15, quad = lane >> 4;
+  const int64_t tile0 = (int64_t)blockIdx.x * NT, n_tiles = tiles_of(a.n);
+  const int steps = (int)steps_of(a.k);
+  const S* const x = static_cast<const S*>(a.x);
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  const S* rows[MT];
+  bool live[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    live[t] = m0 + 16 * t + col < a.m;
+    rows[t] = x + (live[t] ? m0 + 16 * t + col : 0) * a.x_stride;
+  }
+  const i32x4_t neg = minus<T, ZEROS>();
+  f32x4_t tot[MT][NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) tot[t][u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int step = wave; step < steps; step += waves) {
+    i32x4_t w[NT];
+    float s[NT][NG], z[NT][NG];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int64_t tile = min(tile0 + u, n_tiles - 1);  // (what is behind the last is not stored)
+      w[u] = reinterpret_cast<const i32x4_t*>(a.tiles)[(tile * steps + step) * 64 + lane];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int64_t at = (tile * steps * NG + step * NG + g) * 16 + col;
+        s[u][g] = scale_of(a.scales, at, T::code);
+        if constexpr (ZEROS) z[u][g] = 1.0f + (float)a.zeros[at] * 0.0625f;
+      }
+    }
+    i32x4_t f[MT][4][P];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ld_x<T>(rows[t], live[t], step * kTileK + 32 * j + 8 * quad, a.k, f[t][j]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      f32x4_t sums[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        sums[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = g * GS; j < (g + 1) * GS; ++j)
+#pragma unroll
+          for (int p = 0; p < P; ++p) sums[t] = Mma<T>::run(f[t][j][p], neg, sums[t]);
+      }
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        f32x4_t acc[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? sums[t] * z[u][g] : sums[t];
+#pragma unroll
+        for (int j = g * GS; j < (g + 1) * GS; ++j) {
+          const i32x4_t c = codes_of<T>((uint32_t)w[u][j]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int p = 0; p < P; ++p) acc[t] = Mma<T>::run(f[t][j][p], c, acc[t]);
+        }
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tot[t][u][i] = fmaf(s[u][g], acc[t][i], tot[t][u][i]);
+      }
+    }
+  }
+  constexpr int kSums = MT * NT * 256;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) fold[wave * kSums + ((t * NT + u) * 4 + i) * 64 + lane] = tot[t][u][i];
+  __syncthreads();
+  S* const out = static_cast<S*>(a.out);
+  for (int i = threadIdx.x; i < kSums; i += blockDim.x) {
+    float y = 0.0f;
+    for (int v = 0; v < waves; ++v) y += fold[v * kSums + i];
+    const int l = i & 63, r = i >> 6 & 3, u = (i >> 8) % NT, t = (i >> 8) / NT;
+    const int64_t m = m0 + 16 * t + 4 * (l >> 4) + r, n = (tile0 + u) * 16 + (l & 15);
+    if (m < a.m && n < a.n) store_elem(out, m * a.n + n, 16.0f * y, T::code);
+  }
+}
+
+template <class T, int MT, int NT, int GS, bool ZEROS>
+hipError_t run4(const Linear4Args& a, hipStream_t s) {
+  const int steps = (int)steps_of(a.k);
+  int waves = 8;
+  while (waves > 1 && (waves > steps || waves * MT * NT > 64)) waves /= 2;
+  const unsigned gx = (unsigned)((tiles_of(a.n) + NT - 1) / NT);
+  constexpr int64_t kRows = 16 * MT * 32768;  // of a launch
+  for (int64_t m0 = 0; m0 < a.m; m0 += kRows) {
+    Linear4Args part = a;
+    part.m = std::min(kRows, a.m - m0);
+    const int64_t es = sizeof(typename T::storage);
+    part.x = static_cast<const char*>(a.x) + m0 * a.x_stride * es;
+    part.out = static_cast<char*>(a.out) + m0 * a.n * es;
+    const unsigned gy = (unsigned)((part.m + 16 * MT - 1) / (16 * MT));
+    hipLaunchKernelGGL((k_linear4<T, MT, NT, GS, ZEROS>), dim3(gx, gy), dim3(64 * waves), waves * MT * NT * 1024, s, part);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+template <class T, int GS, bool ZEROS>
+hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
+  if (a.m <= 16) return tiles_of(a.n) < 1024 ? run4<T, 1, 1, GS, ZEROS>(a, s) : run4<T, 1, 2, GS, ZEROS>(a, s);
+  if (a.m <= 32) return run4<T, 2, 2, GS, ZEROS>(a, s);
+  return run4<T, 4, 2, GS, ZEROS>(a, s);
+}
+
+template <class T, bool ZEROS>
+hipError_t linear4_g(const Linear4Args& a, hipStream_t s) {
+  switch (a.group) {
+    case 32: return linear4_m<T, 1, ZEROS>(a, s);
+    case 64: return linear4_m<T, 2, ZEROS>(a, s);
+    default: return linear4_m<T, 4, ZEROS>(a, s);
+  }
+}
+
+template <class T>
+hipError_t linear4_t(const Linear4Args& a, hipStream_t s) {
+  return a.zeros != nullptr ? linear4_g<T, true>(a, s) : linear4_g<T, false>(a, s);
+}
+
+template <class T>
+hipError_t quantize_t(const QuantizeArgs& a, hipStream_t s) {
+  const int64_t items = a.n * ((a.k + a.group - 1) / a.group);
+  const unsigned grid = (unsigned)std::min<int64_t>((items + 15) / 16, 1 << 16);
+  if (a.group == 32) hipLaunchKernelGGL((k_quantize4<T, 2>), dim3(grid), dim3(256), 0, s, a);
+  else if (a.group == 64) hipLaunchKernelGGL((k_quantize4<T, 4>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_quantize4<T, 8>), dim3(grid), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_pack4(const PackArgs& a, hipStream_t s) {
+  const int64_t words = tiles_of(a.n) * steps_of(a.k) * 256;
+  const unsigned grid = (unsigned)std::min<int64_t>((words + 255) / 256, 1 << 16);
+  hipLaunchKernelGGL(k_pack4, dim3(grid), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_quantize4(const QuantizeArgs& a, int dtype, hipStream_t s) {
+  if (dtype == SY_BF16) return quantize_t<BF16>(a, s);
+  if (dtype == SY_F16) return quantize_t<F16>(a, s);
+  return quantize_t<F32>(a, s);
+}
+
+hipError_t launch_linear4(const Linear4Args& a, int dtype, hipStream_t s) {
+  if (dtype == SY_BF16) return linear4_t<BF16>(a, s);
+  if (dtype == SY_F16) return linear4_t<F16>(a, s);
+  return linear4_t<F32>(a, s);
+}
+
+}  // namespace sy

@@ -1,0 +1,260 @@
+// The norm of every query and key head with the rotation to its position, and the split of
+// a fused projection into attention's layout, in one pass each way.
+//
+//   u = x r,  r = 1 / sqrt(mean(x^2) + eps)         over a head's channels
+//   y = R_t (g u)    channel i of the first half turns with channel i of the second
+//
+//   backward, from dy:  e = R_t^T dy,  dg = sum e u,  dx = r (g e - u mean(g e u))
+#include <algorithm>
+
+#include "sy_launch.hpp"
+
+namespace sy {
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / 64;
+
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+
+// VE neighbouring channels as fp32.
+template <class T, int VE>
+__device__ __forceinline__ void ld_part(const typename T::storage* p, float (&f)[VE]) {
+  i32x4_t x;
+  if constexpr (VE == T::ce) {
+    x = *reinterpret_cast<const i32x4_t*>(p);
+  } else {
+    const i32x2_t y = *reinterpret_cast<const i32x2_t*>(p);
+    x = i32x4_t{y[0], y[1], 0, 0};
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) f[e] = elem<T>(x, e);
+}
+template <class T, int VE>
+__device__ __forceinline__ void st_part(typename T::storage* p, const float (&f)[VE]) {
+  float g[T::ce] = {};
+#pragma unroll
+  for (int e = 0; e < VE; ++e) g[e] = f[e];
+  const i32x4_t x = pack<T>(g);
+  if constexpr (VE == T::ce) *reinterpret_cast<i32x4_t*>(p) = x;
+  else *reinterpret_cast<i32x2_t*>(p) = i32x2_t{x[0], x[1]};
+}
+
+// L lanes a head, each with the two parts of VE channels that turn together (lanes past the
+// head do nothing); a wave has 64 / L neighbouring tokens of one head, so it writes one run
+// of memory, and keeps their angles while it goes over its heads: every `heads` of the four
+// waves of gridDim.y workgroups.
+template <class T, int VE, int L, bool BWD>
+__global__ void __launch_bounds__(kBlock) k_head_norm(const HeadNormArgs a) {
+  using S = typename T::storage;
+  constexpr int kSlots = 64 / L;
+  const int lane = threadIdx.x & 63, part = lane % L, slot = lane / L;
+  const int half = a.hd / 2, ch = part * VE;
+  const bool in_row = ch < half;
+  const int rows = a.heads + 2 * a.kv_heads;
+  const int first = (int)blockIdx.y * kWaves + wave_id(), every = (int)gridDim.y * kWaves;
+  const float inv_hd = 1.0f / (float)a.hd;
+  float gain[2][2][VE];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        gain[w][h][e] = in_row ? load_elem(w == 0 ? a.q_gain : a.k_gain, h * half + ch + e, a.gain_dtype) : 0.0f;
+  [[maybe_unused]] float dg[2][2][VE];
+  if constexpr (BWD) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) dg[w][h][e] = 0.0f;
+  }
+  for (int64_t t0 = (int64_t)blockIdx.x * kSlots; t0 < a.n_tok; t0 += (int64_t)gridDim.x * kSlots) {
+    const int64_t tok = t0 + slot;
+    const bool live = in_row && tok < a.n_tok;
+    const int64_t b = live ? tok / a.seq : 0;
+    const int t = live ? (int)(tok % a.seq) : 0;
+    float co[VE], si[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      co[e] = live ? a.cosv[(int64_t)t * half + ch + e] : 0.0f;
+      si[e] = live ? a.sinv[(int64_t)t * half + ch + e] : 0.0f;
+    }
+    for (int row = first; row < rows; row += every) {
+      const int which = row < a.heads ? 0 : row < a.heads + a.kv_heads ? 1 : 2;
+      const int head = which == 0 ? row : row - a.heads - (which == 1 ? 0 : a.kv_heads);
+      const int64_t packed = (tok * rows + row) * a.hd + ch;
+      S* const base = static_cast<S*>(which == 0 ? a.q : which == 1 ? a.k : a.v);
+      const int64_t* const st = a.strides[which];
+      S* const split = base + b * st[0] + head * st[1] + t * st[2] + ch;
+      const S* const x = static_cast<const S*>(a.qkv) + packed;
+      float u[2][VE], y[2][VE];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) u[h][e] = y[h][e] = 0.0f;
+      if (live) {
+        if (BWD || which == 2) {
+          const S* const from = BWD ? split : x;
+          ld_part<T, VE>(from, y[0]);
+          ld_part<T, VE>(from + half, y[1]);
+        }
+        if (which < 2) {
+          ld_part<T, VE>(x, u[0]);
+          ld_part<T, VE>(x + half, u[1]);
+        }
+      }
+      if (which < 2) {
+        const float r = head_rinv<VE, L>(u[0], u[1], inv_hd, a.eps);
+        if constexpr (BWD) {
+          float c = 0.0f;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) turn(y[0][e], y[1][e], co[e], -si[e]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              u[h][e] *= r;
+              const float t1 = y[h][e] * u[h][e];
+              dg[0][h][e] += which == 0 ? t1 : 0.0f;
+              dg[1][h][e] += which == 0 ? 0.0f : t1;
+              const float g = which == 0 ? gain[0][h][e] : gain[1][h][e];
+              c = fmaf(g, t1, c);
+              y[h][e] *= g;
+            }
+          c = lane_sum<L>(c) * inv_hd;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) y[h][e] = r * (y[h][e] - u[h][e] * c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            y[0][e] = u[0][e] * (r * (which == 0 ? gain[0][0][e] : gain[1][0][e]));
+            y[1][e] = u[1][e] * (r * (which == 0 ? gain[0][1][e] : gain[1][1][e]));
+            turn(y[0][e], y[1][e], co[e], si[e]);
+          }
+        }
+      }
+      if (live) {
+        S* const to = BWD ? static_cast<S*>(a.dqkv) + packed : split;
+        st_part<T, VE>(to, y[0]);
+        st_part<T, VE>(to + half, y[1]);
+      }
+    }
+  }
+  if constexpr (BWD) {
+    // The wave's tokens, then the workgroup's waves, in a fixed order.
+    __shared__ float fold[kWaves][2][2][L * VE];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          float x = dg[w][h][e];
+#pragma unroll
+          for (int d = L; d < 64; d *= 2) x += __shfl_xor(x, d);
+          if (slot == 0) fold[wave_id()][w][h][part * VE + e] = x;
+        }
+    __syncthreads();
+    const int64_t at = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    for (int i = threadIdx.x; i < 2 * a.hd; i += kBlock) {
+      const int w = i / a.hd, c = i % a.hd, h = c / half;
+      float x = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kWaves; ++v) x += fold[v][w][h][c - h * half];
+      a.partial[((int64_t)w * a.rows + at) * a.hd + c] = x;
+    }
+  }
+}
+
+// Eight columns a workgroup, 32 strands of rows folded in order.
+__global__ void __launch_bounds__(kBlock)
+k_head_norm_gains(const float* partial, int rows, int hd, void* dq_gain, void* dk_gain, int dtype) {
+  __shared__ float fold[32][8];
+  const int c0 = (int)blockIdx.x * 8, w = c0 / hd, c = c0 % hd + (threadIdx.x & 7), strand = threadIdx.x >> 3;
+  const float* const p = partial + (int64_t)w * rows * hd + c;
+  float x = 0.0f;
+#pragma unroll 8
+  for (int r = strand; r < rows; r += 32) x += p[(int64_t)r * hd];
+  fold[strand][threadIdx.x & 7] = x;
+  __syncthreads();
+  if (strand != 0) return;
+  x = 0.0f;
+#pragma unroll
+  for (int s = 0; s < 32; ++s) x += fold[s][threadIdx.x & 7];
+  store_elem(w == 0 ? dq_gain : dk_gain, c, x, dtype);
+}
+
+// Channels a lane has of each half, and the lanes of a head.
+int part_of(int hd, int dtype) { return dtype != SY_F32 && hd % 16 == 0 ? 8 : 4; }
+int lanes_of(int hd, int ve) {
+  int l = 1;
+  while (l * ve < hd / 2) l *= 2;
+  return l;
+}
+
+// Workgroups over the tokens, and over the heads where tokens alone are too few.
+void grid_of(const HeadNormArgs& a, int dtype, unsigned* gx, unsigned* gy) {
+  const int slots = 64 / lanes_of(a.hd, part_of(a.hd, dtype));
+  const int64_t groups = (a.n_tok + slots - 1) / slots;
+  *gx = (unsigned)std::min<int64_t>(groups, 2048);
+  const int most = (a.heads + 2 * a.kv_heads + kWaves - 1) / kWaves;
+  *gy = (unsigned)std::min<int64_t>(most, std::max<int64_t>(1, 1024 / *gx));
+}
+
+template <class T, int VE, int L>
+hipError_t run_norm(const HeadNormArgs& a, hipStream_t s) {
+  unsigned gx, gy;
+  grid_of(a, T::code, &gx, &gy);
+  if (a.dqkv != nullptr) hipLaunchKernelGGL((k_head_norm<T, VE, L, true>), dim3(gx, gy), dim3(kBlock), 0, s, a);
+  else hipLaunchKernelGGL((k_head_norm<T, VE, L, false>), dim3(gx, gy), dim3(kBlock), 0, s, a);
+  return hipGetLastError();
+}
+
+template <class T, int VE>
+hipError_t norm_lanes(const HeadNormArgs& a, hipStream_t s) {
+  switch (lanes_of(a.hd, VE)) {
+    case 1: return run_norm<T, VE, 1>(a, s);
+    case 2: return run_norm<T, VE, 2>(a, s);
+    case 4: return run_norm<T, VE, 4>(a, s);
+    case 8: return run_norm<T, VE, 8>(a, s);
+    case 16: return run_norm<T, VE, 16>(a, s);
+    case 32: return run_norm<T, VE, 32>(a, s);
+    default: return hipErrorInvalidConfiguration;
+  }
+}
+
+template <class T>
+hipError_t norm_t(const HeadNormArgs& a, hipStream_t s) {
+  if constexpr (T::ce == 8) {
+    if (part_of(a.hd, T::code) == 8) return norm_lanes<T, 8>(a, s);
+  }
+  return norm_lanes<T, 4>(a, s);
+}
+
+}  // namespace
+
+int head_norm_rows(const HeadNormArgs& a, int dtype) {
+  unsigned gx, gy;
+  grid_of(a, dtype, &gx, &gy);
+  return (int)(gx * gy);
+}
+
+hipError_t launch_head_norm(const HeadNormArgs& a, int dtype, hipStream_t s) {
+  if (dtype == SY_BF16) return norm_t<BF16>(a, s);
+  if (dtype == SY_F16) return norm_t<F16>(a, s);
+  return norm_t<F32>(a, s);
+}
+
+hipError_t launch_head_norm_gains(const HeadNormArgs& a, void* dq_gain, void* dk_gain, hipStream_t s) {
+  hipLaunchKernelGGL(k_head_norm_gains, dim3((unsigned)(2 * a.hd / 8)), dim3(kBlock), 0, s, a.partial, a.rows, a.hd,
+                     dq_gain, dk_gain, a.gain_dtype);
+  return hipGetLastError();
+}
+
+}  // namespace sy

@@ -81,6 +81,8 @@ bool needs_grad(const Tensor& a, const Tensor& b) {
   return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
 }
 
+bool tracked(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
 at::TensorOptions f32_on(const Tensor& t) { return t.options().dtype(at::kFloat).requires_grad(false); }
 
 // Sizes of stacked sources; `ok` false where the Python path has to see the call.
@@ -531,6 +533,111 @@ std::optional<variable_list> rope_qkv(const Tensor& qkv, const Tensor& cosv, con
   return rope_forward(qkv, cosv, sinv);
 }
 
+// The gains of a norm over heads of hd: of the activations' dtype or fp32, both the same.
+bool gains_ok(const Tensor& q_gain, const Tensor& k_gain, const Tensor& like, int64_t hd) {
+  for (const Tensor* g : {&q_gain, &k_gain})
+    if (!plain(*g) || g->dim() != 1 || g->size(0) != hd || g->device() != like.device() ||
+        g->scalar_type() != q_gain.scalar_type() ||
+        (g->scalar_type() != like.scalar_type() && g->scalar_type() != at::kFloat))
+      return false;
+  return true;
+}
+
+variable_list head_norm_forward(const Tensor& qkv, const Tensor& gq, const Tensor& gk, const Tensor& cosv,
+                                const Tensor& sinv, int64_t kv, double eps) {
+  const c10::DeviceGuard guard(qkv.device());
+  const int64_t b = qkv.size(0), t = qkv.size(1), h = qkv.size(2) - 2 * kv, hd = qkv.size(3);
+  variable_list r;
+  for (int k = 0; k < 3; ++k)
+    r.push_back(at::empty({b, k == 0 ? h : kv, t, hd}, qkv.options().requires_grad(false)));
+  check(sy_qk_norm_rope(qkv.data_ptr(), gq.data_ptr(), gk.data_ptr(), cosv.data_ptr<float>(), sinv.data_ptr<float>(),
+                        r[0].data_ptr(), r[1].data_ptr(), r[2].data_ptr(), b * t, t, h, kv, hd, code_of(qkv),
+                        code_of(gq), (float)eps, stream_of(qkv)),
+        "sy_qk_norm_rope");
+  return r;
+}
+
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& qkv_in, const Tensor& gq_in, const Tensor& gk_in,
+                               const Tensor& cosv, const Tensor& sinv, int64_t kv, double eps) {
+    Tensor qkv = dense(qkv_in);
+    if (!aligned16(qkv)) qkv = qkv.clone();
+    const Tensor gq = dense(gq_in), gk = dense(gk_in);
+    ctx->save_for_backward({qkv, gq, gk, cosv, sinv});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["kv"] = kv;
+    return head_norm_forward(qkv, gq, gk, cosv, sinv, kv, eps);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &qkv = saved[0], &gq = saved[1], &gk = saved[2];
+    const c10::DeviceGuard guard(qkv.device());
+    const double eps = ctx->saved_data["eps"].toDouble();
+    const int64_t b = qkv.size(0), t = qkv.size(1), kv = ctx->saved_data["kv"].toInt(), h = qkv.size(2) - 2 * kv,
+                  hd = qkv.size(3);
+    if (!kernel_backward(grads)) {  // the same from torch operations
+      const Tensor c = saved[3].reshape({-1, hd / 2}).slice(0, 0, t), s = saved[4].reshape({-1, hd / 2}).slice(0, 0, t);
+      const auto parts = qkv.transpose(1, 2).split_with_sizes({h, kv, kv}, 1);
+      variable_list dx, dg;
+      for (int k = 0; k < 2; ++k) {
+        const Tensor x = parts[k].to(at::kFloat), gain = (k == 0 ? gq : gk).to(at::kFloat);
+        const auto p = grads[k].to(at::kFloat).chunk(2, -1);
+        const Tensor e = at::cat({p[0] * c + p[1] * s, p[1] * c - p[0] * s}, -1);
+        const Tensor r = x.square().mean(-1, /*keepdim=*/true).add(eps).rsqrt(), u = x * r;
+        dx.push_back((r * (e * gain - u * (e * gain * u).mean(-1, /*keepdim=*/true))).to(qkv.scalar_type()));
+        dg.push_back((e * u).sum(at::IntArrayRef{0, 1, 2}).to(gq.scalar_type()));
+      }
+      dx.push_back(grads[2]);
+      return {at::cat(dx, 1).transpose(1, 2), dg[0], dg[1], Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+    int64_t strides[9];
+    for (int k = 0; k < 3; ++k) {
+      Tensor& g = grads[k];
+      bool fits = g.stride(3) == 1 && aligned16(g);
+      for (int d = 0; d < 3; ++d) fits = fits && g.stride(d) >= 0 && g.stride(d) % chunk(g) == 0;
+      if (!fits) g = g.clone(at::MemoryFormat::Contiguous);
+      for (int d = 0; d < 3; ++d) strides[3 * k + d] = g.stride(d);
+    }
+    Tensor dqkv = at::empty(qkv.sizes(), qkv.options().requires_grad(false));
+    Tensor dgq = at::empty({hd}, gq.options().requires_grad(false));
+    Tensor dgk = at::empty({hd}, gk.options().requires_grad(false));
+    const int64_t bytes = sy_qk_norm_rope_bwd_bytes(b * t, h, kv, hd, code_of(qkv));
+    if (bytes < 0) check(bytes, "sy_qk_norm_rope_bwd_bytes");
+    const Tensor ws = at::empty({std::max<int64_t>(1, bytes / 4)}, f32_on(qkv));
+    check(sy_qk_norm_rope_bwd(qkv.data_ptr(), gq.data_ptr(), gk.data_ptr(), saved[3].data_ptr<float>(),
+                              saved[4].data_ptr<float>(), grads[0].data_ptr(), grads[1].data_ptr(),
+                              grads[2].data_ptr(), strides, dqkv.data_ptr(), dgq.data_ptr(), dgk.data_ptr(),
+                              ws.data_ptr(), ws.numel() * 4, b * t, t, h, kv, hd, code_of(qkv), code_of(gq),
+                              (float)eps, stream_of(qkv)),
+          "sy_qk_norm_rope_bwd");
+    return {dqkv, dgq, dgk, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// qkv [B, T, heads + 2 kv, hd] (kv 0: a third of the heads), gains [hd], tables [>= T, (1,) hd/2]
+// -> (q, k, v), each [B, heads of it, T, hd].
+std::optional<variable_list> qk_norm_rope(const Tensor& qkv_in, const Tensor& gq, const Tensor& gk, const Tensor& cosv,
+                                          const Tensor& sinv, int64_t kv, double eps) {
+  if (!ordinary() || !plain(qkv_in) || qkv_in.dim() != 4 || qkv_in.numel() == 0 || !plain(cosv) || !plain(sinv))
+    return std::nullopt;
+  const int64_t rows = qkv_in.size(2), hd = qkv_in.size(3);
+  if (kv == 0) {
+    if (rows % 3 != 0) return std::nullopt;
+    kv = rows / 3;
+  }
+  if (kv < 1 || rows - 2 * kv < 1 || rows > 0xffff || hd % 8 != 0 || hd > 256 || !gains_ok(gq, gk, qkv_in, hd))
+    return std::nullopt;
+  for (const Tensor* t : {&cosv, &sinv})
+    if (t->scalar_type() != at::kFloat || t->device() != qkv_in.device() || !t->is_contiguous() || tracked(*t) ||
+        (t->dim() != 2 && t->dim() != 3) || t->size(-1) != hd / 2 || t->numel() != t->size(0) * t->size(-1) ||
+        t->size(0) < qkv_in.size(1))
+      return std::nullopt;
+  if (tracked(qkv_in) || tracked(gq) || tracked(gk)) return QkNormRope::apply(qkv_in, gq, gk, cosv, sinv, kv, eps);
+  Tensor qkv = dense(qkv_in);
+  if (!aligned16(qkv)) qkv = qkv.clone();
+  return head_norm_forward(qkv, dense(gq), dense(gk), cosv, sinv, kv, eps);
+}
+
 struct SwiGlu : torch::autograd::Function<SwiGlu> {
   static Tensor run(const Tensor& gu) {
     const c10::DeviceGuard guard(gu.device());
@@ -574,13 +681,15 @@ std::optional<Tensor> swiglu(const Tensor& gu) {
 
 // -------------------------------------------------------------------- serving
 
-bool whole(const Tensor& t) {  // a dense int32 GPU tensor that nothing intercepts
+// A dense GPU tensor of another type that nothing intercepts.
+bool whole_of(const Tensor& t, at::ScalarType type) {
   using c10::DispatchKey;
   constexpr c10::DispatchKeySet wrapped{DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
                                         DispatchKey::Batched, DispatchKey::Functionalize};
-  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == at::kInt &&
+  return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.scalar_type() == type &&
          !t.unsafeGetTensorImpl()->is_python_dispatch() && !t.key_set().has_any(wrapped);
 }
+bool whole(const Tensor& t) { return whole_of(t, at::kInt); }
 
 void changed(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -624,8 +733,6 @@ bool paged_of(const Tensor& like, int64_t heads, const Tensor& k, const Tensor& 
   return true;
 }
 
-bool tracked(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
-
 // The caller's output, if it is one the kernels can write.
 bool out_ok(const std::optional<Tensor>& out, const Tensor& like, int64_t n_tok, int64_t heads, int64_t hd) {
   return !out.has_value() ||
@@ -637,7 +744,8 @@ bool out_ok(const std::optional<Tensor>& out, const Tensor& like, int64_t n_tok,
 std::optional<Tensor> paged_append(const Tensor& qkv_in, const Tensor& cosv, const Tensor& sinv, const Tensor& k,
                                    const Tensor& v, const Tensor& table, const Tensor& lengths,
                                    const std::optional<Tensor>& starts, int64_t prefix_len,
-                                   const std::optional<Tensor>& out) {
+                                   const std::optional<Tensor>& out, const std::optional<Tensor>& q_gain,
+                                   const std::optional<Tensor>& k_gain, double eps) {
   sy_paged c;
   if (qkv_in.dim() != 3 || qkv_in.size(0) < 1 || k.dim() != 4) return std::nullopt;
   const int64_t heads = qkv_in.size(1) - 2 * k.size(1);
@@ -649,14 +757,27 @@ std::optional<Tensor> paged_append(const Tensor& qkv_in, const Tensor& cosv, con
     if (!plain(*t) || t->scalar_type() != at::kFloat || t->device() != qkv_in.device() || !t->is_contiguous() ||
         t->dim() < 2 || t->size(-1) * 2 != c.hd || t->numel() != t->size(0) * t->size(-1) || tracked(*t))
       return std::nullopt;
-  if (cosv.sizes() != sinv.sizes()) return std::nullopt;
+  if (cosv.sizes() != sinv.sizes() || q_gain.has_value() != k_gain.has_value()) return std::nullopt;
+  const bool norm = q_gain.has_value();
+  if (norm && (!gains_ok(*q_gain, *k_gain, qkv_in, c.hd) || tracked(*q_gain) || tracked(*k_gain))) return std::nullopt;
   const c10::DeviceGuard guard(qkv_in.device());
-  const Tensor qkv = qkv_in.stride(2) == 1 && qkv_in.stride(0) >= 0 && qkv_in.stride(1) >= 0 ? qkv_in : qkv_in.contiguous();
+  const bool fits = qkv_in.stride(2) == 1 && qkv_in.stride(0) >= 0 && qkv_in.stride(1) >= 0 &&
+                    (!norm || (qkv_in.stride(0) % 4 == 0 && qkv_in.stride(1) % 4 == 0 &&
+                               reinterpret_cast<uintptr_t>(qkv_in.data_ptr()) % (4 * qkv_in.element_size()) == 0));
+  const Tensor qkv = fits ? qkv_in : qkv_in.clone(at::MemoryFormat::Contiguous);
   Tensor q = out.has_value() ? *out : at::empty({c.n_tok, heads, c.hd}, qkv.options().requires_grad(false));
-  check(sy_paged_append(&c, qkv.data_ptr(), qkv.stride(0), qkv.stride(1), cosv.data_ptr<float>(),
-                        sinv.data_ptr<float>(), cosv.size(0), prefix_len, q.data_ptr(), out.has_value() ? 0 : 1,
-                        stream_of(qkv)),
-        "sy_paged_append");
+  if (norm) {
+    const Tensor gq = dense(*q_gain), gk = dense(*k_gain);
+    check(sy_paged_append_norm(&c, qkv.data_ptr(), qkv.stride(0), qkv.stride(1), gq.data_ptr(), gk.data_ptr(),
+                               code_of(gq), (float)eps, cosv.data_ptr<float>(), sinv.data_ptr<float>(), cosv.size(0),
+                               prefix_len, q.data_ptr(), out.has_value() ? 0 : 1, stream_of(qkv)),
+          "sy_paged_append_norm");
+  } else {
+    check(sy_paged_append(&c, qkv.data_ptr(), qkv.stride(0), qkv.stride(1), cosv.data_ptr<float>(),
+                          sinv.data_ptr<float>(), cosv.size(0), prefix_len, q.data_ptr(), out.has_value() ? 0 : 1,
+                          stream_of(qkv)),
+          "sy_paged_append");
+  }
   changed(k);
   changed(v);
   if (out.has_value()) changed(q);
@@ -731,6 +852,103 @@ std::optional<Tensor> sample_tokens(const Tensor& logits_in, const Tensor& u, do
   return tokens;
 }
 
+std::optional<Tensor> adjust_logits(const Tensor& logits_in, double repetition, double presence, double frequency,
+                                    const std::optional<Tensor>& tokens, const std::optional<Tensor>& lengths,
+                                    const std::optional<Tensor>& prompts, const std::optional<Tensor>& repetitions,
+                                    const std::optional<Tensor>& presences, const std::optional<Tensor>& frequencies,
+                                    const std::optional<Tensor>& bias, const std::optional<Tensor>& allowed,
+                                    const std::optional<Tensor>& out) {
+  if (!ordinary() || !plain(logits_in) || tracked(logits_in) || logits_in.dim() != 2 || logits_in.numel() == 0 ||
+      logits_in.size(1) > (1 << 30))
+    return std::nullopt;
+  const int64_t b = logits_in.size(0), v = logits_in.size(1);
+  const auto dev = logits_in.device();
+  sy_adjusting how{};
+  how.repetition = repetition, how.presence = presence, how.frequency = frequency;
+  how.tokens_bytes = 8;
+  if (tokens.has_value()) {
+    const Tensor& t = *tokens;
+    if (!(whole_of(t, at::kLong) || whole(t)) || t.device() != dev || t.dim() != 2 || t.size(0) != b ||
+        t.size(1) > 0x7fffffff || t.stride(0) < 0 || (t.size(1) > 1 && t.stride(1) != 1))
+      return std::nullopt;
+    how.tokens = t.data_ptr(), how.tokens_stride = t.stride(0), how.n_tokens = t.size(1);
+    how.tokens_bytes = (int32_t)t.element_size();
+  } else if (lengths.has_value() || prompts.has_value()) {
+    return std::nullopt;
+  }
+  const std::pair<const std::optional<Tensor>*, const int32_t**> ints[] = {{&lengths, &how.lengths},
+                                                                          {&prompts, &how.prompt_lengths}};
+  for (const auto& [t, p] : ints)
+    if (t->has_value()) {
+      if (!whole(**t) || (*t)->dim() != 1 || (*t)->size(0) != b || !(*t)->is_contiguous() || (*t)->device() != dev)
+        return std::nullopt;
+      *p = (*t)->data_ptr<int32_t>();
+    }
+  const std::pair<const std::optional<Tensor>*, const float**> floats[] = {
+      {&repetitions, &how.repetitions}, {&presences, &how.presences}, {&frequencies, &how.frequencies}};
+  for (const auto& [t, p] : floats)
+    if (t->has_value()) {
+      if (!plain(**t) || tracked(**t) || (*t)->scalar_type() != at::kFloat || (*t)->dim() != 1 || (*t)->size(0) != b ||
+          !(*t)->is_contiguous() || (*t)->device() != dev)
+        return std::nullopt;
+      *p = (*t)->data_ptr<float>();
+    }
+  if (bias.has_value()) {
+    const Tensor& t = *bias;
+    if (!plain(t) || tracked(t) || (t.scalar_type() != at::kFloat && t.scalar_type() != logits_in.scalar_type()) ||
+        t.device() != dev || t.dim() < 1 || t.dim() > 2 || t.size(-1) != v || (v > 1 && t.stride(-1) != 1) ||
+        (t.dim() == 2 && (t.size(0) != b || t.stride(0) < 0)))
+      return std::nullopt;
+    how.bias = t.data_ptr(), how.bias_dtype = code_of(t), how.bias_stride = t.dim() == 2 ? t.stride(0) : 0;
+  }
+  if (allowed.has_value()) {
+    const Tensor& t = *allowed;
+    const bool words = whole(t);
+    const int64_t n = words ? (v + 31) / 32 : v;
+    if ((!words && !whole_of(t, at::kBool)) || t.device() != dev || t.dim() < 1 || t.dim() > 2 || t.size(-1) != n ||
+        (n > 1 && t.stride(-1) != 1) || (t.dim() == 2 && (t.size(0) != b || t.stride(0) < 0)))
+      return std::nullopt;
+    how.mask = t.data_ptr(), how.mask_kind = words ? 1 : 2, how.mask_stride = t.dim() == 2 ? t.stride(0) : 0;
+  }
+  if (out.has_value() && (!plain(*out) || tracked(*out) || out->sizes() != logits_in.sizes() || out->device() != dev ||
+                          out->scalar_type() != logits_in.scalar_type() || (v > 1 && out->stride(1) != 1) ||
+                          (b > 1 && out->stride(0) < v)))
+    return std::nullopt;
+  const c10::DeviceGuard guard(dev);
+  const bool rows = (logits_in.stride(1) == 1 || v == 1) && logits_in.stride(0) >= 0;
+  const Tensor x = rows ? logits_in : logits_in.contiguous();
+  Tensor y = out.has_value() ? *out : at::empty({b, v}, x.options().requires_grad(false));
+  check(sy_adjust(x.data_ptr(), y.data_ptr(), &how, b, v, x.stride(0), y.stride(0), code_of(x), stream_of(x)),
+        "sy_adjust");
+  if (out.has_value()) changed(y);
+  return y;
+}
+
+std::optional<Tensor> linear4(const Tensor& x_in, const Tensor& tiles, const Tensor& scales,
+                              const std::optional<Tensor>& zeros, int64_t n, int64_t k, int64_t group) {
+  if (!ordinary() || !plain(x_in) || tracked(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || x_in.size(-1) != k ||
+      !whole(tiles) || !plain(scales) || tracked(scales) || scales.scalar_type() != x_in.scalar_type() ||
+      tiles.device() != x_in.device() || scales.device() != x_in.device() || !tiles.is_contiguous() ||
+      !scales.is_contiguous() || !aligned16(tiles) || (group != 32 && group != 64 && group != 128) || n < 1 ||
+      tiles.numel() != (n + 15) / 16 * ((k + 127) / 128) * 256 || scales.numel() != tiles.numel() * 8 / group ||
+      x_in.numel() / k > 0x7fffffff)
+    return std::nullopt;
+  if (zeros.has_value() && (!whole_of(*zeros, at::kByte) || zeros->device() != x_in.device() ||
+                            !zeros->is_contiguous() || zeros->numel() != scales.numel()))
+    return std::nullopt;
+  const c10::DeviceGuard guard(x_in.device());
+  Tensor x = x_in.dim() == 2 ? x_in : x_in.reshape({-1, k});
+  if ((k > 1 && x.stride(1) != 1) || x.stride(0) < 0) x = x.contiguous();
+  auto sizes = x_in.sizes().vec();
+  sizes.back() = n;
+  Tensor out = at::empty(sizes, x.options().requires_grad(false));
+  check(sy_linear4(x.data_ptr(), x.stride(0), tiles.data_ptr(), scales.data_ptr(),
+                   zeros.has_value() ? zeros->data_ptr<uint8_t>() : nullptr, out.data_ptr(), x.size(0), n, k, group,
+                   code_of(x), stream_of(x)),
+        "sy_linear4");
+  return out;
+}
+
 }  // namespace
 
 // The interpreter's lock is released during a call, as ctypes does.
@@ -745,7 +963,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rms_norm", &rms_norm, free_lock);
   m.def("rope_qkv", &rope_qkv, free_lock);
   m.def("swiglu", &swiglu, free_lock);
+  m.def("qk_norm_rope", &qk_norm_rope, free_lock);
   m.def("paged_append", &paged_append, free_lock);
   m.def("paged_attention", &paged_attention, free_lock);
+  m.def("adjust_logits", &adjust_logits, free_lock);
   m.def("sample_tokens", &sample_tokens, free_lock);
+  m.def("linear4", &linear4, free_lock);
 }

@@ -84,6 +84,16 @@ class Sampling(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("temperatures", "top_ps", "min_ps", "top_ks")])
 
 
+class Adjusting(ctypes.Structure):
+    """Mirror of ``sy_adjusting``."""
+
+    _fields_ = ([(n, ctypes.c_double) for n in ("repetition", "presence", "frequency")]
+                + [(n, ctypes.c_void_p) for n in ("repetitions", "presences", "frequencies", "tokens", "lengths",
+                                                  "prompt_lengths", "bias", "mask")]
+                + [(n, ctypes.c_int64) for n in ("tokens_stride", "n_tokens", "bias_stride", "mask_stride")]
+                + [(n, ctypes.c_int32) for n in ("tokens_bytes", "bias_dtype", "mask_kind")])
+
+
 #: Every symbol include/switchyard.h declares, with (restype, argtypes).
 SIGNATURES = {
     "sy_abi_version": (_i32, []),
@@ -134,6 +144,16 @@ SIGNATURES = {
     "sy_paged_attention": (_i32, [ctypes.POINTER(Paged), _vp, _i64, _i64, _vp, _vp, _i64, ctypes.c_float, _i32,
                                   _vp, _i64, _vp]),
     "sy_sample": (_i32, [_vp, _vp, _vp, ctypes.POINTER(Sampling), _i64, _i64, _i64, _i32, _vp]),
+    "sy_qk_norm_rope": (_i32, [_vp] * 8 + [_i64] * 5 + [_i32, _i32, ctypes.c_float, _vp]),
+    "sy_qk_norm_rope_bwd_bytes": (_i64, [_i64] * 4 + [_i32]),
+    "sy_qk_norm_rope_bwd": (_i32, [_vp] * 8 + [ctypes.POINTER(_i64)] + [_vp] * 4 + [_i64] * 6
+                            + [_i32, _i32, ctypes.c_float, _vp]),
+    "sy_paged_append_norm": (_i32, [ctypes.POINTER(Paged), _vp, _i64, _i64, _vp, _vp, _i32, ctypes.c_float, _vp, _vp,
+                                    _i64, _i64, _vp, _i32, _vp]),
+    "sy_adjust": (_i32, [_vp, _vp, ctypes.POINTER(Adjusting), _i64, _i64, _i64, _i64, _i32, _vp]),
+    "sy_quantize4": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "sy_pack4": (_i32, [_vp] * 6 + [_i64] * 3 + [_i32, _vp]),
+    "sy_linear4": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp]),
     "sy_bw_probe": (_i32, [_i32, _vp, _vp, _i64, _vp]),
     "sy_probe_grid": (_i64, [_i64]),
     "sy_tuning_set": (_i32, [ctypes.POINTER(Tuning)]),

@@ -37,6 +37,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from .hip_op import _ptr
+from .reference import DEFAULT_EPS
 
 __all__ = ["paged_append", "paged_attention"]
 
@@ -109,24 +110,31 @@ def _changed(*tensors) -> None:
 def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cache: torch.Tensor,
                  v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                  starts: torch.Tensor | None = None, *, prefix_len: int = 0,
-                 out: torch.Tensor | None = None) -> torch.Tensor:
+                 out: torch.Tensor | None = None, q_gain: torch.Tensor | None = None,
+                 k_gain: torch.Tensor | None = None, eps: float = DEFAULT_EPS) -> torch.Tensor:
     """Rotate a fused projection's queries and keys to their positions, write the keys and
     values into the cache and return the queries ``[n_tok, heads, head_dim]``.
 
     ``qkv [n_tok, heads + 2 kv_heads, head_dim]`` holds queries, keys and values;
     ``cos``, ``sin`` are fp32 ``[positions, head_dim / 2]`` (``[positions, 1, ...]`` as
     the decoder's). Row ``i`` of ``n`` new ones stands at ``lengths[b] - n + i``, behind
-    ``prefix_len``. Arithmetic is fp32, every output rounded once."""
+    ``prefix_len``. Arithmetic is fp32, every output rounded once.
+
+    With ``q_gain`` and ``k_gain`` (``[head_dim]``, of qkv's dtype or fp32) every query and key
+    head is normalised before it turns, as ``rope_op.qk_norm_rope`` does:
+    ``x / sqrt(mean(x^2) + eps) * gain``."""
     if (_lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths) and qkv.is_cuda
             and type(prefix_len) is int and (starts is None or _lib.ordinary(starts))
-            and (out is None or _lib.ordinary(out))):
-        q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out)
+            and (out is None or _lib.ordinary(out)) and (q_gain is None or _lib.ordinary(q_gain))
+            and (k_gain is None or _lib.ordinary(k_gain))):
+        q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out,
+                                       q_gain, k_gain, eps)
         if q is not None:
             return q
     if torch.compiler.is_compiling():
         return _append_untraced(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len=prefix_len,
-                                out=out)
-    _no_backward("paged_append", qkv, cos, sin, k_cache, v_cache, out)
+                                out=out, q_gain=q_gain, k_gain=k_gain, eps=eps)
+    _no_backward("paged_append", qkv, cos, sin, k_cache, v_cache, out, q_gain, k_gain)
     _need(qkv.ndim == 3, f"qkv must be [n_tok, heads + 2 kv_heads, head_dim], got {tuple(qkv.shape)}")
     _need(k_cache.ndim == 4, "k_cache must be [n_pages, kv_heads, page, head_dim]")
     heads = qkv.shape[1] - 2 * k_cache.shape[1]
@@ -140,14 +148,27 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
     shape = (c.n_tok, heads, c.hd)
     if out is not None:
         _validate_out(out, qkv, shape)
+    _need((q_gain is None) == (k_gain is None), "q_gain and k_gain go together")
+    for name, g in (("q_gain", q_gain), ("k_gain", k_gain)):
+        _need(g is None or (g.shape == (c.hd,) and g.device == qkv.device and g.dtype == q_gain.dtype
+                            and g.dtype in (qkv.dtype, torch.float32)),
+              f"{name} must be a [{c.hd}] tensor on the same CUDA device, of qkv's dtype or fp32, as the other gain is")
     if qkv.stride(2) != 1:
         qkv = qkv.contiguous()
+    if q_gain is not None:
+        q_gain, k_gain = q_gain.contiguous(), k_gain.contiguous()
+        if qkv.stride(0) % 4 or qkv.stride(1) % 4 or qkv.data_ptr() % (4 * qkv.element_size()):
+            qkv = qkv.clone(memory_format=torch.contiguous_format)
     q = torch.empty(shape, device=qkv.device, dtype=qkv.dtype) if out is None else out
     with torch.cuda.device(qkv.device):
-        rc = _lib.lib().sy_paged_append(ctypes.byref(c), _ptr(qkv), qkv.stride(0), qkv.stride(1), _ptr(cos), _ptr(sin),
-                                        cos.shape[0], prefix_len, _ptr(q), int(out is None),
-                                        _lib.stream_ptr(qkv.device))
-    _lib.check(rc, "sy_paged_append")
+        args = (_ptr(cos), _ptr(sin), cos.shape[0], prefix_len, _ptr(q), int(out is None), _lib.stream_ptr(qkv.device))
+        rows = (ctypes.byref(c), _ptr(qkv), qkv.stride(0), qkv.stride(1))
+        if q_gain is None:
+            rc = _lib.lib().sy_paged_append(*rows, *args)
+        else:
+            rc = _lib.lib().sy_paged_append_norm(*rows, _ptr(q_gain), _ptr(k_gain), _lib.dtype_code(q_gain.dtype),
+                                                 float(eps), *args)
+    _lib.check(rc, "sy_paged_append" if q_gain is None else "sy_paged_append_norm")
     _changed(k_cache, v_cache, out)
     return q
 

@@ -352,6 +352,22 @@ int sy_rms_norm_bwd(const void* x, const void* w, const void* grad_out, const fl
 int sy_rope_qkv(void* qkv, void* q, void* k, void* v, const float* cosv, const float* sinv,
                 int64_t n_tok, int64_t seq, int64_t heads, int64_t hd, int dtype, int backward,
                 void* stream);
+/* The same behind an RMSNorm of every query and key head, u = x g / sqrt(mean(x^2) + eps):
+ * qkv [n_tok][heads + 2 kv_heads][hd] (queries, keys, values) to q [n_tok/seq][heads][seq][hd]
+ * and k, v [n_tok/seq][kv_heads][seq][hd]; q_gain, k_gain [hd] of qkv's dtype or fp32; hd a
+ * multiple of 8, at most 256. The gradient reads dq, dk, dv with strides (elements, multiples
+ * of a 16-byte chunk) for batch, head and token, three each, rows of hd dense, and writes dqkv
+ * and the gains' gradients, summed over tokens in a fixed order in a workspace of
+ * sy_qk_norm_rope_bwd_bytes bytes. No reference counterpart. */
+int sy_qk_norm_rope(const void* qkv, const void* q_gain, const void* k_gain, const float* cosv, const float* sinv,
+                    void* q, void* k, void* v, int64_t n_tok, int64_t seq, int64_t heads, int64_t kv_heads,
+                    int64_t hd, int dtype, int gain_dtype, float eps, void* stream);
+int64_t sy_qk_norm_rope_bwd_bytes(int64_t n_tok, int64_t heads, int64_t kv_heads, int64_t hd, int dtype);
+int sy_qk_norm_rope_bwd(const void* qkv, const void* q_gain, const void* k_gain, const float* cosv,
+                        const float* sinv, const void* dq, const void* dk, const void* dv,
+                        const int64_t strides[9], void* dqkv, void* dq_gain, void* dk_gain, void* workspace,
+                        int64_t workspace_bytes, int64_t n_tok, int64_t seq, int64_t heads, int64_t kv_heads,
+                        int64_t hd, int dtype, int gain_dtype, float eps, void* stream);
 /* SwiGLU: out [n_tok][f] = silu(gate) * up over gate_up [n_tok][2 f], gate first;
  * f a multiple of a 16-byte chunk. The gradient writes d gate_up [n_tok][2 f]. */
 int sy_swiglu(const void* gate_up, void* out, int64_t n_tok, int64_t f, int dtype, void* stream);
@@ -411,6 +427,13 @@ int sy_paged_append(const sy_paged* c, const void* qkv, int64_t tok_stride, int6
                     const float* cosv, const float* sinv, int64_t n_pos, int64_t prefix_len, void* q,
                     int fill, void* stream);
 
+/* The same with every query and key head normalised before it turns, as sy_qk_norm_rope does;
+ * q_gain, k_gain [hd] of the cache's dtype or fp32. qkv's rows of heads start at multiples of
+ * four elements. */
+int sy_paged_append_norm(const sy_paged* c, const void* qkv, int64_t tok_stride, int64_t head_stride,
+                         const void* q_gain, const void* k_gain, int gain_dtype, float eps, const float* cosv,
+                         const float* sinv, int64_t n_pos, int64_t prefix_len, void* q, int fill, void* stream);
+
 /* out[i] = sum_j softmax_j(scale <q_i, k_j>) v_j over the keys up to row i's own position
  * (and the whole prefix); q row i at q + i q_tok_stride + head q_head_stride (16-byte
  * aligned), out [n_tok][heads][hd] dense. Query head h reads kv head h kv_heads / heads.
@@ -442,6 +465,57 @@ typedef struct sy_sampling {
 } sy_sampling;
 int sy_sample(const void* logits, const float* u, int64_t* tokens, const sy_sampling* how, int64_t n_rows,
               int64_t vocab, int64_t row_stride, int dtype, void* stream);
+
+/* Logits [n_rows][vocab] (rows row_stride apart) before sampling, to out (rows out_stride
+ * apart, which may be the logits themselves). A token among the first lengths[row] (NULL: all)
+ * of the n_tokens in the row's history has x / repetition where x > 0 and x repetition
+ * elsewhere, less frequency times its occurrences from prompt_lengths[row] (NULL: 0) on, less
+ * presence if there are any. Then biases [vocab] (rows bias_stride apart; 0: shared) are
+ * added, and tokens that the mask does not allow are -inf: kind 1 is 32 tokens to a 32-bit
+ * word, the lowest bit first, kind 2 a byte each; rows mask_stride words or bytes apart (0:
+ * shared). Tokens outside [0, vocab) are passed over. Each of the three settings is a number,
+ * or with its pointer set a device array of one a row. Computed in fp64 and fp32, rounded
+ * once. No reference counterpart. */
+typedef struct sy_adjusting {
+  double repetition;
+  double presence;
+  double frequency;
+  const float* repetitions;
+  const float* presences;
+  const float* frequencies;
+  const void* tokens; /* [n_rows][n_tokens], rows tokens_stride elements apart */
+  const int32_t* lengths;
+  const int32_t* prompt_lengths;
+  const void* bias;
+  const void* mask;
+  int64_t tokens_stride;
+  int64_t n_tokens;
+  int64_t bias_stride;
+  int64_t mask_stride;
+  int32_t tokens_bytes; /* 4 or 8 */
+  int32_t bias_dtype;   /* SY_F32 or the logits' */
+  int32_t mask_kind;    /* 0: all are allowed */
+} sy_adjusting;
+int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_rows, int64_t vocab,
+              int64_t row_stride, int64_t out_stride, int dtype, void* stream);
+
+/* Projections with 4-bit weights: out[i][j] = sum_c x[i][c] s[j][c / group] (codes[j][c] -
+ * zeros[j][c / group]), codes 0 to 15, zeros 8 where there are none; group 32, 64 or 128; n
+ * features and k columns of up to 2^24. One dtype for x, out and the scales.
+ *
+ * codes are [n][(k + 1) / 2] bytes of two columns, the even one in the low half; scales and
+ * zeros [n][ceil(k / group)]. sy_quantize4 makes them from weights [n][k] (rows row_stride
+ * apart): symmetric, codes 1 to 15, without zeros; over the range of each group with them.
+ * sy_pack4 lays them out for sy_linear4: tiles of 1024 bytes for 16 features by 128 columns,
+ * ceil(n / 16) ceil(k / 128) of them, 16-byte aligned; tile_scales and tile_zeros
+ * [ceil(n / 16)][ceil(k / 128) 128 / group][16]. Rows of x are x_stride elements apart and
+ * start anywhere; a row with an infinity or NaN gives NaN. No reference counterpart. */
+int sy_quantize4(const void* w, int64_t row_stride, uint8_t* codes, void* scales, uint8_t* zeros, int64_t n,
+                 int64_t k, int64_t group, int dtype, void* stream);
+int sy_pack4(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* tiles, void* tile_scales,
+             uint8_t* tile_zeros, int64_t n, int64_t k, int64_t group, int dtype, void* stream);
+int sy_linear4(const void* x, int64_t x_stride, const void* tiles, const void* tile_scales, const uint8_t* tile_zeros,
+               void* out, int64_t m, int64_t n, int64_t k, int64_t group, int dtype, void* stream);
 
 /* Speed-of-light ceiling: out[t] = sum_n v_n[t] with the forward's geometry and
  * bytes but no softmax. Replaces speed_of_light (src/switchyard/triton_op.py:153-191). */

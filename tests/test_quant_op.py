@@ -1,0 +1,208 @@
+"""Projections with 4-bit weights on the GPU against float64.
+
+Tolerances. Products of x and 1 + c / 16 are exact in fp32. A group's sum is off by at most
+(group + 40) 2^-23 of A = sum |x| (1 + c / 16) + (1 + z / 16) sum |x| (an addition each, the
+matrix instruction's inner ones cut off instead of rounded), and sums over groups by (groups +
+8) 2^-24 of what they add up. fp32 rows are three bf16 numbers, so three times the additions.
+The output is rounded once: eps / 2 of the value."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover
+    pytest.skip("needs a HIP device", allow_module_level=True)
+
+from oracle.reference import dtype_floor, rel_l2  # noqa: E402
+from switchyard import _lib  # noqa: E402
+from switchyard.quant_op import Linear4, Weight4, linear4, quantize4  # noqa: E402
+
+DEV = "cuda"
+BF, HF, F = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _codes(n, k, group, dtype, zeros, seed):
+    g = _gen(seed)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    shape = (n, -(-k // group))
+    scales = (0.01 + 0.02 * torch.rand(shape, generator=g)).to(dtype)
+    z = torch.randint(0, 16, shape, generator=g, dtype=torch.uint8) if zeros else None
+    padded = torch.nn.functional.pad(codes, (0, k % 2))
+    return codes, padded[:, 0::2] | padded[:, 1::2] << 4, scales, z
+
+
+def _check(x, codes, scales, zeros, group, got):
+    x6, s6 = x.cpu().double(), scales.double()
+    n, k = codes.shape
+    z6 = torch.full(scales.shape, 8.0, dtype=torch.float64) if zeros is None else zeros.double()
+    out = torch.zeros(x6.shape[0], n, dtype=torch.float64)
+    off = torch.zeros_like(out)
+    planes = 3 if x.dtype == F else 1
+    total = torch.zeros_like(out)
+    for g in range(scales.shape[1]):
+        at = slice(g * group, min(k, (g + 1) * group))
+        xs, c = x6[:, at], codes[:, at].double()
+        part = xs @ (c - z6[:, g:g + 1]).T * s6[:, g]
+        a = 16 * s6[:, g].abs() * (xs.abs() @ (1 + c / 16).T + xs.abs().sum(1, keepdim=True) * (1 + z6[:, g] / 16))
+        out += part
+        off += a * planes * (group + 40) * 2.0**-23
+        total += part.abs()
+    off += total * (scales.shape[1] + 8) * 2.0**-24
+    u = torch.finfo(x.dtype).eps / 2
+    tiny = torch.finfo(x.dtype).smallest_normal if x.dtype == HF else 0.0  # (fp16's small numbers have a fixed step)
+    tol = off + u * (out.abs() + off) + tiny * u
+    diff = (got.cpu().double() - out).abs()
+    assert (diff <= tol).all(), (diff / tol.clamp_min(1e-300)).max().item()
+    if x6.shape[0] * n > 200:
+        assert rel_l2(got.cpu(), out) <= (2e-6 if x.dtype == F else 1.10 * dtype_floor(out, x.dtype))
+
+
+SIZES = [(1, 16, 128), (1, 1, 1), (3, 17, 33), (16, 64, 256), (17, 100, 130), (5, 777, 1001), (33, 48, 640), (64, 130, 96),
+         (65, 33, 2048), (130, 200, 257), (300, 70, 384), (2, 1030, 4096), (1, 16400, 128)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype,zeros", [(BF, False), (BF, True), (HF, True), (F, False), (F, True)])
+def test_product(m, n, k, group, dtype, zeros):
+    codes, packed, scales, z = _codes(n, k, group, dtype, zeros, seed=n + k)
+    x = torch.randn(m, k, generator=_gen(m)).to(dtype)
+    w = Weight4.from_codes(packed.to(DEV), scales.to(DEV), None if z is None else z.to(DEV), in_features=k, group=group)
+    got = linear4(x.to(DEV), w)
+    assert got.shape == (m, n) and got.dtype == dtype
+    _check(x, codes, scales, z, group, got)
+    c, s, zz = w.codes()
+    assert torch.equal(c.cpu(), codes) and torch.equal(s.cpu(), scales)
+    assert (zz is None) == (z is None) and (z is None or torch.equal(zz.cpu(), z))
+
+
+def test_activations_that_share_a_sign_and_large_zero_points():
+    """Where the two sums of a group nearly cancel."""
+    codes, packed, scales, z = _codes(96, 512, 128, BF, True, seed=3)
+    z = (z.int() + 12).to(torch.uint8)  # past the codes' range
+    x = (100.0 + torch.randn(20, 512, generator=_gen(4))).to(BF)
+    w = Weight4.from_codes(packed.to(DEV), scales.to(DEV), z.to(DEV), in_features=512, group=128)
+    _check(x, codes, scales, z, 128, linear4(x.to(DEV), w))
+
+
+def test_rows_of_any_shape_start_and_stride():
+    codes, packed, scales, _ = _codes(40, 130, 64, BF, False, seed=5)
+    w = Weight4.from_codes(packed.to(DEV), scales.to(DEV), in_features=130, group=64)
+    x = torch.randn(6, 130, generator=_gen(6)).to(BF)
+    want = linear4(x.to(DEV), w)
+    wide = torch.full((6, 200), float("nan"), dtype=BF)
+    wide[:, 7:137] = x
+    assert torch.equal(linear4(wide.to(DEV)[:, 7:137], w), want)
+    assert torch.equal(linear4(x.to(DEV).t().contiguous().t(), w), want)
+    assert torch.equal(linear4(x.to(DEV).view(2, 3, 130), w), want.view(2, 3, 40))
+    assert torch.equal(linear4(x.to(DEV)[:1].expand(4, 130), w), want[:1].expand(4, 40))
+    assert torch.equal(linear4(x.to(DEV)[0], w), want[0])
+    assert linear4(x.to(DEV)[:0], w).shape == (0, 40)
+    assert linear4(torch.empty(3, 0, 130, dtype=BF, device=DEV), w).shape == (3, 0, 40)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_rows_with_infinities_do_not_touch_others(dtype):
+    codes, packed, scales, _ = _codes(64, 256, 64, dtype, False, seed=7)
+    w = Weight4.from_codes(packed.to(DEV), scales.to(DEV), in_features=256, group=64)
+    x = torch.randn(20, 256, generator=_gen(8)).to(dtype)
+    bad = x.clone()
+    bad[3, 100], bad[11, 5], bad[17, 255] = math.inf, math.nan, -math.inf
+    got, want = linear4(bad.to(DEV), w), linear4(x.to(DEV), w)
+    rows = [i for i in range(20) if i not in (3, 11, 17)]
+    assert got[[3, 11, 17]].isnan().all() and torch.equal(got[rows], want[rows])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("n,k,group", [(5, 64, 32), (33, 200, 64), (16, 129, 128), (1, 1, 32), (70, 512, 128)])
+def test_quantized_weights_are_the_nearest(n, k, group, symmetric, dtype):
+    w = torch.randn(n, k, generator=_gen(n)).to(dtype)
+    w[0, :group] = 0.0  # a group of zeros
+    q = quantize4(w.to(DEV), group, symmetric=symmetric)
+    c, s, z = (None if t is None else t.cpu() for t in q.codes())
+    of = torch.arange(k) // group
+    w6, s6 = w.double(), s.double()
+    z6 = torch.full(s.shape, 8.0, dtype=torch.float64) if z is None else z.double()
+    for g in range(s.shape[1]):
+        part = w6[:, g * group:(g + 1) * group]
+        top = part.abs().amax(1) / 7 if symmetric else (part.amax(1).clamp_min(0) - part.amin(1).clamp_max(0)) / 15
+        assert ((s6[:, g] - top).abs() <= torch.finfo(dtype).eps / 2 * top + 2.0**-24 * top).all()
+    # Nearest to the kept scale, but for quotients within 2^-23 of a half and ends of the range.
+    best = (w6 / s6[:, of].clamp_min(1e-300)).clamp(-100, 100) + z6[:, of]
+    near = best.clamp(1 if symmetric else 0, 15)
+    live = s6[:, of] > 0
+    assert ((c.double() - near).abs()[live] <= 0.5 + 1e-5).all()
+    assert (c[~live] == 8 if symmetric else c[~live] == z6[:, of][~live]).all()
+    assert torch.equal(q.dequantize().cpu().double(), ((c.double() - z6[:, of]) * s6[:, of]).float().double())
+
+
+def test_the_module_its_state_and_autocast():
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(200, 96, bias=False, device=DEV)
+    m = Linear4.from_linear(lin, 32, symmetric=False)
+    x = torch.randn(7, 200, device=DEV)
+    want = m(x)
+    assert torch.equal(want, linear4(x, m.weight4))
+    other = Linear4(quantize4(torch.randn(96, 200, device=DEV), 32, symmetric=False))
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other(x), want)
+    half = Linear4(quantize4(lin.weight.detach().bfloat16(), 32))
+    with torch.autocast("cuda", dtype=BF):
+        assert torch.equal(half(x), half(x.bfloat16()))
+    with pytest.raises(ValueError, match="dtype"):
+        half(x)
+    with pytest.raises(ValueError, match="bias"):
+        Linear4.from_linear(torch.nn.Linear(8, 8, device=DEV))
+
+
+def test_gradients_and_tangents_are_refused():
+    w = quantize4(torch.randn(32, 64, device=DEV))
+    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        linear4(x, w)
+    with torch.no_grad():
+        linear4(x, w)
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="tangents"):
+        linear4(fwad.make_dual(x.detach(), torch.ones_like(x)), w)
+
+
+def test_another_stream_a_graph_and_two_calls_at_once():
+    w = quantize4(torch.randn(512, 1024, device=DEV).bfloat16())
+    x = torch.randn(9, 1024, device=DEV).bfloat16()
+    want = linear4(x, w)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(linear4(x, w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = linear4(x, w)
+    for i in range(3):
+        x.copy_(torch.randn(9, 1024, device=DEV).bfloat16())
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, linear4(x, w))
+
+
+def test_the_python_path_gives_the_same(monkeypatch):
+    w = quantize4(torch.randn(80, 100, device=DEV), 32, symmetric=False)
+    x = torch.randn(4, 100, device=DEV)
+    want = linear4(x, w)
+    monkeypatch.setattr(_lib, "ordinary", lambda *t: False)
+    assert torch.equal(linear4(x, w), want) and torch.equal(linear4(x.t().contiguous().t(), w), want)
