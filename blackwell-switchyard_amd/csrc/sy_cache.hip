@@ -180,76 +180,105 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
 
 // The same behind a norm of every query and key head, u = x r g with r = 1 / sqrt(mean(x^2) +
 // eps): L lanes a head, a power of two, of which the ones past it do nothing, each with two
-// chunks of VE elements that turn together; the sum of squares stays among them.
+// chunks of VE elements that turn together; the sum of squares stays among them. `split` waves
+// share a token's heads, kAhead rounds of them on their way before the first is needed, and
+// before the token's place is known.
 template <class T, int VE, int L>
-__global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a) {
+__global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a, int split, int first) {
   using S = typename T::storage;
+  constexpr int kHeads = 64 / L, kAhead = 3;  // heads of a wave's round
   const CacheArgs& c = a.c;
-  const int half = c.hd / 2, part = threadIdx.x % L, ch = part * VE;
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int half = c.hd / 2, ch = lane % L * VE;
   const int rows = c.heads + 2 * c.kv_heads;
   const float inv_hd = 1.0f / (float)c.hd;
   const bool in_head = ch < half;
   S* const q = static_cast<S*>(a.q);
-  for (int tok = blockIdx.x; tok < c.n_tok; tok += gridDim.x) {
-    const S* const from = static_cast<const S*>(a.qkv) + tok * a.tok_stride;
-    const int b = find_seq(c, tok);
-    if (b < 0) {
-      if (a.fill && outside(c, tok)) {
-        const Chunk<T, VE> zero{};
-        for (int i = threadIdx.x; i < c.heads * c.hd / VE; i += kBlock)
-          st_chunk<T, VE>(q + (int64_t)tok * c.heads * c.hd + i * VE, zero);
-      }
-      continue;
+  const int tok = first + (int)blockIdx.x * (kWaves / split) + wave / split;
+  if (tok >= c.n_tok) return;
+  const S* const from = static_cast<const S*>(a.qkv) + tok * a.tok_stride + ch;
+  int head = wave % split * kHeads + lane / L;
+  Chunk<T, VE> lo[kAhead], hi[kAhead];
+  const auto load = [&]() {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = head + i * split * kHeads;
+      lo[i] = hi[i] = Chunk<T, VE>{};
+      if (!in_head || h >= rows) continue;
+      lo[i] = ld_chunk<T, VE>(from + h * a.head_stride);
+      hi[i] = ld_chunk<T, VE>(from + h * a.head_stride + half);
     }
-    const Seq s = seq_of(c, b);
-    const int j = s.len - s.n + (tok - s.row0);  // position among the sequence's own tokens
-    const int64_t at = j + a.offset;
-    uint64_t dst = 0;
-    bool placed = j >= 0 && j < c.cap && at < a.n_pos;
-    if (placed) {
-      const int id = c.table[b * c.table_stride + (j >> c.page_shift)];
-      placed = (unsigned)id < (unsigned)c.n_pages;
-      if (placed) dst = row_at(c, id, j);
+  };
+  load();
+  float gain[2][2][VE] = {};
+  if (in_head) {
+    const bool wide = a.gain_dtype == F32::code;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      ld_gains<T, VE>(a.q_gain, h * half + ch, wide, gain[0][h]);
+      ld_gains<T, VE>(a.k_gain, h * half + ch, wide, gain[1][h]);
     }
-    // (Whole waves go round together: their lanes add up their squares.)
-    for (int head0 = 0; head0 < rows; head0 += kBlock / L) {
-      const int head = head0 + threadIdx.x / L;
-      const bool live = in_head && head < rows;
-      Chunk<T, VE> lo{}, hi{};
-      if (live) {
-        const S* const src = from + head * a.head_stride + ch;
-        lo = ld_chunk<T, VE>(src);
-        hi = ld_chunk<T, VE>(src + half);
+  }
+  const int b = find_seq(c, tok);
+  if (b < 0) {
+    if (a.fill && outside(c, tok)) {
+      const Chunk<T, VE> zero{};
+      for (int i = wave % split * 64 + lane; i < c.heads * c.hd / VE; i += split * 64)
+        st_chunk<T, VE>(q + (int64_t)tok * c.heads * c.hd + i * VE, zero);
+    }
+    return;
+  }
+  const Seq s = seq_of(c, b);
+  const int j = s.len - s.n + (tok - s.row0);  // position among the sequence's own tokens
+  const int64_t at = j + a.offset;
+  uint64_t dst = 0;
+  bool placed = j >= 0 && j < c.cap && at < a.n_pos;
+  float co[VE] = {}, si[VE] = {};
+  if (placed) {
+    const int id = c.table[b * c.table_stride + (j >> c.page_shift)];
+    if (in_head) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        co[e] = a.cosv[at * half + ch + e];
+        si[e] = a.sinv[at * half + ch + e];
       }
-      const float r = head_rinv<VE, L>(lo.f, hi.f, inv_hd, a.eps);
-      if (!live) continue;
-      if (head < c.heads + c.kv_heads && placed) {
-        const float* const cp = a.cosv + at * half + ch;
-        const float* const sp = a.sinv + at * half + ch;
-        const void* const g = head < c.heads ? a.q_gain : a.k_gain;
+    }
+    placed = (unsigned)id < (unsigned)c.n_pages;
+    if (placed) dst = row_at(c, id, j);
+  }
+  // (The bounds are the wave's: its lanes add up their squares.)
+  for (int round = wave % split * kHeads; round < rows; round += kAhead * split * kHeads) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = head + i * split * kHeads;
+      const float r = head_rinv<VE, L>(lo[i].f, hi[i].f, inv_hd, a.eps);
+      if (!in_head || h >= rows) continue;
+      const bool key = h >= c.heads, turned = h < c.heads + c.kv_heads;
+      if (turned) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          lo.f[e] *= r * load_elem(g, ch + e, a.gain_dtype);
-          hi.f[e] *= r * load_elem(g, half + ch + e, a.gain_dtype);
-          turn(lo.f[e], hi.f[e], cp[e], sp[e]);
+          lo[i].f[e] *= r * (key ? gain[1][0][e] : gain[0][0][e]);
+          hi[i].f[e] *= r * (key ? gain[1][1][e] : gain[0][1][e]);
+          turn(lo[i].f[e], hi[i].f[e], co[e], si[e]);
         }
       }
       S* out;
-      if (head < c.heads) {
+      if (!key) {
         if (!placed) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) lo.f[e] = hi.f[e] = __int_as_float(0x7fc00000);
+          for (int e = 0; e < VE; ++e) lo[i].f[e] = hi[i].f[e] = __int_as_float(0x7fc00000);
         }
-        out = q + ((int64_t)tok * c.heads + head) * c.hd + ch;
+        out = q + ((int64_t)tok * c.heads + h) * c.hd + ch;
       } else {
         if (!placed) continue;
-        const bool key = head < c.heads + c.kv_heads;
-        const int h = head - c.heads - (key ? 0 : c.kv_heads);
-        out = bytes_on(static_cast<S*>(key ? c.k : c.v) + h * c.head_stride + ch, dst);
+        const int kv = h - c.heads - (turned ? 0 : c.kv_heads);
+        out = bytes_on(static_cast<S*>(turned ? c.k : c.v) + kv * c.head_stride + ch, dst);
       }
-      st_chunk<T, VE>(out, lo);
-      st_chunk<T, VE>(out + half, hi);
+      st_chunk<T, VE>(out, lo[i]);
+      st_chunk<T, VE>(out + half, hi[i]);
     }
+    head += kAhead * split * kHeads;
+    if (round + kAhead * split * kHeads < rows) load();
   }
 }
 
@@ -1867,9 +1896,18 @@ hipError_t append_t(const AppendArgs& a, hipStream_t s) {
 
 template <class T, int VE, int L>
 hipError_t append_norm_t(const AppendArgs& a, hipStream_t s) {
-  const unsigned grid = (unsigned)std::min(a.c.n_tok, 1 << 20);
-  hipLaunchKernelGGL((k_append_norm<T, VE, L>), dim3(grid), dim3(kBlock), 0, s, a);
-  return hipGetLastError();
+  // A workgroup for a token, or where they are many a wave.
+  const int split = a.c.n_tok < 1024 ? kWaves : 1;
+  constexpr int kTokens = 1 << 23;  // of a launch
+  for (int at = 0; at < a.c.n_tok; at += kTokens) {
+    const int n = std::min(kTokens, a.c.n_tok - at);
+    hipLaunchKernelGGL((k_append_norm<T, VE, L>), dim3((unsigned)((n + kWaves / split - 1) / (kWaves / split))),
+                       dim3(kBlock), 0, s, a, split, at);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.c.n_tok - at <= kTokens) break;
+  }
+  return hipSuccess;
 }
 
 template <class T, int VE>

@@ -1357,7 +1357,7 @@ int sy_pack4(const uint8_t* codes, const void* scales, const uint8_t* zeros, voi
   const int rc = quant_sizes(n, k, group, dtype);
   if (rc != SY_OK) return rc;
   if (!codes || !scales || !tiles || !tile_scales || !zeros != !tile_zeros) return SY_ERR_NULL;
-  if (!al16(tiles)) return SY_ERR_SHAPE;
+  if (!al16(tiles) || !al16(tile_scales) || reinterpret_cast<uintptr_t>(tile_zeros) % 4 != 0) return SY_ERR_SHAPE;
   const PackArgs a{codes, scales, zeros, static_cast<uint32_t*>(tiles), tile_scales, tile_zeros, n, k, (int)group,
                    (int)esize(dtype)};
   return status(launch_pack4(a, (hipStream_t)stream));
@@ -1371,7 +1371,7 @@ int sy_linear4(const void* x, int64_t x_stride, const void* tiles, const void* t
   if (x_stride < 0) return SY_ERR_STRIDE;
   if (m == 0) return SY_OK;
   if (!x || !tiles || !tile_scales || !out) return SY_ERR_NULL;
-  if (!al16(tiles)) return SY_ERR_SHAPE;
+  if (!al16(tiles) || !al16(tile_scales) || reinterpret_cast<uintptr_t>(tile_zeros) % 4 != 0) return SY_ERR_SHAPE;
   const Linear4Args a{x, x_stride, static_cast<const uint32_t*>(tiles), tile_scales, tile_zeros, out, m, n, (int)k,
                       (int)group};
   return status(launch_linear4(a, dtype, (hipStream_t)stream));

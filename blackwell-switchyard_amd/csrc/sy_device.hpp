@@ -716,6 +716,24 @@ __device__ __forceinline__ float lane_sum(float x) {
   return x;
 }
 
+// VE (4 or 8) gains from p + i on, as fp32: of T, or fp32 with `wide`. They start anywhere.
+template <class T, int VE>
+__device__ __forceinline__ void ld_gains(const void* p, int i, bool wide, float (&f)[VE]) {
+  if (T::code == F32::code || wide) {
+#pragma unroll
+    for (int q = 0; q < VE / 4; ++q) {
+      const i32x4_t w = *reinterpret_cast<const i32x4_f32_t*>(static_cast<const float*>(p) + i + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * q + e] = __int_as_float(w[e]);
+    }
+  } else {
+    i32x4_t w = {0, 0, 0, 0};
+    __builtin_memcpy(&w, static_cast<const uint16_t*>(p) + i, 2 * VE);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) f[e] = elem<T>(w, e);
+  }
+}
+
 // 1 / sqrt(mean(x^2) + eps) of a head that L lanes hold, VE channels of each half a lane, and
 // the rotation of a pair. The contractions are written out, so that every kernel rounds alike.
 template <int VE, int L>

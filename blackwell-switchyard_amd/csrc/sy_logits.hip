@@ -12,7 +12,6 @@ namespace sy {
 
 namespace {
 
-typedef int i32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_any_t __attribute__((ext_vector_type(2), aligned(1)));
 
 constexpr int kBlock = 256;
@@ -53,41 +52,92 @@ __device__ __forceinline__ void count(uint32_t* seen, int64_t token, int lo, int
   else atomicOr(&seen[at], kPrompt);
 }
 
-// A workgroup takes a slice of one row. It reads the row's whole history and counts in LDS
-// what falls into its slice, in whole numbers, so in any order; then one pass over the
-// logits. Chunks that stay as they are in place are not touched, and those with nothing
-// allowed are not read.
-template <class T>
-__global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice, int slices) {
+// The row's first `len` tokens, eight a thread on their way at a time.
+template <class I>
+__device__ __forceinline__ void count_all(uint32_t* seen, const I* t, int64_t len, int64_t prompt, int lo, int n) {
+  constexpr int kAhead = 8;
+  for (int64_t i0 = threadIdx.x; i0 < len; i0 += kBlock * kAhead) {
+    I x[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t i = i0 + j * kBlock;
+      x[j] = i < len ? t[i] : (I)-1;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) count(seen, x[j], lo, n, i0 + j * kBlock >= prompt);
+  }
+}
+
+// CE neighbouring numbers at p as fp32; those from `n` on are zero.
+template <class T, int CE> __device__ __forceinline__ void ld_row_part(const void* p, int n, float (&f)[CE]) {
   using S = typename T::storage;
-  constexpr int CE = T::ce;
+  const S* const s = static_cast<const S*>(p);
+  if (n >= CE) {
+#pragma unroll
+    for (int q = 0; q < CE / T::ce; ++q) {
+      const i32x4_t w = *reinterpret_cast<const i32x4_any_t*>(s + q * T::ce);
+#pragma unroll
+      for (int e = 0; e < T::ce; ++e) f[q * T::ce + e] = elem<T>(w, e);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < CE; ++e) f[e] = e < n ? load_elem(s, e, T::code) : 0.0f;
+  }
+}
+
+// A workgroup takes a slice of one row, IT chunks a thread, all of them on their way while it
+// reads the row's history and counts in LDS what falls into its slice: in whole numbers, so in
+// any order. Chunks with nothing allowed are not read; in place and without a bias only those
+// are that something was counted in, and all that stay as they are are not written.
+template <class T, int IT>
+__global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slices) {
+  using S = typename T::storage;
+  constexpr int CE = T::ce, kSlice = kBlock * CE * IT;
+  constexpr uint32_t all = (1u << CE) - 1u;
   extern __shared__ uint32_t seen[];
   const int64_t row = blockIdx.x / slices;
-  const int lo = (int)(blockIdx.x % slices) * slice, n = min(slice, a.vocab - lo);
+  const int lo = (int)(blockIdx.x % slices) * kSlice, n = min(kSlice, a.vocab - lo);
+  const S* const x = static_cast<const S*>(a.logits) + row * a.row_stride + lo;
+  S* const y = static_cast<S*>(a.out) + row * a.out_stride + lo;
+  const bool in_place = static_cast<const void*>(x) == static_cast<const void*>(y);
+  const bool lazy = in_place && a.bias == nullptr;
+  uint32_t keep[IT];
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const int c = (k * kBlock + threadIdx.x) * CE;
+    keep[k] = c < n ? allowed<CE>(a, row, lo + c, c + CE <= n) : 0u;
+  }
+  float v[IT][CE];
+  if (!lazy) {
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const int c = (k * kBlock + threadIdx.x) * CE;
+#pragma unroll
+      for (int e = 0; e < CE; ++e) v[k][e] = 0.0f;
+      if (keep[k] != 0) ld_row_part<T, CE>(x + c, n - c, v[k]);
+    }
+  }
   const double r = a.repetitions != nullptr ? a.repetitions[row] : a.repetition;
   const double p = a.presences != nullptr ? a.presences[row] : a.presence;
   const double f = a.frequencies != nullptr ? a.frequencies[row] : a.frequency;
   const bool counted = a.tokens != nullptr && (r != 1.0 || p != 0.0 || f != 0.0);
   if (counted) {
-    for (int i = threadIdx.x; i < slice; i += kBlock) seen[i] = 0;
+#pragma unroll
+    for (int k = 0; k < IT; ++k)
+#pragma unroll
+      for (int q = 0; q < CE / 4; ++q)
+        *reinterpret_cast<i32x4_t*>(seen + (k * kBlock + threadIdx.x) * CE + 4 * q) = i32x4_t{0, 0, 0, 0};
     __syncthreads();
     const int64_t len = a.lengths != nullptr ? min(max((int64_t)a.lengths[row], (int64_t)0), a.n_tokens) : a.n_tokens;
     const int64_t prompt = a.prompts != nullptr ? a.prompts[row] : 0;
-    if (a.tokens64) {
-      const int64_t* const t = static_cast<const int64_t*>(a.tokens) + row * a.tokens_stride;
-      for (int64_t i = threadIdx.x; i < len; i += kBlock) count(seen, t[i], lo, n, i >= prompt);
-    } else {
-      const int32_t* const t = static_cast<const int32_t*>(a.tokens) + row * a.tokens_stride;
-      for (int64_t i = threadIdx.x; i < len; i += kBlock) count(seen, t[i], lo, n, i >= prompt);
-    }
+    if (a.tokens64) count_all(seen, static_cast<const int64_t*>(a.tokens) + row * a.tokens_stride, len, prompt, lo, n);
+    else count_all(seen, static_cast<const int32_t*>(a.tokens) + row * a.tokens_stride, len, prompt, lo, n);
     __syncthreads();
   }
-  const S* const x = static_cast<const S*>(a.logits) + row * a.row_stride + lo;
-  S* const y = static_cast<S*>(a.out) + row * a.out_stride + lo;
-  const bool in_place = static_cast<const void*>(x) == static_cast<const void*>(y);
-  for (int c = threadIdx.x * CE; c < n; c += kBlock * CE) {
-    const bool full = c + CE <= n;
-    const uint32_t keep = allowed<CE>(a, row, lo + c, full);
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const int c = (k * kBlock + threadIdx.x) * CE;
+    if (c >= n) break;
     uint32_t cnt[CE], any = 0;
 #pragma unroll
     for (int e = 0; e < CE; ++e) cnt[e] = 0;
@@ -99,55 +149,47 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
         for (int e = 0; e < 4; ++e) cnt[4 * q + e] = (uint32_t)w[e], any |= (uint32_t)w[e];
       }
     }
-    if (in_place && a.bias == nullptr && any == 0 && keep == (1u << CE) - 1u) continue;
-    float v[CE];
+    if (lazy) {
+      const uint32_t there = n - c >= CE ? all : (1u << (n - c)) - 1u;
+      if (any == 0 && (keep[k] & there) == there) continue;
 #pragma unroll
-    for (int e = 0; e < CE; ++e) v[e] = 0.0f;
-    if (keep != 0) {
-      if (full) {
-        const i32x4_t w = *reinterpret_cast<const i32x4_any_t*>(x + c);
+      for (int e = 0; e < CE; ++e) v[k][e] = 0.0f;
+      if (keep[k] != 0) ld_row_part<T, CE>(x + c, n - c, v[k]);
+    }
+    if (any != 0) {
 #pragma unroll
-        for (int e = 0; e < CE; ++e) v[e] = elem<T>(w, e);
-      } else {
-#pragma unroll
-        for (int e = 0; e < CE; ++e)
-          if (c + e < n) v[e] = load_elem(x, c + e, T::code);
+      for (int e = 0; e < CE; ++e) {
+        if (cnt[e] == 0) continue;
+        const uint32_t said = cnt[e] & ~kPrompt;
+        const double z = v[k][e];
+        v[k][e] = (float)((z > 0.0 ? z / r : z * r) - (said != 0 ? f * said + p : 0.0));
       }
-      if (any != 0) {
+    }
+    if (a.bias != nullptr && keep[k] != 0) {
+      const int64_t at = row * a.bias_stride + lo + c;
+      float b[CE];
+      if (a.bias_f32) ld_row_part<F32, CE>(static_cast<const float*>(a.bias) + at, n - c, b);
+      else ld_row_part<T, CE>(static_cast<const S*>(a.bias) + at, n - c, b);
 #pragma unroll
-        for (int e = 0; e < CE; ++e) {
-          if (cnt[e] == 0) continue;
-          const uint32_t said = cnt[e] & ~kPrompt;
-          const double z = v[e];
-          v[e] = (float)((z > 0.0 ? z / r : z * r) - (said != 0 ? f * said + p : 0.0));
-        }
-      }
-      if (a.bias != nullptr) {
-        const int64_t at = row * a.bias_stride + lo + c;
-#pragma unroll
-        for (int e = 0; e < CE; ++e)
-          if (c + e < n) v[e] += load_elem(a.bias, at + e, a.bias_f32 ? F32::code : T::code);
-      }
+      for (int e = 0; e < CE; ++e) v[k][e] += b[e];
     }
 #pragma unroll
     for (int e = 0; e < CE; ++e)
-      if ((keep >> e & 1u) == 0) v[e] = -__builtin_inff();
-    const i32x4_t w = pack<T>(v);
-    if (full) {
-      *reinterpret_cast<i32x4_any_t*>(y + c) = w;
+      if ((keep[k] >> e & 1u) == 0) v[k][e] = -__builtin_inff();
+    if (c + CE <= n) {
+      *reinterpret_cast<i32x4_any_t*>(y + c) = pack<T>(v[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < CE; ++e)
-        if (c + e < n) store_elem(y, c + e, v[e], T::code);
+        if (c + e < n) store_elem(y, c + e, v[k][e], T::code);
     }
   }
 }
 
-template <class T>
-hipError_t adjust_t(const AdjustArgs& a, hipStream_t s) {
-  int slice = 4096;
-  while (slice > 1024 && a.n_rows * ((a.vocab + slice - 1) / slice) < 1024) slice /= 2;
-  const int slices = (a.vocab + slice - 1) / slice;
+template <class T, int IT>
+hipError_t adjust_it(const AdjustArgs& a, hipStream_t s) {
+  constexpr int kSlice = kBlock * T::ce * IT;
+  const int slices = (a.vocab + kSlice - 1) / kSlice;
   const int64_t rows = std::max<int64_t>(1, (1 << 22) / slices);  // of a launch: 2^30 threads
   for (int64_t r0 = 0; r0 < a.n_rows; r0 += rows) {
     AdjustArgs part = a;
@@ -163,12 +205,20 @@ hipError_t adjust_t(const AdjustArgs& a, hipStream_t s) {
     if (a.frequencies) part.frequencies += r0;
     if (a.bias) part.bias = static_cast<const char*>(a.bias) + r0 * a.bias_stride * (a.bias_f32 ? 4 : es);
     if (a.mask) part.mask = static_cast<const char*>(a.mask) + r0 * a.mask_stride * (a.mask_bytes ? 1 : 4);
-    hipLaunchKernelGGL((k_adjust<T>), dim3((unsigned)(part.n_rows * slices)), dim3(kBlock),
-                       a.tokens ? slice * sizeof(uint32_t) : 0, s, part, slice, slices);
+    hipLaunchKernelGGL((k_adjust<T, IT>), dim3((unsigned)(part.n_rows * slices)), dim3(kBlock),
+                       a.tokens ? kSlice * sizeof(uint32_t) : 0, s, part, slices);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
+}
+
+template <class T>
+hipError_t adjust_t(const AdjustArgs& a, hipStream_t s) {
+  const int64_t chunks = a.n_rows * ((a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce));  // workgroups of one each
+  if (chunks >= 4096) return adjust_it<T, 4>(a, s);
+  if (chunks >= 2048) return adjust_it<T, 2>(a, s);
+  return adjust_it<T, 1>(a, s);
 }
 
 }  // namespace

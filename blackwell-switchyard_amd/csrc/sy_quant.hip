@@ -4,6 +4,7 @@
 //
 // with whole codes c in 0..15 and, without zero points, z = 8.
 #include <algorithm>
+#include <type_traits>
 
 #include "sy_launch.hpp"
 
@@ -22,7 +23,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // at columns 32 j + 8 (l / 16) + (0..7), which is what the lane brings to the matrix
 // instruction over columns 32 j .. 32 j + 31. The nibble of column c of a word lies at bits
 // 4 p + 3, p = c / 2 + 4 (c % 2), so one mask leaves a pair of columns in the two halves.
-// Scales and zero points are [feature tile][group][16], with the groups of whole tiles.
+// Scales and zero points are [feature tile][column tile][16][groups of the tile].
 constexpr int kTileK = 128;
 
 __host__ __device__ constexpr int64_t tiles_of(int64_t n) { return (n + 15) / 16; }
@@ -50,10 +51,12 @@ __global__ void __launch_bounds__(256) k_pack4(const PackArgs a) {
     a.tiles[i] = w << 3 | w >> 29;
   }
   // Groups that only pad a tile have scale zero.
-  const int64_t groups = (a.k + a.group - 1) / a.group, padded = (int64_t)steps * (kTileK / a.group);
-  const int64_t cells = tiles_of(a.n) * padded * 16;
+  const int64_t groups = (a.k + a.group - 1) / a.group;
+  const int ng = kTileK / a.group;
+  const int64_t cells = tiles_of(a.n) * steps * 16 * ng;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (int64_t)gridDim.x * 256) {
-    const int64_t n = i / (padded * 16) * 16 + (i & 15), g = (i >> 4) % padded;
+    const int64_t tile = i / ng >> 4;
+    const int64_t n = tile / steps * 16 + (i / ng & 15), g = tile % steps * ng + i % ng;
     const bool in = n < a.n && g < groups;
     if (a.esize == 4)
       static_cast<uint32_t*>(a.scales_out)[i] = in ? static_cast<const uint32_t*>(a.scales)[n * groups + g] : 0u;
@@ -171,41 +174,64 @@ template <class T, bool ZEROS> __device__ __forceinline__ i32x4_t minus() {
   return i32x4_t{(int)x, (int)x, (int)x, (int)x};
 }
 
-typedef int i32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 
-// Eight elements of a row from column k on, as Mma<T>::planes fragments; zero behind the row
-// and where the lane has no row. Rows start anywhere.
-template <class T>
-__device__ __forceinline__ void ld_x(const typename T::storage* row, bool live, int k, int k_end,
-                                     i32x4_t (&f)[Mma<T>::planes]) {
-  using S = typename T::storage;
-  constexpr int W = 8 * sizeof(S) / 16;
-  i32x4_t raw[W];
+// Eight elements of a row as they lie in memory, from column k on; WHOLE: all are before
+// k_end, else those behind it are zero. Rows start anywhere.
+template <class T> struct Raw {
+  static constexpr int words = 8 * sizeof(typename T::storage) / 16;
+  i32x4_t x[words];
+};
+template <class T, bool WHOLE>
+__device__ __forceinline__ Raw<T> ld_x(const typename T::storage* row, int k, int k_end) {
+  Raw<T> r;
+  constexpr int W = Raw<T>::words;
+  if (WHOLE || (W == 2 && k + 8 <= k_end)) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) raw[i] = i32x4_t{0, 0, 0, 0};
-  if (live && k + 8 <= k_end) {
+    for (int i = 0; i < W; ++i) r.x[i] = *reinterpret_cast<const i32x4_any_t*>(row + k + i * (8 / W));
+  } else if constexpr (W == 2) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) raw[i] = *reinterpret_cast<const i32x4_any_t*>(row + k + i * (8 / W));
-  } else if (live) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (k + e >= k_end) continue;
-      if constexpr (sizeof(S) == 4) raw[e / 4][e % 4] = __float_as_int(row[k + e]);
-      else raw[0][e / 2] |= (int)((uint32_t)row[k + e] << (16 * (e % 2)));
+    for (int e = 0; e < 8; ++e) r.x[e / 4][e % 4] = k + e < k_end ? __float_as_int(row[k + e]) : 0;
+  } else {
+    // The row's last eight, with those before k shifted out.
+    typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
+    u64x2_t x = {0, 0};
+    int past = k - (k_end - 8);
+    if (k_end >= 8) {
+      const i32x4_t y = *reinterpret_cast<const i32x4_any_t*>(row + min(k, k_end - 8));
+      x = __builtin_bit_cast(u64x2_t, y);
+    } else {  // a row of fewer
+      past = k;
+#pragma unroll 1
+      for (int e = k_end - 1; e >= 0; --e) {
+        x[1] = x[1] << 16 | x[0] >> 48;
+        x[0] = x[0] << 16 | row[e];
+      }
     }
+    if (past > 0) {
+      const int bits = 16 * (past & 3);
+      if (past & 4) x = u64x2_t{x[1], 0};
+      if (bits != 0) x = u64x2_t{x[0] >> bits | x[1] << (64 - bits), x[1] >> bits};
+      if (past >= 8) x = u64x2_t{0, 0};
+    }
+    r.x[0] = __builtin_bit_cast(i32x4_t, x);
   }
-  if constexpr (W == 1) {
-    f[0] = raw[0];
+  return r;
+}
+
+// Its fragments: itself, or the three bf16 parts of each element.
+template <class T> __device__ __forceinline__ void parts_of(const Raw<T>& r, i32x4_t (&f)[Mma<T>::planes]) {
+  if constexpr (Raw<T>::words == 1) {
+    f[0] = r.x[0];
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int i = 0; i < 4; ++i) {
       float x[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) x[h] = __int_as_float(raw[(2 * r + h) / 4][(2 * r + h) % 4]);
+      for (int h = 0; h < 2; ++h) x[h] = __int_as_float(r.x[(2 * i + h) / 4][(2 * i + h) % 4]);
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
         const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]);
-        f[p][r] = (int)((b & 0xffff0000u) | a >> 16);
+        f[p][i] = (int)((b & 0xffff0000u) | a >> 16);
         x[0] -= __uint_as_float(a & 0xffff0000u);
         x[1] -= __uint_as_float(b & 0xffff0000u);
       }
@@ -213,12 +239,32 @@ __device__ __forceinline__ void ld_x(const typename T::storage* row, bool live, 
   }
 }
 
-__device__ __forceinline__ float scale_of(const void* p, int64_t i, int dtype) { return load_elem(p, i, dtype); }
+// The N scales and zero points of a column in a tile, in one load each.
+template <class T, int N> __device__ __forceinline__ void ld_scales(const typename T::storage* p, float (&s)[N]) {
+  typename T::storage raw[N];
+  __builtin_memcpy(raw, __builtin_assume_aligned(p, N * sizeof(raw[0])), sizeof(raw));
+#pragma unroll
+  for (int g = 0; g < N; ++g) s[g] = load_elem(raw, g, T::code);
+}
+template <int N> __device__ __forceinline__ void ld_zeros(const uint8_t* p, float (&z)[N]) {
+  uint8_t raw[N];
+  __builtin_memcpy(raw, __builtin_assume_aligned(p, N), sizeof(raw));
+#pragma unroll
+  for (int g = 0; g < N; ++g) z[g] = 1.0f + (float)raw[g] * 0.0625f;
+}
 
-// Few rows: a workgroup has NT feature tiles and 16 MT rows, its waves share the columns out
-// tile by tile and fold their sums in LDS in their order. GS: 32-column pieces of a group.
-template <class T, int MT, int NT, int GS, bool ZEROS>
-__global__ void __launch_bounds__(512) k_linear4(const Linear4Args a) {
+// What a wave needs of one column tile.
+template <class T, int MT, int NT, int NG, bool ZEROS> struct Step {
+  i32x4_t w[NT];
+  float s[NT][NG], z[NT][NG];
+  Raw<T> x[MT][4];
+};
+
+// A workgroup has NT feature tiles and 16 MT rows; its waves share the columns out tile by tile
+// and fold their sums in LDS in their order. GS: 32-column pieces of a group. PIPE: a wave asks
+// for its next column tile before it works on the present one.
+template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
+__global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4(const Linear4Args a) {
   using S = typename T::storage;
   constexpr int P = Mma<T>::planes, NG = 4 / GS;
   extern __shared__ float fold[];
@@ -226,40 +272,68 @@ __global__ void __launch_bounds__(512) k_linear4(const Linear4Args a) {
   const int col = lane & 15, quad = lane >> 4;
   const int64_t tile0 = (int64_t)blockIdx.x * NT, n_tiles = tiles_of(a.n);
   const int steps = (int)steps_of(a.k);
-  const S* const x = static_cast<const S*>(a.x);
   const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
-  const S* rows[MT];
-  bool live[MT];
+  // Rows behind the last are the last one's again: their sums are not stored. STAGED: a load is
+  // four whole rows of a tile, 256 bytes each, which go through LDS to the lanes that need them.
+  const S* rows[MT][STAGED ? 4 : 1];
+  const int x_k = STAGED ? 8 * col : 8 * quad;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    live[t] = m0 + 16 * t + col < a.m;
-    rows[t] = x + (live[t] ? m0 + 16 * t + col : 0) * a.x_stride;
-  }
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < (STAGED ? 4 : 1); ++j)
+      rows[t][j] = static_cast<const S*>(a.x) + min(m0 + 16 * t + (STAGED ? 4 * j + quad : col), a.m - 1) * a.x_stride;
+  i32x4_t* const stage = reinterpret_cast<i32x4_t*>(fold) + wave * (MT * 256);
   const i32x4_t neg = minus<T, ZEROS>();
   f32x4_t tot[MT][NT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int u = 0; u < NT; ++u) tot[t][u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int step = wave; step < steps; step += waves) {
-    i32x4_t w[NT];
-    float s[NT][NG], z[NT][NG];
+  // Where the feature tiles begin (those behind the last are the last one: not stored either).
+  const char *w_at[NT], *s_at[NT], *z_at[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const int64_t tile = min(tile0 + u, n_tiles - 1) * steps;
+    w_at[u] = reinterpret_cast<const char*>(a.tiles) + tile * 1024;
+    s_at[u] = static_cast<const char*>(a.scales) + tile * (16 * NG * (int)sizeof(S));
+    if constexpr (ZEROS) z_at[u] = reinterpret_cast<const char*>(a.zeros) + tile * (16 * NG);
+  }
+  using Tile = Step<T, MT, NT, NG, ZEROS>;
+  const auto load = [&](int step, Tile& r, auto whole) {
+    const uint32_t cell = (uint32_t)(step * 16 + col) * NG;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const int64_t tile = min(tile0 + u, n_tiles - 1);  // (what is behind the last is not stored)
-      w[u] = reinterpret_cast<const i32x4_t*>(a.tiles)[(tile * steps + step) * 64 + lane];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const int64_t at = (tile * steps * NG + step * NG + g) * 16 + col;
-        s[u][g] = scale_of(a.scales, at, T::code);
-        if constexpr (ZEROS) z[u][g] = 1.0f + (float)a.zeros[at] * 0.0625f;
-      }
+      r.w[u] = *reinterpret_cast<const i32x4_t*>(w_at[u] + (uint32_t)(step * 1024 + lane * 16));
+      ld_scales<T, NG>(reinterpret_cast<const S*>(s_at[u] + cell * (uint32_t)sizeof(S)), r.s[u]);
+      if constexpr (ZEROS) ld_zeros<NG>(reinterpret_cast<const uint8_t*>(z_at[u] + cell), r.z[u]);
     }
-    i32x4_t f[MT][4][P];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ld_x<T>(rows[t], live[t], step * kTileK + 32 * j + 8 * quad, a.k, f[t][j]);
+      for (int j = 0; j < 4; ++j)
+        r.x[t][j] = ld_x<T, decltype(whole)::value>(rows[t][STAGED ? j : 0], step * kTileK + x_k + (STAGED ? 0 : 32 * j), a.k);
+  };
+  const auto add = [&](const Tile& r) {
+    i32x4_t f[MT][4][P];
+    if constexpr (STAGED) {
+      // Chunk c of a row lies at c ^ row: neither side has two lanes on a bank. (Only this wave
+      // reads what it wrote.)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) stage[t * 256 + (4 * j + quad) * 16 + (col ^ (4 * j + quad))] = r.x[t][j].x[0];
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[t][j][0] = stage[t * 256 + col * 16 + ((4 * j + quad) ^ col)];
+      __builtin_amdgcn_wave_barrier();
+    } else {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) parts_of<T>(r.x[t][j], f[t][j]);
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       f32x4_t sums[MT];
@@ -275,10 +349,10 @@ __global__ void __launch_bounds__(512) k_linear4(const Linear4Args a) {
       for (int u = 0; u < NT; ++u) {
         f32x4_t acc[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? sums[t] * z[u][g] : sums[t];
+        for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? sums[t] * r.z[u][g] : sums[t];
 #pragma unroll
         for (int j = g * GS; j < (g + 1) * GS; ++j) {
-          const i32x4_t c = codes_of<T>((uint32_t)w[u][j]);
+          const i32x4_t c = codes_of<T>((uint32_t)r.w[u][j]);
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -287,11 +361,39 @@ __global__ void __launch_bounds__(512) k_linear4(const Linear4Args a) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tot[t][u][i] = fmaf(s[u][g], acc[t][i], tot[t][u][i]);
+          for (int i = 0; i < 4; ++i) tot[t][u][i] = fmaf(r.s[u][g], acc[t][i], tot[t][u][i]);
       }
     }
+  };
+  // Whole tiles, with the next one's loads on their way where a wave has several (asked for
+  // again behind the last: a branch around loads would wait for all of them); then the rest.
+  const int full = a.k / kTileK;
+  Tile r;
+  if constexpr (PIPE) {
+    Tile next;
+    int step = wave;
+    if (step < full) load(step, r, std::true_type{});
+    while (step < full) {
+      load(min(step + waves, full - 1), next, std::true_type{});
+      add(r);
+      step += waves;
+      if (step >= full) break;
+      load(min(step + waves, full - 1), r, std::true_type{});
+      add(next);
+      step += waves;
+    }
+  } else {
+    for (int step = wave; step < full; step += waves) {
+      load(step, r, std::true_type{});
+      add(r);
+    }
+  }
+  if (full < steps && full % waves == wave) {
+    load(full, r, std::false_type{});
+    add(r);
   }
   constexpr int kSums = MT * NT * 256;
+  if constexpr (STAGED) __syncthreads();  // (the sums go where the waves' rows were)
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -309,13 +411,15 @@ __global__ void __launch_bounds__(512) k_linear4(const Linear4Args a) {
   }
 }
 
-template <class T, int MT, int NT, int GS, bool ZEROS>
+template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
 hipError_t run4(const Linear4Args& a, hipStream_t s) {
   const int steps = (int)steps_of(a.k);
-  int waves = 8;
-  while (waves > 1 && (waves > steps || waves * MT * NT > 64)) waves /= 2;
+  int waves = WAVES;
+  while (waves > 1 && waves > steps) waves /= 2;
   const unsigned gx = (unsigned)((tiles_of(a.n) + NT - 1) / NT);
-  constexpr int64_t kRows = 16 * MT * 32768;  // of a launch
+  const int lds = waves * MT * (STAGED ? std::max(4, NT) : NT) * 1024;
+  static_assert(WAVES * MT * NT <= 64 && (!STAGED || WAVES * MT <= 16), "at most 64 KiB of LDS");
+  constexpr int64_t kRows = 16 * MT * 256;  // of a launch: at most 2^28 workgroups
   for (int64_t m0 = 0; m0 < a.m; m0 += kRows) {
     Linear4Args part = a;
     part.m = std::min(kRows, a.m - m0);
@@ -323,18 +427,31 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
     part.x = static_cast<const char*>(a.x) + m0 * a.x_stride * es;
     part.out = static_cast<char*>(a.out) + m0 * a.n * es;
     const unsigned gy = (unsigned)((part.m + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((k_linear4<T, MT, NT, GS, ZEROS>), dim3(gx, gy), dim3(64 * waves), waves * MT * NT * 1024, s, part);
+    hipLaunchKernelGGL((k_linear4<T, MT, NT, WAVES, STAGED, PIPE, GS, ZEROS>), dim3(gx, gy), dim3(64 * waves), lds, s,
+                       part);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
+// The tile by rows and feature tiles: RULES
 template <class T, int GS, bool ZEROS>
 hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
-  if (a.m <= 16) return tiles_of(a.n) < 1024 ? run4<T, 1, 1, GS, ZEROS>(a, s) : run4<T, 1, 2, GS, ZEROS>(a, s);
-  if (a.m <= 32) return run4<T, 2, 2, GS, ZEROS>(a, s);
-  return run4<T, 4, 2, GS, ZEROS>(a, s);
+  const int64_t tiles = tiles_of(a.n);
+  if constexpr (T::code == F32::code) {
+    return tiles < 1024 ? run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s) : run4<T, 1, 2, 8, false, false, GS, ZEROS>(a, s);
+  } else {
+    const bool wide = tiles >= (a.m > 16 ? 512 : 1024);
+    if (a.m <= 8)
+      return wide ? run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
+    if (a.m <= 16)
+      return wide ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
+    if (a.m >= 512) return run4<T, 4, 4, 4, true, false, GS, ZEROS>(a, s);
+    if (!wide) return run4<T, 2, 1, 8, true, false, GS, ZEROS>(a, s);
+    return a.k < 4096 && a.m <= 32 ? run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s)
+                                   : run4<T, 2, 4, 4, true, true, GS, ZEROS>(a, s);
+  }
 }
 
 template <class T, bool ZEROS>

@@ -55,14 +55,15 @@ __global__ void __launch_bounds__(kBlock) k_head_norm(const HeadNormArgs a) {
   const int rows = a.heads + 2 * a.kv_heads;
   const int first = (int)blockIdx.y * kWaves + wave_id(), every = (int)gridDim.y * kWaves;
   const float inv_hd = 1.0f / (float)a.hd;
-  float gain[2][2][VE];
+  float gain[2][2][VE] = {};
+  if (in_row) {
+    const bool wide = a.gain_dtype == F32::code;
 #pragma unroll
-  for (int w = 0; w < 2; ++w)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        gain[w][h][e] = in_row ? load_elem(w == 0 ? a.q_gain : a.k_gain, h * half + ch + e, a.gain_dtype) : 0.0f;
+    for (int h = 0; h < 2; ++h) {
+      ld_gains<T, VE>(a.q_gain, h * half + ch, wide, gain[0][h]);
+      ld_gains<T, VE>(a.k_gain, h * half + ch, wide, gain[1][h]);
+    }
+  }
   [[maybe_unused]] float dg[2][2][VE];
   if constexpr (BWD) {
 #pragma unroll

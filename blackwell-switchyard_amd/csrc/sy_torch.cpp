@@ -929,12 +929,13 @@ std::optional<Tensor> linear4(const Tensor& x_in, const Tensor& tiles, const Ten
   if (!ordinary() || !plain(x_in) || tracked(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || x_in.size(-1) != k ||
       !whole(tiles) || !plain(scales) || tracked(scales) || scales.scalar_type() != x_in.scalar_type() ||
       tiles.device() != x_in.device() || scales.device() != x_in.device() || !tiles.is_contiguous() ||
-      !scales.is_contiguous() || !aligned16(tiles) || (group != 32 && group != 64 && group != 128) || n < 1 ||
+      !scales.is_contiguous() || !aligned16(tiles) || !aligned16(scales) || (group != 32 && group != 64 && group != 128) || n < 1 ||
       tiles.numel() != (n + 15) / 16 * ((k + 127) / 128) * 256 || scales.numel() != tiles.numel() * 8 / group ||
       x_in.numel() / k > 0x7fffffff)
     return std::nullopt;
   if (zeros.has_value() && (!whole_of(*zeros, at::kByte) || zeros->device() != x_in.device() ||
-                            !zeros->is_contiguous() || zeros->numel() != scales.numel()))
+                            !zeros->is_contiguous() || zeros->numel() != scales.numel() ||
+                            reinterpret_cast<uintptr_t>(zeros->data_ptr()) % 4 != 0))
     return std::nullopt;
   const c10::DeviceGuard guard(x_in.device());
   Tensor x = x_in.dim() == 2 ? x_in : x_in.reshape({-1, k});

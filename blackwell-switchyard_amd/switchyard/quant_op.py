@@ -41,7 +41,7 @@ def _check_sizes(out_features: int, in_features: int, group: int) -> None:
 class Weight4:
     """4-bit weights ``[out_features, in_features]`` in tiles of 16 rows by 128 columns
     (``tiles`` int32 ``[row tiles, column tiles, 64, 4]``; ``scales`` and ``zeros``, which may be
-    None, ``[row tiles, groups of whole tiles, 16]``). Made by ``quantize4`` or ``from_codes``."""
+    None, ``[row tiles, column tiles, 16, groups of a tile]``). Made by ``quantize4`` or ``from_codes``."""
 
     __slots__ = ("tiles", "scales", "zeros", "out_features", "in_features", "group")
 
@@ -51,12 +51,12 @@ class Weight4:
         rows, cols = -(-out_features // 16), -(-in_features // _TILE_K)
         _need(tiles.shape == (rows, cols, 64, 4) and tiles.dtype == torch.int32 and tiles.is_contiguous()
               and tiles.data_ptr() % 16 == 0, f"tiles must be a dense int32 [{rows}, {cols}, 64, 4] tensor")
-        shape = (rows, cols * (_TILE_K // group), 16)
+        shape = (rows, cols, 16, _TILE_K // group)
         _lib.dtype_code(scales.dtype)
-        _need(scales.shape == shape and scales.is_contiguous() and scales.device == tiles.device,
-              f"scales must be a dense {list(shape)} tensor on the tiles' device")
+        _need(scales.shape == shape and scales.is_contiguous() and scales.device == tiles.device
+              and scales.data_ptr() % 16 == 0, f"scales must be a dense {list(shape)} tensor on the tiles' device")
         _need(zeros is None or (zeros.shape == shape and zeros.dtype == torch.uint8 and zeros.is_contiguous()
-                                and zeros.device == tiles.device),
+                                and zeros.device == tiles.device and zeros.data_ptr() % 4 == 0),
               f"zeros must be a dense uint8 {list(shape)} tensor on the tiles' device")
         self.tiles, self.scales, self.zeros = tiles, scales, zeros
         self.out_features, self.in_features, self.group = out_features, in_features, group
@@ -80,7 +80,7 @@ class Weight4:
         _need(codes.is_cuda, "codes must be on a CUDA device")
         dev, rows, cols = codes.device, -(-n // 16), -(-k // _TILE_K)
         tiles = torch.empty(rows, cols, 64, 4, device=dev, dtype=torch.int32)
-        tile_scales = torch.empty(rows, cols * (_TILE_K // group), 16, device=dev, dtype=scales.dtype)
+        tile_scales = torch.empty(rows, cols, 16, _TILE_K // group, device=dev, dtype=scales.dtype)
         tile_zeros = None if zeros is None else torch.empty(tile_scales.shape, device=dev, dtype=torch.uint8)
         codes, scales = codes.detach().contiguous(), scales.detach().contiguous()
         zeros = None if zeros is None else zeros.contiguous()
@@ -98,7 +98,7 @@ class Weight4:
         order = torch.tensor([c // 2 + 4 * (c % 2) for c in range(8)], device=w.device, dtype=torch.int32)
         c = (w[..., None] >> (4 * order)) & 15  # [row tile, column tile, 16 (column) + row, word, column]
         c = c.unflatten(2, (4, 16)).permute(0, 3, 1, 4, 2, 5).reshape(-1, self.tiles.shape[1] * _TILE_K)
-        by_rows = lambda x: x.transpose(1, 2).flatten(0, 1)[:n, :g].contiguous()  # noqa: E731
+        by_rows = lambda x: x.transpose(1, 2).flatten(2, 3).flatten(0, 1)[:n, :g].contiguous()  # noqa: E731
         return (c[:n, :k].to(torch.uint8).contiguous(), by_rows(self.scales),
                 None if self.zeros is None else by_rows(self.zeros))
 

@@ -507,8 +507,9 @@ int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_
  * zeros [n][ceil(k / group)]. sy_quantize4 makes them from weights [n][k] (rows row_stride
  * apart): symmetric, codes 1 to 15, without zeros; over the range of each group with them.
  * sy_pack4 lays them out for sy_linear4: tiles of 1024 bytes for 16 features by 128 columns,
- * ceil(n / 16) ceil(k / 128) of them, 16-byte aligned; tile_scales and tile_zeros
- * [ceil(n / 16)][ceil(k / 128) 128 / group][16]. Rows of x are x_stride elements apart and
+ * ceil(n / 16) ceil(k / 128) of them, tile_scales and tile_zeros [ceil(n / 16)][ceil(k / 128)]
+ * [16][128 / group]; tiles and tile_scales start at 16-byte boundaries, tile_zeros at 4-byte
+ * ones. Rows of x are x_stride elements apart and
  * start anywhere; a row with an infinity or NaN gives NaN. No reference counterpart. */
 int sy_quantize4(const void* w, int64_t row_stride, uint8_t* codes, void* scales, uint8_t* zeros, int64_t n,
                  int64_t k, int64_t group, int dtype, void* stream);
