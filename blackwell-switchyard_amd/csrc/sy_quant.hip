@@ -411,6 +411,182 @@ __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4
   }
 }
 
+// The sum of a chunk's eight elements, added to acc.
+template <class T> __device__ __forceinline__ float sum8(const i32x4_t& x, float acc) {
+  constexpr int one = (int)Mma<T>::one;
+  return dot<T>(x, i32x4_t{one, one, one, one}, acc);
+}
+
+// Many rows: a workgroup has 64 rows by 64 NT features. Four waves with NT feature tiles each
+// share a column tile of the rows in LDS, double-buffered; two such groups of waves take every
+// other column tile and add up at the end. A tile's sums over each group's columns are formed
+// where it is written to LDS, by the lanes that hold it.
+template <class T, int NT, int GS, bool ZEROS>
+__global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
+  using S = typename T::storage;
+  constexpr int NG = 4 / GS, MT = 4, kRows = 16 * MT, kChunks = kRows * 16;
+  __shared__ __align__(16) i32x4_t stage[2][2][kChunks];
+  __shared__ __align__(16) float sums[2][2][NG][kRows];
+  static_assert(sizeof(stage) >= 4 * MT * NT * 1024, "the first group's sums fit");
+  // Neighbouring blocks on one XCD: workgroups go to the eight of them in turn.
+  const int per = (blocks + 7) / 8, block = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= per || block >= blocks) return;
+  const int lane = threadIdx.x & 63, wave = wave_id(), part = wave >> 2;
+  const int col = lane & 15, quad = lane >> 4;
+  const int64_t n_tiles = tiles_of(a.n), m0 = (int64_t)(block / n_blocks) * kRows;
+  const int64_t tile0 = ((int64_t)(block % n_blocks) * 4 + (wave & 3)) * NT;
+  const int steps = (int)steps_of(a.k);
+  // A thread of a group loads four chunks of the tile: rows r0, r0 + 16, r0 + 32, r0 + 48.
+  const int r0 = threadIdx.x >> 4 & 15, c0 = threadIdx.x & 15;
+  const S* rows[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) rows[i] = static_cast<const S*>(a.x) + min(m0 + r0 + 16 * i, a.m - 1) * a.x_stride;
+  const char *w_at[NT], *s_at[NT], *z_at[NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    const int64_t tile = min(tile0 + u, n_tiles - 1) * steps;
+    w_at[u] = reinterpret_cast<const char*>(a.tiles) + tile * 1024;
+    s_at[u] = static_cast<const char*>(a.scales) + tile * (16 * NG * (int)sizeof(S));
+    if constexpr (ZEROS) z_at[u] = reinterpret_cast<const char*>(a.zeros) + tile * (16 * NG);
+  }
+  struct alignas(NG * sizeof(S)) Scales {
+    S x[NG];
+  };
+  struct alignas(NG) Zeros {
+    uint8_t x[NG];
+  };
+  struct Weights {  // as they lie in memory
+    i32x4_t w[NT];
+    Scales s[NT];
+    Zeros z[NT];
+  };
+  const auto load_w = [&](int step, Weights& r) {
+    const uint32_t cell = (uint32_t)(step * 16 + col) * NG;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      r.w[u] = *reinterpret_cast<const i32x4_t*>(w_at[u] + (uint32_t)(step * 1024 + lane * 16));
+      r.s[u] = *reinterpret_cast<const Scales*>(s_at[u] + cell * (uint32_t)sizeof(S));
+      if constexpr (ZEROS) r.z[u] = *reinterpret_cast<const Zeros*>(z_at[u] + cell);
+    }
+  };
+  const auto load_x = [&](int step, Raw<T> (&x)[MT]) {
+    const int k = step * kTileK + 8 * c0;
+    if ((step + 1) * kTileK <= a.k) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[i] = ld_x<T, true>(rows[i], k, a.k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) x[i] = ld_x<T, false>(rows[i], k, a.k);
+    }
+  };
+  const auto put = [&](int buffer, const Raw<T> (&x)[MT]) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      stage[part][buffer][(r0 + 16 * i) * 16 + (c0 ^ r0)] = x[i].x[0];
+      const float s = lane_sum<4 * GS>(sum8<T>(x[i].x[0], 0.0f)) * (ZEROS ? -1.0f : -1.5f);
+      if (c0 % (4 * GS) == 0) sums[part][buffer][c0 / (4 * GS)][r0 + 16 * i] = s;
+    }
+  };
+  f32x4_t tot[MT][NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) tot[t][u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto add = [&](int buffer, const Weights& r) {
+    const i32x4_t* const at = stage[part][buffer] + col * 16;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      i32x4_t f[GS][MT];
+      f32x4_t from[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) from[t] = *reinterpret_cast<const f32x4_t*>(&sums[part][buffer][g][16 * t + 4 * quad]);
+#pragma unroll
+      for (int j = 0; j < GS; ++j)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) f[j][t] = at[t * 256 + ((4 * (g * GS + j) + quad) ^ col)];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        f32x4_t acc[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? from[t] * (1.0f + (float)r.z[u].x[g] * 0.0625f) : from[t];
+#pragma unroll
+        for (int j = 0; j < GS; ++j) {
+          const i32x4_t c = codes_of<T>((uint32_t)r.w[u][g * GS + j]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[t] = Mma<T>::run(f[j][t], c, acc[t]);
+        }
+        const float s = load_elem(r.s[u].x, g, T::code);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tot[t][u][i] = fmaf(s, acc[t][i], tot[t][u][i]);
+      }
+    }
+  };
+  // Both groups go round as often; one may have nothing to add in the last round.
+  const int last = steps - 1, rounds = (steps + 1) / 2;
+  Raw<T> x[MT];
+  Weights w, next;
+  load_w(min(part, last), w);
+  load_x(min(part, last), x);
+  put(0, x);
+  __syncthreads();
+  const auto round = [&](int i, const Weights& now, Weights& then) {
+    const int step = 2 * i + part, at = min(step + 2, last);
+    load_w(at, then);
+    load_x(at, x);
+    if (step <= last) add(i & 1, now);
+    put((i + 1) & 1, x);
+    __syncthreads();
+  };
+  for (int i = 0; i < rounds; i += 2) {
+    round(i, w, next);
+    if (i + 1 < rounds) round(i + 1, next, w);
+  }
+  // The second group's sums to the first, a lane's own.
+  float* const mine = reinterpret_cast<float*>(stage) + (wave & 3) * (MT * NT * 256) + lane;
+  if (part == 1) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[((t * NT + u) * 4 + i) * 64] = tot[t][u][i];
+  }
+  __syncthreads();
+  if (part == 1) return;
+  S* const out = static_cast<S*>(a.out);
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + 16 * t + 4 * quad + i, n = (tile0 + u) * 16 + col;
+        if (m < a.m && n < a.n)
+          store_elem(out, m * a.n + n, 16.0f * (tot[t][u][i] + mine[((t * NT + u) * 4 + i) * 64]), T::code);
+      }
+}
+
+template <class T, int NT, int GS, bool ZEROS>
+hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
+  const int n_blocks = (int)((tiles_of(a.n) + 4 * NT - 1) / (4 * NT));  // (at most 2^18)
+  const int64_t rows = 64 * ((1 << 21) / n_blocks);  // of a launch: 2^30 threads
+  for (int64_t m0 = 0; m0 < a.m; m0 += rows) {
+    Linear4Args part = a;
+    part.m = std::min(rows, a.m - m0);
+    const int64_t es = sizeof(typename T::storage);
+    part.x = static_cast<const char*>(a.x) + m0 * a.x_stride * es;
+    part.out = static_cast<char*>(a.out) + m0 * a.n * es;
+    const int blocks = (int)((part.m + 63) / 64) * n_blocks;
+    hipLaunchKernelGGL((k_linear4_many<T, NT, GS, ZEROS>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(512), 0, s,
+                       part, n_blocks, blocks);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
 hipError_t run4(const Linear4Args& a, hipStream_t s) {
   const int steps = (int)steps_of(a.k);
@@ -435,22 +611,38 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
   return hipSuccess;
 }
 
-// The tile by rows and feature tiles: RULES
+// The kernel and its tile by rows and feature tiles; us on both sides, bf16.
+//   up to 8 rows     straight from memory: a load's lanes touch few lines. 8 rows of 32000 x 2048
+//                    8.2, through LDS 9.4. Past 1024 feature tiles four a workgroup, 1 row of
+//                    32000 x 2048 8.1, one 8.7; below one, 6144 x 2048 3.6, four 5.
+//   up to 16         through LDS. 16 rows of 2048 x 2048 3.4, straight 4.3; of 28672 x 8192 29.6,
+//                    straight 35.7, one feature tile 43.
+//   up to 32, or few blocks of 64 rows
+//                    32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
+//                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
+//                    many: 28672 x 8192 38.5, without 43.
+//   else             64 rows and the most features that leave workgroups for six CUs of ten: 2048
+//                    rows of 2048 x 5632 59 with 256 features, 72 with 128, 82 with 64, 87 as
+//                    above; 128 rows of 11264 x 2048 29, 19, 24, 21; 128 of 2048 x 5632 56, 35, 26,
+//                    13 (32 and 64 workgroups).
 template <class T, int GS, bool ZEROS>
 hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
   const int64_t tiles = tiles_of(a.n);
   if constexpr (T::code == F32::code) {
     return tiles < 1024 ? run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s) : run4<T, 1, 2, 8, false, false, GS, ZEROS>(a, s);
   } else {
-    const bool wide = tiles >= (a.m > 16 ? 512 : 1024);
     if (a.m <= 8)
-      return wide ? run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
+      return tiles >= 1024 ? run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
     if (a.m <= 16)
-      return wide ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
-    if (a.m >= 512) return run4<T, 4, 4, 4, true, false, GS, ZEROS>(a, s);
-    if (!wide) return run4<T, 2, 1, 8, true, false, GS, ZEROS>(a, s);
-    return a.k < 4096 && a.m <= 32 ? run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s)
-                                   : run4<T, 2, 4, 4, true, true, GS, ZEROS>(a, s);
+      return tiles >= 1024 ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
+    if (a.m > 32) {
+      const auto blocks = [&](int nt) { return (a.m + 63) / 64 * ((tiles + 4 * nt - 1) / (4 * nt)); };
+      if (blocks(4) >= 160) return run4_many<T, 4, GS, ZEROS>(a, s);
+      if (blocks(2) >= 160) return run4_many<T, 2, GS, ZEROS>(a, s);
+      if (blocks(1) >= 160) return run4_many<T, 1, GS, ZEROS>(a, s);
+    }
+    if (tiles < 512) return run4<T, 2, 1, 8, true, false, GS, ZEROS>(a, s);
+    return a.k < 4096 ? run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 2, 4, 4, true, true, GS, ZEROS>(a, s);
   }
 }
 
