@@ -6,6 +6,7 @@
 //
 //   backward, from dy:  e = R_t^T dy,  dg = sum e u,  dx = r (g e - u mean(g e u))
 #include <algorithm>
+#include <type_traits>
 
 #include "sy_launch.hpp"
 
@@ -42,125 +43,127 @@ __device__ __forceinline__ void st_part(typename T::storage* p, const float (&f)
 }
 
 // L lanes a head, each with the two parts of VE channels that turn together (lanes past the
-// head do nothing); a wave has 64 / L neighbouring tokens of one head, so it writes one run
-// of memory, and keeps their angles while it goes over its heads: every `heads` of the four
-// waves of gridDim.y workgroups.
+// head do nothing); a wave has 64 / L neighbouring tokens of one head, so it writes one run of
+// memory. The waves of gridDim.y workgroups share the heads out in runs: a wave goes over its
+// queries, then its keys, then its values, and over all its tokens for each, two heads at a
+// time on their way; it holds one gain, and the sums of one gain's gradient, at a time.
 template <class T, int VE, int L, bool BWD>
 __global__ void __launch_bounds__(kBlock) k_head_norm(const HeadNormArgs a) {
   using S = typename T::storage;
-  constexpr int kSlots = 64 / L;
+  constexpr int kSlots = 64 / L, kAhead = 2;
+  [[maybe_unused]] __shared__ float fold[BWD ? kWaves : 1][2][2][L * VE];
   const int lane = threadIdx.x & 63, part = lane % L, slot = lane / L;
   const int half = a.hd / 2, ch = part * VE;
   const bool in_row = ch < half;
   const int rows = a.heads + 2 * a.kv_heads;
-  const int first = (int)blockIdx.y * kWaves + wave_id(), every = (int)gridDim.y * kWaves;
+  const int per = (rows + (int)gridDim.y * kWaves - 1) / ((int)gridDim.y * kWaves);
+  const int first = ((int)blockIdx.y * kWaves + wave_id()) * per, last = min(rows, first + per);
   const float inv_hd = 1.0f / (float)a.hd;
-  float gain[2][2][VE] = {};
-  if (in_row) {
-    const bool wide = a.gain_dtype == F32::code;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      ld_gains<T, VE>(a.q_gain, h * half + ch, wide, gain[0][h]);
-      ld_gains<T, VE>(a.k_gain, h * half + ch, wide, gain[1][h]);
-    }
-  }
-  [[maybe_unused]] float dg[2][2][VE];
-  if constexpr (BWD) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
+  // Rows [lo, hi) of which (0 queries, 1 keys, 2 values), the first of which is row `from`.
+  const auto run = [&](auto kind, int from, int lo, int hi) {
+    constexpr int which = decltype(kind)::value;
+    constexpr bool kTurned = which < 2;
+    float gain[2][VE] = {};
+    [[maybe_unused]] float dg[2][VE] = {};
+    if (kTurned && in_row) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) dg[w][h][e] = 0.0f;
-  }
-  for (int64_t t0 = (int64_t)blockIdx.x * kSlots; t0 < a.n_tok; t0 += (int64_t)gridDim.x * kSlots) {
-    const int64_t tok = t0 + slot;
-    const bool live = in_row && tok < a.n_tok;
-    const int64_t b = live ? tok / a.seq : 0;
-    const int t = live ? (int)(tok % a.seq) : 0;
-    float co[VE], si[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      co[e] = live ? a.cosv[(int64_t)t * half + ch + e] : 0.0f;
-      si[e] = live ? a.sinv[(int64_t)t * half + ch + e] : 0.0f;
+        ld_gains<T, VE>(which == 0 ? a.q_gain : a.k_gain, h * half + ch, a.gain_dtype == F32::code, gain[h]);
     }
-    for (int row = first; row < rows; row += every) {
-      const int which = row < a.heads ? 0 : row < a.heads + a.kv_heads ? 1 : 2;
-      const int head = which == 0 ? row : row - a.heads - (which == 1 ? 0 : a.kv_heads);
-      const int64_t packed = (tok * rows + row) * a.hd + ch;
-      S* const base = static_cast<S*>(which == 0 ? a.q : which == 1 ? a.k : a.v);
-      const int64_t* const st = a.strides[which];
-      S* const split = base + b * st[0] + head * st[1] + t * st[2] + ch;
-      const S* const x = static_cast<const S*>(a.qkv) + packed;
-      float u[2][VE], y[2][VE];
+    S* const base = static_cast<S*>(which == 0 ? a.q : which == 1 ? a.k : a.v);
+    const int64_t head_stride = a.strides[which][1];
+    for (int64_t t0 = (int64_t)blockIdx.x * kSlots; t0 < a.n_tok && lo < hi; t0 += (int64_t)gridDim.x * kSlots) {
+      const int64_t tok = t0 + slot;
+      const bool live = in_row && tok < a.n_tok;
+      const int64_t b = live ? tok / a.seq : 0;
+      const int t = live ? (int)(tok % a.seq) : 0;
+      [[maybe_unused]] float co[VE] = {}, si[VE] = {};
+      if (kTurned && live) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) u[h][e] = y[h][e] = 0.0f;
-      if (live) {
-        if (BWD || which == 2) {
-          const S* const from = BWD ? split : x;
-          ld_part<T, VE>(from, y[0]);
-          ld_part<T, VE>(from + half, y[1]);
-        }
-        if (which < 2) {
-          ld_part<T, VE>(x, u[0]);
-          ld_part<T, VE>(x + half, u[1]);
+        for (int e = 0; e < VE; ++e) {
+          co[e] = a.cosv[(int64_t)t * half + ch + e];
+          si[e] = a.sinv[(int64_t)t * half + ch + e];
         }
       }
-      if (which < 2) {
-        const float r = head_rinv<VE, L>(u[0], u[1], inv_hd, a.eps);
-        if constexpr (BWD) {
-          float c = 0.0f;
+      S* const split = base + b * a.strides[which][0] + t * a.strides[which][2] + ch;
+      const int64_t packed = tok * rows * a.hd + ch;
+      for (int row0 = lo; row0 < hi; row0 += kAhead) {
+        float u[kAhead][2][VE], y[kAhead][2][VE];
 #pragma unroll
-          for (int e = 0; e < VE; ++e) turn(y[0][e], y[1][e], co[e], -si[e]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              u[h][e] *= r;
-              const float t1 = y[h][e] * u[h][e];
-              dg[0][h][e] += which == 0 ? t1 : 0.0f;
-              dg[1][h][e] += which == 0 ? 0.0f : t1;
-              const float g = which == 0 ? gain[0][h][e] : gain[1][h][e];
-              c = fmaf(g, t1, c);
-              y[h][e] *= g;
-            }
-          c = lane_sum<L>(c) * inv_hd;
+        for (int i = 0; i < kAhead; ++i) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < VE; ++e) y[h][e] = r * (y[h][e] - u[h][e] * c);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            y[0][e] = u[0][e] * (r * (which == 0 ? gain[0][0][e] : gain[1][0][e]));
-            y[1][e] = u[1][e] * (r * (which == 0 ? gain[0][1][e] : gain[1][1][e]));
-            turn(y[0][e], y[1][e], co[e], si[e]);
+            for (int e = 0; e < VE; ++e) u[i][h][e] = y[i][h][e] = 0.0f;
+          const int row = row0 + i;
+          if (!live || row >= hi) continue;
+          const S* const x = static_cast<const S*>(a.qkv) + packed + row * a.hd;
+          if (BWD || !kTurned) {
+            const S* const src = BWD ? split + (row - from) * head_stride : x;
+            ld_part<T, VE>(src, y[i][0]);
+            ld_part<T, VE>(src + half, y[i][1]);
+          }
+          if (kTurned) {
+            ld_part<T, VE>(x, u[i][0]);
+            ld_part<T, VE>(x + half, u[i][1]);
           }
         }
-      }
-      if (live) {
-        S* const to = BWD ? static_cast<S*>(a.dqkv) + packed : split;
-        st_part<T, VE>(to, y[0]);
-        st_part<T, VE>(to + half, y[1]);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if constexpr (kTurned) {
+            const float r = head_rinv<VE, L>(u[i][0], u[i][1], inv_hd, a.eps);
+            if constexpr (BWD) {
+              float c = 0.0f;
+#pragma unroll
+              for (int e = 0; e < VE; ++e) turn(y[i][0][e], y[i][1][e], co[e], -si[e]);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                  u[i][h][e] *= r;
+                  const float eu = y[i][h][e] * u[i][h][e];
+                  dg[h][e] += eu;
+                  c = fmaf(gain[h][e], eu, c);
+                }
+              c = lane_sum<L>(c) * inv_hd;
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) y[i][h][e] = r * fmaf(gain[h][e], y[i][h][e], -u[i][h][e] * c);
+            } else {
+#pragma unroll
+              for (int e = 0; e < VE; ++e) {
+                y[i][0][e] = u[i][0][e] * (r * gain[0][e]);
+                y[i][1][e] = u[i][1][e] * (r * gain[1][e]);
+                turn(y[i][0][e], y[i][1][e], co[e], si[e]);
+              }
+            }
+          }
+          const int row = row0 + i;
+          if (!live || row >= hi) continue;
+          S* const to = BWD ? static_cast<S*>(a.dqkv) + packed + row * a.hd : split + (row - from) * head_stride;
+          st_part<T, VE>(to, y[i][0]);
+          st_part<T, VE>(to + half, y[i][1]);
+        }
       }
     }
-  }
-  if constexpr (BWD) {
-    // The wave's tokens, then the workgroup's waves, in a fixed order.
-    __shared__ float fold[kWaves][2][2][L * VE];
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
+    if constexpr (BWD && kTurned) {  // the wave's tokens, in a fixed order
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          float x = dg[w][h][e];
+          float x = dg[h][e];
 #pragma unroll
           for (int d = L; d < 64; d *= 2) x += __shfl_xor(x, d);
-          if (slot == 0) fold[wave_id()][w][h][part * VE + e] = x;
+          if (slot == 0) fold[wave_id()][which][h][part * VE + e] = x;
         }
+    }
+  };
+  const int keys = a.heads, values = a.heads + a.kv_heads;
+  run(std::integral_constant<int, 0>{}, 0, first, min(last, keys));
+  run(std::integral_constant<int, 1>{}, keys, max(first, keys), min(last, values));
+  run(std::integral_constant<int, 2>{}, values, max(first, values), last);
+  if constexpr (BWD) {  // then the workgroup's waves
     __syncthreads();
     const int64_t at = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
     for (int i = threadIdx.x; i < 2 * a.hd; i += kBlock) {
