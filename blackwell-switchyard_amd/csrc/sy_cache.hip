@@ -198,15 +198,19 @@ __global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a, int 
   if (tok >= c.n_tok) return;
   const S* const from = static_cast<const S*>(a.qkv) + tok * a.tok_stride + ch;
   int head = wave % split * kHeads + lane / L;
-  Chunk<T, VE> lo[kAhead], hi[kAhead];
+  i32x4_t raw[kAhead][2];  // (as they lie in memory: half the registers)
   const auto load = [&]() {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int h = head + i * split * kHeads;
-      lo[i] = hi[i] = Chunk<T, VE>{};
+      raw[i][0] = raw[i][1] = i32x4_t{0, 0, 0, 0};
       if (!in_head || h >= rows) continue;
-      lo[i] = ld_chunk<T, VE>(from + h * a.head_stride);
-      hi[i] = ld_chunk<T, VE>(from + h * a.head_stride + half);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const S* const p = from + h * a.head_stride + k * half;
+        if constexpr (VE == T::ce) raw[i][k] = *reinterpret_cast<const i32x4_t*>(p);
+        else __builtin_memcpy(&raw[i][k], __builtin_assume_aligned(p, 8), 8);
+      }
     }
   };
   load();
@@ -251,22 +255,25 @@ __global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a, int 
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int h = head + i * split * kHeads;
-      const float r = head_rinv<VE, L>(lo[i].f, hi[i].f, inv_hd, a.eps);
+      Chunk<T, VE> lo, hi;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) lo.f[e] = elem<T>(raw[i][0], e), hi.f[e] = elem<T>(raw[i][1], e);
+      const float r = head_rinv<VE, L>(lo.f, hi.f, inv_hd, a.eps);
       if (!in_head || h >= rows) continue;
       const bool key = h >= c.heads, turned = h < c.heads + c.kv_heads;
       if (turned) {
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          lo[i].f[e] *= r * (key ? gain[1][0][e] : gain[0][0][e]);
-          hi[i].f[e] *= r * (key ? gain[1][1][e] : gain[0][1][e]);
-          turn(lo[i].f[e], hi[i].f[e], co[e], si[e]);
+          lo.f[e] *= r * (key ? gain[1][0][e] : gain[0][0][e]);
+          hi.f[e] *= r * (key ? gain[1][1][e] : gain[0][1][e]);
+          turn(lo.f[e], hi.f[e], co[e], si[e]);
         }
       }
       S* out;
       if (!key) {
         if (!placed) {
 #pragma unroll
-          for (int e = 0; e < VE; ++e) lo[i].f[e] = hi[i].f[e] = __int_as_float(0x7fc00000);
+          for (int e = 0; e < VE; ++e) lo.f[e] = hi.f[e] = __int_as_float(0x7fc00000);
         }
         out = q + ((int64_t)tok * c.heads + h) * c.hd + ch;
       } else {
@@ -274,8 +281,8 @@ __global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a, int 
         const int kv = h - c.heads - (turned ? 0 : c.kv_heads);
         out = bytes_on(static_cast<S*>(turned ? c.k : c.v) + kv * c.head_stride + ch, dst);
       }
-      st_chunk<T, VE>(out, lo[i]);
-      st_chunk<T, VE>(out + half, hi[i]);
+      st_chunk<T, VE>(out, lo);
+      st_chunk<T, VE>(out + half, hi);
     }
     head += kAhead * split * kHeads;
     if (round + kAhead * split * kHeads < rows) load();

@@ -177,7 +177,11 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
     for (int e = 0; e < CE; ++e)
       if ((keep[k] >> e & 1u) == 0) v[k][e] = -__builtin_inff();
     if (c + CE <= n) {
-      *reinterpret_cast<i32x4_any_t*>(y + c) = pack<T>(v[k]);
+      // (Where there is much to write it goes past the caches: 256 rows of 50257 in fp32 25.8 ->
+      // 23.9 us; 8 of 32000 in bf16 8.1 -> 8.6.)
+      i32x4_any_t* const to = reinterpret_cast<i32x4_any_t*>(y + c);
+      if constexpr (IT == 4) __builtin_nontemporal_store((i32x4_any_t)pack<T>(v[k]), to);
+      else *to = pack<T>(v[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < CE; ++e)
