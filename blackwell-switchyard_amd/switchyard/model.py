@@ -52,7 +52,12 @@ value they read. Two mechanisms handle that:
     version check, which the slot writes would otherwise trip.
 
 Generation. ``Transformer.decode`` appends new tokens to a ``DecodeState`` (paged keys and
-values of every layer) and returns the next logits; ``generate`` samples from them.
+values of every layer) and returns the next logits; ``generate`` samples from them, with
+penalties, biases and masks where they are asked for. ``quantize4_`` replaces the projections
+by 4-bit ones.
+
+With ``ModelConfig.qk_norm`` every query and key head has an RMSNorm of its own before it
+turns (no reference counterpart), which is one kernel with the rotation.
 """
 
 from __future__ import annotations
@@ -70,7 +75,10 @@ from . import _lib
 from .baselines import folded_form
 from .cache_op import paged_append, paged_attention
 from .hip_op import block_attn_res_hip
+from .logits_op import adjust_logits
+from .quant_op import Linear4
 from .reference import DEFAULT_EPS, BlockAttnRes
+from .rope_op import qk_norm_rope
 from .sample_op import sample_tokens
 
 __all__ = [
@@ -111,6 +119,7 @@ class ModelConfig:
     tie_embeddings: bool = True
     residual: str = "standard"
     sources: str = "arena"
+    qk_norm: bool = False
 
     def __post_init__(self) -> None:
         problems = []
@@ -235,14 +244,24 @@ class Rotary(nn.Module):
 
 class Attention(nn.Module):
     """Causal multi-head attention: one fused QKV projection (one GEMM),
-    rotary positions, ``scaled_dot_product_attention`` on contiguous
-    ``[B, H, T, hd]`` operands, and the output projection."""
+    rotary positions (behind a norm of every query and key head with ``qk_norm``),
+    ``scaled_dot_product_attention`` on contiguous ``[B, H, T, hd]`` operands, and the
+    output projection."""
 
     def __init__(self, cfg: ModelConfig) -> None:
         super().__init__()
         self.heads, self.hd = cfg.n_heads, cfg.head_dim
         self.qkv = nn.Linear(cfg.d_model, 3 * cfg.d_model, bias=False)
         self.out = nn.Linear(cfg.d_model, cfg.d_model, bias=False)
+        self.q_norm = RMSNorm(cfg.head_dim, cfg.norm_eps) if cfg.qk_norm else None
+        self.k_norm = RMSNorm(cfg.head_dim, cfg.norm_eps) if cfg.qk_norm else None
+
+    def head_gains(self) -> tuple[Tensor, Tensor, float] | None:
+        """Gains and eps of the head norms, where one kernel may stand in for both."""
+        q, k = self.q_norm, self.k_norm
+        if q is None or not _only_forward(q, RMSNorm) or not _only_forward(k, RMSNorm) or q.eps != k.eps:
+            return None
+        return q.weight, k.weight, q.eps
 
     def forward(self, x: Tensor, rotary: Rotary) -> Tensor:
         if isinstance(rotary, _CacheStep):
@@ -253,9 +272,17 @@ class Attention(nn.Module):
         if _only_forward(rotary, Rotary):
             cos, sin = rotary.cos, rotary.sin
             if _lib.ordinary(qkv, cos, sin) and qkv.is_cuda:
-                split = _lib.native().rope_qkv(qkv, cos, sin)
+                if self.q_norm is None:
+                    split = _lib.native().rope_qkv(qkv, cos, sin)
+                else:
+                    gains = self.head_gains()
+                    if gains is not None and _lib.ordinary(*gains[:2]):
+                        split = _lib.native().qk_norm_rope(qkv.view(b, t, 3 * self.heads, self.hd), *gains[:2], cos, sin,
+                                                           self.heads, gains[2])
         if split is None:
             q, k, v = qkv.unbind(2)
+            if self.q_norm is not None:
+                q, k = self.q_norm(q), self.k_norm(k)
             q, k = rotary(q), rotary(k)
             split = [y.transpose(1, 2).contiguous() for y in (q, k, v)]
         q, k, v = split
@@ -363,8 +390,16 @@ class _CacheStep:
         self.layer += 1
         n_tok, d = x.shape[1:]
         qkv = attn.qkv(x).view(n_tok, 3 * attn.heads, attn.hd)
+        norm = {}
+        if attn.q_norm is not None:
+            gains = attn.head_gains()
+            if gains is None:  # norms that are more than their kernel
+                q, k, v = qkv.view(n_tok, 3, attn.heads, attn.hd).unbind(1)
+                qkv = torch.cat((attn.q_norm(q).to(v.dtype), attn.k_norm(k).to(v.dtype), v), 1)
+            else:
+                norm = {"q_gain": gains[0], "k_gain": gains[1], "eps": gains[2]}
         q = paged_append(qkv, st.cos, st.sin, st.k[layer], st.v[layer], self.table, self.lengths, self.starts,
-                         prefix_len=self.prefix_len)
+                         prefix_len=self.prefix_len, **norm)
         y = paged_attention(q, st.k[layer], st.v[layer], self.table, self.lengths, self.starts, **self.more)
         return attn.out(y.view(1, n_tok, d))
 
@@ -678,15 +713,34 @@ class Transformer(nn.Module):
         return logits
 
     @torch.no_grad()
+    def quantize4_(self, group: int = 64, *, symmetric: bool = True) -> Transformer:
+        """Replace every projection and the LM head by their 4-bit forms (``quant_op.Linear4``), for
+        inference; norms, the embedding and the AttnRes parameters stay. Returns the model."""
+        for layer in self.layers:
+            for owner, name in ((layer.attn, "qkv"), (layer.attn, "out"), (layer.mlp, "gate_up"), (layer.mlp, "down")):
+                if not isinstance(getattr(owner, name), Linear4):
+                    setattr(owner, name, Linear4.from_linear(getattr(owner, name), group, symmetric=symmetric))
+        if not isinstance(self.lm_head, Linear4):
+            self.lm_head = Linear4.from_linear(self.lm_head, group, symmetric=symmetric)
+        return self
+
+    @torch.no_grad()
     def generate(self, prompts, n_new: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
-                 prefix: Tensor | None = None, u: Tensor | None = None, generator=None, page: int = 64) -> Tensor:
+                 repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, bias: Tensor | None = None,
+                 allowed=None, prefix: Tensor | None = None, u: Tensor | None = None, generator=None,
+                 page: int = 64) -> Tensor:
         """``n_new`` tokens behind each prompt, ``[batch, n_new]`` (int64).
 
         ``prompts`` is ``[batch, T]`` or a list of 1-D tensors of any lengths of at least one;
         ``prefix`` a 1-D tensor of tokens that come before all of them, computed once. The
         settings are those of ``sample_op.sample_tokens``; its uniform numbers are ``u
-        [n_new, batch]`` or drawn from ``generator``. Where a model's logits are all NaN the
-        tokens are -1 (and the model goes on from token 0)."""
+        [n_new, batch]`` or drawn from ``generator``. Where a model's logits are all NaN, or a mask
+        allows nothing, the tokens are -1 (and the model goes on from token 0).
+
+        Penalties, ``bias`` and ``allowed`` are those of ``logits_op.adjust_logits``; a row's
+        history is the prefix, its prompt and what it has been given since. ``allowed`` may be a
+        function of the new tokens so far (``[batch, i]``) that returns the next step's mask, or
+        None where it allows everything."""
         rows = list(prompts)
         if not rows or any(r.ndim != 1 or r.numel() == 0 for r in rows):
             raise ValueError("prompts must be 1-D tensors of at least one token each")
@@ -705,9 +759,27 @@ class Transformer(nn.Module):
         starts = torch.tensor([0, *lens], dtype=torch.int32).cumsum(0, dtype=torch.int32).to(dev)
         logits = self.decode(torch.cat([r.to(dev) for r in rows]), state, starts)
         out = torch.empty(len(rows), n_new, device=dev, dtype=torch.int64)
+        penalties = dict(repetition_penalty=repetition_penalty, presence_penalty=presence_penalty,
+                         frequency_penalty=frequency_penalty)
+        past = {}
+        if any(isinstance(p, Tensor) for p in penalties.values()) or penalties != dict(
+                repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0):
+            tokens = torch.full((len(rows), shared + max(lens) + n_new), -1, device=dev, dtype=torch.int64)
+            prompts_end = (starts.diff() + shared).contiguous()
+            for r, row in zip(rows, tokens):
+                if shared:
+                    row[:shared] = prefix
+                row[shared:shared + r.numel()] = r
+            past = dict(tokens=tokens, lengths=prompts_end.clone(), prompt_lengths=prompts_end)
         for i in range(n_new):
+            mask = allowed(out[:, :i]) if callable(allowed) else allowed
+            if past or bias is not None or mask is not None:
+                logits = adjust_logits(logits, **past, **penalties, bias=bias, allowed=mask, out=logits)
             tokens = sample_tokens(logits, u[i], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
             out[:, i] = tokens
+            if past:
+                past["tokens"].scatter_(1, past["lengths"].long()[:, None], tokens[:, None])
+                past["lengths"] += 1
             if i + 1 < n_new:
                 logits = self.decode(tokens.clamp(min=0)[:, None], state)
         return out

@@ -139,32 +139,35 @@ def quantize4(w: torch.Tensor, group: int = 64, *, symmetric: bool = True) -> We
 def linear4(x: torch.Tensor, weight: Weight4) -> torch.Tensor:
     """``x [..., in_features]`` times the weights, ``[..., out_features]``; x has the scales'
     dtype. A row with an infinity or NaN gives NaN."""
-    if _lib.ordinary(x, weight.tiles, weight.scales) and x.is_cuda and (weight.zeros is None or _lib.ordinary(weight.zeros)):
-        y = _lib.native().linear4(x, weight.tiles, weight.scales, weight.zeros, weight.out_features, weight.in_features,
-                                  weight.group)
+    return _linear4(x, weight.tiles, weight.scales, weight.zeros, weight.out_features, weight.in_features, weight.group)
+
+
+def _linear4(x, tiles, scales, zeros, n: int, k: int, group: int) -> torch.Tensor:
+    if _lib.ordinary(x, tiles, scales) and x.is_cuda and (zeros is None or _lib.ordinary(zeros)):
+        y = _lib.native().linear4(x, tiles, scales, zeros, n, k, group)
         if y is not None:
             return y
     if torch.compiler.is_compiling():
-        return _untraced(x, weight)
-    _no_backward("linear4", x, weight.scales)
-    n, k = weight.out_features, weight.in_features
+        return _untraced(x, tiles, scales, zeros, n, k, group)
+    _no_backward("linear4", x, scales)
+    Weight4(tiles, scales, zeros, n, k, group)  # (checks them)
     _need(x.ndim >= 1 and x.shape[-1] == k, f"x must have {k} columns, got {tuple(x.shape)}")
-    _need(x.dtype == weight.scales.dtype, f"x must have the weights' dtype {weight.scales.dtype}, got {x.dtype}")
-    _need(x.is_cuda and x.device == weight.tiles.device, f"x must be on the weights' CUDA device {weight.tiles.device}")
-    rows = x.reshape(-1, k)
+    _need(x.dtype == scales.dtype, f"x must have the weights' dtype {scales.dtype}, got {x.dtype}")
+    _need(x.is_cuda and x.device == tiles.device, f"x must be on the weights' CUDA device, which is {tiles.device}")
+    rows = x.reshape(-1, k) if x.numel() else x.new_empty(0, k)
     if k > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
     out = torch.empty(*x.shape[:-1], n, device=x.device, dtype=x.dtype)
     if rows.shape[0] > 0:
         with torch.cuda.device(x.device):
-            rc = _lib.lib().sy_linear4(_ptr(rows), rows.stride(0), _ptr(weight.tiles), _ptr(weight.scales),
-                                       None if weight.zeros is None else _ptr(weight.zeros), _ptr(out), rows.shape[0], n,
-                                       k, weight.group, _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
+            rc = _lib.lib().sy_linear4(_ptr(rows), rows.stride(0), _ptr(tiles), _ptr(scales),
+                                       None if zeros is None else _ptr(zeros), _ptr(out), rows.shape[0], n, k, group,
+                                       _lib.dtype_code(x.dtype), _lib.stream_ptr(x.device))
         _lib.check(rc, "sy_linear4")
     return out
 
 
-_untraced = torch.compiler.disable(linear4)  # what a compiler's trace calls
+_untraced = torch.compiler.disable(_linear4)  # what a compiler's trace calls
 
 
 class Linear4(nn.Module):
@@ -190,7 +193,7 @@ class Linear4(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dtype != self.scales.dtype and torch.is_autocast_enabled("cuda"):
             x = x.to(self.scales.dtype)
-        return linear4(x, self.weight4)
+        return _linear4(x, self.tiles, self.scales, self.zeros, self.out_features, self.in_features, self.group)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}"
