@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
   const double r = a.repetitions != nullptr ? a.repetitions[row] : a.repetition;
   const double p = a.presences != nullptr ? a.presences[row] : a.presence;
   const double f = a.frequencies != nullptr ? a.frequencies[row] : a.frequency;
+  const double inv_r = 1.0 / r;  // (its rounding is 2^-53, and a division a token was 1 us)
   const bool counted = a.tokens != nullptr && (r != 1.0 || p != 0.0 || f != 0.0);
   if (counted) {
 #pragma unroll
@@ -159,10 +160,10 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
     if (any != 0) {
 #pragma unroll
       for (int e = 0; e < CE; ++e) {
-        if (cnt[e] == 0) continue;
         const uint32_t said = cnt[e] & ~kPrompt;
         const double z = v[k][e];
-        v[k][e] = (float)((z > 0.0 ? z / r : z * r) - (said != 0 ? f * said + p : 0.0));
+        const double y = fma(z, z > 0.0 ? inv_r : r, said != 0 ? -fma(f, (double)said, p) : 0.0);
+        v[k][e] = cnt[e] != 0 ? (float)y : v[k][e];
       }
     }
     if (a.bias != nullptr && keep[k] != 0) {

@@ -175,22 +175,15 @@ template <class T, bool ZEROS> __device__ __forceinline__ i32x4_t minus() {
 }
 
 
-// Eight elements of a row as they lie in memory, from column k on; WHOLE: all are before
-// k_end, else those behind it are zero. Rows start anywhere.
-template <class T> struct Raw {
-  static constexpr int words = 8 * sizeof(typename T::storage) / 16;
-  i32x4_t x[words];
-};
+// 16 bytes of a row from column k on; WHOLE: all are before k_end, else those behind it are
+// zero. Rows start anywhere.
 template <class T, bool WHOLE>
-__device__ __forceinline__ Raw<T> ld_x(const typename T::storage* row, int k, int k_end) {
-  Raw<T> r;
-  constexpr int W = Raw<T>::words;
-  if (WHOLE || (W == 2 && k + 8 <= k_end)) {
+__device__ __forceinline__ i32x4_t ld_x(const typename T::storage* row, int k, int k_end) {
+  if (WHOLE) return *reinterpret_cast<const i32x4_any_t*>(row + k);
+  i32x4_t r = {0, 0, 0, 0};
+  if constexpr (T::ce == 4) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) r.x[i] = *reinterpret_cast<const i32x4_any_t*>(row + k + i * (8 / W));
-  } else if constexpr (W == 2) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r.x[e / 4][e % 4] = k + e < k_end ? __float_as_int(row[k + e]) : 0;
+    for (int e = 0; e < 4; ++e) r[e] = k + e < k_end ? __float_as_int(row[k + e]) : 0;
   } else {
     // The row's last eight, with those before k shifted out.
     typedef uint64_t u64x2_t __attribute__((ext_vector_type(2)));
@@ -213,10 +206,16 @@ __device__ __forceinline__ Raw<T> ld_x(const typename T::storage* row, int k, in
       if (bits != 0) x = u64x2_t{x[0] >> bits | x[1] << (64 - bits), x[1] >> bits};
       if (past >= 8) x = u64x2_t{0, 0};
     }
-    r.x[0] = __builtin_bit_cast(i32x4_t, x);
+    r = __builtin_bit_cast(i32x4_t, x);
   }
   return r;
 }
+
+// Eight elements of a row.
+template <class T> struct Raw {
+  static constexpr int words = 8 / T::ce;
+  i32x4_t x[words];
+};
 
 // Its fragments: itself, or the three bf16 parts of each element.
 template <class T> __device__ __forceinline__ void parts_of(const Raw<T>& r, i32x4_t (&f)[Mma<T>::planes]) {
@@ -274,15 +273,18 @@ __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4
   const int steps = (int)steps_of(a.k);
   const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
   // Rows behind the last are the last one's again: their sums are not stored. STAGED: a load is
-  // four whole rows of a tile, 256 bytes each, which go through LDS to the lanes that need them.
-  const S* rows[MT][STAGED ? 4 : 1];
-  const int x_k = STAGED ? 8 * col : 8 * quad;
+  // whole rows of a tile, four of 256 bytes or two of 512, which go through LDS to the lanes
+  // that need them.
+  constexpr int W = Raw<T>::words, kChunks = kTileK / T::ce, kLoads = kChunks / 4;  // of a row, and of 16 rows
+  const int r0 = lane / kChunks, c0 = lane % kChunks;
+  const S* rows[MT][STAGED ? kLoads : 1];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int j = 0; j < (STAGED ? 4 : 1); ++j)
-      rows[t][j] = static_cast<const S*>(a.x) + min(m0 + 16 * t + (STAGED ? 4 * j + quad : col), a.m - 1) * a.x_stride;
-  i32x4_t* const stage = reinterpret_cast<i32x4_t*>(fold) + wave * (MT * 256);
+    for (int j = 0; j < (STAGED ? kLoads : 1); ++j)
+      rows[t][j] = static_cast<const S*>(a.x) +
+                   min(m0 + 16 * t + (STAGED ? 16 / kLoads * j + r0 : col), a.m - 1) * a.x_stride;
+  i32x4_t* const stage = reinterpret_cast<i32x4_t*>(fold) + wave * (MT * 16 * kChunks);
   const i32x4_t neg = minus<T, ZEROS>();
   f32x4_t tot[MT][NT];
 #pragma unroll
@@ -310,8 +312,10 @@ __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        r.x[t][j] = ld_x<T, decltype(whole)::value>(rows[t][STAGED ? j : 0], step * kTileK + x_k + (STAGED ? 0 : 32 * j), a.k);
+      for (int j = 0; j < kLoads; ++j) {
+        const int k = step * kTileK + (STAGED ? T::ce * c0 : 32 * (j / W) + 8 * quad + T::ce * (j % W));
+        r.x[t][j / W].x[j % W] = ld_x<T, decltype(whole)::value>(rows[t][STAGED ? j : 0], k, a.k);
+      }
   };
   const auto add = [&](const Tile& r) {
     i32x4_t f[MT][4][P];
@@ -321,12 +325,20 @@ __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) stage[t * 256 + (4 * j + quad) * 16 + (col ^ (4 * j + quad))] = r.x[t][j].x[0];
+        for (int j = 0; j < kLoads; ++j) {
+          const int row = 16 / kLoads * j + r0;
+          stage[(t * 16 + row) * kChunks + (c0 ^ row)] = r.x[t][j / W].x[j % W];
+        }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[t][j][0] = stage[t * 256 + col * 16 + ((4 * j + quad) ^ col)];
+        for (int j = 0; j < 4; ++j) {
+          Raw<T> x;
+#pragma unroll
+          for (int i = 0; i < W; ++i) x.x[i] = stage[(t * 16 + col) * kChunks + (((4 * j + quad) * W + i) ^ col)];
+          parts_of<T>(x, f[t][j]);
+        }
       __builtin_amdgcn_wave_barrier();
     } else {
 #pragma unroll
@@ -469,7 +481,7 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
       if constexpr (ZEROS) r.z[u] = *reinterpret_cast<const Zeros*>(z_at[u] + cell);
     }
   };
-  const auto load_x = [&](int step, Raw<T> (&x)[MT]) {
+  const auto load_x = [&](int step, i32x4_t (&x)[MT]) {
     const int k = step * kTileK + 8 * c0;
     if ((step + 1) * kTileK <= a.k) {
 #pragma unroll
@@ -479,11 +491,11 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
       for (int i = 0; i < MT; ++i) x[i] = ld_x<T, false>(rows[i], k, a.k);
     }
   };
-  const auto put = [&](int buffer, const Raw<T> (&x)[MT]) {
+  const auto put = [&](int buffer, const i32x4_t (&x)[MT]) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      stage[part][buffer][(r0 + 16 * i) * 16 + (c0 ^ r0)] = x[i].x[0];
-      const float s = lane_sum<4 * GS>(sum8<T>(x[i].x[0], 0.0f)) * (ZEROS ? -1.0f : -1.5f);
+      stage[part][buffer][(r0 + 16 * i) * 16 + (c0 ^ r0)] = x[i];
+      const float s = lane_sum<4 * GS>(sum8<T>(x[i], 0.0f)) * (ZEROS ? -1.0f : -1.5f);
       if (c0 % (4 * GS) == 0) sums[part][buffer][c0 / (4 * GS)][r0 + 16 * i] = s;
     }
   };
@@ -525,7 +537,7 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
   };
   // Both groups go round as often; one may have nothing to add in the last round.
   const int last = steps - 1, rounds = (steps + 1) / 2;
-  Raw<T> x[MT];
+  i32x4_t x[MT];
   Weights w, next;
   load_w(min(part, last), w);
   load_x(min(part, last), x);
@@ -593,8 +605,9 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
   int waves = WAVES;
   while (waves > 1 && waves > steps) waves /= 2;
   const unsigned gx = (unsigned)((tiles_of(a.n) + NT - 1) / NT);
-  const int lds = waves * MT * (STAGED ? std::max(4, NT) : NT) * 1024;
-  static_assert(WAVES * MT * NT <= 64 && (!STAGED || WAVES * MT <= 16), "at most 64 KiB of LDS");
+  constexpr int kRows16 = T::ce == 8 ? 4 : 8;  // KiB of a column tile of 16 rows
+  const int lds = waves * MT * (STAGED ? std::max(kRows16, NT) : NT) * 1024;
+  static_assert(WAVES * MT * NT <= 64 && (!STAGED || WAVES * MT * kRows16 <= 64), "at most 64 KiB of LDS");
   constexpr int64_t kRows = 16 * MT * 256;  // of a launch: at most 2^28 workgroups
   for (int64_t m0 = 0; m0 < a.m; m0 += kRows) {
     Linear4Args part = a;
@@ -611,25 +624,34 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
   return hipSuccess;
 }
 
-// The kernel and its tile by rows and feature tiles; us on both sides, bf16.
+// The kernel and its tile by rows and feature tiles; us on both sides, bf16 unless stated.
 //   up to 8 rows     straight from memory: a load's lanes touch few lines. 8 rows of 32000 x 2048
 //                    8.2, through LDS 9.4. Past 1024 feature tiles four a workgroup, 1 row of
 //                    32000 x 2048 8.1, one 8.7; below one, 6144 x 2048 3.6, four 5.
+//                    fp32: two from 256 on, 1 row of 6144 x 2048 5.6, one 7.0; 5 rows of 1408 x
+//                    2048 5.6, one 5.3.
 //   up to 16         through LDS. 16 rows of 2048 x 2048 3.4, straight 4.3; of 28672 x 8192 29.6,
 //                    straight 35.7, one feature tile 43.
 //   up to 32, or few blocks of 64 rows
 //                    32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
 //                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
 //                    many: 28672 x 8192 38.5, without 43.
-//   else             64 rows and the most features that leave workgroups for six CUs of ten: 2048
-//                    rows of 2048 x 5632 59 with 256 features, 72 with 128, 82 with 64, 87 as
-//                    above; 128 rows of 11264 x 2048 29, 19, 24, 21; 128 of 2048 x 5632 56, 35, 26,
-//                    13 (32 and 64 workgroups).
+//   else             64 rows and 64 NT features, for which a CU needs 2.7 (NT 4), 1.6 (2) or 1.3 us
+//                    (1; two at once 1.9) for two column tiles: the one that is done first on 256
+//                    CUs. 2048 rows of 2048 x 5632 59, 72, 82, and 87 as above; 128 rows of 11264 x
+//                    2048 29, 19, 24, 21; 128 of 2048 x 5632 56, 35, 26, 13 (32 to 128 workgroups).
+//   fp32 past 8      through LDS, 16 rows a workgroup, and up to four feature tiles: 16 rows of 2048
+//                    x 5632 10.4 with one, 12.4 with two, 15.6 with four, 15.1 straight; 64 of 2048
+//                    x 2048 8.3, 6.7, 7.9, 10.9; 16 of 11264 x 2048 11.9, 10.5, 8.9, 17.3.
 template <class T, int GS, bool ZEROS>
 hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
   const int64_t tiles = tiles_of(a.n);
   if constexpr (T::code == F32::code) {
-    return tiles < 1024 ? run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s) : run4<T, 1, 2, 8, false, false, GS, ZEROS>(a, s);
+    if (a.m <= 8)
+      return tiles >= 256 ? run4<T, 1, 2, 8, false, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
+    const int64_t blocks = tiles * ((a.m + 15) / 16);
+    if (blocks < 256) return run4<T, 1, 1, 8, true, false, GS, ZEROS>(a, s);
+    return blocks < 704 ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
   } else {
     if (a.m <= 8)
       return tiles >= 1024 ? run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
@@ -637,9 +659,13 @@ hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
       return tiles >= 1024 ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
     if (a.m > 32) {
       const auto blocks = [&](int nt) { return (a.m + 63) / 64 * ((tiles + 4 * nt - 1) / (4 * nt)); };
-      if (blocks(4) >= 160) return run4_many<T, 4, GS, ZEROS>(a, s);
-      if (blocks(2) >= 160) return run4_many<T, 2, GS, ZEROS>(a, s);
-      if (blocks(1) >= 160) return run4_many<T, 1, GS, ZEROS>(a, s);
+      if (blocks(1) >= 160) {
+        const double t4 = 2.7 * (double)((blocks(4) + 255) / 256), t2 = 1.6 * (double)((blocks(2) + 255) / 256);
+        const int64_t rest = blocks(1) % 512;
+        const double t1 = 1.9 * (double)(blocks(1) / 512) + (rest > 256 ? 1.9 : rest > 0 ? 1.3 : 0.0);
+        if (t4 <= t2 && t4 <= t1) return run4_many<T, 4, GS, ZEROS>(a, s);
+        return t2 <= t1 ? run4_many<T, 2, GS, ZEROS>(a, s) : run4_many<T, 1, GS, ZEROS>(a, s);
+      }
     }
     if (tiles < 512) return run4<T, 2, 1, 8, true, false, GS, ZEROS>(a, s);
     return a.k < 4096 ? run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 2, 4, 4, true, true, GS, ZEROS>(a, s);
