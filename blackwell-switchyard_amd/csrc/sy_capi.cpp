@@ -1298,7 +1298,7 @@ int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_
   if (!valid_dtype(dtype)) return SY_ERR_DTYPE;
   if (how->bias && how->bias_dtype != dtype && how->bias_dtype != SY_F32) return SY_ERR_DTYPE;
   if (n_rows < 0 || n_rows > 0x7fffffff || vocab < 1 || vocab > (1 << 30) || how->n_tokens < 0 ||
-      how->n_tokens > 0x7fffffff || (how->tokens_bytes != 4 && how->tokens_bytes != 8) || how->mask_kind < 0 ||
+      how->n_tokens > (1 << 30) || (how->tokens_bytes != 4 && how->tokens_bytes != 8) || how->mask_kind < 0 ||
       how->mask_kind > 2)
     return SY_ERR_SHAPE;
   if (row_stride < 0 || out_stride < 0 || (n_rows > 1 && out_stride < vocab) || how->tokens_stride < 0 ||

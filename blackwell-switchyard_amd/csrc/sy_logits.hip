@@ -45,27 +45,43 @@ __device__ __forceinline__ uint32_t allowed(const AdjustArgs& a, int64_t row, in
   return static_cast<const uint32_t*>(a.mask)[row * a.mask_stride + (v >> 5)] >> (v & 31) & all;
 }
 
-__device__ __forceinline__ void count(uint32_t* seen, int64_t token, int lo, int n, bool said) {
-  const int64_t at = token - lo;
-  if ((uint64_t)at >= (uint64_t)n) return;
-  if (said) atomicAdd(&seen[at], 1u);
-  else atomicOr(&seen[at], kPrompt);
+// A barrier for what is in LDS alone: loads from memory stay on their way across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// The row's first `len` tokens, eight a thread on their way at a time.
-template <class I>
-__device__ __forceinline__ void count_all(uint32_t* seen, const I* t, int64_t len, int64_t prompt, int lo, int n) {
-  constexpr int kAhead = 8;
-  for (int64_t i0 = threadIdx.x; i0 < len; i0 += kBlock * kAhead) {
-    I x[kAhead];
+// Eight tokens a thread of a row of `n_tokens`, from i0 on; what is no token of 31 bits is -1.
+constexpr int kAhead = 8;
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void ld_tokens(const AdjustArgs& a, int64_t row, int i0, int (&x)[kAhead]) {
+  const int first = i0 + (int)threadIdx.x;
+  if (a.tokens64) {
+    const u32x2_t* const t = static_cast<const u32x2_t*>(a.tokens) + row * a.tokens_stride + first;
+    u32x2_t w[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int64_t i = i0 + j * kBlock;
-      x[j] = i < len ? t[i] : (I)-1;
-    }
+    for (int j = 0; j < kAhead; ++j) w[j] = first + j * kBlock < (int)a.n_tokens ? t[j * kBlock] : u32x2_t{0, 1};
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) count(seen, x[j], lo, n, i0 + j * kBlock >= prompt);
+    for (int j = 0; j < kAhead; ++j) x[j] = w[j][1] == 0 ? (int)w[j][0] : -1;
+  } else {
+    const int* const t = static_cast<const int*>(a.tokens) + row * a.tokens_stride + first;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) x[j] = first + j * kBlock < (int)a.n_tokens ? t[j * kBlock] : -1;
   }
+}
+
+// A chunk as it lies in memory; elements from `n` on are zero.
+template <class T> __device__ __forceinline__ i32x4_t ld_chunk(const typename T::storage* p, int n) {
+  if (n >= T::ce) return *reinterpret_cast<const i32x4_any_t*>(p);
+  i32x4_t r = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < T::ce; ++e) {
+    if (e >= n) continue;
+    if constexpr (T::ce == 4) r[e] = __float_as_int(p[e]);
+    else r[e / 2] |= (int)((uint32_t)p[e] << (16 * (e % 2)));
+  }
+  return r;
 }
 
 // CE neighbouring numbers at p as fp32; those from `n` on are zero.
@@ -85,16 +101,36 @@ template <class T, int CE> __device__ __forceinline__ void ld_row_part(const voi
   }
 }
 
-// A workgroup takes a slice of one row, IT chunks a thread, all of them on their way while it
-// reads the row's history and counts in LDS what falls into its slice: in whole numbers, so in
-// any order. Chunks with nothing allowed are not read; in place and without a bias only those
-// are that something was counted in, and all that stay as they are are not written.
+// The elements of a chunk that `keep` has a bit for; -inf for the others.
+template <class T> __device__ __forceinline__ i32x4_t masked(const i32x4_t& x, uint32_t keep) {
+  constexpr int kInf = T::code == F32::code ? (int)0xff800000 : T::code == BF16::code ? (int)0xff80ff80 : (int)0xfc00fc00;
+  const auto all = [&](int e) { return (int)(keep << (31 - e)) >> 31; };
+  i32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = T::ce == 4 ? all(i) : (all(2 * i) & 0xffff) | (all(2 * i + 1) & (int)0xffff0000);
+    r[i] = (x[i] & m) | (kInf & ~m);
+  }
+  return r;
+}
+
+// A workgroup takes a slice of one row, IT chunks a thread, all of them on their way (and left
+// as they come) while it deals with the row's history. It counts in LDS what falls into its
+// slice, in whole numbers, so in any order, and lists the tokens that are there; then penalises
+// those, a thread each, puts the results in the counts' places and sets a bit for each (worked
+// out in the chunks that hold them, 82 rows of 92375 in fp16 with 1290 tokens 13.9 us, so 9.7;
+// 8 rows with 3808 tokens 5.5, so 7.3). Then one pass over the chunks. Those with
+// nothing allowed are not read; in place and without a bias only those are that something was
+// counted in, and all that stay as they are are not written.
 template <class T, int IT>
 __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slices) {
   using S = typename T::storage;
   constexpr int CE = T::ce, kSlice = kBlock * CE * IT;
   constexpr uint32_t all = (1u << CE) - 1u;
   extern __shared__ uint32_t seen[];
+  uint32_t* const there = seen + kSlice;  // a bit a token
+  uint32_t* const listed = there + kSlice / 32;
+  uint16_t* const list = reinterpret_cast<uint16_t*>(listed + 1);
   const int64_t row = blockIdx.x / slices;
   const int lo = (int)(blockIdx.x % slices) * kSlice, n = min(kSlice, a.vocab - lo);
   const S* const x = static_cast<const S*>(a.logits) + row * a.row_stride + lo;
@@ -107,86 +143,100 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
     const int c = (k * kBlock + threadIdx.x) * CE;
     keep[k] = c < n ? allowed<CE>(a, row, lo + c, c + CE <= n) : 0u;
   }
-  float v[IT][CE];
-  if (!lazy) {
+  int ahead[kAhead];
+  if (a.tokens != nullptr) ld_tokens(a, row, 0, ahead);
+  i32x4_t raw[IT];
 #pragma unroll
-    for (int k = 0; k < IT; ++k) {
-      const int c = (k * kBlock + threadIdx.x) * CE;
-#pragma unroll
-      for (int e = 0; e < CE; ++e) v[k][e] = 0.0f;
-      if (keep[k] != 0) ld_row_part<T, CE>(x + c, n - c, v[k]);
-    }
+  for (int k = 0; k < IT; ++k) {
+    const int c = (k * kBlock + threadIdx.x) * CE;
+    raw[k] = i32x4_t{0, 0, 0, 0};
+    if (!lazy && keep[k] != 0) raw[k] = ld_chunk<T>(x + c, n - c);
   }
   const double r = a.repetitions != nullptr ? a.repetitions[row] : a.repetition;
   const double p = a.presences != nullptr ? a.presences[row] : a.presence;
   const double f = a.frequencies != nullptr ? a.frequencies[row] : a.frequency;
-  const double inv_r = 1.0 / r;  // (its rounding is 2^-53, and a division a token was 1 us)
   const bool counted = a.tokens != nullptr && (r != 1.0 || p != 0.0 || f != 0.0);
   if (counted) {
+    const int len = a.lengths != nullptr ? min(a.lengths[row], (int)a.n_tokens) : (int)a.n_tokens;
+    const int prompt = a.prompts != nullptr ? a.prompts[row] : 0;
 #pragma unroll
-    for (int k = 0; k < IT; ++k)
+    for (int k = 0; k < IT * CE / 4; ++k)
+      *reinterpret_cast<i32x4_t*>(seen + (k * kBlock + threadIdx.x) * 4) = i32x4_t{0, 0, 0, 0};
+    if (threadIdx.x < kSlice / 128) *reinterpret_cast<i32x4_t*>(there + threadIdx.x * 4) = i32x4_t{0, 0, 0, 0};
+    if (threadIdx.x == 0) *listed = 0;
+    lds_barrier();
+    for (int i0 = 0; i0 < len; i0 += kBlock * kAhead) {
+      int next[kAhead];
+      if (i0 + kBlock * kAhead < len) ld_tokens(a, row, i0 + kBlock * kAhead, next);
+      uint32_t before[kAhead];
 #pragma unroll
-      for (int q = 0; q < CE / 4; ++q)
-        *reinterpret_cast<i32x4_t*>(seen + (k * kBlock + threadIdx.x) * CE + 4 * q) = i32x4_t{0, 0, 0, 0};
-    __syncthreads();
-    const int64_t len = a.lengths != nullptr ? min(max((int64_t)a.lengths[row], (int64_t)0), a.n_tokens) : a.n_tokens;
-    const int64_t prompt = a.prompts != nullptr ? a.prompts[row] : 0;
-    if (a.tokens64) count_all(seen, static_cast<const int64_t*>(a.tokens) + row * a.tokens_stride, len, prompt, lo, n);
-    else count_all(seen, static_cast<const int32_t*>(a.tokens) + row * a.tokens_stride, len, prompt, lo, n);
-    __syncthreads();
+      for (int j = 0; j < kAhead; ++j) {
+        const int i = i0 + j * kBlock + (int)threadIdx.x;
+        ahead[j] -= lo;
+        before[j] = 1;
+        if (i >= len || (uint32_t)ahead[j] >= (uint32_t)n) continue;
+        before[j] = i >= prompt ? atomicAdd(&seen[ahead[j]], 1u) : atomicOr(&seen[ahead[j]], kPrompt);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        if (before[j] == 0) list[atomicAdd(listed, 1u)] = (uint16_t)ahead[j];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) ahead[j] = next[j];
+    }
+    lds_barrier();
+    const int count = (int)*listed;
+    for (int i = threadIdx.x; i < count; i += kBlock) {
+      const int at = list[i];
+      const uint32_t said = seen[at] & ~kPrompt;
+      const double z = load_elem(x, at, T::code);
+      seen[at] = __float_as_uint((float)((z > 0.0 ? z / r : z * r) - (said != 0 ? fma(f, (double)said, p) : 0.0)));
+      atomicOr(&there[at >> 5], 1u << (at & 31));
+    }
+    lds_barrier();
   }
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
     const int c = (k * kBlock + threadIdx.x) * CE;
     if (c >= n) break;
-    uint32_t cnt[CE], any = 0;
-#pragma unroll
-    for (int e = 0; e < CE; ++e) cnt[e] = 0;
-    if (counted) {
-#pragma unroll
-      for (int q = 0; q < CE / 4; ++q) {
-        const i32x4_t w = *reinterpret_cast<const i32x4_t*>(seen + c + 4 * q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) cnt[4 * q + e] = (uint32_t)w[e], any |= (uint32_t)w[e];
-      }
-    }
+    const uint32_t set = counted ? there[c >> 5] >> (c & 31) & all : 0u;
     if (lazy) {
-      const uint32_t there = n - c >= CE ? all : (1u << (n - c)) - 1u;
-      if (any == 0 && (keep[k] & there) == there) continue;
-#pragma unroll
-      for (int e = 0; e < CE; ++e) v[k][e] = 0.0f;
-      if (keep[k] != 0) ld_row_part<T, CE>(x + c, n - c, v[k]);
+      const uint32_t inside = n - c >= CE ? all : (1u << (n - c)) - 1u;
+      if (set == 0 && (keep[k] & inside) == inside) continue;
+      if (keep[k] != 0) raw[k] = ld_chunk<T>(x + c, n - c);
     }
-    if (any != 0) {
+    if ((set != 0 || a.bias != nullptr) && keep[k] != 0) {
+      float v[CE];
 #pragma unroll
-      for (int e = 0; e < CE; ++e) {
-        const uint32_t said = cnt[e] & ~kPrompt;
-        const double z = v[k][e];
-        const double y = fma(z, z > 0.0 ? inv_r : r, said != 0 ? -fma(f, (double)said, p) : 0.0);
-        v[k][e] = cnt[e] != 0 ? (float)y : v[k][e];
+      for (int e = 0; e < CE; ++e) v[e] = elem<T>(raw[k], e);
+      if (set != 0) {
+#pragma unroll
+        for (int q = 0; q < CE / 4; ++q) {
+          const i32x4_t w = *reinterpret_cast<const i32x4_t*>(seen + c + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * q + e] = set >> (4 * q + e) & 1u ? __int_as_float(w[e]) : v[4 * q + e];
+        }
       }
-    }
-    if (a.bias != nullptr && keep[k] != 0) {
-      const int64_t at = row * a.bias_stride + lo + c;
-      float b[CE];
-      if (a.bias_f32) ld_row_part<F32, CE>(static_cast<const float*>(a.bias) + at, n - c, b);
-      else ld_row_part<T, CE>(static_cast<const S*>(a.bias) + at, n - c, b);
+      if (a.bias != nullptr) {
+        const int64_t at = row * a.bias_stride + lo + c;
+        float b[CE];
+        if (a.bias_f32) ld_row_part<F32, CE>(static_cast<const float*>(a.bias) + at, n - c, b);
+        else ld_row_part<T, CE>(static_cast<const S*>(a.bias) + at, n - c, b);
 #pragma unroll
-      for (int e = 0; e < CE; ++e) v[k][e] += b[e];
+        for (int e = 0; e < CE; ++e) v[e] += b[e];
+      }
+      raw[k] = pack<T>(v);
     }
-#pragma unroll
-    for (int e = 0; e < CE; ++e)
-      if ((keep[k] >> e & 1u) == 0) v[k][e] = -__builtin_inff();
+    if (a.mask != nullptr) raw[k] = masked<T>(raw[k], keep[k]);
     if (c + CE <= n) {
       // (Where there is much to write it goes past the caches: 256 rows of 50257 in fp32 25.8 ->
-      // 23.9 us; 8 of 32000 in bf16 8.1 -> 8.6.)
+      // 23.9 us, 82 of 92375 in fp16 10.9 -> 9.7; 8 of 32000 in bf16 8.1 -> 8.6.)
       i32x4_any_t* const to = reinterpret_cast<i32x4_any_t*>(y + c);
-      if constexpr (IT == 4) __builtin_nontemporal_store((i32x4_any_t)pack<T>(v[k]), to);
-      else *to = pack<T>(v[k]);
+      if constexpr (CE * IT == 16) __builtin_nontemporal_store((i32x4_any_t)raw[k], to);
+      else *to = raw[k];
     } else {
 #pragma unroll
       for (int e = 0; e < CE; ++e)
-        if (c + e < n) store_elem(y, c + e, v[k][e], T::code);
+        if (c + e < n) store_elem(y, c + e, elem<T>(raw[k], e), T::code);
     }
   }
 }
@@ -196,6 +246,8 @@ hipError_t adjust_it(const AdjustArgs& a, hipStream_t s) {
   constexpr int kSlice = kBlock * T::ce * IT;
   const int slices = (a.vocab + kSlice - 1) / kSlice;
   const int64_t rows = std::max<int64_t>(1, (1 << 22) / slices);  // of a launch: 2^30 threads
+  // A count and a bit a token, and the tokens that are there.
+  const int lds = a.tokens ? kSlice * 4 + kSlice / 8 + 4 + 2 * (int)std::min<int64_t>(kSlice, a.n_tokens) : 0;
   for (int64_t r0 = 0; r0 < a.n_rows; r0 += rows) {
     AdjustArgs part = a;
     part.n_rows = std::min(rows, a.n_rows - r0);
@@ -211,19 +263,23 @@ hipError_t adjust_it(const AdjustArgs& a, hipStream_t s) {
     if (a.bias) part.bias = static_cast<const char*>(a.bias) + r0 * a.bias_stride * (a.bias_f32 ? 4 : es);
     if (a.mask) part.mask = static_cast<const char*>(a.mask) + r0 * a.mask_stride * (a.mask_bytes ? 1 : 4);
     hipLaunchKernelGGL((k_adjust<T, IT>), dim3((unsigned)(part.n_rows * slices)), dim3(kBlock),
-                       a.tokens ? kSlice * sizeof(uint32_t) : 0, s, part, slices);
+                       lds, s, part, slices);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
+// Slices as long as leave every CU workgroups: each reads the row's whole history. Past 4096
+// tokens the counts would leave too few workgroups to a CU: 98 rows of 116414 in bf16 with 1290
+// tokens 15.9 us with slices of 8192, 13.8 with 4096.
 template <class T>
 hipError_t adjust_t(const AdjustArgs& a, hipStream_t s) {
   const int64_t chunks = a.n_rows * ((a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce));  // workgroups of one each
-  if (chunks >= 4096) return adjust_it<T, 4>(a, s);
-  if (chunks >= 2048) return adjust_it<T, 2>(a, s);
-  return adjust_it<T, 1>(a, s);
+  if constexpr (T::ce == 4) {
+    if (chunks >= 4096) return adjust_it<T, 4>(a, s);
+  }
+  return chunks >= 2048 ? adjust_it<T, 2>(a, s) : adjust_it<T, 1>(a, s);
 }
 
 }  // namespace

@@ -869,7 +869,7 @@ std::optional<Tensor> adjust_logits(const Tensor& logits_in, double repetition, 
   if (tokens.has_value()) {
     const Tensor& t = *tokens;
     if (!(whole_of(t, at::kLong) || whole(t)) || t.device() != dev || t.dim() != 2 || t.size(0) != b ||
-        t.size(1) > 0x7fffffff || t.stride(0) < 0 || (t.size(1) > 1 && t.stride(1) != 1))
+        t.size(1) > (1 << 30) || t.stride(0) < 0 || (t.size(1) > 1 && t.stride(1) != 1))
       return std::nullopt;
     how.tokens = t.data_ptr(), how.tokens_stride = t.stride(0), how.n_tokens = t.size(1);
     how.tokens_bytes = (int32_t)t.element_size();

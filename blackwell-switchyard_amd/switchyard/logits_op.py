@@ -34,6 +34,8 @@ def _need(ok: bool, message: str) -> None:
 
 def _split(name: str, x):
     """A setting as (number, tensor or None); numbers are checked here."""
+    if type(x) is float and (x > 0 or name != "repetition_penalty") and abs(x) < math.inf:
+        return x, None
     if isinstance(x, torch.Tensor):
         return 1.0, x
     if not isinstance(x, numbers.Real) or not math.isfinite(x):
@@ -69,7 +71,7 @@ def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, l
     p, ps = _split("presence_penalty", presence_penalty)
     f, fs = _split("frequency_penalty", frequency_penalty)
     more = (tokens, lengths, prompt_lengths, rs, ps, fs, bias, allowed, out)
-    if _lib.ordinary(logits) and logits.is_cuda and all(x is None or _lib.ordinary(x) for x in more):
+    if _lib.ordinary(logits, *[x for x in more if x is not None]) and logits.is_cuda:
         y = _lib.native().adjust_logits(logits, r, p, f, *more)
         if y is not None:
             return y
@@ -91,6 +93,7 @@ def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, l
     else:
         _need(tokens.ndim == 2 and tokens.shape[0] == b and tokens.dtype in (torch.int64, torch.int32)
               and tokens.device == dev, f"tokens must be int64 or int32 [{b}, L] on the same CUDA device as logits")
+        _need(tokens.shape[1] <= 1 << 30, "a history must hold at most 2^30 tokens")
         if tokens.shape[1] > 1 and tokens.stride(1) != 1:
             tokens = tokens.contiguous()
         keep.append(tokens)
