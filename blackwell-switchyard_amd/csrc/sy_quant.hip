@@ -630,8 +630,9 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
 //                    32000 x 2048 8.1, one 8.7; below one, 6144 x 2048 3.6, four 5.
 //                    fp32: two from 256 on, 1 row of 6144 x 2048 5.6, one 7.0; 5 rows of 1408 x
 //                    2048 5.6, one 5.3.
-//   up to 16         through LDS. 16 rows of 2048 x 2048 3.4, straight 4.3; of 28672 x 8192 29.6,
-//                    straight 35.7, one feature tile 43.
+//   up to 16         through LDS, four feature tiles from 512 on. 16 rows of 2048 x 2048 3.4,
+//                    straight 4.3; of 11264 x 2048 5.8, one feature tile 10.7; of 28672 x 8192
+//                    29.6, straight 35.7, one feature tile 43.
 //   up to 32, or few blocks of 64 rows
 //                    32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
 //                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
@@ -656,7 +657,7 @@ hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
     if (a.m <= 8)
       return tiles >= 1024 ? run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
     if (a.m <= 16)
-      return tiles >= 1024 ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
+      return tiles >= 512 ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
     if (a.m > 32) {
       const auto blocks = [&](int nt) { return (a.m + 63) / 64 * ((tiles + 4 * nt - 1) / (4 * nt)); };
       if (blocks(1) >= 160) {

@@ -125,8 +125,7 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_cach
     ``x / sqrt(mean(x^2) + eps) * gain``."""
     if (_lib.ordinary(qkv, cos, sin, k_cache, v_cache, page_table, lengths) and qkv.is_cuda
             and type(prefix_len) is int and (starts is None or _lib.ordinary(starts))
-            and (out is None or _lib.ordinary(out)) and (q_gain is None or _lib.ordinary(q_gain))
-            and (k_gain is None or _lib.ordinary(k_gain))):
+            and (out is None or _lib.ordinary(out)) and (q_gain is None or _lib.ordinary(q_gain, k_gain))):
         q = _lib.native().paged_append(qkv, cos, sin, k_cache, v_cache, page_table, lengths, starts, prefix_len, out,
                                        q_gain, k_gain, eps)
         if q is not None:

@@ -172,7 +172,7 @@ _untraced = torch.compiler.disable(_linear4)  # what a compiler's trace calls
 
 class Linear4(nn.Module):
     """A projection with 4-bit weights, for inference. Under autocast activations are taken in
-    the scales' dtype."""
+    the scales' dtype and the output has autocast's."""
 
     def __init__(self, weight: Weight4) -> None:
         super().__init__()
@@ -191,9 +191,10 @@ class Linear4(nn.Module):
         return Weight4(self.tiles, self.scales, self.zeros, self.out_features, self.in_features, self.group)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if x.dtype != self.scales.dtype and torch.is_autocast_enabled("cuda"):
-            x = x.to(self.scales.dtype)
-        return _linear4(x, self.tiles, self.scales, self.zeros, self.out_features, self.in_features, self.group)
+        args = (self.tiles, self.scales, self.zeros, self.out_features, self.in_features, self.group)
+        if torch.is_autocast_enabled("cuda"):
+            return _linear4(x.to(self.scales.dtype), *args).to(torch.get_autocast_dtype("cuda"))
+        return _linear4(x, *args)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, group={self.group}"

@@ -202,6 +202,18 @@ def test_sixteen_bit_generation_runs_in_every_part(dtype):
     assert got.shape == (2, 8) and ((got >= 0) & (got < 300)).all()
 
 
+def test_a_quantized_decoder_under_autocast():
+    m = _model().quantize4_(64)
+    with torch.autocast("cuda", dtype=torch.bfloat16), torch.no_grad():
+        state = DecodeState(m, 2, 40, page=16)
+        assert state.k.dtype == torch.bfloat16
+        idx = _tokens(2, 20)
+        got = m.decode(idx, state)
+        want = m(idx)[:, -1]
+        assert got.dtype == want.dtype and (got - want).float().norm() <= 0.03 * want.float().norm()  # bf16 all the way
+        assert m.generate(idx, 3, repetition_penalty=1.2).shape == (2, 3)
+
+
 def test_a_captured_step_of_all_of_them():
     """Norm, rotation and append, attention, projections, penalties and sampling as one graph,
     replayed for tokens and lengths that change on the device."""
