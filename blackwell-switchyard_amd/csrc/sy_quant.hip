@@ -150,23 +150,28 @@ template <> struct Mma<F32> : Mma<BF16> {
 
 __device__ __forceinline__ uint32_t ror(uint32_t x, int n) { return __builtin_amdgcn_alignbit(x, x, n); }
 
-// The eight weights of a word as 1 + c / 16.
-template <class T> __device__ __forceinline__ i32x4_t codes_of(uint32_t w) {
-  constexpr uint32_t M = Mma<T>::mask, B = Mma<T>::one;
-  i32x4_t r;
-  if constexpr (T::code == F16::code) {
-    r[0] = (int)((w << 3 & M) | B);
-    r[1] = (int)((w >> 1 & M) | B);
-    r[2] = (int)((w >> 5 & M) | B);
-    r[3] = (int)((ror(w, 9) & M) | B);
-  } else {
-    r[0] = (int)((w & M) | B);
-    r[1] = (int)((w >> 4 & M) | B);
-    r[2] = (int)((w >> 8 & M) | B);
-    r[3] = (int)((ror(w, 12) & M) | B);
+// The eight weights of a word as 1 + c / 16. Mask and one are held in registers, opaque to the
+// compiler, which else takes them as literals and splits each and-or in two (2048 rows of 2048 x
+// 5632 58 us, so FUSED_US).
+template <class T> struct Codes {
+  uint32_t mask = Mma<T>::mask, one = Mma<T>::one;
+  __device__ __forceinline__ Codes() { asm("" : "+v"(mask), "+v"(one)); }
+  __device__ __forceinline__ i32x4_t operator()(uint32_t w) const {
+    i32x4_t r;
+    if constexpr (T::code == F16::code) {
+      r[0] = (int)((w << 3 & mask) | one);
+      r[1] = (int)((w >> 1 & mask) | one);
+      r[2] = (int)((w >> 5 & mask) | one);
+      r[3] = (int)((ror(w, 9) & mask) | one);
+    } else {
+      r[0] = (int)((w & mask) | one);
+      r[1] = (int)((w >> 4 & mask) | one);
+      r[2] = (int)((w >> 8 & mask) | one);
+      r[3] = (int)((ror(w, 12) & mask) | one);
+    }
+    return r;
   }
-  return r;
-}
+};
 
 // -1, or -1.5 = -(1 + 8 / 16), in every element: what the sum over x is taken against.
 template <class T, bool ZEROS> __device__ __forceinline__ i32x4_t minus() {
@@ -286,6 +291,7 @@ __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4
                    min(m0 + 16 * t + (STAGED ? 16 / kLoads * j + r0 : col), a.m - 1) * a.x_stride;
   i32x4_t* const stage = reinterpret_cast<i32x4_t*>(fold) + wave * (MT * 16 * kChunks);
   const i32x4_t neg = minus<T, ZEROS>();
+  const Codes<T> codes;
   f32x4_t tot[MT][NT];
 #pragma unroll
   for (int t = 0; t < MT; ++t)
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4
         for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? sums[t] * r.z[u][g] : sums[t];
 #pragma unroll
         for (int j = g * GS; j < (g + 1) * GS; ++j) {
-          const i32x4_t c = codes_of<T>((uint32_t)r.w[u][j]);
+          const i32x4_t c = codes((uint32_t)r.w[u][j]);
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -448,6 +454,7 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
   const int64_t n_tiles = tiles_of(a.n), m0 = (int64_t)(block / n_blocks) * kRows;
   const int64_t tile0 = ((int64_t)(block % n_blocks) * 4 + (wave & 3)) * NT;
   const int steps = (int)steps_of(a.k);
+  const Codes<T> codes;
   // A thread of a group loads four chunks of the tile: rows r0, r0 + 16, r0 + 32, r0 + 48.
   const int r0 = threadIdx.x >> 4 & 15, c0 = threadIdx.x & 15;
   const S* rows[MT];
@@ -523,7 +530,7 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
         for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? from[t] * (1.0f + (float)r.z[u].x[g] * 0.0625f) : from[t];
 #pragma unroll
         for (int j = 0; j < GS; ++j) {
-          const i32x4_t c = codes_of<T>((uint32_t)r.w[u][g * GS + j]);
+          const i32x4_t c = codes((uint32_t)r.w[u][g * GS + j]);
 #pragma unroll
           for (int t = 0; t < MT; ++t) acc[t] = Mma<T>::run(f[j][t], c, acc[t]);
         }
