@@ -151,8 +151,8 @@ template <> struct Mma<F32> : Mma<BF16> {
 __device__ __forceinline__ uint32_t ror(uint32_t x, int n) { return __builtin_amdgcn_alignbit(x, x, n); }
 
 // The eight weights of a word as 1 + c / 16. Mask and one are held in registers, opaque to the
-// compiler, which else takes them as literals and splits each and-or in two (2048 rows of 2048 x
-// 5632 58 us, so FUSED_US).
+// compiler, which else takes them as literals and splits each and-or in two (us: 2048 rows of 2048
+// x 5632 58, so 57; 32 of 11264 x 2048 8.0, so 7.6).
 template <class T> struct Codes {
   uint32_t mask = Mma<T>::mask, one = Mma<T>::one;
   __device__ __forceinline__ Codes() { asm("" : "+v"(mask), "+v"(one)); }
@@ -436,16 +436,17 @@ template <class T> __device__ __forceinline__ float sum8(const i32x4_t& x, float
 }
 
 // Many rows: a workgroup has 64 rows by 64 NT features. Four waves with NT feature tiles each
-// share a column tile of the rows in LDS, double-buffered; two such groups of waves take every
-// other column tile and add up at the end. A tile's sums over each group's columns are formed
+// share a column tile of the rows in LDS, double-buffered; with PARTS 2, two such groups of
+// waves take every other column tile and add up at the end. A tile's sums over each group's columns are formed
 // where it is written to LDS, by the lanes that hold it.
-template <class T, int NT, int GS, bool ZEROS>
-__global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
+template <class T, int NT, int PARTS, int GS, bool ZEROS>
+__global__ void __launch_bounds__(256 * PARTS) __attribute__((amdgpu_waves_per_eu(2)))
+k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
   using S = typename T::storage;
   constexpr int NG = 4 / GS, MT = 4, kRows = 16 * MT, kChunks = kRows * 16;
-  __shared__ __align__(16) i32x4_t stage[2][2][kChunks];
-  __shared__ __align__(16) float sums[2][2][NG][kRows];
-  static_assert(sizeof(stage) >= 4 * MT * NT * 1024, "the first group's sums fit");
+  __shared__ __align__(16) i32x4_t stage[PARTS][2][kChunks];
+  __shared__ __align__(16) float sums[PARTS][2][NG][kRows];
+  static_assert(PARTS == 1 || sizeof(stage) >= 4 * MT * NT * 1024, "the second group's sums fit");
   // Neighbouring blocks on one XCD: workgroups go to the eight of them in turn.
   const int per = (blocks + 7) / 8, block = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
   if ((int)(blockIdx.x / 8) >= per || block >= blocks) return;
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
     }
   };
   // Both groups go round as often; one may have nothing to add in the last round.
-  const int last = steps - 1, rounds = (steps + 1) / 2;
+  const int last = steps - 1, rounds = (steps + PARTS - 1) / PARTS;
   i32x4_t x[MT];
   Weights w, next;
   load_w(min(part, last), w);
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
   put(0, x);
   __syncthreads();
   const auto round = [&](int i, const Weights& now, Weights& then) {
-    const int step = 2 * i + part, at = min(step + 2, last);
+    const int step = PARTS * i + part, at = min(step + PARTS, last);
     load_w(at, then);
     load_x(at, x);
     if (step <= last) add(i & 1, now);
@@ -564,16 +565,18 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
   }
   // The second group's sums to the first, a lane's own.
   float* const mine = reinterpret_cast<float*>(stage) + (wave & 3) * (MT * NT * 256) + lane;
-  if (part == 1) {
+  if constexpr (PARTS == 2) {
+    if (part == 1) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[((t * NT + u) * 4 + i) * 64] = tot[t][u][i];
+          for (int i = 0; i < 4; ++i) mine[((t * NT + u) * 4 + i) * 64] = tot[t][u][i];
+    }
+    __syncthreads();
+    if (part == 1) return;
   }
-  __syncthreads();
-  if (part == 1) return;
   S* const out = static_cast<S*>(a.out);
 #pragma unroll
   for (int t = 0; t < MT; ++t)
@@ -583,11 +586,12 @@ __global__ void __launch_bounds__(512) k_linear4_many(const Linear4Args a, int n
       for (int i = 0; i < 4; ++i) {
         const int64_t m = m0 + 16 * t + 4 * quad + i, n = (tile0 + u) * 16 + col;
         if (m < a.m && n < a.n)
-          store_elem(out, m * a.n + n, 16.0f * (tot[t][u][i] + mine[((t * NT + u) * 4 + i) * 64]), T::code);
+          store_elem(out, m * a.n + n, 16.0f * (PARTS == 2 ? tot[t][u][i] + mine[((t * NT + u) * 4 + i) * 64] : tot[t][u][i]),
+                     T::code);
       }
 }
 
-template <class T, int NT, int GS, bool ZEROS>
+template <class T, int NT, int PARTS, int GS, bool ZEROS>
 hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
   const int n_blocks = (int)((tiles_of(a.n) + 4 * NT - 1) / (4 * NT));  // (at most 2^18)
   const int64_t rows = 64 * ((1 << 21) / n_blocks);  // of a launch: 2^30 threads
@@ -598,7 +602,7 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
     part.x = static_cast<const char*>(a.x) + m0 * a.x_stride * es;
     part.out = static_cast<char*>(a.out) + m0 * a.n * es;
     const int blocks = (int)((part.m + 63) / 64) * n_blocks;
-    hipLaunchKernelGGL((k_linear4_many<T, NT, GS, ZEROS>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(512), 0, s,
+    hipLaunchKernelGGL((k_linear4_many<T, NT, PARTS, GS, ZEROS>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(256 * PARTS), 0, s,
                        part, n_blocks, blocks);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -640,17 +644,28 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
 //   up to 16         through LDS, four feature tiles from 512 on. 16 rows of 2048 x 2048 3.4,
 //                    straight 4.3; of 11264 x 2048 5.8, one feature tile 10.7; of 28672 x 8192
 //                    29.6, straight 35.7, one feature tile 43.
-//   up to 32, or few blocks of 64 rows
-//                    32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
+//   up to 32         32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
 //                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
 //                    many: 28672 x 8192 38.5, without 43.
-//   else             64 rows and 64 NT features, for which a CU needs 2.7 (NT 4), 1.6 (2) or 1.3 us
-//                    (1; two at once 1.9) for two column tiles: the one that is done first on 256
-//                    CUs. 2048 rows of 2048 x 5632 59, 72, 82, and 87 as above; 128 rows of 11264 x
-//                    2048 29, 19, 24, 21; 128 of 2048 x 5632 56, 35, 26, 13 (32 to 128 workgroups).
+//   else             that, or 64 rows by 64 NT features with one or two groups of waves, whichever
+//                    the costs below say is done first. Two groups where workgroups have a CU
+//                    each, one where two of them share it and each hides the other's waits: 2048
+//                    rows of 2048 x 5632 61 (NT 4, two groups), 65 (one), 70 and 64 (NT 2), 81
+//                    (NT 1), 86 (32 rows); 4096 of 11264 x 2048 281, 237, 328 and 281, 355, 387;
+//                    128 of 11264 x 2048 29, 31, 19 and 21, 24, 20; 512 of 2048 x 5632 53, 63, 36
+//                    and 41, 27, 25.
 //   fp32 past 8      through LDS, 16 rows a workgroup, and up to four feature tiles: 16 rows of 2048
 //                    x 5632 10.4 with one, 12.4 with two, 15.6 with four, 15.1 straight; 64 of 2048
 //                    x 2048 8.3, 6.7, 7.9, 10.9; 16 of 11264 x 2048 11.9, 10.5, 8.9, 17.3.
+
+// What a workgroup of 64 rows costs a column tile, in us, on 256 CUs: `alone` where each has a CU
+// to itself, `full` where two share every CU (0: they do not).
+double many_cost(int64_t blocks, double alone, double full) {
+  if (full == 0.0) return (double)((blocks + 255) / 256) * alone;
+  const int64_t rest = blocks % 512;
+  return (double)(blocks / 512) * full + (rest > 256 ? full : rest > 0 ? alone : 0.0);
+}
+
 template <class T, int GS, bool ZEROS>
 hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
   const int64_t tiles = tiles_of(a.n);
@@ -667,12 +682,16 @@ hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
       return tiles >= 512 ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
     if (a.m > 32) {
       const auto blocks = [&](int nt) { return (a.m + 63) / 64 * ((tiles + 4 * nt - 1) / (4 * nt)); };
-      if (blocks(1) >= 160) {
-        const double t4 = 2.7 * (double)((blocks(4) + 255) / 256), t2 = 1.6 * (double)((blocks(2) + 255) / 256);
-        const int64_t rest = blocks(1) % 512;
-        const double t1 = 1.9 * (double)(blocks(1) / 512) + (rest > 256 ? 1.9 : rest > 0 ? 1.3 : 0.0);
-        if (t4 <= t2 && t4 <= t1) return run4_many<T, 4, GS, ZEROS>(a, s);
-        return t2 <= t1 ? run4_many<T, 2, GS, ZEROS>(a, s) : run4_many<T, 1, GS, ZEROS>(a, s);
+      const double rows32 = (double)((a.m + 31) / 32);
+      const double cost[] = {tiles < 512 ? 0.1 + 0.4e-3 * rows32 * (double)tiles : 0.3 + 0.21e-3 * rows32 * (double)tiles,
+                             many_cost(blocks(4), 1.38, 0.0), many_cost(blocks(4), 1.45, 2.3),
+                             many_cost(blocks(2), 0.8, 0.0), many_cost(blocks(1), 0.62, 0.93)};
+      switch (std::min_element(cost, cost + 5) - cost) {
+        case 1: return run4_many<T, 4, 2, GS, ZEROS>(a, s);
+        case 2: return run4_many<T, 4, 1, GS, ZEROS>(a, s);
+        case 3: return run4_many<T, 2, 2, GS, ZEROS>(a, s);
+        case 4: return run4_many<T, 1, 2, GS, ZEROS>(a, s);
+        default: break;
       }
     }
     if (tiles < 512) return run4<T, 2, 1, 8, true, false, GS, ZEROS>(a, s);
