@@ -636,14 +636,17 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
 }
 
 // The kernel and its tile by rows and feature tiles; us on both sides, bf16 unless stated.
-//   up to 8 rows     straight from memory: a load's lanes touch few lines. 8 rows of 32000 x 2048
-//                    8.2, through LDS 9.4. Past 1024 feature tiles four a workgroup, 1 row of
-//                    32000 x 2048 8.1, one 8.7; below one, 6144 x 2048 3.6, four 5.
-//                    fp32: two from 256 on, 1 row of 6144 x 2048 5.6, one 7.0; 5 rows of 1408 x
-//                    2048 5.6, one 5.3.
-//   up to 16         through LDS, four feature tiles from 512 on. 16 rows of 2048 x 2048 3.4,
-//                    straight 4.3; of 11264 x 2048 5.8, one feature tile 10.7; of 28672 x 8192
-//                    29.6, straight 35.7, one feature tile 43.
+//   1 and 2 rows     straight from memory, where a load's lanes touch few lines: 1 row of 6144 x
+//                    2048 3.5 (through LDS 3.6 at best), of 20000 x 2048 6.2 (7.5). Four feature
+//                    tiles a workgroup where there is much to read: 1 row of 28672 x 8192 25.6, one
+//                    33; of 20000 x 2048 7.6. Up to 8 rows of much likewise: 8 of 28672 x 8192 27.1,
+//                    through LDS 28.0.
+//                    Not for rows at odd places: 8 rows of 9055 x 3715 22, through LDS 8.5.
+//   up to 16         through LDS, one to four feature tiles: 8 rows of 2048 x 5632 4.6 with one, 5.5
+//                    with two, straight 5.7; of 6144 x 2048 4.9, 3.6, 4.7, with four 5.0; 16 of 28672
+//                    x 8192 43, 33, 35.7, 29.6. At odd places four: 8 of 9055 x 3715 10.6 with two.
+//                    fp32 up to 8 rows straight from memory, two feature tiles from 256 on: 1 row of
+//                    6144 x 2048 5.6, one 7.0; 5 of 1408 x 2048 5.6, one 5.3.
 //   up to 32         32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
 //                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
 //                    many: 28672 x 8192 38.5, without 43.
@@ -676,10 +679,15 @@ hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
     if (blocks < 256) return run4<T, 1, 1, 8, true, false, GS, ZEROS>(a, s);
     return blocks < 704 ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
   } else {
-    if (a.m <= 8)
-      return tiles >= 1024 ? run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
-    if (a.m <= 16)
-      return tiles >= 512 ? run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
+    const int64_t work = tiles * steps_of(a.k);  // tiles of weights
+    const bool even = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.x_stride * 2) % 4 == 0;
+    if (a.m <= 2 && (even || a.m == 1) && work < 40000) return run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
+    if (a.m <= 8 && even && work >= 30000) return run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s);
+    if (a.m <= 16) {
+      if (tiles < 256) return run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
+      return even && tiles < (a.m <= 8 ? 1536 : 1024) ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s)
+                                                      : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
+    }
     if (a.m > 32) {
       const auto blocks = [&](int nt) { return (a.m + 63) / 64 * ((tiles + 4 * nt - 1) / (4 * nt)); };
       const double rows32 = (double)((a.m + 31) / 32);

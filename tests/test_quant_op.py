@@ -70,7 +70,9 @@ SIZES = [(1, 16, 128), (1, 1, 1), (3, 17, 33), (16, 64, 256), (17, 100, 130), (5
          (65, 33, 2048), (130, 200, 257), (300, 70, 384), (2, 1030, 4096), (1, 16400, 128), (6, 16390, 200), (12, 80, 2300), (13, 16385, 136), (20, 8201, 300),
          (40, 8195, 150), (25, 8200, 4101), (600, 80, 200), (513, 130, 7), (9, 33, 5),
          (700, 3900, 140), (130, 10300, 260), (70, 10250, 380), (65, 2600, 5),
-         (525, 7530, 70), (340, 5530, 290), (45, 12200, 136), (41, 19200, 257)]
+         (525, 7530, 70), (340, 5530, 290), (45, 12200, 136), (41, 19200, 257),
+         (2, 100, 300), (2, 100, 301), (7, 100, 300), (8, 5000, 300), (12, 5000, 301), (6, 24600, 130), (3, 16000, 3900),
+         (5, 16000, 3901), (2, 16000, 5200)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
