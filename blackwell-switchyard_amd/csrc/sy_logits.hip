@@ -14,7 +14,6 @@ namespace {
 
 typedef uint32_t u32x2_any_t __attribute__((ext_vector_type(2), aligned(1)));
 
-constexpr int kBlock = 256;
 constexpr uint32_t kPrompt = 0x80000000u;  // of a token's count: it was in the prompt
 
 // Which of CE tokens from v on are allowed, a bit each.
@@ -55,6 +54,7 @@ __device__ __forceinline__ void lds_barrier() {
 // Eight tokens a thread of a row of `n_tokens`, from i0 on; what is no token of 31 bits is -1.
 constexpr int kAhead = 8;
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <int kBlock>
 __device__ __forceinline__ void ld_tokens(const AdjustArgs& a, int64_t row, int i0, int (&x)[kAhead]) {
   const int first = i0 + (int)threadIdx.x;
   if (a.tokens64) {
@@ -122,7 +122,7 @@ template <class T> __device__ __forceinline__ i32x4_t masked(const i32x4_t& x, u
 // 8 rows with 3808 tokens 5.5, so 7.3). Then one pass over the chunks. Those with
 // nothing allowed are not read; in place and without a bias only those are that something was
 // counted in, and all that stay as they are are not written.
-template <class T, int IT>
+template <class T, int IT, int kBlock>
 __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slices) {
   using S = typename T::storage;
   constexpr int CE = T::ce, kSlice = kBlock * CE * IT;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
     keep[k] = c < n ? allowed<CE>(a, row, lo + c, c + CE <= n) : 0u;
   }
   int ahead[kAhead];
-  if (a.tokens != nullptr) ld_tokens(a, row, 0, ahead);
+  if (a.tokens != nullptr) ld_tokens<kBlock>(a, row, 0, ahead);
   i32x4_t raw[IT];
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
     lds_barrier();
     for (int i0 = 0; i0 < len; i0 += kBlock * kAhead) {
       int next[kAhead];
-      if (i0 + kBlock * kAhead < len) ld_tokens(a, row, i0 + kBlock * kAhead, next);
+      if (i0 + kBlock * kAhead < len) ld_tokens<kBlock>(a, row, i0 + kBlock * kAhead, next);
       uint32_t before[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slice
   }
 }
 
-template <class T, int IT>
+template <class T, int IT, int kBlock>
 hipError_t adjust_it(const AdjustArgs& a, hipStream_t s) {
   constexpr int kSlice = kBlock * T::ce * IT;
   const int slices = (a.vocab + kSlice - 1) / kSlice;
@@ -262,7 +262,7 @@ hipError_t adjust_it(const AdjustArgs& a, hipStream_t s) {
     if (a.frequencies) part.frequencies += r0;
     if (a.bias) part.bias = static_cast<const char*>(a.bias) + r0 * a.bias_stride * (a.bias_f32 ? 4 : es);
     if (a.mask) part.mask = static_cast<const char*>(a.mask) + r0 * a.mask_stride * (a.mask_bytes ? 1 : 4);
-    hipLaunchKernelGGL((k_adjust<T, IT>), dim3((unsigned)(part.n_rows * slices)), dim3(kBlock),
+    hipLaunchKernelGGL((k_adjust<T, IT, kBlock>), dim3((unsigned)(part.n_rows * slices)), dim3(kBlock),
                        lds, s, part, slices);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -271,15 +271,20 @@ hipError_t adjust_it(const AdjustArgs& a, hipStream_t s) {
 }
 
 // Slices as long as leave every CU workgroups: each reads the row's whole history. Past 4096
-// tokens the counts would leave too few workgroups to a CU: 98 rows of 116414 in bf16 with 1290
-// tokens 15.9 us with slices of 8192, 13.8 with 4096.
+// tokens of a 16-bit row the counts would leave too few workgroups to a CU: 98 rows of 116414 in
+// bf16 with 1290 tokens 15.9 us with slices of 8192, 13.8 with 4096. Where rows are few and
+// histories long, 1024 threads read them faster: 8 rows of 32000 in bf16 with 2000 tokens 5.0
+// us, 4000 5.6, 14000 9.2, with 256 threads 5.0, 6.9 and 16.0; but 98 rows of 116414 with 4000
+// 27.4 and 20.5.
 template <class T>
 hipError_t adjust_t(const AdjustArgs& a, hipStream_t s) {
-  const int64_t chunks = a.n_rows * ((a.vocab + kBlock * T::ce - 1) / (kBlock * T::ce));  // workgroups of one each
+  if (a.tokens != nullptr && a.n_tokens > 2048 && a.n_rows * ((a.vocab + 1024 * T::ce - 1) / (1024 * T::ce)) <= 512)
+    return adjust_it<T, 1, 1024>(a, s);
+  const int64_t chunks = a.n_rows * ((a.vocab + 256 * T::ce - 1) / (256 * T::ce));  // workgroups of one each
   if constexpr (T::ce == 4) {
-    if (chunks >= 4096) return adjust_it<T, 4>(a, s);
+    if (chunks >= 4096) return adjust_it<T, 4, 256>(a, s);
   }
-  return chunks >= 2048 ? adjust_it<T, 2>(a, s) : adjust_it<T, 1>(a, s);
+  return chunks >= 2048 ? adjust_it<T, 2, 256>(a, s) : adjust_it<T, 1, 256>(a, s);
 }
 
 }  // namespace

@@ -91,7 +91,7 @@ def _run(x, tokens, lengths, prompts, s, **more):
         **more))
 
 
-SHAPES = [(1, 1, 1), (2, 7, 5), (3, 33, 64), (5, 1000, 300), (2, 1023, 9), (1, 1025, 2000), (4, 4097, 77), (9, 50257, 500),
+SHAPES = [(2, 5000, 9000), (1, 1, 1), (2, 7, 5), (3, 33, 64), (5, 1000, 300), (2, 1023, 9), (1, 1025, 2000), (4, 4097, 77), (9, 50257, 500),
           (130, 300, 40), (2, 131072, 3000)]
 
 
