@@ -666,7 +666,7 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
 //                    with two, straight 5.7; of 6144 x 2048 4.9, 3.6, 4.7, with four 5.0; 16 of 28672
 //                    x 8192 43, 33, 35.7, 29.6. At odd places four: 8 of 9055 x 3715 10.6 with two.
 //                    fp32 up to 8 rows straight from memory, two feature tiles from 256 on: 1 row of
-//                    6144 x 2048 5.6, one 7.0; 5 of 1408 x 2048 5.6, one 5.3.
+//                    6144 x 2048 6.0, one 7.2; 5 of 1408 x 2048 6.1, one 4.9.
 //   up to 32         32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
 //                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
 //                    many: 28672 x 8192 38.5, without 43.
@@ -678,8 +678,11 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
 //                    128 of 11264 x 2048 29, 31, 19 and 21, 24, 20; 512 of 2048 x 5632 53, 63, 36
 //                    and 41, 27, 25.
 //   fp32 past 8      through LDS, 16 rows a workgroup, and up to four feature tiles: 16 rows of 2048
-//                    x 5632 10.4 with one, 12.4 with two, 15.6 with four, 15.1 straight; 64 of 2048
-//                    x 2048 8.3, 6.7, 7.9, 10.9; 16 of 11264 x 2048 11.9, 10.5, 8.9, 17.3.
+//                    x 5632 11.2 with one, 14.2 with two, 19.7 with four, 12.6 straight; 64 of 2048
+//                    x 2048 8.7, 7.3, 9.3, 10.6; 16 of 11264 x 2048 11.6, 11.1, 10.3, 15.3. 32 rows
+//                    and four feature tiles where all CUs have work and every wave a few column
+//                    tiles: 2048 rows of 2048 x 5632 200, 16 rows 296; 512 of 2048 x 2048 26, 36;
+//                    but 128 of 2048 x 5632 38, 20, and 239 of 22848 x 704 73, 63.
 
 // What a workgroup of 64 rows costs a column tile, in us, on 256 CUs: `alone` where each has a CU
 // to itself, `full` where two share every CU (0: they do not).
@@ -696,6 +699,7 @@ hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
     if (a.m <= 8)
       return tiles >= 256 ? run4<T, 1, 2, 8, false, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
     const int64_t blocks = tiles * ((a.m + 15) / 16);
+    if (steps_of(a.k) >= 16 && tiles * ((a.m + 31) / 32) >= 4 * 256) return run4<T, 2, 4, 4, true, false, GS, ZEROS>(a, s);
     if (blocks < 256) return run4<T, 1, 1, 8, true, false, GS, ZEROS>(a, s);
     return blocks < 704 ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
   } else {

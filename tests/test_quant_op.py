@@ -71,7 +71,7 @@ def _check(x, codes, scales, zeros, group, got):
 
 
 SIZES = [(1, 16, 128), (1, 1, 1), (3, 17, 33), (16, 64, 256), (17, 100, 130), (5, 777, 1001), (33, 48, 640), (64, 130, 96),
-         (65, 33, 2048), (130, 200, 257), (300, 70, 384), (2, 1030, 4096), (1, 16400, 128), (6, 16390, 200), (12, 80, 2300), (13, 16385, 136), (20, 8201, 300),
+         (65, 33, 2048), (130, 200, 257), (300, 70, 384), (2, 1030, 4096), (1, 16400, 128), (6, 16390, 200), (12, 80, 2300), (13, 16385, 136), (20, 8201, 300), (690, 780, 2049),
          (40, 8195, 150), (25, 8200, 4101), (600, 80, 200), (513, 130, 7), (9, 33, 5),
          (700, 3900, 140), (130, 10300, 260), (70, 10250, 380), (65, 2600, 5),
          (525, 7530, 70), (340, 5530, 290), (45, 12200, 136), (41, 19200, 257),
