@@ -182,7 +182,9 @@ __global__ void __launch_bounds__(kBlock) k_append(const AppendArgs a) {
 // eps): L lanes a head, a power of two, of which the ones past it do nothing, each with two
 // chunks of VE elements that turn together; the sum of squares stays among them. `split` waves
 // share a token's heads, kAhead rounds of them on their way before the first is needed, and
-// before the token's place is known.
+// before the token's place is known. Memory bounds it: 6728 tokens of 40 heads of 64 in fp16 move
+// 70 MB in 17.2 us, 4.1 TB/s (loads after the place, 35.6); 8 single tokens of 48 heads of 128
+// take 4.1, three dependent loads.
 template <class T, int VE, int L>
 __global__ void __launch_bounds__(kBlock) k_append_norm(const AppendArgs a, int split, int first) {
   using S = typename T::storage;

@@ -121,7 +121,9 @@ template <class T> __device__ __forceinline__ i32x4_t masked(const i32x4_t& x, u
 // out in the chunks that hold them, 82 rows of 92375 in fp16 with 1290 tokens 13.9 us, so 9.7;
 // 8 rows with 3808 tokens 5.5, so 7.3). Then one pass over the chunks. Those with
 // nothing allowed are not read; in place and without a bias only those are that something was
-// counted in, and all that stay as they are are not written.
+// counted in, and all that stay as they are are not written. Memory bounds many rows: 256 of
+// 50257 in fp32 with 1500 tokens, biases and a mask 106 MB in 24.5 us, 4.3 TB/s; latency, of
+// the history above all, few: 8 of 32000 in bf16 with 4000 tokens 6.0.
 template <class T, int IT, int kBlock>
 __global__ void __launch_bounds__(kBlock) k_adjust(const AdjustArgs a, int slices) {
   using S = typename T::storage;

@@ -29,6 +29,7 @@ constexpr int kTileK = 128;
 __host__ __device__ constexpr int64_t tiles_of(int64_t n) { return (n + 15) / 16; }
 __host__ __device__ constexpr int64_t steps_of(int64_t k) { return (k + kTileK - 1) / kTileK; }
 
+// Once for a weight: 28672 x 8192 in 206 us.
 __global__ void __launch_bounds__(256) k_pack4(const PackArgs a) {
   const int64_t words = tiles_of(a.n) * steps_of(a.k) * 256;
   const int64_t row_bytes = (a.k + 1) / 2;
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(256) k_pack4(const PackArgs a) {
 // max |w| / 7, c = round(w / s) + 8 (1 to 15); with zero points s = (max - min) / 15 over a
 // range that holds zero, z = round(-min / s), c = round(w / s) + z. s is rounded to the
 // weights' type first, so the codes fit the scale that is kept; a group of zeros has s = 0.
+// Once for a weight too: 28672 x 8192 in bf16 in 360 us, 1.6 TB/s.
 template <class T, int E>
 __global__ void __launch_bounds__(256) k_quantize4(const QuantizeArgs a) {
   using S = typename T::storage;
@@ -286,7 +288,11 @@ template <class T, int MT, int NT, int NG, bool ZEROS> struct Step {
 
 // A workgroup has NT feature tiles and 16 MT rows; its waves share the columns out tile by tile
 // and fold their sums in LDS in their order. GS: 32-column pieces of a group. PIPE: a wave asks
-// for its next column tile before it works on the present one.
+// for its next column tile before it works on the present one. The weights' bytes bound it where
+// there are many: 16 rows of 28672 x 8192 29.1 us, 4.3 TB/s (its waves wait half their time, the
+// vector units work 43% of it), 1 row of 32000 x 2048 7.4, 4.6; else latency, 1 row of 6144 x
+// 2048 4.1. More waves or tiles ahead, loads past the caches and other orders of the columns
+// gained nothing there.
 template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
 __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4(const Linear4Args a) {
   using S = typename T::storage;
@@ -457,8 +463,11 @@ template <class T> __device__ __forceinline__ float sum8(const i32x4_t& x, float
 
 // Many rows: a workgroup has 64 rows by 64 NT features. Four waves with NT feature tiles each
 // share a column tile of the rows in LDS, double-buffered; with PARTS 2, two such groups of
-// waves take every other column tile and add up at the end. A tile's sums over each group's columns are formed
-// where it is written to LDS, by the lanes that hold it.
+// waves take every other column tile and add up at the end. A tile's sums over each group's
+// columns are formed where it is written to LDS, by the lanes that hold it. Vector instructions
+// bound it, next to waits: 2048 rows of 2048 x 5632 take 57 us, 815 TFLOP/s, of which they work
+// 55% (codes to numbers and scaling, a third each) and the matrix units 37%; the library's
+// product with bf16 weights 54.5.
 template <class T, int NT, int PARTS, int GS, bool ZEROS>
 __global__ void __launch_bounds__(256 * PARTS) __attribute__((amdgpu_waves_per_eu(2)))
 k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
