@@ -557,6 +557,28 @@ variable_list head_norm_forward(const Tensor& qkv, const Tensor& gq, const Tenso
   return r;
 }
 
+// Under capture, what a backward hands to nodes of a stream outside of it (those of the leaves,
+// where an eager graph of them lives) would take that stream into the capture, which ends the
+// process.
+void check_capture(const Tensor& t) {
+  const auto now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
+  const auto captures = [](hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return s != nullptr && hipStreamIsCapturing(s, &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+  };
+  if (!captures(now.stream())) return;
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.function) continue;
+    const auto other = edge.function->stream();
+    TORCH_CHECK(!other.has_value() || *other == now.unwrap() ||
+                    captures(c10::hip::HIPStreamMasqueradingAsCUDA(*other).stream()),
+                "qk_norm_rope: a backward is captured while an eager graph of the same leaves lives; drop its outputs "
+                "before the capture");
+  }
+}
+
 struct QkNormRope : torch::autograd::Function<QkNormRope> {
   static variable_list forward(AutogradContext* ctx, const Tensor& qkv_in, const Tensor& gq_in, const Tensor& gk_in,
                                const Tensor& cosv, const Tensor& sinv, int64_t kv, double eps) {
@@ -572,6 +594,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &qkv = saved[0], &gq = saved[1], &gk = saved[2];
     const c10::DeviceGuard guard(qkv.device());
+    check_capture(qkv);
     const double eps = ctx->saved_data["eps"].toDouble();
     const int64_t b = qkv.size(0), t = qkv.size(1), kv = ctx->saved_data["kv"].toInt(), h = qkv.size(2) - 2 * kv,
                   hd = qkv.size(3);

@@ -34,6 +34,9 @@ def qk_norm_rope(qkv: torch.Tensor, q_gain: torch.Tensor, k_gain: torch.Tensor, 
     ``[hd]``, of qkv's dtype or fp32; ``hd`` is a multiple of 8, at most 256. Arithmetic is fp32,
     every output and gradient rounded once; the gains' gradients are summed in a fixed order.
 
+    A backward that is captured into a graph while an eager graph of the same leaves lives is
+    refused: it would take the leaves' stream into the capture.
+
     Calls that no kernel may stand in for (tracing, transforms, tensor subclasses) run as torch
     operations on the same numbers."""
     if (_lib.ordinary(qkv, q_gain, k_gain, cos, sin) and qkv.is_cuda

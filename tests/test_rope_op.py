@@ -9,6 +9,7 @@ fp32, at most n 2^-24 of the sum of their sizes."""
 
 from __future__ import annotations
 
+import gc
 import math
 
 import pytest
@@ -245,6 +246,37 @@ def test_replays_of_a_captured_training_step():
         g.replay()
         torch.cuda.synchronize()
         for o, w in zip(held, step()):
+            assert torch.equal(o, w)
+
+
+def test_a_captured_backward_next_to_an_eager_graph_of_its_leaves_is_refused():
+    x = _rand(2, 30, 6, 32, dtype=BF, seed=1).to(DEV).requires_grad_()
+    gq, gk = ((1 + 0.3 * _rand(32, dtype=BF, seed=s)).to(DEV).requires_grad_() for s in (2, 3))
+    cos, sin = (z.to(DEV) for z in _tables(30, 32))
+
+    def step():
+        outs = qk_norm_rope(x, gq, gk, cos, sin, eps=EPS)
+        return torch.autograd.grad(outs, (x, gq, gk), [torch.ones_like(o) for o in outs])
+
+    want = step()
+    alive = qk_norm_rope(x, gq, gk, cos, sin, eps=EPS)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured while an eager graph"):
+        with torch.cuda.graph(g):
+            step()
+    torch.cuda.synchronize()
+    for o, w in zip(step(), want):
+        assert torch.equal(o, w)
+    del alive, g
+    gc.collect()  # (the exception's frames hold the refused step's)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = step()
+    for _ in range(2):
+        g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(held, want):
             assert torch.equal(o, w)
 
 
