@@ -1306,6 +1306,16 @@ int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_
     return SY_ERR_STRIDE;
   if (n_rows == 0) return SY_OK;
   if (!logits || !out || (how->mask_kind != 0 && !how->mask) || (how->n_tokens != 0 && !how->tokens)) return SY_ERR_NULL;
+  if (logits != out || (n_rows > 1 && row_stride != out_stride)) {  // in place, or apart: no third
+    const int64_t es = esize(dtype), row = vocab * es, step = row_stride * es;
+    const int64_t from = (int64_t)reinterpret_cast<uintptr_t>(logits), to = (int64_t)reinterpret_cast<uintptr_t>(out);
+    const bool meet = from < to + (n_rows - 1) * out_stride * es + row && to < from + (n_rows - 1) * step + row;
+    if (meet && (n_rows == 1 || row_stride != out_stride)) return SY_ERR_STRIDE;
+    if (meet) {
+      const int64_t off = (to - from) % step < 0 ? (to - from) % step + step : (to - from) % step;
+      if (off < row || step - off < row) return SY_ERR_STRIDE;
+    }
+  }
   AdjustArgs a{};
   a.logits = logits;
   a.out = out;

@@ -58,7 +58,8 @@ def adjust_logits(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, l
                   prompt_lengths: torch.Tensor | None = None, repetition_penalty=1.0, presence_penalty=0.0,
                   frequency_penalty=0.0, bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
-    """``logits [B, V]`` adjusted, as a new tensor or in ``out``, which may be ``logits``.
+    """``logits [B, V]`` adjusted, as a new tensor or in ``out``, which may be ``logits``
+    (and overlaps with them in no other way).
 
     ``tokens [B, L]`` (int64 or int32) is each row's history, of which the first ``lengths``
     count (int32 ``[B]``; all without it) and the first ``prompt_lengths`` (int32 ``[B]``; none

@@ -467,7 +467,7 @@ int sy_sample(const void* logits, const float* u, int64_t* tokens, const sy_samp
               int64_t vocab, int64_t row_stride, int dtype, void* stream);
 
 /* Logits [n_rows][vocab] (rows row_stride apart) before sampling, to out (rows out_stride
- * apart, which may be the logits themselves). A token among the first lengths[row] (NULL: all)
+ * apart, which may be the logits themselves but no other rows that overlap with theirs). A token among the first lengths[row] (NULL: all)
  * of the n_tokens in the row's history has x / repetition where x > 0 and x repetition
  * elsewhere, less frequency times its occurrences from prompt_lengths[row] (NULL: 0) on, less
  * presence if there are any. Then biases [vocab] (rows bias_stride apart; 0: shared) are

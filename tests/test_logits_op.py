@@ -145,6 +145,14 @@ def test_in_place_and_strided_rows(dtype):
         assert torch.equal(_run(view, tokens, lengths, prompts, s, allowed=allowed), want)
         _run(view, tokens, lengths, prompts, s, allowed=allowed, out=view)
         assert torch.equal(view, want) and (wide[:, :3] == 7).all() and (wide[:, 5004:] == 7).all()
+        halves = torch.full((6, 2, 5001), 7.0, dtype=dtype, device=DEV)  # rows between the logits'
+        halves[:, 0] = x.to(DEV)
+        _run(halves[:, 0], tokens, lengths, prompts, s, allowed=allowed, out=halves[:, 1])
+        assert torch.equal(halves[:, 0].cpu(), x) and torch.equal(halves[:, 1], want)
+        with pytest.raises(RuntimeError, match="sy_adjust"):
+            adjust_logits(wide[:, :5001], out=wide[:, 1:5002])
+        with pytest.raises(RuntimeError, match="sy_adjust"):
+            adjust_logits(wide[:5, :5001], out=wide[1:, :5001])
         turned = x.to(DEV).t().contiguous().t()
         assert torch.equal(_run(turned, tokens, lengths, prompts, s, allowed=allowed), want)
         assert torch.equal(_run(x, tokens.t().contiguous().t(), lengths, prompts, s, allowed=allowed), want)

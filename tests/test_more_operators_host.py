@@ -88,6 +88,14 @@ def test_bad_adjustments_are_refused():
     assert _adjust(n_rows=0, logits=None, out=None) == OK
 
 
+@pytest.mark.parametrize("size,dtype", [(2, BF), (4, F)])
+def test_adjusted_rows_are_in_place_or_apart(size, dtype):
+    for off, kw in [(1, {}), (299, {}), (-299, {}), (100, {}), (0, dict(out_stride=101)), (0, dict(row_stride=0)),
+                    (10, dict(n_rows=1)), (99, dict(row_stride=250, out_stride=250)),
+                    (151, dict(row_stride=250, out_stride=250)), (350, dict(row_stride=0, out_stride=200, logits=FAKE + 500 * size))]:
+        assert _adjust(out=FAKE + size * off, dtype=dtype, **kw) == STRIDE, (off, kw)
+
+
 def test_bad_4_bit_weights_are_refused():
     lib = _lib.lib()
 
