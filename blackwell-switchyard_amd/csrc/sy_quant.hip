@@ -461,20 +461,51 @@ template <class T> __device__ __forceinline__ float sum8(const i32x4_t& x, float
   return dot<T>(x, i32x4_t{one, one, one, one}, acc);
 }
 
+// 16 bytes a lane from memory to LDS, lane i's at byte `at` + 16 i of the workgroup's LDS; done
+// when vmcnt says so. The compiler does not count these loads: a wait of its own for an earlier
+// one would wait for them too.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ uint32_t lds_byte(void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)p;
+}
+
+// N bytes, 1 to 8, as they lie in memory.
+template <int N> struct Bytes {
+  uint32_t w[(N + 3) / 4];
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (N == 1) w[0] = *reinterpret_cast<const uint8_t*>(p);
+    else if constexpr (N == 2) w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else __builtin_memcpy(w, __builtin_assume_aligned(p, N), N);
+  }
+  __device__ __forceinline__ void wait() {
+#pragma unroll
+    for (uint32_t& x : w) asm volatile("" : "+v"(x));
+  }
+  __device__ __forceinline__ uint32_t half(int i) const { return w[i / 2] >> (16 * (i % 2)) & 0xffffu; }
+  __device__ __forceinline__ uint32_t byte(int i) const { return w[i / 4] >> (8 * (i % 4)) & 0xffu; }
+};
+
 // Many rows: a workgroup has 64 rows by 64 NT features. Four waves with NT feature tiles each
 // share a column tile of the rows in LDS, double-buffered; with PARTS 2, two such groups of
 // waves take every other column tile and add up at the end. A tile's sums over each group's
-// columns are formed where it is written to LDS, by the lanes that hold it. Vector instructions
-// bound it, next to waits: 2048 rows of 2048 x 5632 take 57 us, 815 TFLOP/s, of which they work
-// 55% (codes to numbers and scaling, a third each) and the matrix units 37%; the library's
-// product with bf16 weights 54.5.
-template <class T, int NT, int PARTS, int GS, bool ZEROS>
+// columns are formed where it is written to LDS, by the lanes that hold it; DIRECT: the tile goes
+// straight to LDS, for which rows start at 16-byte boundaries, and each wave takes the sums off
+// the matrix units (us: 512 rows of 2048 x 5632 27.0, so 24.6; 4096 of 11264 x 2048 229, so 219;
+// 2048 of 2048 x 5632 58.2, so 57.5). Vector instructions bound it, next to waits: the last of
+// those is 820 TFLOP/s; codes to numbers and scaling are a third of them each. The library's
+// product with bf16 weights takes 54.5.
+template <class T, int NT, int PARTS, bool DIRECT, int GS, bool ZEROS>
 __global__ void __launch_bounds__(256 * PARTS) __attribute__((amdgpu_waves_per_eu(2)))
 k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
   using S = typename T::storage;
   constexpr int NG = 4 / GS, MT = 4, kRows = 16 * MT, kChunks = kRows * 16;
   __shared__ __align__(16) i32x4_t stage[PARTS][2][kChunks];
-  __shared__ __align__(16) float sums[PARTS][2][NG][kRows];
+  __shared__ __align__(16) float sums[PARTS][2][NG][kRows];  // (not DIRECT)
   static_assert(PARTS == 1 || sizeof(stage) >= 4 * MT * NT * 1024, "the second group's sums fit");
   // Neighbouring blocks on one XCD: workgroups go to the eight of them in turn.
   const int per = (blocks + 7) / 8, block = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
@@ -498,24 +529,18 @@ k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
     s_at[u] = static_cast<const char*>(a.scales) + tile * (16 * NG * (int)sizeof(S));
     if constexpr (ZEROS) z_at[u] = reinterpret_cast<const char*>(a.zeros) + tile * (16 * NG);
   }
-  struct alignas(NG * sizeof(S)) Scales {
-    S x[NG];
-  };
-  struct alignas(NG) Zeros {
-    uint8_t x[NG];
-  };
-  struct Weights {  // as they lie in memory
+  struct Weights {
     i32x4_t w[NT];
-    Scales s[NT];
-    Zeros z[NT];
+    Bytes<NG * (int)sizeof(S)> s[NT];
+    Bytes<NG> z[NT];
   };
   const auto load_w = [&](int step, Weights& r) {
     const uint32_t cell = (uint32_t)(step * 16 + col) * NG;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       r.w[u] = *reinterpret_cast<const i32x4_t*>(w_at[u] + (uint32_t)(step * 1024 + lane * 16));
-      r.s[u] = *reinterpret_cast<const Scales*>(s_at[u] + cell * (uint32_t)sizeof(S));
-      if constexpr (ZEROS) r.z[u] = *reinterpret_cast<const Zeros*>(z_at[u] + cell);
+      r.s[u].load(s_at[u] + cell * (uint32_t)sizeof(S));
+      if constexpr (ZEROS) r.z[u].load(z_at[u] + cell);
     }
   };
   const auto load_x = [&](int step, i32x4_t (&x)[MT]) {
@@ -532,6 +557,7 @@ k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       stage[part][buffer][(r0 + 16 * i) * 16 + (c0 ^ r0)] = x[i];
+      if (DIRECT) continue;
       const float s = lane_sum<4 * GS>(sum8<T>(x[i], 0.0f)) * (ZEROS ? -1.0f : -1.5f);
       if (c0 % (4 * GS) == 0) sums[part][buffer][c0 / (4 * GS)][r0 + 16 * i] = s;
     }
@@ -548,23 +574,32 @@ k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
       i32x4_t f[GS][MT];
       f32x4_t from[MT];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) from[t] = *reinterpret_cast<const f32x4_t*>(&sums[part][buffer][g][16 * t + 4 * quad]);
+      for (int t = 0; t < MT; ++t)
+        from[t] = DIRECT ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}
+                         : *reinterpret_cast<const f32x4_t*>(&sums[part][buffer][g][16 * t + 4 * quad]);
 #pragma unroll
       for (int j = 0; j < GS; ++j)
 #pragma unroll
         for (int t = 0; t < MT; ++t) f[j][t] = at[t * 256 + ((4 * (g * GS + j) + quad) ^ col)];
+      if constexpr (DIRECT) {
+#pragma unroll
+        for (int j = 0; j < GS; ++j)
+#pragma unroll
+          for (int t = 0; t < MT; ++t) from[t] = Mma<T>::run(f[j][t], minus<T, ZEROS>(), from[t]);
+      }
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         f32x4_t acc[MT];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? from[t] * (1.0f + (float)r.z[u].x[g] * 0.0625f) : from[t];
+        for (int t = 0; t < MT; ++t) acc[t] = ZEROS ? from[t] * (1.0f + (float)r.z[u].byte(g) * 0.0625f) : from[t];
 #pragma unroll
         for (int j = 0; j < GS; ++j) {
           const i32x4_t c = codes((uint32_t)r.w[u][g * GS + j], 0.0f);
 #pragma unroll
           for (int t = 0; t < MT; ++t) acc[t] = Mma<T>::run(f[j][t], c, acc[t]);
         }
-        const float s = load_elem(r.s[u].x, g, T::code);
+        const S raw = (S)r.s[u].half(g);
+        const float s = load_elem(&raw, 0, T::code);
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -576,16 +611,49 @@ k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
   const int last = steps - 1, rounds = (steps + PARTS - 1) / PARTS;
   i32x4_t x[MT];
   Weights w, next;
+  // A column tile to LDS, straight where all of it is there.
+  const uint32_t stage_at = lds_byte(&stage[part][0][(wave & 3) * 64]);
+  const auto fill = [&](int step, int buffer) {
+    if ((step + 1) * kTileK <= a.k) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        load_to_lds(rows[i] + step * kTileK + 8 * (c0 ^ r0),
+                    __builtin_amdgcn_readfirstlane(stage_at + (buffer * kChunks + i * 256) * 16));
+    } else {
+      load_x(step, x);
+      put(buffer, x);
+    }
+  };
+  const auto landed = [&](Weights& r) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      asm volatile("" : "+v"(r.w[u]));
+      r.s[u].wait();
+      if constexpr (ZEROS) r.z[u].wait();
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
   load_w(min(part, last), w);
-  load_x(min(part, last), x);
-  put(0, x);
+  if constexpr (DIRECT) {
+    fill(min(part, last), 0);
+    landed(w);
+  } else {
+    load_x(min(part, last), x);
+    put(0, x);
+  }
   __syncthreads();
   const auto round = [&](int i, const Weights& now, Weights& then) {
     const int step = PARTS * i + part, at = min(step + PARTS, last);
     load_w(at, then);
-    load_x(at, x);
-    if (step <= last) add(i & 1, now);
-    put((i + 1) & 1, x);
+    if constexpr (DIRECT) {
+      fill(at, (i + 1) & 1);
+      if (step <= last) add(i & 1, now);
+      landed(then);
+    } else {
+      load_x(at, x);
+      if (step <= last) add(i & 1, now);
+      put((i + 1) & 1, x);
+    }
     __syncthreads();
   };
   for (int i = 0; i < rounds; i += 2) {
@@ -620,8 +688,8 @@ k_linear4_many(const Linear4Args a, int n_blocks, int blocks) {
       }
 }
 
-template <class T, int NT, int PARTS, int GS, bool ZEROS>
-hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
+template <class T, int NT, int PARTS, bool DIRECT, int GS, bool ZEROS>
+hipError_t run4_direct(const Linear4Args& a, hipStream_t s) {
   const int n_blocks = (int)((tiles_of(a.n) + 4 * NT - 1) / (4 * NT));  // (at most 2^18)
   const int64_t rows = 64 * ((1 << 21) / n_blocks);  // of a launch: 2^30 threads
   for (int64_t m0 = 0; m0 < a.m; m0 += rows) {
@@ -631,7 +699,7 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
     part.x = static_cast<const char*>(a.x) + m0 * a.x_stride * es;
     part.out = static_cast<char*>(a.out) + m0 * a.n * es;
     const int blocks = (int)((part.m + 63) / 64) * n_blocks;
-    hipLaunchKernelGGL((k_linear4_many<T, NT, PARTS, GS, ZEROS>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(256 * PARTS), 0, s,
+    hipLaunchKernelGGL((k_linear4_many<T, NT, PARTS, DIRECT, GS, ZEROS>), dim3((unsigned)(blocks + 7) / 8 * 8), dim3(256 * PARTS), 0, s,
                        part, n_blocks, blocks);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -662,6 +730,12 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
+}
+
+template <class T, int NT, int PARTS, int GS, bool ZEROS>
+hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
+  const bool direct = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0;
+  return direct ? run4_direct<T, NT, PARTS, true, GS, ZEROS>(a, s) : run4_direct<T, NT, PARTS, false, GS, ZEROS>(a, s);
 }
 
 // The kernel and its tile by rows and feature tiles; us on both sides, bf16 unless stated.

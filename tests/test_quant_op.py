@@ -73,7 +73,8 @@ def _check(x, codes, scales, zeros, group, got):
 SIZES = [(1, 16, 128), (1, 1, 1), (3, 17, 33), (16, 64, 256), (17, 100, 130), (5, 777, 1001), (33, 48, 640), (64, 130, 96),
          (65, 33, 2048), (130, 200, 257), (300, 70, 384), (2, 1030, 4096), (1, 16400, 128), (6, 16390, 200), (12, 80, 2300), (13, 16385, 136), (20, 8201, 300), (690, 780, 2049),
          (40, 8195, 150), (25, 8200, 4101), (600, 80, 200), (513, 130, 7), (9, 33, 5),
-         (700, 3900, 140), (130, 10300, 260), (70, 10250, 380), (65, 2600, 5),
+         (700, 3900, 140), (130, 10300, 260), (70, 10250, 380), (65, 2600, 5), (700, 3900, 144), (130, 10300, 264),
+         (70, 10250, 384), (340, 5530, 1000), (525, 7530, 8), (512, 2048, 1104), (1030, 5000, 520),
          (525, 7530, 70), (340, 5530, 290), (45, 12200, 136), (41, 19200, 257),
          (2, 100, 300), (2, 100, 301), (7, 100, 300), (8, 5000, 300), (12, 5000, 301), (6, 24600, 130), (3, 16000, 3900),
          (5, 16000, 3901), (2, 16000, 5200)]
@@ -128,6 +129,13 @@ def test_rows_of_any_shape_start_and_stride():
     assert torch.equal(linear4(x.to(DEV).view(2, 3, 130), w), want.view(2, 3, 40))
     assert torch.equal(linear4(x.to(DEV)[:1].expand(4, 130), w), want[:1].expand(4, 40))
     assert torch.equal(linear4(x.to(DEV)[0], w), want[0])
+    codes, packed, scales, z = _codes(6000, 264, 32, BF, True, seed=8)  # rows that go straight to LDS, or do not
+    many = Weight4.from_codes(packed.to(DEV), scales.to(DEV), z.to(DEV), in_features=264, group=32)
+    y = torch.randn(300, 264, generator=_gen(9)).to(BF)
+    for start in (8, 7, 10):
+        at = torch.full((300, 280), float("nan"), dtype=BF)
+        at[:, start:start + 264] = y
+        _check(y, codes, scales, z, 32, linear4(at.to(DEV)[:, start:start + 264], many))
     assert linear4(x.to(DEV)[:0], w).shape == (0, 40)
     assert linear4(torch.empty(3, 0, 130, dtype=BF, device=DEV), w).shape == (3, 0, 40)
 
