@@ -292,9 +292,11 @@ template <class T, int MT, int NT, int NG, bool ZEROS> struct Step {
 // there are many: 16 rows of 28672 x 8192 29.1 us, 4.3 TB/s (its waves wait half their time, the
 // vector units work 43% of it), 1 row of 32000 x 2048 7.4, 4.6; else latency, 1 row of 6144 x
 // 2048 4.1. More waves or tiles ahead, loads past the caches and other orders of the columns
-// gained nothing there.
+// gained nothing there. (32 rows by 64 features are bound to two waves a SIMD: with the registers
+// of three the compiler asks for less at a time, 32 rows of 28672 x 8192 58 us for 42.)
 template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
-__global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES) k_linear4(const Linear4Args a) {
+__global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES)
+__attribute__((amdgpu_waves_per_eu(WAVES < 16 ? 2 : 4, MT * NT == 8 ? 2 : 8))) k_linear4(const Linear4Args a) {
   using S = typename T::storage;
   constexpr int P = Mma<T>::planes, NG = 4 / GS;
   extern __shared__ float fold[];
@@ -750,16 +752,14 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
 //                    x 8192 43, 33, 35.7, 29.6. At odd places four: 8 of 9055 x 3715 10.6 with two.
 //                    fp32 up to 8 rows straight from memory, two feature tiles from 256 on: 1 row of
 //                    6144 x 2048 6.0, one 7.2; 5 of 1408 x 2048 6.1, one 4.9.
-//   up to 32         32 rows a workgroup, four feature tiles from 512 on: 32 rows of 11264 x 2048
-//                    7.8, one 9.3; of 2048 x 5632 12, one 7.1. Column tiles ahead where a wave has
-//                    many: 28672 x 8192 38.5, without 43.
-//   else             that, or 64 rows by 64 NT features with one or two groups of waves, whichever
-//                    the costs below say is done first. Two groups where workgroups have a CU
-//                    each, one where two of them share it and each hides the other's waits: 2048
-//                    rows of 2048 x 5632 61 (NT 4, two groups), 65 (one), 70 and 64 (NT 2), 81
-//                    (NT 1), 86 (32 rows); 4096 of 11264 x 2048 281, 237, 328 and 281, 355, 387;
-//                    128 of 11264 x 2048 29, 31, 19 and 21, 24, 20; 512 of 2048 x 5632 53, 63, 36
-//                    and 41, 27, 25.
+//   more             16 or 32 rows a workgroup through LDS, or 64 with one or two groups of waves,
+//                    whichever the costs below say is done first. In their order: 32 rows of 2048 x
+//                    5632 5.1, 6.2, 7.9, 10.5, of the last four 21 at best; 24 of 28672 x 8192 79,
+//                    49, 49, 39, 54 at best; 128 of 6144 x 2048 23, 12.2, 12.4, 13.8, 22.3, 23.4,
+//                    15.1, 11.3; 256 of 11264 x 2048 73, 36, 40, 36, 24.2, 24.2, 27.3, 25.0; 2048 of
+//                    2048 x 5632 57.5, 62.1, 68.8 and 81.2 with the last four. Of 207 shapes (17 to
+//                    1400 rows, 300 to 30000 features, 200 to 9000 columns, groups of 64 and 128)
+//                    the choice takes 2% longer than the best on average, 38% at most.
 //   fp32 past 8      through LDS, 16 rows a workgroup, and up to four feature tiles: 16 rows of 2048
 //                    x 5632 11.2 with one, 14.2 with two, 19.7 with four, 12.6 straight; 64 of 2048
 //                    x 2048 8.7, 7.3, 9.3, 10.6; 16 of 11264 x 2048 11.6, 11.1, 10.3, 15.3. 32 rows
@@ -767,13 +767,20 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
 //                    tiles: 2048 rows of 2048 x 5632 200, 16 rows 296; 512 of 2048 x 2048 26, 36;
 //                    but 128 of 2048 x 5632 38, 20, and 239 of 22848 x 704 73, 63.
 
-// What a workgroup of 64 rows costs a column tile, in us, on 256 CUs: `alone` where each has a CU
-// to itself, `full` where two share every CU (0: they do not).
-double many_cost(int64_t blocks, double alone, double full) {
-  if (full == 0.0) return (double)((blocks + 255) / 256) * alone;
-  const int64_t rest = blocks % 512;
-  return (double)(blocks / 512) * full + (rest > 256 ? full : rest > 0 ? alone : 0.0);
-}
+// A launch's time in us, fitted to those shapes on 256 CUs: base + step (column tiles + more) for
+// each round of up to 512 workgroups that fill the CUs twice over; the last counts as 1 / full of
+// that if there are 256 in it or fewer.
+struct Cost {
+  int rows, tiles;  // of a workgroup
+  double base, step, more, full;
+  double of(int64_t m, int64_t n_tiles, int64_t steps) const {
+    const int64_t blocks = (m + rows - 1) / rows * ((n_tiles + tiles - 1) / tiles), rest = blocks % 512;
+    return base + step * ((double)steps + more) * ((double)(blocks / 512) * full + (rest > 256 ? full : rest > 0 ? 1.0 : 0.0));
+  }
+};
+constexpr Cost kCosts[] = {{16, 1, 3.0, 0.056, 1.0, 3.2}, {16, 2, 2.8, 0.099, 4.0, 1.8}, {16, 4, 3.4, 0.14, 4.0, 2.3},
+                           {32, 4, 3.1, 0.20, 9.0, 2.3},  {64, 16, 0.5, 1.1, 7.0, 2.1},  {64, 16, 4.0, 1.2, 3.0, 1.7},
+                           {64, 8, 0.5, 0.69, 8.0, 1.9},  {64, 4, 2.5, 0.45, 6.0, 1.8}};
 
 template <class T, int GS, bool ZEROS>
 hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
@@ -795,22 +802,22 @@ hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
       return even && tiles < (a.m <= 8 ? 1536 : 1024) ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s)
                                                       : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
     }
-    if (a.m > 32) {
-      const auto blocks = [&](int nt) { return (a.m + 63) / 64 * ((tiles + 4 * nt - 1) / (4 * nt)); };
-      const double rows32 = (double)((a.m + 31) / 32);
-      const double cost[] = {tiles < 512 ? 0.1 + 0.4e-3 * rows32 * (double)tiles : 0.3 + 0.21e-3 * rows32 * (double)tiles,
-                             many_cost(blocks(4), 1.38, 0.0), many_cost(blocks(4), 1.45, 2.3),
-                             many_cost(blocks(2), 0.8, 0.0), many_cost(blocks(1), 0.62, 0.93)};
-      switch (std::min_element(cost, cost + 5) - cost) {
-        case 1: return run4_many<T, 4, 2, GS, ZEROS>(a, s);
-        case 2: return run4_many<T, 4, 1, GS, ZEROS>(a, s);
-        case 3: return run4_many<T, 2, 2, GS, ZEROS>(a, s);
-        case 4: return run4_many<T, 1, 2, GS, ZEROS>(a, s);
-        default: break;
-      }
+    int best = 0;
+    double least = 0.0;
+    for (int i = 0; i < 8; ++i) {
+      const double us = kCosts[i].of(a.m, tiles, steps_of(a.k));
+      if (i == 0 || us < least) best = i, least = us;
     }
-    if (tiles < 512) return run4<T, 2, 1, 8, true, false, GS, ZEROS>(a, s);
-    return a.k < 4096 ? run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s) : run4<T, 2, 4, 4, true, true, GS, ZEROS>(a, s);
+    switch (best) {
+      case 0: return run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
+      case 1: return run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s);
+      case 2: return run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
+      case 3: return run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s);
+      case 4: return run4_many<T, 4, 2, GS, ZEROS>(a, s);
+      case 5: return run4_many<T, 4, 1, GS, ZEROS>(a, s);
+      case 6: return run4_many<T, 2, 2, GS, ZEROS>(a, s);
+      default: return run4_many<T, 1, 2, GS, ZEROS>(a, s);
+    }
   }
 }
 
