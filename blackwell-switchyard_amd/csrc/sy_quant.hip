@@ -287,14 +287,13 @@ template <class T, int MT, int NT, int NG, bool ZEROS> struct Step {
 };
 
 // A workgroup has NT feature tiles and 16 MT rows; its waves share the columns out tile by tile
-// and fold their sums in LDS in their order. GS: 32-column pieces of a group. PIPE: a wave asks
-// for its next column tile before it works on the present one. The weights' bytes bound it where
+// and fold their sums in LDS in their order. GS: 32-column pieces of a group. The weights' bytes bound it where
 // there are many: 16 rows of 28672 x 8192 29.1 us, 4.3 TB/s (its waves wait half their time, the
-// vector units work 43% of it), 1 row of 32000 x 2048 7.4, 4.6; else latency, 1 row of 6144 x
+// vector units work 43% of it), 8 rows of 32000 x 2048 8.0, 4.3; else latency, 1 row of 6144 x
 // 2048 4.1. More waves or tiles ahead, loads past the caches and other orders of the columns
 // gained nothing there. (32 rows by 64 features are bound to two waves a SIMD: with the registers
 // of three the compiler asks for less at a time, 32 rows of 28672 x 8192 58 us for 42.)
-template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
+template <class T, int MT, int NT, int WAVES, bool STAGED, int GS, bool ZEROS>
 __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES)
 __attribute__((amdgpu_waves_per_eu(WAVES < 16 ? 2 : 4, MT * NT == 8 ? 2 : 8))) k_linear4(const Linear4Args a) {
   using S = typename T::storage;
@@ -411,28 +410,12 @@ __attribute__((amdgpu_waves_per_eu(WAVES < 16 ? 2 : 4, MT * NT == 8 ? 2 : 8))) k
       }
     }
   };
-  // Whole tiles, with the next one's loads on their way where a wave has several (asked for
-  // again behind the last: a branch around loads would wait for all of them); then the rest.
+  // Whole tiles, then the rest.
   const int full = a.k / kTileK;
   Tile r;
-  if constexpr (PIPE) {
-    Tile next;
-    int step = wave;
-    if (step < full) load(step, r, std::true_type{});
-    while (step < full) {
-      load(min(step + waves, full - 1), next, std::true_type{});
-      add(r);
-      step += waves;
-      if (step >= full) break;
-      load(min(step + waves, full - 1), r, std::true_type{});
-      add(next);
-      step += waves;
-    }
-  } else {
-    for (int step = wave; step < full; step += waves) {
-      load(step, r, std::true_type{});
-      add(r);
-    }
+  for (int step = wave; step < full; step += waves) {
+    load(step, r, std::true_type{});
+    add(r);
   }
   if (full < steps && full % waves == wave) {
     load(full, r, std::false_type{});
@@ -709,7 +692,7 @@ hipError_t run4_direct(const Linear4Args& a, hipStream_t s) {
   return hipSuccess;
 }
 
-template <class T, int MT, int NT, int WAVES, bool STAGED, bool PIPE, int GS, bool ZEROS>
+template <class T, int MT, int NT, int WAVES, bool STAGED, int GS, bool ZEROS>
 hipError_t run4(const Linear4Args& a, hipStream_t s) {
   const int steps = (int)steps_of(a.k);
   int waves = WAVES;
@@ -726,7 +709,7 @@ hipError_t run4(const Linear4Args& a, hipStream_t s) {
     part.x = static_cast<const char*>(a.x) + m0 * a.x_stride * es;
     part.out = static_cast<char*>(a.out) + m0 * a.n * es;
     const unsigned gy = (unsigned)((part.m + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((k_linear4<T, MT, NT, WAVES, STAGED, PIPE, GS, ZEROS>), dim3(gx, gy), dim3(64 * waves), lds, s,
+    hipLaunchKernelGGL((k_linear4<T, MT, NT, WAVES, STAGED, GS, ZEROS>), dim3(gx, gy), dim3(64 * waves), lds, s,
                        part);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -741,15 +724,14 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
 }
 
 // The kernel and its tile by rows and feature tiles; us on both sides, bf16 unless stated.
-//   1 and 2 rows     straight from memory, where a load's lanes touch few lines: 1 row of 6144 x
-//                    2048 3.5 (through LDS 3.6 at best), of 20000 x 2048 6.2 (7.5). Four feature
-//                    tiles a workgroup where there is much to read: 1 row of 28672 x 8192 25.6, one
-//                    33; of 20000 x 2048 7.6. Up to 8 rows of much likewise: 8 of 28672 x 8192 27.1,
-//                    through LDS 28.0.
-//                    Not for rows at odd places: 8 rows of 9055 x 3715 22, through LDS 8.5.
-//   up to 16         through LDS, one to four feature tiles: 8 rows of 2048 x 5632 4.6 with one, 5.5
-//                    with two, straight 5.7; of 6144 x 2048 4.9, 3.6, 4.7, with four 5.0; 16 of 28672
-//                    x 8192 43, 33, 35.7, 29.6. At odd places four: 8 of 9055 x 3715 10.6 with two.
+//   up to 16         straight from memory with one or two feature tiles, where a load's lanes touch
+//                    few lines, or through LDS with one, two or four, by the costs below. In their
+//                    order: 1 row of 6144 x 2048 3.5, 3.6, and 4.0 at best through LDS; 8 of 2048 x
+//                    5632 5.7, 7.0, 4.6, 5.5, 7.8; of 32000 x 2048 12.4, 8.9, 15.7, 9.4, 10.5; 16 of
+//                    28672 x 8192 56, 41, 49, 32.7, 29.5; 9 of 17951 x 1092 6.4, 5.1, 7.5, 7.4, 8.8.
+//                    Of 296 shapes the choice takes 3% longer than the best on average, 43% at most.
+//                    More than one row at odd places goes through LDS: 8 rows of 9055 x 3715 8.5,
+//                    straight 22.
 //                    fp32 up to 8 rows straight from memory, two feature tiles from 256 on: 1 row of
 //                    6144 x 2048 6.0, one 7.2; 5 of 1408 x 2048 6.1, one 4.9.
 //   more             16 or 32 rows a workgroup through LDS, or 64 with one or two groups of waves,
@@ -769,50 +751,67 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
 
 // A launch's time in us, fitted to those shapes on 256 CUs: base + step (column tiles + more) for
 // each round of up to 512 workgroups that fill the CUs twice over; the last counts as 1 / full of
-// that if there are 256 in it or fewer.
+// that if there are 256 in it or fewer. Up to 16 rows the smaller workgroups fill in evenly, and
+// each row adds its part of a step.
 struct Cost {
   int rows, tiles;  // of a workgroup
-  double base, step, more, full;
-  double of(int64_t m, int64_t n_tiles, int64_t steps) const {
+  double base, step, more, full, row;
+  double of(int64_t m, int64_t n_tiles, int steps) const {
     const int64_t blocks = (m + rows - 1) / rows * ((n_tiles + tiles - 1) / tiles), rest = blocks % 512;
-    return base + step * ((double)steps + more) * ((double)(blocks / 512) * full + (rest > 256 ? full : rest > 0 ? 1.0 : 0.0));
+    return base + step * (steps + more) * ((double)(blocks / 512) * full + (rest > 256 ? full : rest > 0 ? 1.0 : 0.0));
+  }
+  double few(int64_t m, int64_t n_tiles, int steps) const {
+    const int64_t blocks = (n_tiles + tiles - 1) / tiles;
+    return base + step * (steps + more) * (1.0 + row * (double)m) *
+                      (blocks <= 256 ? 1.0 : 1.0 + (full - 1.0) * (double)(blocks - 256) / 256.0);
   }
 };
-constexpr Cost kCosts[] = {{16, 1, 3.0, 0.056, 1.0, 3.2}, {16, 2, 2.8, 0.099, 4.0, 1.8}, {16, 4, 3.4, 0.14, 4.0, 2.3},
-                           {32, 4, 3.1, 0.20, 9.0, 2.3},  {64, 16, 0.5, 1.1, 7.0, 2.1},  {64, 16, 4.0, 1.2, 3.0, 1.7},
-                           {64, 8, 0.5, 0.69, 8.0, 1.9},  {64, 4, 2.5, 0.45, 6.0, 1.8}};
+constexpr Cost kCosts[] = {{16, 1, 3.0, 0.056, 1.0, 3.2, 0.0}, {16, 2, 2.8, 0.099, 4.0, 1.8, 0.0},
+                           {16, 4, 3.4, 0.14, 4.0, 2.3, 0.0},  {32, 4, 3.1, 0.20, 9.0, 2.3, 0.0},
+                           {64, 16, 0.5, 1.1, 7.0, 2.1, 0.0},  {64, 16, 4.0, 1.2, 3.0, 1.7, 0.0},
+                           {64, 8, 0.5, 0.69, 8.0, 1.9, 0.0},  {64, 4, 2.5, 0.45, 6.0, 1.8, 0.0}};
+// Two that take rows straight from memory, three through LDS.
+constexpr Cost kFewCosts[] = {{16, 1, 2.6, 0.039, 0.0, 2.3, 0.085}, {16, 2, 2.4, 0.085, 2.0, 2.0, 0.036},
+                              {16, 1, 3.1, 0.041, 0.0, 3.2, 0.012}, {16, 2, 2.6, 0.096, 3.0, 2.1, 0.011},
+                              {16, 4, 3.4, 0.13, 3.0, 3.3, 0.007}};
+template <class F>
+int cheapest(const Cost* costs, int from, int to, const F& us) {
+  int best = from;
+  double least = us(costs[from]);
+  for (int i = from + 1; i < to; ++i) {
+    const double x = us(costs[i]);
+    if (x < least) best = i, least = x;
+  }
+  return best;
+}
 
 template <class T, int GS, bool ZEROS>
 hipError_t linear4_m(const Linear4Args& a, hipStream_t s) {
   const int64_t tiles = tiles_of(a.n);
   if constexpr (T::code == F32::code) {
     if (a.m <= 8)
-      return tiles >= 256 ? run4<T, 1, 2, 8, false, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
+      return tiles >= 256 ? run4<T, 1, 2, 8, false, GS, ZEROS>(a, s) : run4<T, 1, 1, 8, false, GS, ZEROS>(a, s);
     const int64_t blocks = tiles * ((a.m + 15) / 16);
-    if (steps_of(a.k) >= 16 && tiles * ((a.m + 31) / 32) >= 4 * 256) return run4<T, 2, 4, 4, true, false, GS, ZEROS>(a, s);
-    if (blocks < 256) return run4<T, 1, 1, 8, true, false, GS, ZEROS>(a, s);
-    return blocks < 704 ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s) : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
+    if (steps_of(a.k) >= 16 && tiles * ((a.m + 31) / 32) >= 4 * 256) return run4<T, 2, 4, 4, true, GS, ZEROS>(a, s);
+    if (blocks < 256) return run4<T, 1, 1, 8, true, GS, ZEROS>(a, s);
+    return blocks < 704 ? run4<T, 1, 2, 8, true, GS, ZEROS>(a, s) : run4<T, 1, 4, 8, true, GS, ZEROS>(a, s);
   } else {
-    const int64_t work = tiles * steps_of(a.k);  // tiles of weights
-    const bool even = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.x_stride * 2) % 4 == 0;
-    if (a.m <= 2 && (even || a.m == 1) && work < 40000) return run4<T, 1, 1, 8, false, false, GS, ZEROS>(a, s);
-    if (a.m <= 8 && even && work >= 30000) return run4<T, 1, 4, 8, false, true, GS, ZEROS>(a, s);
+    const int steps = (int)steps_of(a.k);
     if (a.m <= 16) {
-      if (tiles < 256) return run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
-      return even && tiles < (a.m <= 8 ? 1536 : 1024) ? run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s)
-                                                      : run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
+      const bool even = (reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)a.x_stride * 2) % 4 == 0;
+      switch (cheapest(kFewCosts, a.m == 1 || even ? 0 : 2, 5, [&](const Cost& c) { return c.few(a.m, tiles, steps); })) {
+        case 0: return run4<T, 1, 1, 8, false, GS, ZEROS>(a, s);
+        case 1: return run4<T, 1, 2, 8, false, GS, ZEROS>(a, s);
+        case 2: return run4<T, 1, 1, 16, true, GS, ZEROS>(a, s);
+        case 3: return run4<T, 1, 2, 8, true, GS, ZEROS>(a, s);
+        default: return run4<T, 1, 4, 8, true, GS, ZEROS>(a, s);
+      }
     }
-    int best = 0;
-    double least = 0.0;
-    for (int i = 0; i < 8; ++i) {
-      const double us = kCosts[i].of(a.m, tiles, steps_of(a.k));
-      if (i == 0 || us < least) best = i, least = us;
-    }
-    switch (best) {
-      case 0: return run4<T, 1, 1, 16, true, false, GS, ZEROS>(a, s);
-      case 1: return run4<T, 1, 2, 8, true, false, GS, ZEROS>(a, s);
-      case 2: return run4<T, 1, 4, 8, true, false, GS, ZEROS>(a, s);
-      case 3: return run4<T, 2, 4, 8, true, false, GS, ZEROS>(a, s);
+    switch (cheapest(kCosts, 0, 8, [&](const Cost& c) { return c.of(a.m, tiles, steps); })) {
+      case 0: return run4<T, 1, 1, 16, true, GS, ZEROS>(a, s);
+      case 1: return run4<T, 1, 2, 8, true, GS, ZEROS>(a, s);
+      case 2: return run4<T, 1, 4, 8, true, GS, ZEROS>(a, s);
+      case 3: return run4<T, 2, 4, 8, true, GS, ZEROS>(a, s);
       case 4: return run4_many<T, 4, 2, GS, ZEROS>(a, s);
       case 5: return run4_many<T, 4, 1, GS, ZEROS>(a, s);
       case 6: return run4_many<T, 2, 2, GS, ZEROS>(a, s);

@@ -75,7 +75,7 @@ SIZES = [(1, 16, 128), (1, 1, 1), (3, 17, 33), (16, 64, 256), (17, 100, 130), (5
          (40, 8195, 150), (25, 8200, 4101), (600, 80, 200), (513, 130, 7), (9, 33, 5),
          (700, 3900, 140), (130, 10300, 260), (70, 10250, 380), (65, 2600, 5), (700, 3900, 144), (130, 10300, 264),
          (70, 10250, 384), (340, 5530, 1000), (340, 5530, 1001), (525, 7530, 8), (512, 2048, 1104), (178, 5187, 103),
-         (1030, 5000, 520), (18, 4213, 1458), (49, 6261, 560),
+         (1030, 5000, 520), (18, 4213, 1458), (49, 6261, 560), (15, 20100, 1002),
          (525, 7530, 70), (340, 5530, 290), (45, 12200, 136), (41, 19200, 257),
          (2, 100, 300), (2, 100, 301), (7, 100, 300), (8, 5000, 300), (12, 5000, 301), (6, 24600, 130), (3, 16000, 3900),
          (5, 16000, 3901), (2, 16000, 5200)]
