@@ -289,9 +289,9 @@ template <class T, int MT, int NT, int NG, bool ZEROS> struct Step {
 // A workgroup has NT feature tiles and 16 MT rows; its waves share the columns out tile by tile
 // and fold their sums in LDS in their order. GS: 32-column pieces of a group. The weights' bytes bound it where
 // there are many: 16 rows of 28672 x 8192 29.1 us, 4.3 TB/s (its waves wait half their time, the
-// vector units work 43% of it), 8 rows of 32000 x 2048 8.0, 4.3; else latency, 1 row of 6144 x
-// 2048 4.1. More waves or tiles ahead, loads past the caches and other orders of the columns
-// gained nothing there. (32 rows by 64 features are bound to two waves a SIMD: with the registers
+// vector units work 43% of it), 8 rows of 32000 x 2048 8.2, 4.2; else latency, 1 row of 6144 x
+// 2048 4.1. More waves, a wave's next tile asked for ahead, loads past the caches and other orders
+// of the columns gained nothing over all shapes. (32 rows by 64 features are bound to two waves a SIMD: with the registers
 // of three the compiler asks for less at a time, 32 rows of 28672 x 8192 58 us for 42.)
 template <class T, int MT, int NT, int WAVES, bool STAGED, int GS, bool ZEROS>
 __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES)
