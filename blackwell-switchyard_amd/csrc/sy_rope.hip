@@ -105,8 +105,9 @@ __global__ void __launch_bounds__(kBlock) k_head_norm(const HeadNormArgs a) {
           }
         }
         if constexpr (kTurned) {
-          const float r = head_rinv<VE, L>(u[0], u[1], inv_hd, a.eps);
+          float r = head_rinv<VE, L>(u[0], u[1], inv_hd, a.eps);
           if constexpr (BWD) {
+            if (!live) r = 0.0f;  // (without eps the root of nothing is infinite, and dg takes every slot's)
             float c = 0.0f;
 #pragma unroll
             for (int e = 0; e < VE; ++e) turn(y[0][e], y[1][e], co[e], -si[e]);

@@ -378,3 +378,12 @@ def test_rows_of_no_sequence_stay():
     out = torch.full((6, 2, hd), 9.0, device=DEV)
     paged_append(x, cos, sin, k, v, table, n, starts, q_gain=g, k_gain=g, out=out)
     assert (out[[0, 4, 5]] == 9).all() and torch.equal(out[1:4], q[1:4])
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 8), (1, 3, 4, 2, 64), (1, 17, 5, 1, 72), (2, 9, 3, 3, 80), (1, 1, 2, 1, 128),
+                                   (2, 130, 2, 2, 64)], ids=str)
+@pytest.mark.parametrize("dtype,gains", [(BF, BF), (HF, F), (F, F)])
+def test_an_eps_of_zero(shape, dtype, gains, monkeypatch):
+    """Places behind the last token hold no head: nothing of theirs is in the gains' gradients."""
+    monkeypatch.setitem(globals(), "EPS", 0.0)  # (the oracle's and the calls' alike)
+    test_forward_and_backward(shape, dtype, gains)
