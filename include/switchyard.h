@@ -505,7 +505,8 @@ int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_
  *
  * codes are [n][(k + 1) / 2] bytes of two columns, the even one in the low half; scales and
  * zeros [n][ceil(k / group)]. sy_quantize4 makes them from weights [n][k] (rows row_stride
- * apart): symmetric, codes 1 to 15, without zeros; over the range of each group with them.
+ * apart): symmetric, codes 1 to 15, without zeros; over the range of each group with them. A
+ * group with an infinity or NaN has the scale NaN.
  * sy_pack4 lays them out for sy_linear4: tiles of 1024 bytes for 16 features by 128 columns,
  * ceil(n / 16) ceil(k / 128) of them, tile_scales and tile_zeros [ceil(n / 16)][ceil(k / 128)]
  * [16][128 / group]; tiles and tile_scales start at 16-byte boundaries, tile_zeros at 4-byte

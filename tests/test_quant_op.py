@@ -238,3 +238,29 @@ def test_the_python_path_gives_the_same(monkeypatch):
     want = linear4(x, w)
     monkeypatch.setattr(_lib, "ordinary", lambda *t: False)
     assert torch.equal(linear4(x, w), want) and torch.equal(linear4(x.t().contiguous().t(), w), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_weights_that_are_no_numbers_show(group, symmetric, dtype):
+    """A group with one is NaN: in its scale, its weights and the products; the others are as without it."""
+    n, k = 40, 300
+    w = torch.randn(n, k, generator=_gen(1)).to(dtype)
+    bad = w.clone()
+    bad[1, 70], bad[2, 130], bad[3, 299] = math.nan, math.inf, -math.inf
+    bad[4, :group], bad[5, 9], bad[5, 11] = math.nan, math.inf, -math.inf
+    hit = torch.zeros(n, -(-k // group), dtype=torch.bool)
+    for row, col in ((1, 70), (2, 130), (3, 299), (4, 0), (5, 9)):
+        hit[row, col // group] = True
+    q, p = quantize4(bad.to(DEV), group, symmetric=symmetric), quantize4(w.to(DEV), group, symmetric=symmetric)
+    of = torch.arange(k) // group
+    (c, s, z), (wc, ws, wz) = q.codes(), p.codes()
+    assert torch.equal(s.isnan().cpu(), hit) and torch.equal(s[~hit.to(DEV)], ws[~hit.to(DEV)])
+    assert torch.equal(c.cpu()[~hit[:, of]], wc.cpu()[~hit[:, of]])
+    assert z is None or torch.equal(z.cpu()[~hit], wz.cpu()[~hit])
+    assert torch.equal(q.dequantize().isnan().cpu(), hit[:, of])
+    for m in (3, 20, 300):
+        x = torch.randn(m, k, generator=_gen(m)).to(dtype).to(DEV)
+        got, want = linear4(x, q), linear4(x, p)
+        assert got[:, 1:6].isnan().all() and torch.equal(got[:, 6:], want[:, 6:]) and torch.equal(got[:, 0], want[:, 0])
