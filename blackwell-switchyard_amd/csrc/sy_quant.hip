@@ -70,8 +70,10 @@ __global__ void __launch_bounds__(256) k_pack4(const PackArgs a) {
 // Rounding to codes: sixteen lanes a group, each with group / 16 neighbours. Symmetric: s =
 // max |w| / 7, c = round(w / s) + 8 (1 to 15); with zero points s = (max - min) / 15 over a
 // range that holds zero, z = round(-min / s), c = round(w / s) + z. s is rounded to the
-// weights' type first, so the codes fit the scale that is kept; a group of zeros has s = 0, one
-// with an infinity or NaN s = NaN, which its products show (minima and maxima pass over NaN).
+// weights' type first, so the codes fit the scale that is kept; where that leaves the group's ends
+// half a step or more outside the codes (s a few of the type's smallest steps, or 0) s is the next
+// number up. A group of zeros has s = 0, one with an infinity or NaN s = NaN, which its products
+// show (minima and maxima pass over NaN).
 // Once for a weight too: 28672 x 8192 in bf16 in 360 us, 1.6 TB/s.
 template <class T, int E>
 __global__ void __launch_bounds__(256) k_quantize4(const QuantizeArgs a) {
@@ -98,9 +100,11 @@ __global__ void __launch_bounds__(256) k_quantize4(const QuantizeArgs a) {
       lo = fminf(lo, __shfl_xor(lo, d, 16));
       hi = fmaxf(hi, __shfl_xor(hi, d, 16));
     }
-    float f[T::ce] = {a.zeros != nullptr ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f};
+    const float range = a.zeros != nullptr ? hi - lo : fmaxf(hi, -lo), spans = a.zeros != nullptr ? 15.0f : 7.0f;
+    float f[T::ce] = {range / spans};
     if (__ballot(!finite) >> (threadIdx.x & 48) & 0xffff) f[0] = __int_as_float(0x7fc00000);
-    const i32x4_t kept = pack<T>(f);
+    i32x4_t kept = pack<T>(f);
+    if (range > 0.0f && range / elem<T>(kept, 0) >= spans + 0.5f) ++kept[0];  // (the other elements are 0)
     const float s = elem<T>(kept, 0);
     const auto steps_in = [s](float x) { return s > 0.0f ? rintf(x / s) : 0.0f; };
     const float z = a.zeros != nullptr ? fminf(fmaxf(steps_in(-lo), 0.0f), 15.0f) : 8.0f;

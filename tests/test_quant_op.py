@@ -264,3 +264,33 @@ def test_weights_that_are_no_numbers_show(group, symmetric, dtype):
         x = torch.randn(m, k, generator=_gen(m)).to(dtype).to(DEV)
         got, want = linear4(x, q), linear4(x, p)
         assert got[:, 1:6].isnan().all() and torch.equal(got[:, 6:], want[:, 6:]) and torch.equal(got[:, 0], want[:, 0])
+
+
+@pytest.mark.parametrize("dtype,step", [(HF, 2.0**-24), (BF, 2.0**-133), (F, 2.0**-149)])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_small_weights_fit_the_scale_that_is_kept(dtype, step, symmetric):
+    """Groups whose scale is a few of the type's last steps: rounded down it would leave the ends
+    out of the codes' reach, or all of the group where it is 0."""
+    n, group = 250, 32
+    top = torch.arange(1, n + 1, dtype=torch.float64)
+    w = top[:, None] * (2 * torch.rand(n, 64, generator=_gen(2), dtype=torch.float64) - 1)
+    w[:, 0], w[:, 1], w[:, 40] = top, -top, top  # both ends; the second group's top alone
+    w = (w.round() * step).to(dtype)
+    assert (w.double()[:, 0] == top * step).all()
+    q = quantize4(w.to(DEV), group, symmetric=symmetric)
+    c, s, z = (None if t is None else t.cpu().double() for t in q.codes())
+    of = torch.arange(64) // group
+    w6, z = w.double(), torch.full_like(s, 8.0) if z is None else z
+    assert (s > 0).all()
+    off = (w6 / s[:, of] - (c - z[:, of])).abs()
+    if symmetric:
+        # 0.5 where nothing is cut off; quotients are fp32's, 2^-24 of at most 7.5.
+        assert off.max() <= 0.5 + 1e-5 and c.min() >= 1
+    else:
+        # A zero point is up to half a step off, and the range up to half a step past 15.
+        assert off.max() <= 1.0 + 1e-5
+    for g in range(2):  # no larger than one of the type's steps over what fits
+        part = w6[:, g * group:(g + 1) * group]
+        fits = part.abs().amax(1) / 7 if symmetric else (part.amax(1).clamp_min(0) - part.amin(1).clamp_max(0)) / 15
+        # (quotients of up to 34 steps: the type has all of them)
+        assert (s[:, g] <= fits + step).all() and (s[:, g] >= fits - step / 2 * (1 + 1e-5)).all()
