@@ -101,10 +101,10 @@ __global__ void __launch_bounds__(256) k_quantize4(const QuantizeArgs a) {
       hi = fmaxf(hi, __shfl_xor(hi, d, 16));
     }
     const float range = a.zeros != nullptr ? hi - lo : fmaxf(hi, -lo), spans = a.zeros != nullptr ? 15.0f : 7.0f;
-    float f[T::ce] = {range / spans};
+    float f[T::ce] = {isfinite(range) ? range / spans : hi / spans - lo / spans};  // (hi - lo may be past fp32)
     if (__ballot(!finite) >> (threadIdx.x & 48) & 0xffff) f[0] = __int_as_float(0x7fc00000);
     i32x4_t kept = pack<T>(f);
-    if (range > 0.0f && range / elem<T>(kept, 0) >= spans + 0.5f) ++kept[0];  // (the other elements are 0)
+    if (range > 0.0f && isfinite(range) && range / elem<T>(kept, 0) >= spans + 0.5f) ++kept[0];  // (the other elements are 0)
     const float s = elem<T>(kept, 0);
     const auto steps_in = [s](float x) { return s > 0.0f ? rintf(x / s) : 0.0f; };
     const float z = a.zeros != nullptr ? fminf(fmaxf(steps_in(-lo), 0.0f), 15.0f) : 8.0f;

@@ -117,7 +117,8 @@ def quantize4(w: torch.Tensor, group: int = 64, *, symmetric: bool = True) -> We
     """Round weights ``w [N, K]`` to 4 bits: each group to the nearest of ``s (c - 8)`` with ``s =
     max|w| / 7``, or without ``symmetric`` to ``s (c - z)`` over its range with zero, ``s = (max -
     min) / 15``. Scales have w's dtype, to which they are rounded before the codes are chosen (up
-    where the codes would not reach the group's ends else, among the type's last steps). A group with an infinity or NaN has the scale NaN, and all its weights are NaN."""
+    where the codes would not reach the group's ends else, among the type's last steps). A group
+    with an infinity or NaN has the scale NaN, and all its weights are NaN."""
     _need(w.ndim == 2, f"w must be [N, K], got {tuple(w.shape)}")
     n, k = w.shape
     _check_sizes(n, k, group)

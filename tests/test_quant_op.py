@@ -294,3 +294,20 @@ def test_small_weights_fit_the_scale_that_is_kept(dtype, step, symmetric):
         fits = part.abs().amax(1) / 7 if symmetric else (part.amax(1).clamp_min(0) - part.amin(1).clamp_max(0)) / 15
         # (quotients of up to 34 steps: the type has all of them)
         assert (s[:, g] <= fits + step).all() and (s[:, g] >= fits - step / 2 * (1 + 1e-5)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_a_range_past_the_largest_number(dtype):
+    """max - min of finite weights may be none."""
+    w = torch.randn(8, 64, generator=_gen(3)) * 1e37
+    w[:, 3], w[:, 7] = 3e38, -3e38
+    w[1, :32] = w[1, :32].abs().clamp_max(3e38)
+    w = w.to(dtype)
+    q = quantize4(w.to(DEV), 32, symmetric=False)
+    c, s, z = (t.cpu().double() for t in q.codes())
+    of = torch.arange(64) // 32
+    assert torch.isfinite(s).all()
+    top = (w.double().amax() - w.double().amin()) / 15  # of every row's first group but the second's
+    assert ((s[2:, 0] - top).abs() <= (torch.finfo(dtype).eps / 2 + 2.0**-22) * top).all()
+    best = w.double() / s[:, of] + z[:, of]
+    assert ((c - best.clamp(0, 15)).abs() <= 0.5 + 1e-5).all() and (best >= -0.55).all() and (best <= 15.55).all()
