@@ -40,7 +40,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_gain: torch.Tensor, k_gain: torch.Tensor, 
     Calls that no kernel may stand in for (tracing, transforms, tensor subclasses) run as torch
     operations on the same numbers."""
     if (_lib.ordinary(qkv, q_gain, k_gain, cos, sin) and qkv.is_cuda
-            and (kv_heads is None or type(kv_heads) is int)):
+            and (kv_heads is None or (type(kv_heads) is int and kv_heads > 0))):
         r = _lib.native().qk_norm_rope(qkv, q_gain, k_gain, cos, sin, 0 if kv_heads is None else kv_heads, eps)
         if r is not None:
             return tuple(r)

@@ -211,3 +211,8 @@ def test_the_decoder_normalises_heads_on_the_cpu():
         a.q_norm.weight.mul_(4.0)
         a.k_norm.weight.mul_(0.25)
         assert (m(idx) - want).abs().max() <= 1e-5 and (plain(idx) - want).abs().max() > 1e-4
+
+
+def test_no_kv_heads_are_refused():
+    with pytest.raises(ValueError, match="no queries"):
+        qk_norm_rope(torch.zeros(1, 2, 6, 8), torch.ones(8), torch.ones(8), torch.zeros(3, 4), torch.zeros(3, 4), kv_heads=0)

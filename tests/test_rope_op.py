@@ -387,3 +387,11 @@ def test_an_eps_of_zero(shape, dtype, gains, monkeypatch):
     """Places behind the last token hold no head: nothing of theirs is in the gains' gradients."""
     monkeypatch.setitem(globals(), "EPS", 0.0)  # (the oracle's and the calls' alike)
     test_forward_and_backward(shape, dtype, gains)
+
+
+def test_no_kv_heads_are_refused():
+    x, g = torch.zeros(1, 2, 6, 16, device=DEV, dtype=BF), torch.ones(16, device=DEV)
+    cos, sin = (z.to(DEV) for z in _tables(2, 16))
+    for kv in (0, -1, 3):
+        with pytest.raises(ValueError, match="no queries"):
+            qk_norm_rope(x, g, g, cos, sin, kv_heads=kv)
