@@ -533,6 +533,12 @@ std::optional<variable_list> rope_qkv(const Tensor& qkv, const Tensor& cosv, con
   return rope_forward(qkv, cosv, sinv);
 }
 
+// A projection as the kernels read it: dense, from a 16-byte boundary on.
+Tensor rows_of(const Tensor& qkv) {
+  const Tensor x = dense(qkv);
+  return aligned16(x) ? x : x.clone();
+}
+
 // The gains of a norm over heads of hd: of the activations' dtype or fp32, both the same.
 bool gains_ok(const Tensor& q_gain, const Tensor& k_gain, const Tensor& like, int64_t hd) {
   for (const Tensor* g : {&q_gain, &k_gain})
@@ -582,17 +588,15 @@ void check_capture(const Tensor& t) {
 struct QkNormRope : torch::autograd::Function<QkNormRope> {
   static variable_list forward(AutogradContext* ctx, const Tensor& qkv_in, const Tensor& gq_in, const Tensor& gk_in,
                                const Tensor& cosv, const Tensor& sinv, int64_t kv, double eps) {
-    Tensor qkv = dense(qkv_in);
-    if (!aligned16(qkv)) qkv = qkv.clone();
-    const Tensor gq = dense(gq_in), gk = dense(gk_in);
-    ctx->save_for_backward({qkv, gq, gk, cosv, sinv});
+    // The inputs themselves, not the copies: a recorded backward's derivative leads to them.
+    ctx->save_for_backward({qkv_in, gq_in, gk_in, cosv, sinv});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["kv"] = kv;
-    return head_norm_forward(qkv, gq, gk, cosv, sinv, kv, eps);
+    return head_norm_forward(rows_of(qkv_in), dense(gq_in), dense(gk_in), cosv, sinv, kv, eps);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &qkv = saved[0], &gq = saved[1], &gk = saved[2];
+    Tensor qkv = saved[0], gq = saved[1], gk = saved[2];
     const c10::DeviceGuard guard(qkv.device());
     check_capture(qkv);
     const double eps = ctx->saved_data["eps"].toDouble();
@@ -613,6 +617,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
       dx.push_back(grads[2]);
       return {at::cat(dx, 1).transpose(1, 2), dg[0], dg[1], Tensor(), Tensor(), Tensor(), Tensor()};
     }
+    qkv = rows_of(qkv), gq = dense(gq), gk = dense(gk);
     int64_t strides[9];
     for (int k = 0; k < 3; ++k) {
       Tensor& g = grads[k];
@@ -656,9 +661,7 @@ std::optional<variable_list> qk_norm_rope(const Tensor& qkv_in, const Tensor& gq
         t->size(0) < qkv_in.size(1))
       return std::nullopt;
   if (tracked(qkv_in) || tracked(gq) || tracked(gk)) return QkNormRope::apply(qkv_in, gq, gk, cosv, sinv, kv, eps);
-  Tensor qkv = dense(qkv_in);
-  if (!aligned16(qkv)) qkv = qkv.clone();
-  return head_norm_forward(qkv, dense(gq), dense(gk), cosv, sinv, kv, eps);
+  return head_norm_forward(rows_of(qkv_in), dense(gq), dense(gk), cosv, sinv, kv, eps);
 }
 
 struct SwiGlu : torch::autograd::Function<SwiGlu> {

@@ -395,3 +395,37 @@ def test_no_kv_heads_are_refused():
     for kv in (0, -1, 3):
         with pytest.raises(ValueError, match="no queries"):
             qk_norm_rope(x, g, g, cos, sin, kv_heads=kv)
+
+
+def test_second_derivatives_of_strided_inputs():
+    """Of rows and gains that the kernels take copies of."""
+    qkv = _rand(2, 4, 6, 16, dtype=F, seed=1).to(DEV)
+    gains = (1 + 0.3 * _rand(16, 2, dtype=F, seed=2)).to(DEV)
+    cos, sin = (z.to(DEV) for z in _tables(4, 16))
+    gs = [_rand(2, 2, 4, 16, dtype=F, seed=4 + i).to(DEV) for i in range(3)]
+    wide, off = torch.zeros(2, 4, 6, 40, device=DEV), torch.zeros(2 * 4 * 6 * 16 + 1, device=DEV)
+    wide[..., 5:21], off[1:] = qkv, qkv.flatten()
+
+    def second(x, a, c):
+        x, a, c = (z.detach().requires_grad_() for z in (x, a, c))
+        first = torch.autograd.grad(qk_norm_rope(x, a, c, cos, sin, eps=EPS), (x, a, c), gs, create_graph=True)
+        return (*first, *torch.autograd.grad(sum(y.square().sum() for y in first), (x, a, c)))
+
+    want = second(qkv, gains[:, 0].contiguous(), gains[:, 1].contiguous())
+    for x in (wide[..., 5:21], off[1:].view(2, 4, 6, 16)):
+        for o, w in zip(second(x, gains[:, 0], gains[:, 1]), want):
+            assert rel_l2(o.detach().cpu(), w.detach().cpu().double()) <= 1e-5  # two fp32 evaluations
+
+
+def test_strided_inputs_that_change_after_the_forward():
+    """As for dense ones: autograd says so instead of taking other numbers."""
+    cos, sin = (z.to(DEV) for z in _tables(4, 16))
+    for dense in (True, False):
+        x = _rand(2, 4, 6, 40, dtype=F, seed=1).to(DEV).requires_grad_()
+        y = x[..., 5:21].clone() if dense else (x * 1.0)[..., 5:21]
+        g = torch.ones(16, device=DEV, requires_grad=True)
+        outs = qk_norm_rope(y, g, g, cos, sin)
+        with torch.no_grad():
+            y.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(outs, (x, g), [torch.ones_like(o) for o in outs])
