@@ -715,13 +715,16 @@ class Transformer(nn.Module):
     @torch.no_grad()
     def quantize4_(self, group: int = 64, *, symmetric: bool = True) -> Transformer:
         """Replace every projection and the LM head by their 4-bit forms (``quant_op.Linear4``), for
-        inference; norms, the embedding and the AttnRes parameters stay. Returns the model."""
+        inference; norms, the embedding and the AttnRes parameters stay. Returns the model.
+        Raises, with nothing replaced, where a projection has a bias, hooks or a forward of its own."""
+        todo = [(self, "lm_head")]
         for layer in self.layers:
-            for owner, name in ((layer.attn, "qkv"), (layer.attn, "out"), (layer.mlp, "gate_up"), (layer.mlp, "down")):
-                if not isinstance(getattr(owner, name), Linear4):
-                    setattr(owner, name, Linear4.from_linear(getattr(owner, name), group, symmetric=symmetric))
-        if not isinstance(self.lm_head, Linear4):
-            self.lm_head = Linear4.from_linear(self.lm_head, group, symmetric=symmetric)
+            todo += [(layer.attn, "qkv"), (layer.attn, "out"), (layer.mlp, "gate_up"), (layer.mlp, "down")]
+        todo = [(owner, name) for owner, name in todo if not isinstance(getattr(owner, name), Linear4)]
+        for owner, name in todo:
+            Linear4.check(getattr(owner, name))
+        for owner, name in todo:
+            setattr(owner, name, Linear4.from_linear(getattr(owner, name), group, symmetric=symmetric))
         return self
 
     @torch.no_grad()

@@ -185,8 +185,19 @@ class Linear4(nn.Module):
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, group: int = 64, *, symmetric: bool = True) -> Linear4:
-        _need(linear.bias is None, "a projection with a bias has no 4-bit form")
+        """The 4-bit form of a projection that is its weights' product and nothing else: no bias, no
+        hooks, no ``forward`` of its own."""
+        cls.check(linear)
         return cls(quantize4(linear.weight, group, symmetric=symmetric))
+
+    @staticmethod
+    def check(linear: nn.Module) -> None:
+        """Raise ValueError where ``from_linear`` would."""
+        _need(getattr(linear, "bias", None) is None, "a projection with a bias has no 4-bit form")
+        _need(isinstance(linear, nn.Linear) and type(linear).forward is nn.Linear.forward and "forward" not in linear.__dict__,
+              f"{type(linear).__name__} is no plain projection: one with a forward of its own has no 4-bit form")
+        _need(not (linear._forward_hooks or linear._forward_pre_hooks or linear._backward_hooks or linear._backward_pre_hooks),
+              "a projection with hooks has no 4-bit form")
 
     @property
     def weight4(self) -> Weight4:

@@ -255,3 +255,11 @@ def test_a_captured_step_of_all_of_them():
         last.copy_(drawn)
         tokens[:, 20 + i] = drawn
         n += 1
+
+
+def test_a_decoder_is_quantized_whole_or_not_at_all():
+    m = _model()
+    m.layers[1].mlp.down.register_forward_hook(lambda mod, a, y: 2 * y)
+    with pytest.raises(ValueError, match="has no 4-bit form"):
+        m.quantize4_()
+    assert not any(isinstance(x, Linear4) for x in m.modules())

@@ -311,3 +311,22 @@ def test_a_range_past_the_largest_number(dtype):
     assert ((s[2:, 0] - top).abs() <= (torch.finfo(dtype).eps / 2 + 2.0**-22) * top).all()
     best = w.double() / s[:, of] + z[:, of]
     assert ((c - best.clamp(0, 15)).abs() <= 0.5 + 1e-5).all() and (best >= -0.55).all() and (best <= 15.55).all()
+
+
+def test_projections_that_are_more_than_their_weights_are_refused():
+    class Twice(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    def plain():
+        return torch.nn.Linear(64, 48, bias=False, device=DEV)
+
+    hooked, before, own = plain(), plain(), plain()
+    hooked.register_forward_hook(lambda m, a, y: 2 * y)
+    before.register_forward_pre_hook(lambda m, a: (2 * a[0],))
+    own.forward = lambda x: x[..., :48]
+    for m in (hooked, before, own, Twice(64, 48, bias=False, device=DEV), torch.nn.Bilinear(4, 4, 8, bias=False, device=DEV)):
+        with pytest.raises(ValueError, match="has no 4-bit form"):
+            Linear4.from_linear(m)
+    scaled = torch.nn.utils.parametrizations.weight_norm(plain())  # its weight is computed, its product the usual one
+    assert torch.equal(Linear4.from_linear(scaled).weight4.dequantize(), quantize4(scaled.weight).dequantize())
