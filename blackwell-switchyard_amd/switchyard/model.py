@@ -284,6 +284,8 @@ class Attention(nn.Module):
             if self.q_norm is not None:
                 q, k = self.q_norm(q), self.k_norm(k)
             q, k = rotary(q), rotary(k)
+            if self.q_norm is not None:  # (gains of another type make wider heads)
+                q, k = q.to(v.dtype), k.to(v.dtype)
             split = [y.transpose(1, 2).contiguous() for y in (q, k, v)]
         q, k, v = split
         y = F.scaled_dot_product_attention(q, k, v, is_causal=True)

@@ -216,3 +216,19 @@ def test_the_decoder_normalises_heads_on_the_cpu():
 def test_no_kv_heads_are_refused():
     with pytest.raises(ValueError, match="no queries"):
         qk_norm_rope(torch.zeros(1, 2, 6, 8), torch.ones(8), torch.ones(8), torch.zeros(3, 4), torch.zeros(3, 4), kv_heads=0)
+
+
+def test_head_norms_of_another_type_than_the_projections_on_the_cpu():
+    torch.manual_seed(0)
+    cfg = ModelConfig(vocab_size=50, d_model=32, n_layers=2, n_heads=2, d_ff=48, n_blocks=2, max_seq_len=16, qk_norm=True)
+    m = Transformer(cfg).bfloat16()
+    idx = torch.randint(0, 50, (2, 9))
+    want = m(idx)
+    for layer in m.layers:
+        layer.attn.q_norm.float()
+        layer.attn.k_norm.float()
+    got, loss = m(idx, idx)
+    loss.backward()
+    assert got.dtype == want.dtype and m.layers[0].attn.q_norm.weight.grad.dtype == torch.float32
+    # The gains are one: the norms round less, by bf16's 2^-8 a few times a layer.
+    assert (got - want).abs().max() <= 2.0**-4 * want.abs().max()
