@@ -395,7 +395,8 @@ class _CacheStep:
         norm = {}
         if attn.q_norm is not None:
             gains = attn.head_gains()
-            if gains is None:  # norms that are more than their kernel
+            # norms that are more than their kernel, or of a type that it does not take next to the projection's
+            if gains is None or gains[0].dtype != gains[1].dtype or gains[0].dtype not in (qkv.dtype, torch.float32):
                 q, k, v = qkv.view(n_tok, 3, attn.heads, attn.hd).unbind(1)
                 qkv = torch.cat((attn.q_norm(q).to(v.dtype), attn.k_norm(k).to(v.dtype), v), 1)
             else:

@@ -263,3 +263,21 @@ def test_a_decoder_is_quantized_whole_or_not_at_all():
     with pytest.raises(ValueError, match="has no 4-bit form"):
         m.quantize4_()
     assert not any(isinstance(x, Linear4) for x in m.modules())
+
+
+def test_gains_of_another_type_than_the_projections():
+    """Every rounding is fp16's, 2^-11; some twenty a layer and as many a logit's terms, in two
+    evaluations: under 2^-5 of the largest logit."""
+    m = _model(dtype=torch.bfloat16, residual="standard")
+    idx = _tokens(2, 20)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+        want = m(idx).float()
+        got = m.decode(idx, DecodeState(m, 2, 30, page=16)).float()
+    assert (got - want[:, -1]).abs().max() <= 2.0**-5 * want.abs().max()
+    mixed = _model(dtype=torch.bfloat16)
+    for layer in mixed.layers:
+        layer.attn.q_norm.float()  # next to a k_norm in bf16
+    with torch.no_grad():
+        want = mixed(idx).float()
+        got = mixed.decode(idx, DecodeState(mixed, 2, 30, page=16)).float()
+    assert (got - want[:, -1]).abs().max() <= 2.0**-2 * want.abs().max()  # bf16's: 2^-8
