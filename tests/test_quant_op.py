@@ -330,3 +330,13 @@ def test_projections_that_are_more_than_their_weights_are_refused():
             Linear4.from_linear(m)
     scaled = torch.nn.utils.parametrizations.weight_norm(plain())  # its weight is computed, its product the usual one
     assert torch.equal(Linear4.from_linear(scaled).weight4.dequantize(), quantize4(scaled.weight).dequantize())
+
+
+@pytest.mark.parametrize("m,n,k", [(4100, 64, 100), (8201, 64, 2048)])
+def test_more_fp32_rows_than_a_launch(m, n, k):
+    test_product(m, n, k, 64, F, True)
+
+
+def test_more_rows_than_a_launch():
+    test_product(4101, 16, 128, 64, BF, True)
+    test_product(4101, 16, 128, 64, HF, False)

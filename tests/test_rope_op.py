@@ -429,3 +429,35 @@ def test_strided_inputs_that_change_after_the_forward():
             y.mul_(2.0)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             torch.autograd.grad(outs, (x, g), [torch.ones_like(o) for o in outs])
+
+
+@pytest.mark.parametrize("shape,dtype", [((3, 5500, 2, 1, 128), BF), ((1, 4099, 2, 1, 256), F), ((1, 131100, 1, 1, 8), HF)], ids=str)
+def test_more_tokens_than_workgroups_at_once(shape, dtype):
+    """Over 2048 groups of tokens each workgroup has a second one."""
+    test_forward_and_backward(shape, dtype, dtype)
+
+
+def test_bad_gains_of_an_append_are_refused(monkeypatch):
+    hd = 32
+    cos, sin = (z.to(DEV) for z in _tables(8, hd))
+    k, v = (torch.zeros(2, 1, 4, hd, device=DEV, dtype=BF) for _ in range(2))
+    table, n = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.full((1,), 3, dtype=torch.int32, device=DEV)
+    g = torch.ones(hd, device=DEV, dtype=BF)
+
+    def call(**kw):
+        return paged_append(_rand(3, 4, hd, dtype=BF, seed=1).to(DEV), cos, sin, k, v, table, n, **kw)
+
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(_lib, "ordinary", lambda *t: False)
+        call(q_gain=g, k_gain=g)
+        before = k.clone(), v.clone()
+        for kw, what in ((dict(q_gain=g), "go together"), (dict(k_gain=g), "go together"),
+                         (dict(q_gain=g[:16], k_gain=g), "q_gain must be"), (dict(q_gain=g, k_gain=g[:16]), "k_gain must be"),
+                         (dict(q_gain=g.half(), k_gain=g.half()), "q_gain must be"),
+                         (dict(q_gain=g, k_gain=g.float()), "k_gain must be"),
+                         (dict(q_gain=g.cpu(), k_gain=g.cpu()), "q_gain must be"),
+                         (dict(q_gain=g[:, None], k_gain=g), "q_gain must be")):
+            with pytest.raises(ValueError, match=what):
+                call(**kw)
+        assert torch.equal(k, before[0]) and torch.equal(v, before[1])
