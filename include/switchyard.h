@@ -358,7 +358,8 @@ int sy_rope_qkv(void* qkv, void* q, void* k, void* v, const float* cosv, const f
  * multiple of 8, at most 256. The gradient reads dq, dk, dv with strides (elements, multiples
  * of a 16-byte chunk) for batch, head and token, three each, rows of hd dense, and writes dqkv
  * and the gains' gradients, summed over tokens in a fixed order in a workspace of
- * sy_qk_norm_rope_bwd_bytes bytes. No reference counterpart. */
+ * sy_qk_norm_rope_bwd_bytes bytes. With no tokens nothing is written, the gains' gradients not
+ * either: a caller that wants their zeros fills them. No reference counterpart. */
 int sy_qk_norm_rope(const void* qkv, const void* q_gain, const void* k_gain, const float* cosv, const float* sinv,
                     void* q, void* k, void* v, int64_t n_tok, int64_t seq, int64_t heads, int64_t kv_heads,
                     int64_t hd, int dtype, int gain_dtype, float eps, void* stream);
