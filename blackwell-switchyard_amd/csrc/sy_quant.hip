@@ -167,8 +167,8 @@ template <> struct Mma<F32> : Mma<BF16> {
 __device__ __forceinline__ uint32_t ror(uint32_t x, int n) { return __builtin_amdgcn_alignbit(x, x, n); }
 
 // The eight weights of a word as 1 + c / 16. Mask and one are held in registers, opaque to the
-// compiler, which else takes them as literals and splits each and-or in two (us: 2048 rows of 2048
-// x 5632 58, so 57; 32 of 11264 x 2048 8.0, so 7.6).
+// compiler, which else takes them as literals and splits each and-or in two (2048 rows of 2048 x
+// 5632 so take 2% less time, 32 of 11264 x 2048 5%).
 template <class T> struct Codes {
   static constexpr float unit = 16.0f;  // of the sums
   uint32_t mask = Mma<T>::mask, one = Mma<T>::one;
@@ -298,12 +298,13 @@ template <class T, int MT, int NT, int NG, bool ZEROS> struct Step {
 };
 
 // A workgroup has NT feature tiles and 16 MT rows; its waves share the columns out tile by tile
-// and fold their sums in LDS in their order. GS: 32-column pieces of a group. The weights' bytes bound it where
-// there are many: 16 rows of 28672 x 8192 29.1 us, 4.3 TB/s (its waves wait half their time, the
-// vector units work 43% of it), 8 rows of 32000 x 2048 8.2, 4.2; else latency, 1 row of 6144 x
-// 2048 4.1. More waves, a wave's next tile asked for ahead, loads past the caches and other orders
-// of the columns gained nothing over all shapes. (32 rows by 64 features are bound to two waves a SIMD: with the registers
-// of three the compiler asks for less at a time, 32 rows of 28672 x 8192 58 us for 42.)
+// and fold their sums in LDS in their order. GS: 32-column pieces of a group. The weights' bytes
+// bound it where there are many: 16 rows of 28672 x 8192 29.3 us, 4.2 TB/s (its waves wait half
+// their time, the vector units work 43% of it), 8 rows of 32000 x 2048 8.2, 4.2; else latency, 1 row
+// of 6144 x 2048 3.7 where launches follow one another. More waves, a wave's next tile asked for
+// ahead, loads past the caches and other orders of the columns gained nothing over all shapes. (32
+// rows by 64 features are bound to two waves a SIMD: with the registers of three the compiler asks
+// for less at a time, and 32 rows of 28672 x 8192 take 1.4 times as long.)
 template <class T, int MT, int NT, int WAVES, bool STAGED, int GS, bool ZEROS>
 __global__ void __launch_bounds__(64 * WAVES < 512 ? 512 : 64 * WAVES)
 __attribute__((amdgpu_waves_per_eu(WAVES < 16 ? 2 : 4, MT * NT == 8 ? 2 : 8))) k_linear4(const Linear4Args a) {
@@ -491,9 +492,9 @@ template <int N> struct Bytes {
 // waves take every other column tile and add up at the end. A tile's sums over each group's
 // columns are formed where it is written to LDS, by the lanes that hold it; DIRECT: the tile goes
 // straight to LDS, for which rows start at 16-byte boundaries, and each wave takes the sums off
-// the matrix units (us: 512 rows of 2048 x 5632 27.0, so 24.6; 4096 of 11264 x 2048 229, so 219;
-// 2048 of 2048 x 5632 58.2, so 57.5). Vector instructions bound it, next to waits: the last of
-// those is 820 TFLOP/s; codes to numbers and scaling are a third of them each. The library's
+// the matrix units (512 rows of 2048 x 5632 so take 9% less time, 4096 of 11264 x 2048 4%, 2048 of
+// 2048 x 5632 1%: 24.2, 221 and 55.8 us). Vector instructions bound it, next to waits: the last of
+// those is 847 TFLOP/s; codes to numbers and scaling are a third of them each. The library's
 // product with bf16 weights takes 54.5.
 template <class T, int NT, int PARTS, bool DIRECT, int GS, bool ZEROS>
 __global__ void __launch_bounds__(256 * PARTS) __attribute__((amdgpu_waves_per_eu(2)))
@@ -734,7 +735,8 @@ hipError_t run4_many(const Linear4Args& a, hipStream_t s) {
   return direct ? run4_direct<T, NT, PARTS, true, GS, ZEROS>(a, s) : run4_direct<T, NT, PARTS, false, GS, ZEROS>(a, s);
 }
 
-// The kernel and its tile by rows and feature tiles; us on both sides, bf16 unless stated.
+// The kernel and its tile by rows and feature tiles; us on both sides, bf16 unless stated, of the
+// sweep that the costs were fitted to (captured launches on one machine; others are up to 6% off).
 //   up to 16         straight from memory with one or two feature tiles, where a load's lanes touch
 //                    few lines, or through LDS with one, two or four, by the costs below. In their
 //                    order: 1 row of 6144 x 2048 3.5, 3.6, and 4.0 at best through LDS; 8 of 2048 x

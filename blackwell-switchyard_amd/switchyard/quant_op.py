@@ -140,7 +140,13 @@ def quantize4(w: torch.Tensor, group: int = 64, *, symmetric: bool = True) -> We
 
 def linear4(x: torch.Tensor, weight: Weight4) -> torch.Tensor:
     """``x [..., in_features]`` times the weights, ``[..., out_features]``; x has the scales'
-    dtype. A row with an infinity or NaN gives NaN."""
+    dtype. A row with an infinity or NaN gives NaN, and so may sums that pass fp32's range on the way
+    (activations past 2^112).
+
+    16-bit rows meet ``1 + c / 16``, less ``(1 + z / 16)`` of their sum over the group: two sums of
+    the size of ``16 s |x| (2 + (c + z) / 16)``, where ``s (c - z) x`` added up directly are of ``s
+    |x| |c - z|``. fp32's error in them, about ten times that of the direct sum, shows past the
+    output's rounding only where a result all but cancels. fp32 rows meet ``c - z``."""
     return _linear4(x, weight.tiles, weight.scales, weight.zeros, weight.out_features, weight.in_features, weight.group)
 
 

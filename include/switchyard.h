@@ -512,7 +512,8 @@ int sy_adjust(const void* logits, void* out, const sy_adjusting* how, int64_t n_
  * ceil(n / 16) ceil(k / 128) of them, tile_scales and tile_zeros [ceil(n / 16)][ceil(k / 128)]
  * [16][128 / group]; tiles and tile_scales start at 16-byte boundaries, tile_zeros at 4-byte
  * ones. Rows of x are x_stride elements apart and
- * start anywhere; a row with an infinity or NaN gives NaN. No reference counterpart. */
+ * start anywhere; a row with an infinity or NaN gives NaN, and so may one with numbers past 2^112,
+ * whose sums pass fp32's range. No reference counterpart. */
 int sy_quantize4(const void* w, int64_t row_stride, uint8_t* codes, void* scales, uint8_t* zeros, int64_t n,
                  int64_t k, int64_t group, int dtype, void* stream);
 int sy_pack4(const uint8_t* codes, const void* scales, const uint8_t* zeros, void* tiles, void* tile_scales,
